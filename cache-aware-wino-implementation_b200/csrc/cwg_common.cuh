@@ -32,6 +32,22 @@ inline cudaError_t smem_attr_once(int bytes) {
   return smem_attr_once(done, (const void *)Kernel, bytes);
 }
 
+// Reads a translation unit's status word and clears it when it is set.
+inline int read_clear_status(unsigned &word, unsigned *status) {
+  unsigned v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, word, sizeof(v));
+  if (e == cudaSuccess && v) {
+    const unsigned zero = 0;
+    e = cudaMemcpyToSymbol(word, &zero, sizeof(zero));
+  }
+  if (e != cudaSuccess) {
+    cwgk_set_cuda_error((int)e);
+    return -3;
+  }
+  *status = v;
+  return 0;
+}
+
 // ---- weight transform G g G^T ------------------------------------------------
 // G for F(2,3), F(4,3) and F(6,3): the unique matrices that make the reference's Bt/At
 // (src/fused_winograd_kernel.py:18-67) compute a 3x3 cross-correlation.

@@ -1,0 +1,604 @@
+// cwg_fp8.cu -- e4m3 quantiser and matrix product with fp32 scales per block of 128
+// (cwg_fp8_quantize, cwg_fp8_matmul).
+//
+//   y[i][j] = act(bias[j] + sum_kb as[i][kb] ws[j / 128][kb] sum_{k in kb} a[i][k] w[j][k])
+//
+// The inner sum over one block of 128 runs on the tensor cores (kind::f8f6f4, e4m3,
+// fp32 accumulators in tensor memory); as soon as a block is done, the promoting
+// warps read it back, scale it and add it to fp32 registers, while the next block's
+// MMAs fill another accumulator.  The scales differ from block to block, so no sum
+// can run across blocks inside the tensor core.
+#include <cstdint>
+
+#include <cuda.h>
+#include <cuda_fp8.h>
+
+#include "../../include/cwg.h"
+#include "cwg_seq.cuh"
+#include "cwg_tcgen05.cuh"
+
+namespace cwg {
+namespace fp8 {
+
+using namespace tc;
+using seq::pack1;
+
+__device__ unsigned int g_fp8_status;
+
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *abort) {
+  return tc::mbar_wait(bar, parity, abort, &g_fp8_status);
+}
+
+// ---- quantiser ---------------------------------------------------------------------
+constexpr float kE4m3Max = 448.f;
+constexpr float kScaleMin = 1.17549435e-38f;  // 2^-126
+
+// max |x| by its bits: NaN is larger than infinity, infinity than any number
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ float scale_of(uint32_t amax) {
+  const float s = __fdiv_rn(__uint_as_float(amax), kE4m3Max);
+  return s < kScaleMin ? kScaleMin : s;  // NaN stays
+}
+__device__ __forceinline__ uint32_t e4m3x4(const float *v, float s) {
+  const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(
+      make_float2(__fdiv_rn(v[0], s), __fdiv_rn(v[1], s)), __NV_SATFINITE, __NV_E4M3);
+  const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(
+      make_float2(__fdiv_rn(v[2], s), __fdiv_rn(v[3], s)), __NV_SATFINITE, __NV_E4M3);
+  return (uint32_t)lo | (uint32_t)hi << 16;
+}
+
+struct QuantArgs {
+  const void *x;
+  uint8_t *q;
+  float *scale;
+  size_t ldx, ldq, lds;
+  int rows, cols, kblocks;
+  long long groups;
+};
+
+// 8 consecutive elements of a row (zeros past the end), and their codes back.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T *p, int n, float (&v)[8]) {
+  if constexpr (VEC) {
+    constexpr int E = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 8; i += E) {
+      float f[E];
+      seq::unpack(i < n ? seq::load_raw<T, E>(p + i) : seq::zero_raw<T, E>(), f);
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[i + e] = i + e < n ? f[e] : 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.f;
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void store8(uint8_t *q, const float (&v)[8], float s, int n) {
+  const uint32_t a = e4m3x4(v, s), b = e4m3x4(v + 4, s);
+  if (VEC && n >= 8) {
+    *reinterpret_cast<uint2 *>(q) = make_uint2(a, b);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) q[i] = (uint8_t)((i < 4 ? a >> 8 * i : b >> 8 * (i - 4)) & 0xff);
+  }
+}
+
+// One half-warp per group of 1 x 128: 8 elements a lane, read once.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) quantize_rows(const QuantArgs a) {
+  const long long g = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int lane = threadIdx.x & 15;
+  const bool ok = g < a.groups;
+  const int row = ok ? (int)(g / a.kblocks) : 0, kb = ok ? (int)(g % a.kblocks) : 0;
+  const int c = kb * 128 + lane * 8;
+  const int n = ok ? a.cols - c : 0;
+  float v[8];
+  load8<T, VEC>(static_cast<const T *>(a.x) + (size_t)row * a.ldx + c, n, v);
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i]));
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float s = scale_of(m);
+  if (ok && lane == 0) a.scale[(size_t)row * a.lds + kb] = s;
+  if (n > 0) store8<VEC>(a.q + (size_t)row * a.ldq + c, v, s, n);
+}
+
+// One CTA per block of 128 x 128, 64 elements a thread held in registers.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) quantize_blocks(const QuantArgs a) {
+  __shared__ uint32_t s_max[8];
+  const int kb = blockIdx.x % a.kblocks, rb = blockIdx.x / a.kblocks;
+  const int c = kb * 128 + (threadIdx.x & 15) * 8, r0 = rb * 128 + (threadIdx.x >> 4);
+  float v[8][8];
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = r0 + i * 16;
+    const int n = r < a.rows ? a.cols - c : 0;
+    load8<T, VEC>(static_cast<const T *>(a.x) + (size_t)(r < a.rows ? r : 0) * a.ldx + c, n,
+                  v[i]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = max(m, abs_bits(v[i][e]));
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, s_max[i]);
+  const float s = scale_of(m);
+  if (threadIdx.x == 0) a.scale[(size_t)rb * a.lds + kb] = s;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = r0 + i * 16;
+    if (r < a.rows && c < a.cols) store8<VEC>(a.q + (size_t)r * a.ldq + c, v[i], s, a.cols - c);
+  }
+}
+
+template <typename T>
+static int quantize(QuantArgs a, int block_rows, cudaStream_t s) {
+  constexpr int E = 16 / (int)sizeof(T);
+  const bool one = a.rows <= 1;
+  // a whole vector at a row's end may reach past cols only if the row does
+  const bool vec = ((uintptr_t)a.x & 15) == 0 && ((uintptr_t)a.q & 7) == 0 &&
+                   a.cols % E == 0 && (one || (a.ldx % E == 0 && a.ldq % 8 == 0));
+  const long long blocks = block_rows == 1 ? (a.groups + 15) / 16 : a.groups;
+  if (blocks > 0x7fffffffLL) return -2;
+  if (block_rows == 1) {
+    if (vec)
+      quantize_rows<T, true><<<(unsigned)blocks, 256, 0, s>>>(a);
+    else
+      quantize_rows<T, false><<<(unsigned)blocks, 256, 0, s>>>(a);
+  } else {
+    if (vec)
+      quantize_blocks<T, true><<<(unsigned)blocks, 256, 0, s>>>(a);
+    else
+      quantize_blocks<T, false><<<(unsigned)blocks, 256, 0, s>>>(a);
+  }
+  cwgk_count_launch();
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) {
+    cwgk_set_cuda_error((int)e);
+    return -3;
+  }
+  return 0;
+}
+
+// ---- matrix product -----------------------------------------------------------------
+// The weights are the MMA's M side: a CTA owns 128 outputs x TN rows of a, so that
+// few rows (decoding) waste no MMA rows and the weight stream is read once.  Operand
+// tiles of 128 k (128 bytes a row) come by TMA with the 128-byte swizzle; four MMAs of
+// k = 32 make a block.  TMEM lane = output, column = row of a.  Promoting warps hold
+// 32 outputs x TN (or TN / 2) sums each; the block's scales as * ws, one per column,
+// are a broadcast read from shared memory that one warp keeps filled ahead.
+// When the tiles leave SMs idle, the k blocks are cut among the CTAs of a cluster,
+// which add their sums through distributed shared memory in rank order: the result
+// does not depend on timing, and no workspace is needed.
+constexpr int kTileK = 128;
+constexpr int kGroupK = 8;  // blocks whose scales are staged together
+
+template <int TN>
+struct Cfg {
+  static constexpr int kPromote = TN > 64 ? 8 : 4;       // promoting warps
+  static constexpr int kCols = TN * 4 / kPromote;        // columns per promoting thread
+  static constexpr int kThreads = (kPromote + 3) * 32;
+  static constexpr int kMinBlocks = TN > 64 ? 1 : 2;
+  static constexpr int kAcc = TN > 64 ? 2 : 4;           // accumulators in flight
+  static constexpr int kTmem = kAcc * TN;
+  static constexpr int kStageBytes = 128 * kTileK + TN * kTileK;
+  static constexpr int kStages = TN > 64 ? 6 : 4;
+  static constexpr int kScaleOff = kStages * kStageBytes;
+  static constexpr int kScaleBytes = 2 * kGroupK * TN * 4;
+  static constexpr int kBarOff = kScaleOff + kScaleBytes;
+  // full[], empty[], acc_full[], acc_empty[], s_full[2], s_empty[2], drain
+  static constexpr int kBars = 2 * kStages + 2 * kAcc + 5;
+  static constexpr int kSmem = kBarOff + 8 * kBars + 16 + 1024;  // + slack to align to 1024
+  static_assert(128 * TN * 4 <= kStages * kStageBytes, "partial sums reuse the stages");
+};
+
+struct MatArgs {
+  const float *a_scale, *w_scale, *bias;
+  void *y;
+  size_t lda_scale, ldw_scale, ldy;
+  int m, n, kblocks, per;  // per: k blocks of one cluster rank
+  int splits, relu, bf16;
+};
+
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, int x, int y,
+                                       uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void mma_fp8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                        uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// K-major operand of 128-byte rows in the 128-byte swizzle: 8-row groups 1024 B apart.
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// kind::f8f6f4: D fp32, A and B e4m3, both K-major.
+__host__ __device__ constexpr uint32_t idesc_fp8(int m, int n) {
+  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float *v) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void store_out(const MatArgs &a, int row, int col, float v,
+                                          float bias) {
+  v += bias;
+  if (a.relu && v < 0.f) v = 0.f;  // NaN stays
+  const size_t at = (size_t)row * a.ldy + col;
+  if (a.bf16)
+    static_cast<__nv_bfloat16 *>(a.y)[at] = pack1<__nv_bfloat16>(v);
+  else
+    static_cast<float *>(a.y)[at] = v;
+}
+
+template <int TN>
+__global__ void __launch_bounds__(Cfg<TN>::kThreads, Cfg<TN>::kMinBlocks)
+    fp8_matmul(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
+               const MatArgs p) {
+  using C = Cfg<TN>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t sbase = (smem_u32(smem_raw) + 1023) & ~1023u;
+  uint8_t *smem = smem_raw + (sbase - smem_u32(smem_raw));
+  const uint32_t full = sbase + C::kBarOff, empty = full + 8 * C::kStages;
+  const uint32_t acc_full = empty + 8 * C::kStages, acc_empty = acc_full + 8 * C::kAcc;
+  const uint32_t s_full = acc_empty + 8 * C::kAcc, s_empty = s_full + 16, drain = s_empty + 16;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + C::kBarOff + 8 * C::kBars);
+  volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
+  const int rank = p.splits > 1 ? (int)cluster_rank() : 0;
+  const int tile = blockIdx.x / p.splits;
+  const int ntiles = (p.n + 127) / 128;
+  const int n0 = (tile % ntiles) * 128, m0 = (tile / ntiles) * TN;
+  const int kb0 = min(rank * p.per, p.kblocks), kb1 = min(kb0 + p.per, p.kblocks);
+  const int nkb = kb1 - kb0;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, 1);
+    }
+    for (int i = 0; i < C::kAcc; ++i) {
+      mbar_init(acc_full + 8 * i, 1);
+      mbar_init(acc_empty + 8 * i, C::kPromote);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + 8 * i, 1);
+      mbar_init(s_empty + 8 * i, C::kPromote);
+    }
+    mbar_init(drain, 1);
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == C::kPromote) {  // the MMA warp owns the tensor memory
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)),
+                 "r"(C::kTmem));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  float acc[C::kCols];
+#pragma unroll
+  for (int j = 0; j < C::kCols; ++j) acc[j] = 0.f;
+
+  if (warp == C::kPromote) {
+    // ---- MMAs
+    constexpr uint32_t idesc = idesc_fp8(128, TN);
+    bool ok = true;
+    for (int i = 0; i < nkb; ++i) {
+      const int st = i % C::kStages, ac = i % C::kAcc;
+      ok = __all_sync(0xffffffffu,
+                      mbar_wait(acc_empty + 8 * ac, ((i / C::kAcc) & 1) ^ 1, abort) &&
+                          mbar_wait(full + 8 * st, (i / C::kStages) & 1, abort));
+      if (!ok) break;
+      tc_fence_after();
+      const uint64_t w = desc_sw128(sbase + st * C::kStageBytes);
+      const uint64_t a = desc_sw128(sbase + st * C::kStageBytes + 128 * kTileK);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)  // 32 bytes along k = 2 descriptor units
+        if (elect_one()) mma_fp8(tmem + ac * TN, w + 2 * k, a + 2 * k, idesc, k > 0);
+      __syncwarp();
+      if (elect_one()) tc_commit(empty + 8 * st);
+      if (elect_one()) tc_commit(acc_full + 8 * ac);
+      __syncwarp();
+    }
+    if (!ok) {  // let what was issued finish before the tensor memory is freed
+      if (elect_one()) tc_commit(drain);
+      __syncwarp();
+      const unsigned long long t0 = globaltimer();
+      while (!mbar_try(drain, 0) && globaltimer() - t0 < kTimeoutNs) {
+      }
+    }
+  } else if (warp == C::kPromote + 1) {
+    // ---- operand tiles
+    int issued = 0;
+    for (int i = 0; i < nkb; ++i) {
+      const int st = i % C::kStages;
+      if (!__all_sync(0xffffffffu,
+                      mbar_wait(empty + 8 * st, ((i / C::kStages) & 1) ^ 1, abort)))
+        break;
+      if (elect_one()) {
+        const uint32_t dst = sbase + st * C::kStageBytes;
+        mbar_expect_tx(full + 8 * st, C::kStageBytes);
+        tma_2d(dst, &map_w, (kb0 + i) * kTileK, n0, full + 8 * st);
+        tma_2d(dst + 128 * kTileK, &map_a, (kb0 + i) * kTileK, m0, full + 8 * st);
+      }
+      __syncwarp();
+      issued = i + 1;
+    }
+    // never leave the CTA with a copy still writing shared memory
+    for (int i = issued - C::kStages > 0 ? issued - C::kStages : 0; i < issued; ++i) {
+      const unsigned long long t0 = globaltimer();
+      while (!mbar_try(full + 8 * (i % C::kStages), (i / C::kStages) & 1) &&
+             globaltimer() - t0 < kTimeoutNs) {
+      }
+    }
+  } else if (warp == C::kPromote + 2) {
+    // ---- scales: as[row][kb] * ws[kb] of kGroupK blocks at a time, one group ahead in
+    // registers
+    float *s_scale = reinterpret_cast<float *>(smem + C::kScaleOff);
+    constexpr int R = (TN + 31) / 32;
+    const float *ws = p.w_scale + (size_t)(n0 / 128) * p.ldw_scale;
+    float v[R][kGroupK];
+    auto fetch = [&](int i0) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int row = m0 + r * 32 + lane;
+        const bool ok = r * 32 + lane < TN && row < p.m;
+        const float *as = p.a_scale + (size_t)(ok ? row : 0) * p.lda_scale;
+#pragma unroll
+        for (int k = 0; k < kGroupK; ++k)
+          v[r][k] = ok && i0 + k < nkb ? as[kb0 + i0 + k] * ws[kb0 + i0 + k] : 0.f;
+      }
+    };
+    fetch(0);
+    for (int i = 0, g = 0; i < nkb; i += kGroupK, ++g) {
+      if (!__all_sync(0xffffffffu, mbar_wait(s_empty + 8 * (g & 1), ((g >> 1) & 1) ^ 1, abort)))
+        break;
+      float *dst = s_scale + (g & 1) * kGroupK * TN;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int k = 0; k < kGroupK; ++k)
+          if (r * 32 + lane < TN) dst[k * TN + r * 32 + lane] = v[r][k];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_full + 8 * (g & 1));
+      if (i + kGroupK < nkb) fetch(i + kGroupK);
+    }
+  } else {
+    // ---- promotion
+    const int quad = warp & 3, half = warp >> 2;
+    const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16) + half * C::kCols;
+    const float *s_scale = reinterpret_cast<const float *>(smem + C::kScaleOff) + half * C::kCols;
+    for (int i = 0; i < nkb; ++i) {
+      const int ac = i % C::kAcc, g = i / kGroupK, k = i % kGroupK;
+      bool ok = true;
+      if (k == 0) ok = mbar_wait(s_full + 8 * (g & 1), (g >> 1) & 1, abort);
+      ok = ok && mbar_wait(acc_full + 8 * ac, (i / C::kAcc) & 1, abort);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      const float *sc = s_scale + ((g & 1) * kGroupK + k) * TN;
+#pragma unroll
+      for (int j0 = 0; j0 < C::kCols; j0 += 16) {
+        float v[16];
+        tmem_ld16(trow + ac * TN + j0, v);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          const float4 f = *reinterpret_cast<const float4 *>(sc + j0 + j);
+          acc[j0 + j] = fmaf(v[j], f.x, acc[j0 + j]);
+          acc[j0 + j + 1] = fmaf(v[j + 1], f.y, acc[j0 + j + 1]);
+          acc[j0 + j + 2] = fmaf(v[j + 2], f.z, acc[j0 + j + 2]);
+          acc[j0 + j + 3] = fmaf(v[j + 3], f.w, acc[j0 + j + 3]);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(acc_empty + 8 * ac);
+        if (k == kGroupK - 1) mbar_arrive(s_empty + 8 * (g & 1));
+      }
+    }
+    const int row = quad * 32 + lane, col = n0 + row;
+    if (p.splits == 1) {
+      if (col < p.n) {
+        const float bias = p.bias ? p.bias[col] : 0.f;
+#pragma unroll
+        for (int j = 0; j < C::kCols; ++j)
+          if (m0 + half * C::kCols + j < p.m)
+            store_out(p, m0 + half * C::kCols + j, col, acc[j], bias);
+      }
+    }
+  }
+  if (p.splits > 1) {
+    // all copies have landed and all MMAs have read them once every role is here
+    __syncthreads();
+    float *part = reinterpret_cast<float *>(smem);  // [column][output]
+    if (warp < C::kPromote) {
+      const int row = (warp & 3) * 32 + lane;
+#pragma unroll
+      for (int j = 0; j < C::kCols; ++j) part[((warp >> 2) * C::kCols + j) * 128 + row] = acc[j];
+    }
+    cluster_sync_all();
+    // rank r finishes the columns r, r + splits, ...
+    const int row = threadIdx.x & 127, lead = (int)(threadIdx.x >> 7);
+    constexpr int kTeams = C::kThreads / 128;
+    const int col = n0 + row;
+    if (lead < kTeams && col < p.n) {
+      const float bias = p.bias ? p.bias[col] : 0.f;
+      for (int j = rank + lead * p.splits; j < TN && m0 + j < p.m; j += kTeams * p.splits) {
+        const uint32_t at = sbase + (uint32_t)(j * 128 + row) * 4;
+        float v = 0.f;
+        for (int r = 0; r < p.splits; ++r) v += ld_cluster(mapa_shared(at, (uint32_t)r));
+        store_out(p, m0 + j, col, v, bias);
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();  // no CTA leaves while another reads its sums
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == C::kPromote) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(C::kTmem));
+  }
+}
+
+// Row-major e4m3 matrix [rows][k], rows ld bytes apart, as tiles of box_rows x 128.
+// Reads outside [rows][k] give zeros.
+static int make_map(CUtensorMap *map, const void *base, long long ld, int rows, int k,
+                    int box_rows) {
+  typedef CUresult (*encode_fn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
+                                const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static std::atomic<encode_fn> found_fn{nullptr};  // the same pointer for every thread
+  encode_fn encode = found_fn.load(std::memory_order_acquire);
+  if (!encode) {
+    void *fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000,
+                                                           cudaEnableDefault, &found);
+    if (e != cudaSuccess || found != cudaDriverEntryPointSuccess || !fn) {
+      cwgk_set_cuda_error((int)(e != cudaSuccess ? e : cudaErrorNotSupported));
+      return -3;
+    }
+    encode = (encode_fn)fn;
+    found_fn.store(encode, std::memory_order_release);
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)(rows > 1 ? ld : ((long long)k + 15) / 16 * 16)};
+  const cuuint32_t box[2] = {kTileK, (cuuint32_t)box_rows}, ones[2] = {1, 1};
+  const CUresult r =
+      encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box,
+             ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    cwgk_set_cuda_error((int)cudaErrorInvalidValue);
+    return -3;
+  }
+  return 0;
+}
+
+template <int TN>
+static int launch(const cwgk_fp8 *op, cudaStream_t s) {
+  using C = Cfg<TN>;
+  CUtensorMap map_a, map_w;
+  int rc = make_map(&map_a, op->a, op->lda, op->m, op->k, TN);
+  if (!rc) rc = make_map(&map_w, op->w, op->ldw, op->n, op->k, 128);
+  if (rc) return rc;
+  MatArgs p;
+  p.a_scale = op->a_scale;
+  p.w_scale = op->w_scale;
+  p.bias = op->bias;
+  p.y = op->y;
+  p.lda_scale = (size_t)op->lda_scale;
+  p.ldw_scale = (size_t)op->ldw_scale;
+  p.ldy = (size_t)op->ldy;
+  p.m = op->m;
+  p.n = op->n;
+  p.kblocks = (op->k + kTileK - 1) / kTileK;
+  p.relu = op->relu;
+  p.bf16 = op->bf16;
+  const long long tiles = (long long)((op->n + 127) / 128) * ((op->m + TN - 1) / TN);
+  int splits = 1;
+  while (splits < 8 && tiles * splits * 2 <= 148 * C::kMinBlocks && p.kblocks >= splits * 4)
+    splits *= 2;
+  p.splits = splits;
+  p.per = (p.kblocks + splits - 1) / splits;
+  if (tiles * splits > 0x7fffffffLL) return -2;
+  cudaError_t e = smem_attr_once<fp8_matmul<TN>>(C::kSmem);
+  if (e == cudaSuccess) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * splits));
+    cfg.blockDim = dim3(C::kThreads);
+    cfg.dynamicSmemBytes = C::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)splits;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, fp8_matmul<TN>, map_a, map_w, p);
+    cwgk_count_launch();
+  }
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    cwgk_set_cuda_error((int)e);
+    return -3;
+  }
+  return 0;
+}
+
+}  // namespace fp8
+}  // namespace cwg
+
+extern "C" {
+
+int cwgk_fp8_quantize(const void *x, long long ldx, void *q, long long ldq, float *scale,
+                      long long lds, int rows, int cols, int block_rows, int bf16, void *stream) {
+  cwg::fp8::QuantArgs a;
+  a.x = x;
+  a.q = static_cast<uint8_t *>(q);
+  a.scale = scale;
+  a.ldx = (size_t)ldx;
+  a.ldq = (size_t)ldq;
+  a.lds = (size_t)lds;
+  a.rows = rows;
+  a.cols = cols;
+  a.kblocks = (cols + 127) / 128;
+  a.groups = (long long)((rows + block_rows - 1) / block_rows) * a.kblocks;
+  return bf16 ? cwg::fp8::quantize<__nv_bfloat16>(a, block_rows, (cudaStream_t)stream)
+              : cwg::fp8::quantize<float>(a, block_rows, (cudaStream_t)stream);
+}
+
+int cwgk_fp8_matmul(const cwgk_fp8 *op, void *stream) {
+  cudaStream_t s = (cudaStream_t)stream;
+  if (op->m <= 16) return cwg::fp8::launch<16>(op, s);
+  if (op->m <= 32) return cwg::fp8::launch<32>(op, s);
+  if (op->m <= 64) return cwg::fp8::launch<64>(op, s);
+  return cwg::fp8::launch<128>(op, s);
+}
+
+int cwgk_fp8_read_clear_status(unsigned *status) {
+  return cwg::read_clear_status(cwg::fp8::g_fp8_status, status);
+}
+
+}  // extern "C"

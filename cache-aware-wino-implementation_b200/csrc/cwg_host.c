@@ -49,6 +49,7 @@ const char *cwg_strerror(int status) {
     case CWG_ENOMEM: return "out of memory";
     case CWG_ENODEV: return "no usable sm_100 device";
     case CWG_ERANGE: return "an operand left the range of the kernel's fp16 arithmetic";
+    case CWG_EINDEX: return "an index in device memory is out of range or given twice";
     default: return "unknown status";
   }
 }
@@ -637,10 +638,14 @@ int cwg_conv3x3_fused_host(const void *x_host, const void *U, const float *bias,
 int cwg_device_status(void *stream) {
   cudaError_t e = cudaStreamSynchronize((cudaStream_t)stream);
   if (e != cudaSuccess) return cuda_fail(e);
-  unsigned st = 0;
-  if (cwgk_read_clear_status(&st)) return CWG_ECUDA;
-  if (st & 1u) return CWG_ETIMEOUT;
-  return st ? CWG_ERANGE : CWG_OK;
+  unsigned st = 0, conv1d = 0, ssm = 0, fp8 = 0;
+  if (cwgk_read_clear_status(&st) || cwgk_conv1d_read_clear_status(&conv1d) ||
+      cwgk_ssm_read_clear_status(&ssm) || cwgk_fp8_read_clear_status(&fp8))
+    return CWG_ECUDA;
+  st |= conv1d | ssm | fp8;
+  if (st & CWGK_STATUS_TIMEOUT) return CWG_ETIMEOUT;
+  if (st & CWGK_STATUS_RANGE) return CWG_ERANGE;
+  return st & CWGK_STATUS_INDEX ? CWG_EINDEX : CWG_OK;
 }
 
 static size_t al256(size_t b) { return (b + 255) / 256 * 256; }

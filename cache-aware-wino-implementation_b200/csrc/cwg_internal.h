@@ -124,9 +124,55 @@ int cwgh_conv_host_serial(const void *x_host, const void *U, const float *bias, 
                           char *xd, char *yd, size_t xbytes, size_t ybytes, int n, int c_in,
                           int c_out, int h, int w, int m, unsigned flags, void *stream);
 
-/* Reads and clears the device status word (after the caller synchronised):
- * bit 0 a bounded wait gave up, bit 1 an fp16 operand left fp16's range. */
+/* Reads and clears the device status word of a translation unit (after the caller
+ * synchronised): bit 0 a bounded wait gave up, bit 1 an fp16 operand left fp16's
+ * range, bit 2 an index in device memory was out of range or given twice. */
+#define CWGK_STATUS_TIMEOUT 1u
+#define CWGK_STATUS_RANGE 2u
+#define CWGK_STATUS_INDEX 4u
 int cwgk_read_clear_status(unsigned *status);
+int cwgk_conv1d_read_clear_status(unsigned *status);
+int cwgk_ssm_read_clear_status(unsigned *status);
+int cwgk_fp8_read_clear_status(unsigned *status);
+
+/* Activations of the sequence layers and the 8-bit product. */
+enum { CWGK_ACT_NONE = 0, CWGK_ACT_RELU = 1, CWGK_ACT_SILU = 2 };
+
+/* Causal convolution (csrc/cwg_conv1d.cu), arguments checked by the host entry. */
+typedef struct cwgk_conv1d {
+  const void *x;
+  long long ldx;
+  const float *w, *bias;
+  void *y;
+  long long ldy;
+  void *state;
+  const int *starts, *slots;
+  const unsigned char *resume;
+  int tokens, n_seq, n_slots, channels, width, act, bf16;
+} cwgk_conv1d;
+int cwgk_conv1d_prompt(const cwgk_conv1d *op, void *stream);
+int cwgk_conv1d_step(const cwgk_conv1d *op, void *stream); /* n_seq rows */
+
+/* Selective scan (csrc/cwg_ssm.cu); op as the public call takes it, checked. */
+struct cwg_ssm;
+size_t cwgk_ssm_workspace_bytes(int tokens, int n_seq, int channels, int states);
+int cwgk_ssm_scan(const struct cwg_ssm *op, void *workspace, size_t workspace_bytes,
+                  void *stream);
+int cwgk_ssm_step(const struct cwg_ssm *op, void *stream);
+
+/* 8-bit product (csrc/cwg_fp8.cu), arguments checked by the host entry. */
+int cwgk_fp8_quantize(const void *x, long long ldx, void *q, long long ldq, float *scale,
+                      long long lds, int rows, int cols, int block_rows, int bf16, void *stream);
+typedef struct cwgk_fp8 {
+  const void *a, *w;
+  long long lda, ldw;
+  const float *a_scale, *w_scale, *bias;
+  long long lda_scale, ldw_scale;
+  void *y;
+  long long ldy;
+  int m, n, k, relu, bf16;
+} cwgk_fp8;
+int cwgk_fp8_matmul(const cwgk_fp8 *op, void *stream);
 
 /* Launch counter shared by all translation units. */
 void cwgk_count_launch(void);

@@ -1,0 +1,125 @@
+// cwg_seq.cuh -- device helpers shared by the sequence layers: rows of mixed
+// types as fp32 vectors, packed sequences and their cache lines.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "cwg_common.cuh"
+
+namespace cwg {
+namespace seq {
+
+// V elements of T, moved as one 16-byte vector (or one element, V = 1).
+template <typename T, int V>
+struct Raw {
+  static_assert(V == 1 || V * sizeof(T) == 16, "one element or one 16-byte vector");
+  using type = uint4;
+};
+template <>
+struct Raw<float, 1> {
+  using type = float;
+};
+template <>
+struct Raw<__nv_bfloat16, 1> {
+  using type = __nv_bfloat16;
+};
+
+template <typename T, int V>
+__device__ __forceinline__ typename Raw<T, V>::type load_raw(const T *p) {
+  return *reinterpret_cast<const typename Raw<T, V>::type *>(p);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_raw(T *p, typename Raw<T, V>::type v) {
+  *reinterpret_cast<typename Raw<T, V>::type *>(p) = v;
+}
+template <typename T, int V>
+__device__ __forceinline__ typename Raw<T, V>::type zero_raw() {
+  if constexpr (V == 1)
+    return from_f32<T>(0.f);
+  else
+    return make_uint4(0, 0, 0, 0);
+}
+
+__device__ __forceinline__ void unpack(float v, float (&f)[1]) { f[0] = v; }
+__device__ __forceinline__ void unpack(__nv_bfloat16 v, float (&f)[1]) { f[0] = to_f32(v); }
+__device__ __forceinline__ void unpack(uint4 v, float (&f)[4]) {
+  f[0] = __uint_as_float(v.x);
+  f[1] = __uint_as_float(v.y);
+  f[2] = __uint_as_float(v.z);
+  f[3] = __uint_as_float(v.w);
+}
+__device__ __forceinline__ void unpack(uint4 v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+  }
+}
+// One rounding, to nearest even (none for fp32).
+template <typename T>
+__device__ __forceinline__ T pack1(float v) {
+  return from_f32<T>(v);
+}
+template <typename T, int V>
+__device__ __forceinline__ typename Raw<T, V>::type pack(const float (&f)[V]) {
+  if constexpr (V == 1) {
+    return from_f32<T>(f[0]);
+  } else if constexpr (V == 4) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                      __float_as_uint(f[3]));
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+__device__ __forceinline__ float silu(float v) { return v / (1.f + expf(-v)); }
+
+__device__ __forceinline__ float softplus(float v) {
+  // above 20 exp(-v) is below half a step of v
+  return v > 20.f ? v : log1pf(expf(v));
+}
+
+// First b in [0, n) with s[b] >= v (n if none); ends for any contents of s.
+__device__ __forceinline__ int lower_bound(const int *s, int n, int v) {
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (s[mid] < v)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+// Whether slots[b] occurs among slots[0 .. b-1]: the calling warp's lanes search
+// together, and all of them get the answer.
+__device__ __forceinline__ bool taken_before(const int *slots, int b, int slot) {
+  bool hit = false;
+  for (int i = (int)(threadIdx.x & 31); i < b; i += 32) hit |= slots[i] == slot;
+  return __any_sync(0xffffffffu, hit) != 0;
+}
+
+// Cache line of sequence b, or -1: no line (a negative slot), or an index that
+// cannot be served (outside the lines, or an earlier sequence's), which `bad`
+// reports.  Called by whole warps with a warp-uniform b.
+__device__ __forceinline__ int line_of(const int *slots, int b, int n_slots, bool &bad) {
+  const int slot = slots ? slots[b] : b;
+  if (slot < 0) return -1;
+  if (slot >= n_slots || (slots && taken_before(slots, b, slot))) {
+    bad = true;
+    return -1;
+  }
+  return slot;
+}
+
+}  // namespace seq
+}  // namespace cwg

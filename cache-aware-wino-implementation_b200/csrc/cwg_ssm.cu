@@ -1,0 +1,379 @@
+// cwg_ssm.cu -- selective state space scan (cwg_ssm_scan, cwg_ssm_step).
+//
+// For every channel c with states i = 0 .. N-1, step d = softplus(dt + dt_bias):
+//   h_i <- exp(d A_i) h_i + d u B_i,   y = (sum_i C_i h_i + D u) z / (1 + exp(-z))
+//
+// A channel's N states are spread over L lanes, four per lane (N padded to 4 L
+// with A = B = C = 0, whose states stay zero), so a warp holds 32 / L channels.
+// exp(d A) is computed as 2^(d (A log2 e)) with ex2.approx (2 ulp); state, decay
+// and sums are fp32.
+#include <cstdint>
+
+#include "../../include/cwg.h"
+#include "cwg_seq.cuh"
+
+namespace cwg {
+namespace ssm {
+
+using namespace seq;
+
+__device__ unsigned int g_ssm_status;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kS = 4;    // states per lane
+constexpr int kTT = 32;  // tokens per tile of the prompt kernel
+
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+struct Args {
+  cwg_ssm p;
+  int per;      // channels per group
+  int cblocks;  // CTAs along one group's channels
+  int run;      // rows per CTA (steps)
+  bool vec_state;
+};
+
+// A lane's four states of one cache line, or zeros.
+__device__ __forceinline__ void load_states(const float *line, int i0, int n, bool vec,
+                                            float (&h)[kS]) {
+  if (vec) {
+    const float4 f = *reinterpret_cast<const float4 *>(line + i0);
+    h[0] = f.x, h[1] = f.y, h[2] = f.z, h[3] = f.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kS; ++i) h[i] = i0 + i < n ? line[i0 + i] : 0.f;
+  }
+}
+__device__ __forceinline__ void store_states(float *line, int i0, int n, bool vec,
+                                             const float (&h)[kS]) {
+  if (vec) {
+    *reinterpret_cast<float4 *>(line + i0) = make_float4(h[0], h[1], h[2], h[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kS; ++i)
+      if (i0 + i < n) line[i0 + i] = h[i];
+  }
+}
+
+// ---- prompts --------------------------------------------------------------------
+// One CTA per (sequence, block of CH channels of one group): it walks the sequence
+// in tiles of kTT tokens.  Per tile the CTA turns dt and u into (d, d u) pairs and
+// B, C into fp32 in shared memory, the lanes run the recurrence over the tile, and
+// the CTA finishes y with full-width row accesses.  The next tile's operands are
+// loaded into registers while the recurrence runs.
+template <int L>
+struct Geo {
+  static constexpr int kCH = L <= 4 ? 64 : 256 / L;
+  static constexpr int kThreads = kCH * L;
+  static constexpr int kNP = kS * L;
+  static constexpr int kTasks = kTT * kCH / 8;  // 8-channel pieces of a tile
+  static constexpr int kPer = (kTasks + kThreads - 1) / kThreads;
+  static constexpr int kPerB = kTT * kNP / kThreads;
+};
+
+// 8 consecutive channels of one row as fp32; channels past `n` read as zero.
+template <typename T, bool VEC>
+struct Piece {
+  static constexpr int kRaw = VEC ? (int)sizeof(T) * 8 / 16 : 8;
+  using R = typename Raw<T, VEC ? 16 / (int)sizeof(T) : 1>::type;
+  R raw[kRaw];
+  __device__ __forceinline__ void load(const T *p, int n) {
+#pragma unroll
+    for (int i = 0; i < kRaw; ++i) {
+      constexpr int E = 8 / kRaw;
+      raw[i] = i * E < n ? load_raw<T, E>(p + i * E) : zero_raw<T, E>();
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+    constexpr int E = 8 / kRaw;
+#pragma unroll
+    for (int i = 0; i < kRaw; ++i) {
+      float g[E];
+      unpack(raw[i], g);
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[i * E + e] = g[e];
+    }
+  }
+  __device__ static __forceinline__ void store(T *p, const float (&f)[8], int n) {
+    constexpr int E = 8 / kRaw;
+#pragma unroll
+    for (int i = 0; i < kRaw; ++i) {
+      float g[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) g[e] = f[i * E + e];
+      if (i * E < n) store_raw<T, E>(p + i * E, pack<T, E>(g));
+    }
+  }
+};
+
+template <typename T, int L, bool VEC>
+__global__ void __launch_bounds__(Geo<L>::kThreads) ssm_prompt(const Args a) {
+  using G = Geo<L>;
+  constexpr int CH = G::kCH, NT = G::kThreads, NP = G::kNP, PER = G::kPer, PERB = G::kPerB;
+  __shared__ __align__(16) float2 s_dx[kTT][CH];
+  __shared__ __align__(16) float s_b[kTT][NP], s_c[kTT][NP];
+  __shared__ __align__(16) float s_y[kTT][CH];
+  const cwg_ssm &p = a.p;
+  const int tid = threadIdx.x;
+  const int cblk = blockIdx.x % a.cblocks;
+  const int group = (blockIdx.x / a.cblocks) % p.groups;
+  const int b = blockIdx.x / (a.cblocks * p.groups);
+  const int in0 = cblk * CH;                // first channel within the group
+  const int c0 = group * a.per + in0;       // first channel
+  const int nch = min(CH, a.per - in0);
+  const int begin = p.starts[b], end = p.starts[b + 1];
+  const bool report = tid == 0 && cblk == 0 && group == 0;
+  if (begin < 0 || end < begin || end > p.tokens) {
+    if (report) atomicOr(&g_ssm_status, CWGK_STATUS_INDEX);
+    return;
+  }
+  bool bad = false;
+  const int slot = p.state ? line_of(p.slots, b, p.n_slots, bad) : -1;
+  if (bad && report) atomicOr(&g_ssm_status, CWGK_STATUS_INDEX);
+  const bool carry = slot >= 0 && p.resume && p.resume[b];
+
+  // the recurrence's view: lane `l` of channel `ch`, states i0 .. i0 + 3
+  const int ch = tid / L, l = tid % L, i0 = l * kS;
+  const bool mine = ch < nch;
+  float A2[kS], h[kS];
+  float *line = p.state + ((size_t)(slot < 0 ? 0 : slot) * p.channels + c0 + ch) * p.states;
+#pragma unroll
+  for (int i = 0; i < kS; ++i) {
+    A2[i] = mine && i0 + i < p.states ? p.A[(size_t)(c0 + ch) * p.states + i0 + i] * kLog2e : 0.f;
+    h[i] = 0.f;
+  }
+  if (carry && mine) load_states(line, i0, p.states, a.vec_state, h);
+
+  // the tile's view: 8-channel pieces
+  Piece<T, VEC> ru[PER], rd[PER], rz[PER], cu[PER], cz[PER];
+  float rb[PERB], rc[PERB];
+  auto fetch = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int task = tid + i * NT;
+      const int t = t0 + task / (CH / 8), c = (task % (CH / 8)) * 8;
+      const int n = task < G::kTasks && t < end ? nch - c : 0;
+      const size_t at = (size_t)t;
+      ru[i].load(static_cast<const T *>(p.u) + at * p.ldu + c0 + c, n);
+      rd[i].load(static_cast<const T *>(p.dt) + at * p.lddt + c0 + c, n);
+      rz[i].load(static_cast<const T *>(p.z) + at * p.ldz + c0 + c, p.z ? n : 0);
+    }
+#pragma unroll
+    for (int i = 0; i < PERB; ++i) {
+      const int e = tid + i * NT;
+      const int t = t0 + e / NP, s = e % NP;
+      const bool ok = t < end && s < p.states;
+      const size_t col = (size_t)group * p.states + s;
+      rb[i] = ok ? to_f32(static_cast<const T *>(p.B)[(size_t)t * p.ldb + col]) : 0.f;
+      rc[i] = ok ? to_f32(static_cast<const T *>(p.C)[(size_t)t * p.ldc + col]) : 0.f;
+    }
+  };
+
+  fetch(begin);
+  for (int t0 = begin; t0 < end; t0 += kTT) {
+    // (d, d u) of every (token, channel); rows past the end have d = 0, which
+    // leaves the states as they are
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int task = tid + i * NT;
+      const int t = task / (CH / 8), c = (task % (CH / 8)) * 8;
+      if (task < G::kTasks) {
+        float u[8], d[8];
+        ru[i].get(u);
+        rd[i].get(d);
+        const bool row = t0 + t < end;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const bool ok = row && c + e < nch;
+          float v = d[e] + (ok && p.dt_bias ? p.dt_bias[c0 + c + e] : 0.f);
+          if (p.flags & CWG_SOFTPLUS) v = softplus(v);
+          s_dx[t][c + e] = ok ? make_float2(v, v * u[e]) : make_float2(0.f, 0.f);
+        }
+      }
+      cu[i] = ru[i];
+      cz[i] = rz[i];
+    }
+#pragma unroll
+    for (int i = 0; i < PERB; ++i) {
+      const int e = tid + i * NT;
+      s_b[e / NP][e % NP] = rb[i];
+      s_c[e / NP][e % NP] = rc[i];
+    }
+    __syncthreads();
+    if (t0 + kTT < end) fetch(t0 + kTT);
+#pragma unroll 4
+    for (int t = 0; t < kTT; ++t) {
+      const float2 dx = s_dx[t][ch];
+      const float4 bv = *reinterpret_cast<const float4 *>(&s_b[t][i0]);
+      const float4 cv = *reinterpret_cast<const float4 *>(&s_c[t][i0]);
+      h[0] = fmaf(ex2(dx.x * A2[0]), h[0], dx.y * bv.x);
+      h[1] = fmaf(ex2(dx.x * A2[1]), h[1], dx.y * bv.y);
+      h[2] = fmaf(ex2(dx.x * A2[2]), h[2], dx.y * bv.z);
+      h[3] = fmaf(ex2(dx.x * A2[3]), h[3], dx.y * bv.w);
+      float y = fmaf(h[0], cv.x, h[1] * cv.y) + fmaf(h[2], cv.z, h[3] * cv.w);
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+      if (l == 0) s_y[t][ch] = y;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int task = tid + i * NT;
+      const int t = task / (CH / 8), c = (task % (CH / 8)) * 8;
+      if (task < G::kTasks && t0 + t < end && c < nch) {
+        float u[8], z[8], y[8];
+        cu[i].get(u);
+        cz[i].get(z);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          y[e] = fmaf(p.D && c + e < nch ? p.D[c0 + c + e] : 0.f, u[e], s_y[t][c + e]);
+          if (p.z) y[e] *= silu(z[e]);
+        }
+        Piece<T, VEC>::store(static_cast<T *>(p.y) + (size_t)(t0 + t) * p.ldy + c0 + c, y,
+                             nch - c);
+      }
+    }
+  }
+  if (slot >= 0 && mine) store_states(line, i0, p.states, a.vec_state, h);
+}
+
+// ---- one token of each sequence ----------------------------------------------------
+// Bound by the states, 8 N bytes per channel in and out; the lanes of a channel
+// compute its step together, a CTA's rows share A.
+template <typename T, int L>
+__global__ void __launch_bounds__(Geo<L>::kThreads) ssm_token(const Args a) {
+  constexpr int CH = Geo<L>::kCH;
+  const cwg_ssm &p = a.p;
+  const int tid = threadIdx.x;
+  const int cblk = blockIdx.x % a.cblocks;
+  const int group = (blockIdx.x / a.cblocks) % p.groups;
+  const int run = blockIdx.x / (a.cblocks * p.groups);
+  const int ch = tid / L, l = tid % L, i0 = l * kS;
+  const int in = cblk * CH + ch, c = group * a.per + in;
+  const bool mine = in < a.per;
+  float A2[kS];
+#pragma unroll
+  for (int i = 0; i < kS; ++i)
+    A2[i] = mine && i0 + i < p.states ? p.A[(size_t)c * p.states + i0 + i] * kLog2e : 0.f;
+  const float bias = mine && p.dt_bias ? p.dt_bias[c] : 0.f;
+  const float skip = mine && p.D ? p.D[c] : 0.f;
+  bool bad = false;
+  const int r1 = min((run + 1) * a.run, p.tokens);
+  for (int r = run * a.run; r < r1; ++r) {
+    const int slot = line_of(p.slots, r, p.n_slots, bad);
+    float *line = p.state + ((size_t)(slot < 0 ? 0 : slot) * p.channels + c) * p.states;
+    const size_t row = (size_t)r;
+    float h[kS] = {0.f, 0.f, 0.f, 0.f}, bv[kS], cv[kS];
+    float u = 0.f, d = 0.f, z = 0.f;
+    if (mine) {
+      if (slot >= 0) load_states(line, i0, p.states, a.vec_state, h);
+      u = to_f32(static_cast<const T *>(p.u)[row * p.ldu + c]);
+      d = to_f32(static_cast<const T *>(p.dt)[row * p.lddt + c]) + bias;
+      if (p.z) z = to_f32(static_cast<const T *>(p.z)[row * p.ldz + c]);
+    }
+#pragma unroll
+    for (int i = 0; i < kS; ++i) {
+      const bool ok = i0 + i < p.states;
+      const size_t col = (size_t)group * p.states + i0 + i;
+      bv[i] = ok ? to_f32(static_cast<const T *>(p.B)[row * p.ldb + col]) : 0.f;
+      cv[i] = ok ? to_f32(static_cast<const T *>(p.C)[row * p.ldc + col]) : 0.f;
+    }
+    if (p.flags & CWG_SOFTPLUS) d = softplus(d);
+    const float du = d * u;
+    float y = 0.f;
+#pragma unroll
+    for (int i = 0; i < kS; ++i) {
+      h[i] = fmaf(ex2(d * A2[i]), h[i], du * bv[i]);
+      y = fmaf(h[i], cv[i], y);
+    }
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+    if (mine) {
+      if (slot >= 0) store_states(line, i0, p.states, a.vec_state, h);
+      if (l == 0) {
+        y = fmaf(skip, u, y);
+        if (p.z) y *= silu(z);
+        static_cast<T *>(p.y)[row * p.ldy + c] = pack1<T>(y);
+      }
+    }
+  }
+  if (bad && tid == 0 && cblk == 0 && group == 0) atomicOr(&g_ssm_status, CWGK_STATUS_INDEX);
+}
+
+static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+static int done() {
+  cwgk_count_launch();
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) {
+    cwgk_set_cuda_error((int)e);
+    return -3;
+  }
+  return 0;
+}
+
+template <typename T, int L>
+static int launch(const cwg_ssm *op, bool step, cudaStream_t s) {
+  using G = Geo<L>;
+  Args a;
+  a.p = *op;
+  if (op->tokens <= 1) a.p.ldu = a.p.lddt = a.p.ldz = a.p.ldy = 0, a.p.ldb = a.p.ldc = 0;
+  a.per = op->channels / op->groups;
+  a.cblocks = (a.per + G::kCH - 1) / G::kCH;
+  a.vec_state = op->states == G::kNP && aligned16(op->state);
+  a.run = 1;
+  const long long rows = step ? (op->tokens + a.run - 1) / a.run : op->n_seq;
+  const long long blocks = rows * a.cblocks * op->groups;
+  if (blocks > 0x7fffffffLL) return -2;
+  if (step) {
+    ssm_token<T, L><<<(unsigned)blocks, G::kThreads, 0, s>>>(a);
+    return done();
+  }
+  constexpr int E = 16 / (int)sizeof(T);
+  const bool vec = a.per % 8 == 0 && aligned16(op->u) && aligned16(op->dt) && aligned16(op->z) &&
+                   aligned16(op->y) && a.p.ldu % E == 0 && a.p.lddt % E == 0 &&
+                   a.p.ldy % E == 0 && (!op->z || a.p.ldz % E == 0);
+  if (vec)
+    ssm_prompt<T, L, true><<<(unsigned)blocks, G::kThreads, 0, s>>>(a);
+  else
+    ssm_prompt<T, L, false><<<(unsigned)blocks, G::kThreads, 0, s>>>(a);
+  return done();
+}
+
+template <typename T>
+static int by_states(const cwg_ssm *op, bool step, cudaStream_t s) {
+  if (op->states <= 4) return launch<T, 1>(op, step, s);
+  if (op->states <= 8) return launch<T, 2>(op, step, s);
+  if (op->states <= 16) return launch<T, 4>(op, step, s);
+  if (op->states <= 32) return launch<T, 8>(op, step, s);
+  return launch<T, 16>(op, step, s);
+}
+
+static int any(const cwg_ssm *op, bool step, cudaStream_t s) {
+  return op->flags & CWG_BF16 ? by_states<__nv_bfloat16>(op, step, s) : by_states<float>(op, step, s);
+}
+
+}  // namespace ssm
+}  // namespace cwg
+
+extern "C" {
+
+size_t cwgk_ssm_workspace_bytes(int tokens, int n_seq, int channels, int states) { return 256; }
+
+int cwgk_ssm_scan(const cwg_ssm *op, void *workspace, size_t workspace_bytes, void *stream) {
+  return cwg::ssm::any(op, false, (cudaStream_t)stream);
+}
+
+int cwgk_ssm_step(const cwg_ssm *op, void *stream) {
+  return cwg::ssm::any(op, true, (cudaStream_t)stream);
+}
+
+int cwgk_ssm_read_clear_status(unsigned *status) {
+  return cwg::read_clear_status(cwg::ssm::g_ssm_status, status);
+}
+
+}  // extern "C"

@@ -35,6 +35,7 @@
 
 #include "../../include/cwg.h"
 #include "cwg_common.cuh"
+#include "cwg_tcgen05.cuh"
 
 namespace cwg {
 namespace tc {
@@ -46,7 +47,6 @@ constexpr int kFPerU = 2;      // frequencies per U stage
 constexpr int kNV = 2;         // V stages
 constexpr int kTmemCols = 512;
 constexpr int kCoreBytes = 4096;               // one 128x16 bf16 operand block
-constexpr unsigned long long kTimeoutNs = 2000000000ull;  // 2 s per wait
 
 // Two accumulation schemes share the kernel:
 //   HALF  ("half-folded", the default): the row pass of the output transform,
@@ -93,77 +93,8 @@ struct Layout {
 __device__ unsigned int g_tc_status;
 
 // ---- PTX wrappers -------------------------------------------------------------
-__device__ __forceinline__ uint32_t smem_u32(const void *p) {
-  return (uint32_t)__cvta_generic_to_shared(p);
-}
-__device__ __forceinline__ unsigned long long globaltimer() {
-  unsigned long long t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-  asm volatile(
-      "{\n\t.reg .b64 st;\n\t"
-      "mbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" ::"r"(bar)
-      : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile(
-      "{\n\t.reg .b64 st;\n\t"
-      "mbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar),
-      "r"(bytes)
-      : "memory");
-}
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.b32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// Bounded wait: true when the phase completed; false on timeout or when another
-// role already aborted (the abort flag lives in shared memory).
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *abort) {
-  if (mbar_try(bar, parity)) return true;
-  const unsigned long long t0 = globaltimer();
-  while (true) {
-    if (mbar_try(bar, parity)) return true;
-    if (*abort) return false;
-    if (globaltimer() - t0 > kTimeoutNs) {
-      *abort = 1;
-      atomicOr(&g_tc_status, 1u);
-      return false;
-    }
-  }
-}
-__device__ __forceinline__ void bulk_g2s(uint32_t dst, const void *src, uint32_t bytes,
-                                         uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
-          "r"(dst),
-      "l"(src), "r"(bytes), "r"(bar)
-      : "memory");
-}
-__device__ __forceinline__ void fence_proxy_async() {
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::
-                   "r"(bar)
-               : "memory");
+  return mbar_wait(bar, parity, abort, &g_tc_status);
 }
 // D[tmem] (+)= A[smem desc] * B[smem desc]^T, bf16 x bf16 -> fp32.
 __device__ __forceinline__ void mma_bf16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
@@ -175,52 +106,8 @@ __device__ __forceinline__ void mma_bf16(uint32_t d_tmem, uint64_t a_desc, uint6
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld4(uint32_t taddr, float (&v)[4]) {
-  uint32_t r0, r1, r2, r3;
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-               : "r"(taddr)
-               : "memory");
-  v[0] = __uint_as_float(r0);
-  v[1] = __uint_as_float(r1);
-  v[2] = __uint_as_float(r2);
-  v[3] = __uint_as_float(r3);
-}
-// One lane of a converged warp (elect.sync).  Issuing tcgen05 instructions this
-// way, from warp-uniform control flow, keeps their operands in uniform
-// registers: a per-lane branch around them costs ~3x in MMA issue rate.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t pred = 0;
-  asm volatile(
-      "{\n\t.reg .pred px;\n\telect.sync _|px, %1;\n\t@px mov.s32 %0, 1;\n\t}"
-      : "+r"(pred)
-      : "r"(0xFFFFFFFFu));
-  return pred != 0;
-}
-
 // Named barrier 1: TMEM address handoff from warp 0 to the epilogue warps.
 constexpr int kBarTmem = 1;
-__device__ __forceinline__ void named_bar_arrive(int id, int count) {
-  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(count) : "memory");
-}
-__device__ __forceinline__ void named_bar_sync(int id, int count) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory");
-}
-__device__ __forceinline__ void tmem_wait_ld() {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
-// Shared-memory matrix descriptor: K-major, no swizzle.  Core matrices are
-// 8 rows x 16 bytes; `lbo` = byte distance between the two K-adjacent core
-// matrices of one MMA step, `sbo` = byte distance between 8-row groups.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-  uint64_t d = 0;
-  d |= (uint64_t)((addr >> 4) & 0x3FFF);
-  d |= (uint64_t)((lbo >> 4) & 0x3FFF) << 16;
-  d |= (uint64_t)((sbo >> 4) & 0x3FFF) << 32;
-  d |= (uint64_t)1 << 46;  // descriptor version for sm_100
-  return d;                // base offset 0, legacy LBO mode, SWIZZLE_NONE
-}
 
 // Instruction descriptor: kind::f16, A = B = bf16 (or both fp16), D = fp32, both
 // K-major.
@@ -685,45 +572,6 @@ static cudaError_t launch(const void *x, const void *U, const float *bias, void 
 // otherwise) relays each of its completed V stages and landed weight stages.
 // Releases (operand stages, accumulators) are multicast commits that arrive on
 // both CTAs' barriers.
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-// shared::cluster address of the same shared-memory offset in CTA `rank`
-__device__ __forceinline__ uint32_t mapa_shared(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-// Arrival on a barrier of another CTA of the cluster.  Default (CTA-scope)
-// release: a cluster-scope release costs ~1.4K cycles per arrival, and what it
-// would order is already complete -- bulk copies by their own mbarrier, thread
-// writes to V by fence.proxy.async and the local barrier the relay observed.
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-// Programmatic dependent launch: wait for the previous grid of the stream to
-// complete (its memory operations visible); allow the next grid to launch.
-__device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void griddep_launch_dependents() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile(
-      "barrier.cluster.arrive.release.aligned;\n\t"
-      "barrier.cluster.wait.acquire.aligned;" ::
-          : "memory");
-}
-// completion of this thread's earlier MMAs -> one arrival on the barrier at
-// offset `bar` of every CTA in `mask`
-__device__ __forceinline__ void tc_commit_pair(uint32_t bar, uint16_t mask) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
-      "[%0], %1;" ::"r"(bar),
-      "h"(mask)
-      : "memory");
-}
 __device__ __forceinline__ void mma_pair_bf16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
                                               uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -733,18 +581,6 @@ __device__ __forceinline__ void mma_pair_bf16(uint32_t d_tmem, uint64_t a_desc, 
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&v)[8]) {
-  uint32_t r[8];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7])
-      : "r"(taddr)
-      : "memory");
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(r[e]);
-}
-
 // y[0..3] += v, one 16-byte vector reduction in L2 (16-byte aligned address).
 __device__ __forceinline__ void red_add_v4(float *y, float4 v) {
   asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(y), "f"(v.x), "f"(v.y),
@@ -2431,18 +2267,7 @@ int cwg_selftest_wait_timeout(void *stream) {
 }
 
 int cwgk_read_clear_status(unsigned *status) {
-  unsigned v = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(&v, tc::g_tc_status, sizeof(v));
-  if (e == cudaSuccess && v) {
-    const unsigned zero = 0;
-    e = cudaMemcpyToSymbol(tc::g_tc_status, &zero, sizeof(zero));
-  }
-  if (e != cudaSuccess) {
-    cwgk_set_cuda_error((int)e);
-    return -3;
-  }
-  *status = v;
-  return 0;
+  return read_clear_status(tc::g_tc_status, status);
 }
 
 }  // extern "C"

@@ -48,6 +48,9 @@ extern "C" {
 #define CWG_ERANGE (-7)       /* an operand left the range of the kernel's fp16 arithmetic
                                  (bf16 F(4,3) tensor-core layers: |x| above ~650 or |g|
                                  above ~900); results invalid, rerun with CWG_TC_X3 */
+#define CWG_EINDEX (-8)       /* an index in device memory (a sequence's offset or its cache
+                                 line) was out of range or given twice; see the sequence
+                                 layers below for what was computed instead */
 
 /* ---- flags for the layer-level calls -------------------------------------- */
 #define CWG_RELU 0x1u        /* fused ReLU after bias */
@@ -72,6 +75,10 @@ extern "C" {
                                 start (barriers, TMEM) while the previous kernel in the stream
                                 finishes, and wait for that kernel's completion before they
                                 touch global memory */
+
+/* ---- flags of the sequence layers and of the 8-bit matrix product ----------- */
+#define CWG_SILU 0x1000u     /* y = v / (1 + exp(-v)) after the bias (causal convolution) */
+#define CWG_SOFTPLUS 0x2000u /* step = log(1 + exp(dt + dt_bias)) instead of dt + dt_bias */
 
 /* Kernel paths reported by cwg_select. */
 #define CWG_PATH_FFMA 1 /* warp register-blocked FFMA fused kernel */
@@ -191,6 +198,109 @@ int cwg_conv3x3_nonfused(const float *x, const float *U, const float *bias, floa
                          void *workspace, size_t workspace_bytes, int n, int c_in, int c_out,
                          int h, int w, int m, unsigned flags, void *stream);
 
+/* ---- sequence layers (DEVICE pointers) -------------------------------------- */
+
+/* The layers of a state space block for serving: a short causal convolution over
+ * time and a selective scan, each for whole prompts and for one token of every
+ * sequence.  No counterpart in the reference.
+ *
+ * Rows are tokens, columns are channels: element (row, column) of an operand is
+ * at row * ld + column, ld in elements and at least the row's width, so that an
+ * operand may be a column range of a wider matrix (a projection's output).  Rows
+ * that are 16-byte aligned and hold whole 16-byte vectors take the vector path;
+ * others are read element by element.  fp32, or bf16 with CWG_BF16 (x, y, u, dt,
+ * B, C, z and the convolution's cache; all weights and the scan's state are fp32).
+ *
+ * Prompts are packed: sequence b is rows starts[b] .. starts[b+1]-1 (device,
+ * int32, n_seq + 1 offsets, ascending, at most `tokens`).  An empty sequence is
+ * allowed; rows that belong to no sequence are neither read nor written.
+ *
+ * State between calls is kept in cache lines, one per sequence: sequence b uses
+ * line slots[b] of `state` (device, int32; NULL: line b).  With resume[b] != 0 a
+ * prompt continues from its line, otherwise (and with resume NULL) it starts from
+ * zeros and the line's old contents are not read; either way the line holds the
+ * state behind the sequence's last token afterwards.  A sequence with a negative
+ * slot has no line: it starts from zeros and nothing is stored.  state may be NULL
+ * for prompts (no sequence has a line).
+ *
+ * Indices are checked on the device, so that none of them can reach outside an
+ * operand: a slot >= n_slots, or one that an earlier sequence of the call has
+ * too, counts as negative, a sequence whose offsets are not
+ * 0 <= starts[b] <= starts[b+1] <= tokens is left out, and
+ * cwg_device_status reports CWG_EINDEX.
+ *
+ * y must not overlap the inputs (disjoint columns of one matrix do not overlap):
+ * CWG_EINVAL.  All calls are asynchronous on `stream`, allocate nothing and can be
+ * captured into a graph. */
+
+/* y[t][c] = act(bias[c] + sum_j w[c][j] x[t - width + 1 + j][c]); rows before the
+ * sequence come from its line.  w fp32 [channels][width], width 2 .. 4, bias fp32
+ * [channels] or NULL, act: CWG_SILU, CWG_RELU or none.  state
+ * [n_slots][width - 1][channels] in x's type: the last inputs, oldest first. */
+int cwg_conv1d_causal(const void *x, long long ldx, const float *w, const float *bias, void *y,
+                      long long ldy, void *state, const int *starts, const int *slots,
+                      const unsigned char *resume, int tokens, int n_seq, int n_slots,
+                      int channels, int width, unsigned flags, void *stream);
+
+/* The same for one token of each of n sequences: row i of x and y, line slots[i]. */
+int cwg_conv1d_causal_step(const void *x, long long ldx, const float *w, const float *bias,
+                           void *y, long long ldy, void *state, const int *slots, int n,
+                           int n_slots, int channels, int width, unsigned flags, void *stream);
+
+/* Selective scan.  With step = dt + dt_bias (through CWG_SOFTPLUS), for every
+ * channel c, its group g = c / (channels / groups), and state i:
+ *   h[c][i] = exp(step[t][c] A[c][i]) h[c][i] + step[t][c] B[t][g][i] u[t][c]
+ *   y[t][c] = (sum_i C[t][g][i] h[c][i] + D[c] u[t][c]) * z[t][c] / (1 + exp(-z[t][c]))
+ * A fp32 [channels][states], B and C rows of groups * states columns, D and
+ * dt_bias fp32 [channels] or NULL, z or NULL (no gate).  state fp32
+ * [n_slots][channels][states].  1 <= states <= 64; groups divides channels. */
+typedef struct cwg_ssm {
+  const void *u, *dt, *B, *C, *z;
+  void *y;
+  long long ldu, lddt, ldb, ldc, ldz, ldy;
+  const float *A, *D, *dt_bias;
+  float *state;
+  const int *starts, *slots;     /* starts, resume: prompts only */
+  const unsigned char *resume;
+  int tokens;                    /* rows: of all prompts, or one per sequence */
+  int n_seq;                     /* prompts only */
+  int n_slots, channels, groups, states;
+  unsigned flags;
+} cwg_ssm;
+
+/* Prompts.  Few, long sequences are cut into chunks of time that run side by side,
+ * in a caller-owned workspace (256-byte aligned, cwg_ssm_workspace_bytes bytes);
+ * workspace NULL: never cut.  Calls whose work overlaps on the GPU need workspaces
+ * of their own. */
+size_t cwg_ssm_workspace_bytes(int tokens, int n_seq, int channels, int states);
+int cwg_ssm_scan(const cwg_ssm *op, void *workspace, size_t workspace_bytes, void *stream);
+
+/* One token of each of op->tokens sequences: row i, line slots[i], updated in place. */
+int cwg_ssm_step(const cwg_ssm *op, void *stream);
+
+/* ---- 8-bit matrix product with scales per block of 128 (DEVICE pointers) ------- */
+
+/* e4m3 values q and fp32 scales of x (fp32, or bf16 with CWG_BF16), [rows][cols]:
+ * each group of block_rows rows x 128 columns (cut at the edges) has
+ *   scale = max(max |x| / 448, 2^-126),  q = e4m3(x / scale), to nearest even.
+ * block_rows 1 (activations) or 128 (weights).  scale [ceil(rows / block_rows)]
+ * [ceil(cols / 128)], rows lds apart.  A group that holds an infinity or NaN has an
+ * infinite or NaN scale, and its values come back as NaN. */
+int cwg_fp8_quantize(const void *x, long long ldx, void *q, long long ldq, float *scale,
+                     long long lds, int rows, int cols, int block_rows, unsigned flags,
+                     void *stream);
+
+/* y[i][j] = act(bias[j] + sum_kb a_scale[i][kb] w_scale[j / 128][kb]
+ *                         sum_{k in block kb of 128} a[i][k] w[j][k])
+ * a e4m3 [m][k], w e4m3 [n][k] (a weight's rows are outputs), as cwg_fp8_quantize
+ * writes them with block_rows 1 and 128; a and w 16-byte aligned with lda and ldw
+ * multiples of 16 (k itself may be any size >= 1).  y fp32 [m][n], or bf16 with
+ * CWG_BF16; bias fp32 [n] or NULL; act: CWG_RELU or none. */
+int cwg_fp8_matmul(const void *a, long long lda, const float *a_scale, long long lda_scale,
+                   const void *w, long long ldw, const float *w_scale, long long ldw_scale,
+                   const float *bias, void *y, long long ldy, int m, int n, int k,
+                   unsigned flags, void *stream);
+
 /* ---- selector, diagnostics ----------------------------------------------- */
 
 /* Chooses m (when m == 0), the kernel path and its blocking for a layer on the
@@ -204,11 +314,12 @@ const char *cwg_strerror(int status);
 int cwg_last_cuda_error(void);
 
 /* Synchronises `stream`, then reads and clears the device-side status word
- * that bounded waits inside the kernels set when they give up, and that the
- * fp16 tensor-core path sets when an operand leaves fp16's range.  Returns
- * CWG_ETIMEOUT if any kernel since the last call timed out, else CWG_ERANGE if
- * an operand overflowed, else CWG_OK (or CWG_ECUDA if the synchronisation
- * itself failed). */
+ * that bounded waits inside the kernels set when they give up, that the fp16
+ * tensor-core path sets when an operand leaves fp16's range, and that the
+ * sequence layers set for a bad index.  Returns CWG_ETIMEOUT if any kernel since
+ * the last call timed out, else CWG_ERANGE if an operand overflowed, else
+ * CWG_EINDEX if an index was bad, else CWG_OK (or CWG_ECUDA if the
+ * synchronisation itself failed). */
 int cwg_device_status(void *stream);
 
 /* Self-test of the failure path: launches one CTA whose bounded device wait can

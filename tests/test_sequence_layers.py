@@ -1,0 +1,393 @@
+"""Causal convolution, selective scan, 8-bit quantiser and product on the GPU, against plain
+64-bit implementations (seq_ref.py) within bounds that count their roundings."""
+import pytest
+import torch
+
+import cwg
+import seq_ref as R
+
+pytestmark = pytest.mark.gpu
+
+DT = {"fp32": torch.float32, "bf16": torch.bfloat16}
+GUARD = 7.25  # exact in both types
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def randn(g, *shape, dtype=torch.float32, std=1.0):
+    return (torch.randn(*shape, generator=g) * std).to(dtype)
+
+
+def wide(t, dev, left, right):
+    """t as the columns left .. of a wider matrix of guard values, on the device."""
+    m = torch.full((t.shape[0], left + t.shape[1] + right), GUARD, dtype=t.dtype, device=dev)
+    v = m[:, left:left + t.shape[1]]
+    v.copy_(t)
+    return m, v
+
+
+def offsets(lens):
+    out = [0]
+    for n in lens:
+        out.append(out[-1] + n)
+    return out
+
+
+def put(v, dev):
+    return None if v is None else v.to(dev)
+
+
+# ---- causal convolution ---------------------------------------------------------------
+LENS = [
+    [1], [2], [40], [0], [0, 0, 5, 0], [1, 1, 1, 2, 3, 4], [31, 1, 0, 33, 2, 95],
+    [32, 32, 64], [3, 29, 3, 200, 1], [700], [1] * 70,
+]
+
+
+def conv_case(dtype, lens, ch, width, kind, seed, bias=True, tail=3, slots="perm", pad=(0, 0)):
+    g = gen(seed)
+    dt = DT[dtype]
+    starts = offsets(lens)
+    T, n = starts[-1] + tail, len(lens)
+    x = randn(g, T, ch, dtype=dt)
+    w = randn(g, ch, width, std=0.6)
+    b = randn(g, ch, std=0.3) if bias else None
+    lines = n + 2
+    state = randn(g, lines, width - 1, ch, dtype=dt)
+    where = torch.randperm(lines, generator=g)[:n].to(torch.int32) if slots == "perm" else None
+    resume = torch.randint(0, 2, (n,), generator=g).to(torch.uint8)
+    return dict(x=x, w=w, bias=b, state=state, starts=starts, slots=where, resume=resume,
+                kind=kind, dt=dt, pad=pad)
+
+
+FLAG = {"silu": cwg.SILU, "relu": cwg.RELU, "none": 0}
+
+
+def run_conv(c, dev):
+    x = wide(c["x"], dev, *c["pad"])[1]
+    ym, y = wide(torch.full_like(c["x"], GUARD), dev, *c["pad"])
+    state = c["state"].to(dev)
+    cwg.conv1d_causal(x, c["w"].to(dev), put(c["bias"], dev), y, state,
+                      torch.tensor(c["starts"], dtype=torch.int32, device=dev),
+                      put(c["slots"], dev), put(c["resume"], dev),
+                      (cwg.BF16 if c["dt"] == torch.bfloat16 else 0) | FLAG[c["kind"]])
+    cwg.device_status()
+    return ym, y, state
+
+
+def check_conv(c, dev):
+    ym, y, state = run_conv(c, dev)
+    want_state = c["state"].clone()
+    for b in range(len(c["starts"]) - 1):
+        s, e = c["starts"][b], c["starts"][b + 1]
+        slot = b if c["slots"] is None else int(c["slots"][b])
+        line = c["state"][slot] if c["resume"][b] else torch.zeros_like(c["state"][slot])
+        want, new = R.conv1d(c["x"][s:e], c["w"], c["bias"], line, c["kind"])
+        R.close(y[s:e], want, f"sequence {b}")
+        want_state[slot] = new.to(c["dt"])
+    assert torch.equal(state.cpu(), want_state)
+    # rows of no sequence and the neighbouring columns are left as they were
+    rest = ym.clone()
+    rest[:c["starts"][-1], c["pad"][0]:c["pad"][0] + c["x"].shape[1]] = GUARD
+    assert (rest == GUARD).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("lens", LENS, ids=str)
+def test_conv1d_sequences(cuda_dev, dtype, lens):
+    check_conv(conv_case(dtype, lens, 96, 4, "silu", 1), cuda_dev)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("width", [2, 3, 4])
+@pytest.mark.parametrize("ch,pad", [(1, (0, 0)), (7, (0, 0)), (40, (8, 8)), (40, (3, 0)),
+                                    (264, (0, 16)), (521, (0, 0)), (1040, (0, 1))])
+def test_conv1d_channels_and_strides(cuda_dev, dtype, width, ch, pad):
+    kind = ("none", "relu", "silu")[(ch + width) % 3]
+    check_conv(conv_case(dtype, [5, 0, 70, 1, 33], ch, width, kind, 2, bias=ch != 40, pad=pad,
+                         slots="perm" if ch % 2 else None), cuda_dev)
+
+
+def test_conv1d_without_cache_lines(cuda_dev):
+    c = conv_case("bf16", [9, 40], 64, 4, "none", 3, tail=0)
+    y = torch.empty_like(c["x"], device=cuda_dev)
+    cwg.conv1d_causal(c["x"].to(cuda_dev), c["w"].to(cuda_dev), None, y, None,
+                      torch.tensor(c["starts"], dtype=torch.int32, device=cuda_dev),
+                      flags=cwg.BF16)
+    for b, (s, e) in enumerate(((0, 9), (9, 49))):
+        want, _ = R.conv1d(c["x"][s:e], c["w"], None, torch.zeros(3, 64), "none")
+        R.close(y[s:e], want, f"sequence {b}")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n,ch,width", [(1, 2048, 4), (3, 7, 2), (17, 136, 3), (130, 72, 4),
+                                        (5, 1, 4)])
+def test_conv1d_step(cuda_dev, dtype, n, ch, width):
+    c = conv_case(dtype, [1] * n, ch, width, "silu", 4, tail=0, pad=(8, 0))
+    xs = wide(c["x"], cuda_dev, 8, 0)[1]
+    y = torch.empty_like(c["x"], device=cuda_dev)
+    state = c["state"].to(cuda_dev)
+    slots = c["slots"].clone()
+    slots[n // 2] = -1 if n > 1 else slots[0]  # a padding row: no line
+    cwg.conv1d_causal_step(xs, c["w"].to(cuda_dev), c["bias"].to(cuda_dev), y, state,
+                           slots.to(cuda_dev),
+                           (cwg.BF16 if dtype == "bf16" else 0) | cwg.SILU)
+    cwg.device_status()
+    want_state = c["state"].clone()
+    for i in range(n):
+        slot = int(slots[i])
+        line = c["state"][slot] if slot >= 0 else torch.zeros_like(c["state"][0])
+        want, new = R.conv1d(c["x"][i:i + 1], c["w"], c["bias"], line, "silu")
+        R.close(y[i:i + 1], want, f"row {i}")
+        if slot >= 0:
+            want_state[slot] = new.to(c["dt"])
+    assert torch.equal(state.cpu(), want_state)
+
+
+# ---- selective scan ----------------------------------------------------------------------
+def ssm_case(dtype, lens, ch, groups, n, seed, gate=True, extras=True, pad=(0, 0), tail=2,
+             slots="perm"):
+    g = gen(seed)
+    dt = DT[dtype]
+    starts = offsets(lens)
+    T, k = starts[-1] + tail, len(lens)
+    c = dict(dt=dt, starts=starts, pad=pad, softplus=extras)
+    c["u"] = randn(g, T, ch, dtype=dt)
+    if extras:
+        c["step"] = randn(g, T, ch, dtype=dt, std=0.7)
+    else:
+        c["step"] = (torch.rand(T, ch, generator=g) * 0.2).to(dt)
+    c["B"], c["C"] = randn(g, T, groups * n, dtype=dt), randn(g, T, groups * n, dtype=dt)
+    c["A"] = -torch.rand(ch, n, generator=g) * n - 0.05
+    c["D"] = randn(g, ch) if extras else None
+    c["bias"] = torch.rand(ch, generator=g) * 6 - 6 if extras else None
+    c["z"] = randn(g, T, ch, dtype=dt) if gate else None
+    c["state"] = randn(g, k + 2, ch, n)
+    c["slots"] = torch.randperm(k + 2, generator=g)[:k].to(torch.int32) if slots else None
+    c["resume"] = torch.randint(0, 2, (k,), generator=g).to(torch.uint8)
+    return c
+
+
+def run_ssm(c, dev, workspace=True, state=None):
+    p = c["pad"]
+    u, step, B, C = (wide(c[k], dev, *p)[1] for k in ("u", "step", "B", "C"))
+    z = None if c["z"] is None else wide(c["z"], dev, *p)[1]
+    ym, y = wide(torch.full_like(c["u"], GUARD), dev, *p)
+    state = c["state"].to(dev) if state is None else state
+    n = len(c["starts"]) - 1
+    T, ch = c["u"].shape
+    ws = None
+    if workspace:
+        ws = torch.empty(cwg.ssm_workspace_bytes(T, n, ch, c["A"].shape[1]), dtype=torch.uint8,
+                         device=dev)
+    cwg.ssm_scan(u, step, c["A"].to(dev), B, C, put(c["D"], dev), put(c["bias"], dev), z, y,
+                 state, torch.tensor(c["starts"], dtype=torch.int32, device=dev),
+                 put(c["slots"], dev), put(c["resume"], dev), ws,
+                 (cwg.BF16 if c["dt"] == torch.bfloat16 else 0) |
+                 (cwg.SOFTPLUS if c["softplus"] else 0))
+    cwg.device_status()
+    return ym, y, state
+
+
+def ssm_want(c, rows, h):
+    groups = c["B"].shape[1] // c["A"].shape[1]
+    B, C = (c[k][rows].unflatten(1, (groups, -1)) for k in ("B", "C"))
+    return R.ssm(c["u"][rows], c["step"][rows], c["A"], B, C, c["D"], c["bias"],
+                 None if c["z"] is None else c["z"][rows], h, c["softplus"])
+
+
+def check_ssm(c, dev, workspace=True):
+    ym, y, state = run_ssm(c, dev, workspace)
+    kept = torch.ones(len(state), dtype=torch.bool)
+    for b in range(len(c["starts"]) - 1):
+        s, e = c["starts"][b], c["starts"][b + 1]
+        slot = b if c["slots"] is None else int(c["slots"][b])
+        h = c["state"][slot] if c["resume"][b] else torch.zeros_like(c["state"][slot])
+        want, new = ssm_want(c, slice(s, e), h)
+        R.close(y[s:e], want, f"sequence {b}")
+        R.close(state[slot], new, f"state of sequence {b}")
+        kept[slot] = False
+    assert torch.equal(state.cpu()[kept], c["state"][kept])
+    rest = ym.clone()
+    rest[:c["starts"][-1], c["pad"][0]:c["pad"][0] + c["u"].shape[1]] = GUARD
+    assert (rest == GUARD).all()
+
+
+@pytest.mark.parametrize("workspace", [True, False])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("lens", LENS[:-1] + [[257, 0, 64]], ids=str)
+def test_ssm_sequences(cuda_dev, dtype, lens, workspace):
+    check_ssm(ssm_case(dtype, lens, 128, 1, 16, 5), cuda_dev, workspace)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n", [1, 3, 4, 8, 12, 16, 23, 32, 64])
+def test_ssm_states(cuda_dev, dtype, n):
+    check_ssm(ssm_case(dtype, [37, 1, 70], 72, 1, n, 6, gate=n % 2 == 0, extras=n != 12),
+              cuda_dev)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("ch,groups,pad", [(1, 1, (0, 0)), (6, 2, (0, 0)), (96, 3, (8, 8)),
+                                           (130, 2, (1, 0)), (256, 4, (0, 8)), (201, 1, (0, 3))])
+def test_ssm_channels_groups_and_strides(cuda_dev, dtype, ch, groups, pad):
+    check_ssm(ssm_case(dtype, [33, 0, 65, 2], ch, groups, 16, 7, pad=pad,
+                       slots="perm" if ch % 2 else None), cuda_dev)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_ssm_long_sequence(cuda_dev, dtype):
+    check_ssm(ssm_case(dtype, [3000, 5], 64, 1, 16, 8), cuda_dev)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("rows,ch,groups,n", [(1, 2048, 1, 16), (5, 6, 2, 12), (33, 264, 1, 64),
+                                              (70, 128, 4, 4), (3, 70, 1, 23), (9, 64, 1, 8)])
+def test_ssm_step(cuda_dev, dtype, rows, ch, groups, n):
+    c = ssm_case(dtype, [1] * rows, ch, groups, n, 9, tail=0, gate=n != 4)
+    dev = cuda_dev
+    slots = c["slots"].clone()
+    if rows > 1:
+        slots[rows // 2] = -1
+    state = c["state"].to(dev)
+    y = torch.empty_like(c["u"], device=dev)
+    cwg.ssm_step(c["u"].to(dev), c["step"].to(dev), c["A"].to(dev), c["B"].to(dev),
+                 c["C"].to(dev), put(c["D"], dev), put(c["bias"], dev), put(c["z"], dev), y,
+                 state, slots.to(dev),
+                 (cwg.BF16 if dtype == "bf16" else 0) | cwg.SOFTPLUS)
+    cwg.device_status()
+    kept = torch.ones(len(state), dtype=torch.bool)
+    for i in range(rows):
+        slot = int(slots[i])
+        h = c["state"][slot] if slot >= 0 else torch.zeros_like(c["state"][0])
+        want, new = ssm_want(c, slice(i, i + 1), h)
+        R.close(y[i:i + 1], want, f"row {i}")
+        if slot >= 0:
+            R.close(state[slot], new, f"state of row {i}")
+            kept[slot] = False
+    assert torch.equal(state.cpu()[kept], c["state"][kept])
+
+
+# ---- indices in device memory -----------------------------------------------------------
+def test_bad_indices_are_reported_and_stay_inside(cuda_dev):
+    """A line out of range or given twice counts as no line, a sequence with bad offsets is
+    left out; nothing outside the operands is touched, and the status says so."""
+    dev = cuda_dev
+    c = conv_case("fp32", [4, 40, 3, 6], 32, 4, "none", 10)
+    c["slots"] = torch.tensor([1, 1, 99, 0], dtype=torch.int32)
+    c["resume"] = torch.ones(4, dtype=torch.uint8)
+    with pytest.raises(cwg.CwgError) as e:
+        run_conv(c, dev)
+    assert e.value.status == cwg.EINDEX
+    cwg.device_status()  # cleared
+    s = ssm_case("fp32", [4, 40, 3, 6], 32, 1, 16, 11)
+    s["slots"], s["resume"] = c["slots"], c["resume"]
+    with pytest.raises(cwg.CwgError) as e:
+        run_ssm(s, dev)
+    assert e.value.status == cwg.EINDEX
+    for bad in ([0, 5, 3, 9], [0, 5, 60, 9], [-3, 5, 7, 9]):
+        c = conv_case("bf16", [3, 3, 3], 32, 4, "none", 12)
+        c["starts"] = bad
+        with pytest.raises(cwg.CwgError) as e:
+            run_conv(c, dev)
+        assert e.value.status == cwg.EINDEX
+        s = ssm_case("bf16", [3, 3, 3], 32, 1, 16, 13)
+        s["starts"] = bad
+        with pytest.raises(cwg.CwgError) as e:
+            run_ssm(s, dev)
+        assert e.value.status == cwg.EINDEX
+
+
+def test_bad_lines_compute_as_no_line(cuda_dev):
+    dev = cuda_dev
+    s = ssm_case("fp32", [4, 40, 3, 6], 32, 1, 16, 14, tail=0)
+    s["resume"] = torch.ones(4, dtype=torch.uint8)
+    s["slots"] = torch.tensor([1, 1, 99, 0], dtype=torch.int32)
+    T, ch = s["u"].shape
+    y, state = torch.empty(T, ch, device=dev), s["state"].to(dev)
+    cwg.ssm_scan(s["u"].to(dev), s["step"].to(dev), s["A"].to(dev), s["B"].to(dev),
+                 s["C"].to(dev), s["D"].to(dev), s["bias"].to(dev), s["z"].to(dev), y, state,
+                 torch.tensor(s["starts"], dtype=torch.int32, device=dev), s["slots"].to(dev),
+                 s["resume"].to(dev), None, cwg.SOFTPLUS)
+    with pytest.raises(cwg.CwgError):
+        cwg.device_status()
+    for b, slot in enumerate([1, -1, -1, 0]):
+        rows = slice(s["starts"][b], s["starts"][b + 1])
+        h = s["state"][slot] if slot >= 0 else torch.zeros_like(s["state"][0])
+        want, new = ssm_want(s, rows, h)
+        R.close(y[rows], want, f"sequence {b}")
+        if slot >= 0:
+            R.close(state[slot], new, f"state of sequence {b}")
+    assert torch.equal(state[2:].cpu(), s["state"][2:])
+
+
+# ---- 8-bit quantiser and product ---------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("rows,cols,pad", [(1, 1, 0), (3, 128, 0), (130, 200, 8), (257, 333, 0),
+                                           (64, 1024, 16), (5, 136, 3)])
+def test_fp8_quantize(cuda_dev, dtype, block_rows, rows, cols, pad):
+    g = gen(rows * cols)
+    x = (torch.randn(rows, cols, generator=g) *
+         torch.exp(4 * torch.randn(rows, 1, generator=g))).to(DT[dtype])
+    if rows > 3:
+        x[2] = 0
+        x[3] *= 1e-30
+    xd = wide(x, cuda_dev, pad, pad)[1]
+    qm = torch.full((rows, cols + 16), 1.0, device=cuda_dev).to(torch.float8_e4m3fn)
+    scale = torch.empty(-(-rows // block_rows), -(-cols // 128), device=cuda_dev)
+    cwg.fp8_quantize(xd, qm[:, :cols], scale, block_rows, cwg.BF16 if dtype == "bf16" else 0)
+    q, s = R.quantize(x, block_rows)
+    assert torch.equal(scale.cpu(), s)
+    assert torch.equal(qm[:, :cols].float().cpu(), q.float())
+    assert (qm[:, cols:].float() == 1.0).all()
+
+
+def test_fp8_quantize_infinity_and_nan(cuda_dev):
+    x = torch.ones(3, 256)
+    x[0, 5], x[1, 130], x[2, 7] = float("inf"), float("nan"), -float("inf")
+    q = torch.empty(3, 256, dtype=torch.float8_e4m3fn, device=cuda_dev)
+    s = torch.empty(3, 2, device=cuda_dev)
+    cwg.fp8_quantize(x.to(cuda_dev), q, s, 1)
+    back = q.float().cpu().view(3, 2, 128) * s.cpu()[:, :, None]
+    hurt = torch.tensor([[True, False], [False, True], [True, False]])
+    assert back[hurt].isnan().all() and (back[~hurt] - 1).abs().max() <= 2.0 ** -4
+
+
+def matmul_case(m, n, k, seed, dtype="fp32"):
+    g = gen(seed)
+    a, a_s = R.quantize(randn(g, m, k) * torch.exp(randn(g, m, 1)), 1)
+    w, w_s = R.quantize(randn(g, n, k, std=k ** -0.5), 128)
+    return a, a_s, w, w_s, randn(g, n, std=0.2)
+
+
+def on_dev(q, dev):
+    """e4m3 rows on 16-byte boundaries, with NaN behind every row's end."""
+    ld = -(-q.shape[1] // 16) * 16
+    t = torch.full((q.shape[0], ld), 0x7f, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
+    t[:, :q.shape[1]].copy_(q)
+    return t[:, :q.shape[1]]
+
+
+def check_matmul(dev, m, n, k, dtype, relu, with_bias, seed=15):
+    a, a_s, w, w_s, bias = matmul_case(m, n, k, seed)
+    ym, y = wide(torch.zeros(m, n, dtype=DT[dtype]), dev, 3, 2)
+    flags = (cwg.BF16 if dtype == "bf16" else 0) | (cwg.RELU if relu else 0)
+    cwg.fp8_matmul(on_dev(a, dev), a_s.to(dev), on_dev(w, dev), w_s.to(dev),
+                   bias.to(dev) if with_bias else None, y, flags)
+    cwg.device_status()
+    R.close(y, R.matmul(a, a_s, w, w_s, bias if with_bias else None, relu, DT[dtype]),
+            f"{m}x{n}x{k}")
+    assert (ym[:, :3] == GUARD).all() and (ym[:, 3 + n:] == GUARD).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("m,n,k", [
+    (1, 1, 1), (1, 128, 128), (1, 300, 100), (4, 1000, 4096), (16, 128, 640), (17, 257, 129),
+    (33, 520, 1000), (64, 384, 256), (65, 130, 1543), (128, 128, 128), (200, 333, 700),
+    (300, 512, 2048), (513, 640, 96),
+])
+def test_fp8_matmul(cuda_dev, dtype, m, n, k):
+    check_matmul(cuda_dev, m, n, k, dtype, relu=(m + n) % 2 == 0, with_bias=m != 16)

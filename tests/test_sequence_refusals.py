@@ -1,0 +1,168 @@
+"""What the sequence layers and the 8-bit product refuse before any CUDA call, through the C
+ABI (fake addresses: nothing is read) and through the Python mirror."""
+import ctypes
+
+import pytest
+import torch
+
+import cwg
+
+X, W, Y, S, I = 0x10000, 0x20000, 0x400000, 0x800000, 0xC00000  # far apart, 16-byte aligned
+
+
+def conv(**kw):
+    a = dict(x=X, ldx=64, w=W, bias=None, y=Y, ldy=64, state=S, starts=I, slots=I, resume=None,
+             tokens=10, n_seq=2, n_slots=4, channels=64, width=4, flags=0)
+    a.update(kw)
+    return cwg.lib().cwg_conv1d_causal(*a.values(), None)
+
+
+def conv_step(**kw):
+    a = dict(x=X, ldx=64, w=W, bias=None, y=Y, ldy=64, state=S, slots=I, n=3, n_slots=4,
+             channels=64, width=4, flags=0)
+    a.update(kw)
+    return cwg.lib().cwg_conv1d_causal_step(*a.values(), None)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(x=None), cwg.EINVAL), (dict(y=None), cwg.EINVAL), (dict(w=None), cwg.EINVAL),
+    (dict(starts=None), cwg.EINVAL), (dict(x=X + 2), cwg.EINVAL), (dict(w=W + 2), cwg.EINVAL),
+    (dict(ldx=63), cwg.EINVAL), (dict(ldy=10), cwg.EINVAL), (dict(tokens=-1), cwg.EINVAL),
+    (dict(tokens=(1 << 30) + 1), cwg.EINVAL), (dict(n_seq=-1), cwg.EINVAL),
+    (dict(channels=0), cwg.EINVAL), (dict(width=1), cwg.EINVAL),
+    (dict(width=5), cwg.EUNSUPPORTED), (dict(flags=cwg.SILU | cwg.RELU), cwg.EINVAL),
+    (dict(flags=cwg.SOFTPLUS), cwg.EINVAL), (dict(flags=cwg.FORCE_TC), cwg.EINVAL),
+    (dict(y=X), cwg.EINVAL),                            # in place
+    (dict(y=X + 64 * 4, ldx=64), cwg.EINVAL),           # one row further
+    (dict(ldx=96, ldy=96, y=X + 63 * 4), cwg.EINVAL),   # one shared column
+    (dict(slots=None, n_slots=1), cwg.EINVAL),          # line b of too few lines
+    (dict(n_slots=-1), cwg.EINVAL), (dict(state=S + 2), cwg.EINVAL),
+    (dict(n_seq=0), cwg.OK), (dict(tokens=0, state=None), cwg.OK),
+])
+def test_conv1d_refuses(kw, status):
+    assert conv(**kw) == status
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(state=None), cwg.EINVAL), (dict(n=-1), cwg.EINVAL), (dict(n=0), cwg.OK),
+    (dict(slots=None, n_slots=2), cwg.EINVAL), (dict(width=5), cwg.EUNSUPPORTED),
+    (dict(y=X), cwg.EINVAL), (dict(ldx=8), cwg.EINVAL),
+])
+def test_conv1d_step_refuses(kw, status):
+    assert conv_step(**kw) == status
+
+
+def ssm(step=False, workspace=None, size=0, **kw):
+    op = cwg.cwg_ssm(u=X, dt=X + 0x40000, B=X + 0x80000, C=X + 0xC0000, z=None, y=Y, ldu=64,
+                     lddt=64, ldb=16, ldc=16, ldz=0, ldy=64, A=W, D=None, dt_bias=None, state=S,
+                     starts=I, slots=I, resume=None, tokens=10, n_seq=2, n_slots=4, channels=64,
+                     groups=1, states=16, flags=0)
+    for k, v in kw.items():
+        setattr(op, k, v)
+    if step:
+        return cwg.lib().cwg_ssm_step(ctypes.byref(op), None)
+    return cwg.lib().cwg_ssm_scan(ctypes.byref(op), workspace, size, None)
+
+
+@pytest.mark.parametrize("step", [False, True])
+@pytest.mark.parametrize("kw", [
+    dict(u=None), dict(dt=None), dict(A=None), dict(B=None), dict(C=None), dict(y=None),
+    dict(ldu=63), dict(lddt=1), dict(ldb=15), dict(ldc=3), dict(ldy=0), dict(z=W, ldz=5),
+    dict(channels=0), dict(groups=0), dict(groups=3), dict(states=0), dict(tokens=-1),
+    dict(A=W + 1), dict(D=W + 2), dict(flags=cwg.SILU), dict(flags=cwg.RELU), dict(y=X),
+    dict(B=Y, ldb=64), dict(slots=None, n_slots=1), dict(state=S + 1),
+], ids=str)
+def test_ssm_refuses(step, kw):
+    assert ssm(step, **kw) == cwg.EINVAL
+
+
+def test_ssm_refuses_and_accepts():
+    assert ssm(states=65, ldb=65, ldc=65) == cwg.EUNSUPPORTED
+    assert ssm(True, state=None) == cwg.EINVAL
+    assert ssm(starts=None) == cwg.EINVAL
+    assert ssm(n_seq=0) == cwg.OK and ssm(True, tokens=0) == cwg.OK
+    assert ssm(tokens=0, state=None) == cwg.OK
+    need = cwg.ssm_workspace_bytes(10, 2, 64, 16)
+    assert need > 0
+    assert ssm(workspace=0x1000001, size=1 << 30) == cwg.EINVAL  # misaligned
+    assert ssm(workspace=0x1000000, size=need - 1) == cwg.EINVAL
+    for bad in ((-1, 1, 64, 16), (10, -1, 64, 16), (10, 1, 0, 16), (10, 1, 64, 65)):
+        assert cwg.ssm_workspace_bytes(*bad) == 0
+
+
+def quantize(**kw):
+    a = dict(x=X, ldx=200, q=Y, ldq=208, scale=S, lds=2, rows=3, cols=200, block_rows=1, flags=0)
+    a.update(kw)
+    return cwg.lib().cwg_fp8_quantize(*a.values(), None)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(x=None), cwg.EINVAL), (dict(q=None), cwg.EINVAL), (dict(scale=None), cwg.EINVAL),
+    (dict(ldx=199), cwg.EINVAL), (dict(ldq=100), cwg.EINVAL), (dict(lds=1), cwg.EINVAL),
+    (dict(block_rows=2), cwg.EINVAL), (dict(cols=0), cwg.EINVAL), (dict(rows=-1), cwg.EINVAL),
+    (dict(flags=cwg.RELU), cwg.EINVAL), (dict(x=X + 1), cwg.EINVAL), (dict(rows=0), cwg.OK),
+])
+def test_fp8_quantize_refuses(kw, status):
+    assert quantize(**kw) == status
+
+
+def matmul(**kw):
+    a = dict(a=X, lda=208, a_scale=S, lda_scale=2, w=W, ldw=208, w_scale=S + 4096, ldw_scale=2,
+             bias=None, y=Y, ldy=300, m=5, n=300, k=200, flags=0)
+    a.update(kw)
+    return cwg.lib().cwg_fp8_matmul(*a.values(), None)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(a=None), cwg.EINVAL), (dict(w=None), cwg.EINVAL), (dict(y=None), cwg.EINVAL),
+    (dict(a_scale=None), cwg.EINVAL), (dict(w_scale=None), cwg.EINVAL),
+    (dict(a=X + 8), cwg.EINVAL), (dict(w=W + 1), cwg.EINVAL), (dict(lda=200), cwg.EINVAL),
+    (dict(ldw=204), cwg.EINVAL), (dict(lda=192), cwg.EINVAL), (dict(ldy=299), cwg.EINVAL),
+    (dict(lda_scale=1), cwg.EINVAL), (dict(ldw_scale=1), cwg.EINVAL), (dict(m=-1), cwg.EINVAL),
+    (dict(n=0), cwg.EINVAL), (dict(k=0), cwg.EINVAL), (dict(flags=cwg.SILU), cwg.EINVAL),
+    (dict(bias=S + 2), cwg.EINVAL), (dict(m=0), cwg.OK),
+])
+def test_fp8_matmul_refuses(kw, status):
+    assert matmul(**kw) == status
+
+
+def test_python_mirror_names_the_wrong_argument():
+    t = torch.zeros(4, 8)
+    i = torch.zeros(2, dtype=torch.int32)
+    w = torch.zeros(8, 4)
+    with pytest.raises(ValueError, match="x is not on a CUDA device"):
+        cwg.conv1d_causal(t, w, None, t, None, i)
+    with pytest.raises(ValueError, match="x is not a matrix"):
+        cwg.conv1d_causal_step(t[0], w, None, t, None)
+    with pytest.raises(ValueError, match="u is not on a CUDA device"):
+        cwg.ssm_scan(t, t, w, t, t, None, None, None, t, None, i)
+    with pytest.raises(ValueError, match="state is missing"):
+        cwg.ssm_step(t, t, w, t, t, None, None, None, t, None)
+    with pytest.raises(ValueError, match="a is not on a CUDA device"):
+        cwg.fp8_matmul(t, t, t, t, None, t)
+    with pytest.raises(ValueError, match="x is not a matrix"):
+        cwg.fp8_quantize(None, t, t, 1)
+
+
+def test_argument_check_helpers():
+    """The checks themselves, on CPU tensors (device -1)."""
+    t = torch.zeros(4, 8)
+    assert cwg._rows(t, "t", torch.float32, 4, 8, -1) == (t.data_ptr(), 8)
+    v = torch.zeros(4, 24)[:, 8:16]
+    assert cwg._rows(v, "v", torch.float32, 4, 8, -1) == (v.data_ptr(), 24)
+    for bad, what in ((t.to(torch.bfloat16), "not torch.float32"), (t[:3], "shape"),
+                      (torch.zeros(8, 4).t(), "strides"), (t[:1].expand(4, 8), "strides"),
+                      (None, "missing"), (torch.zeros(4, 16)[:, ::2], "strides")):
+        with pytest.raises(ValueError, match=what):
+            cwg._rows(bad, "t", torch.float32, 4, 8, -1)
+    assert cwg._arg(None, "t", torch.float32, (4, 8), -1, True) is None
+    for bad, what in ((torch.zeros(4, 16)[:, ::2], "contiguous"), (t.double(), "not torch"),
+                      (t[0], "shape"), (None, "missing")):
+        with pytest.raises(ValueError, match=what):
+            cwg._arg(bad, "t", torch.float32, (4, 8), -1)
+    with pytest.raises(ValueError, match="device"):
+        cwg._arg(t, "t", torch.float32, (4, 8), 0)
+
+
+def test_strerror_of_bad_index():
+    assert "index" in cwg.strerror(cwg.EINDEX)
