@@ -59,11 +59,15 @@ def ref_available() -> bool:
     return os.path.exists(REF_SO)
 
 
+class ReferenceNotBuilt(RuntimeError):
+    """The reference's own C is needed and its source tree was not there to build it from."""
+
+
 def ref() -> ctypes.CDLL:
     global _ref
     if _ref is None:
         if not ref_available():
-            raise RuntimeError(f"reference C not built: {REF_SO}")
+            raise ReferenceNotBuilt(f"reference C not built: {REF_SO}")
         L = ctypes.CDLL(REF_SO)
         L.refl_tiles_f23.argtypes = [_fp, _fp, _fp, _i, _i, _i, _i]
         L.refl_conv_layer_f23.argtypes = [_fp, _fp, _fp, _fp, _i, _i, _i, _i, _i, _i, _i]

@@ -17,6 +17,17 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (B200, sm_100a)")
 
 
+@pytest.hookimpl(wrapper=True)
+def pytest_runtest_call(item):
+    """A comparison with the reference's own C is skipped where its source tree is missing."""
+    import oracle
+
+    try:
+        return (yield)
+    except oracle.ReferenceNotBuilt as e:
+        pytest.skip(str(e))
+
+
 def load_golden(name):
     with np.load(os.path.join(GOLDEN, name)) as z:
         return {k: z[k] for k in z.files}
