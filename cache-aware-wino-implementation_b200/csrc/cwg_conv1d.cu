@@ -8,7 +8,7 @@
 //
 // Prompts: a thread owns one 16-byte vector of channels and a run of consecutive
 // rows, so that a row is read once (plus K - 1 rows of halo per run) and the
-// window slides through registers; eight rows' loads are in flight at a time.
+// window slides through registers while the next four rows are loaded.
 // The K - 1 first rows of a sequence, which need the cache line, are all computed
 // by the thread whose run holds the sequence's first row, and that thread stores
 // the new line after it: no other thread reads a line, so the old line can be
@@ -24,13 +24,13 @@ namespace seq {
 __device__ unsigned int g_seq_status;
 
 constexpr int kConvThreads = 128;
-constexpr int kAhead = 8;          // rows loaded ahead of their use
+constexpr int kAhead = 4;          // rows per step; the next step's are loaded meanwhile
 constexpr int kStartsInSmem = 1024;
 
-template <int ACT>
+template <typename T, int ACT>
 __device__ __forceinline__ float activate(float v) {
   if (ACT == CWGK_ACT_RELU) return v < 0.f ? 0.f : v;  // NaN stays
-  if (ACT == CWGK_ACT_SILU) return silu(v);
+  if (ACT == CWGK_ACT_SILU) return silu<T>(v);
   return v;
 }
 
@@ -69,7 +69,7 @@ __device__ __forceinline__ void load_weights(const ConvArgs &a, int c, bool acti
 }
 
 // act(b + sum_j w[j] h[j]) with h the window's rows, oldest first, x the newest.
-template <int V, int K, int ACT>
+template <typename T, int V, int K, int ACT>
 __device__ __forceinline__ void window_row(const float (&w)[V][K], const float (&b)[V],
                                            const float (&h)[K - 1][V], const float (&x)[V],
                                            float (&y)[V]) {
@@ -78,7 +78,7 @@ __device__ __forceinline__ void window_row(const float (&w)[V][K], const float (
     float s = b[v];
 #pragma unroll
     for (int j = 0; j < K - 1; ++j) s = fmaf(w[v][j], h[j][v], s);
-    y[v] = activate<ACT>(fmaf(w[v][K - 1], x[v], s));
+    y[v] = activate<T, ACT>(fmaf(w[v][K - 1], x[v], s));
   }
 }
 template <int V, int K>
@@ -92,7 +92,7 @@ __device__ __forceinline__ void slide(float (&h)[K - 1][V], const float (&x)[V])
 }
 
 template <typename T, int V, int K, int ACT>
-__global__ void __launch_bounds__(kConvThreads) conv1d_prompt(const ConvArgs a) {
+__global__ void __launch_bounds__(kConvThreads, 4) conv1d_prompt(const ConvArgs a) {
   __shared__ int s_starts[kStartsInSmem + 1];
   const T *x = static_cast<const T *>(a.x);
   T *y = static_cast<T *>(a.y);
@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(kConvThreads) conv1d_prompt(const ConvArgs a) 
       if (i < len) {
         float xv[V], yv[V];
         unpack(load_raw<T, V>(x + (size_t)(begin + i) * a.ldx + c), xv);
-        window_row<V, K, ACT>(w, b, h, xv, yv);
+        window_row<T, V, K, ACT>(w, b, h, xv, yv);
         store_raw<T, V>(y + (size_t)(begin + i) * a.ldy + c, pack<T, V>(yv));
         slide<V, K>(h, xv);
       }
@@ -166,29 +166,45 @@ __global__ void __launch_bounds__(kConvThreads) conv1d_prompt(const ConvArgs a) 
     unpack(t >= 0 && t < a.tokens ? load_raw<T, V>(x + (size_t)t * a.ldx + c) : zero_raw<T, V>(),
            h[j]);
   }
-  for (int t = t0; t < t1; t += kAhead) {
-    typename Raw<T, V>::type raw[kAhead];
+  typename Raw<T, V>::type raw[kAhead], next[kAhead];
+  auto fetch = [&](int t) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
-      raw[i] = t + i < t1 ? load_raw<T, V>(x + (size_t)(t + i) * a.ldx + c) : zero_raw<T, V>();
+      next[i] = t + i < t1 ? load_raw<T, V>(x + (size_t)(t + i) * a.ldx + c) : zero_raw<T, V>();
+  };
+  fetch(t0);
+  for (int t = t0; t < t1; t += kAhead) {
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      if (t + i < t1) {
-        while (s + 1 < a.n_seq && starts[s + 1] <= t + i) {
-          ++s;
-          begin = starts[s];
-          end = starts[s + 1];
-          if (begin < 0 || end > a.tokens) end = begin = 0;
-        }
-        float xv[V];
+    for (int i = 0; i < kAhead; ++i) raw[i] = next[i];
+    fetch(t + kAhead);
+    if (t - begin >= K - 1 && t + kAhead <= end) {  // all of one sequence, as nearly always
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        float xv[V], yv[V];
         unpack(raw[i], xv);
-        if (t + i < end && t + i - begin >= K - 1) {
-          float yv[V];
-          window_row<V, K, ACT>(w, b, h, xv, yv);
-          store_raw<T, V>(y + (size_t)(t + i) * a.ldy + c, pack<T, V>(yv));
-        }
+        window_row<T, V, K, ACT>(w, b, h, xv, yv);
+        store_raw<T, V>(y + (size_t)(t + i) * a.ldy + c, pack<T, V>(yv));
         slide<V, K>(h, xv);
       }
+      continue;
+    }
+#pragma unroll 1
+    for (int i = 0; i < kAhead; ++i) {
+      if (t + i >= t1) break;
+      while (s + 1 < a.n_seq && starts[s + 1] <= t + i) {
+        ++s;
+        begin = starts[s];
+        end = starts[s + 1];
+        if (begin < 0 || end > a.tokens) end = begin = 0;
+      }
+      float xv[V];
+      unpack(i == 0 ? raw[0] : i == 1 ? raw[1] : i == 2 ? raw[2] : raw[3], xv);
+      if (t + i < end && t + i - begin >= K - 1) {
+        float yv[V];
+        window_row<T, V, K, ACT>(w, b, h, xv, yv);
+        store_raw<T, V>(y + (size_t)(t + i) * a.ldy + c, pack<T, V>(yv));
+      }
+      slide<V, K>(h, xv);
     }
   }
 }
@@ -224,7 +240,7 @@ __global__ void __launch_bounds__(kConvThreads) conv1d_step(const ConvArgs a) {
 #pragma unroll
     for (int j = 0; j < K - 1; ++j) unpack(raw[j], h[j]);
     unpack(raw[K - 1], xv);
-    window_row<V, K, ACT>(w, b, h, xv, yv);
+    window_row<T, V, K, ACT>(w, b, h, xv, yv);
     store_raw<T, V>(y + (size_t)r * a.ldy + c, pack<T, V>(yv));
     if (slot >= 0) {
 #pragma unroll

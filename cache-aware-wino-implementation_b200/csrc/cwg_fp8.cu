@@ -85,25 +85,38 @@ __device__ __forceinline__ void store8(uint8_t *q, const float (&v)[8], float s,
   }
 }
 
-// One half-warp per group of 1 x 128: 8 elements a lane, read once.
+// A half-warp per group of 1 x 128, 8 elements a lane; it takes kRowGroups groups, whose
+// loads are all in flight before the first is used.
+constexpr int kRowGroups = 4;
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quantize_rows(const QuantArgs a) {
-  const long long g = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const long long first = (long long)blockIdx.x * (16 * kRowGroups) + (threadIdx.x >> 4);
   const int lane = threadIdx.x & 15;
-  const bool ok = g < a.groups;
-  const int row = ok ? (int)(g / a.kblocks) : 0, kb = ok ? (int)(g % a.kblocks) : 0;
-  const int c = kb * 128 + lane * 8;
-  const int n = ok ? a.cols - c : 0;
-  float v[8];
-  load8<T, VEC>(static_cast<const T *>(a.x) + (size_t)row * a.ldx + c, n, v);
-  uint32_t m = 0;
+  float v[kRowGroups][8];
+  int row[kRowGroups], kb[kRowGroups], n[kRowGroups];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i]));
+  for (int k = 0; k < kRowGroups; ++k) {
+    const long long g = first + k * 16;
+    row[k] = (int)(g / a.kblocks);
+    kb[k] = (int)(g - (long long)row[k] * a.kblocks);
+    n[k] = g < a.groups ? a.cols - (kb[k] * 128 + lane * 8) : 0;
+    load8<T, VEC>(static_cast<const T *>(a.x) + (n[k] > 0 ? (size_t)row[k] * a.ldx : 0) +
+                      kb[k] * 128 + lane * 8,
+                  n[k], v[k]);
+  }
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float s = scale_of(m);
-  if (ok && lane == 0) a.scale[(size_t)row * a.lds + kb] = s;
-  if (n > 0) store8<VEC>(a.q + (size_t)row * a.ldq + c, v, s, n);
+  for (int k = 0; k < kRowGroups; ++k) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[k][i]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float s = scale_of(m);
+    if (n[k] > 0) {
+      if (lane == 0) a.scale[(size_t)row[k] * a.lds + kb[k]] = s;
+      store8<VEC>(a.q + (size_t)row[k] * a.ldq + kb[k] * 128 + lane * 8, v[k], s, n[k]);
+    }
+  }
 }
 
 // One CTA per block of 128 x 128, 64 elements a thread held in registers.
@@ -144,7 +157,7 @@ static int quantize(QuantArgs a, int block_rows, cudaStream_t s) {
   // a whole vector at a row's end may reach past cols only if the row does
   const bool vec = ((uintptr_t)a.x & 15) == 0 && ((uintptr_t)a.q & 7) == 0 &&
                    a.cols % E == 0 && (one || (a.ldx % E == 0 && a.ldq % 8 == 0));
-  const long long blocks = block_rows == 1 ? (a.groups + 15) / 16 : a.groups;
+  const long long blocks = block_rows == 1 ? (a.groups + 16 * kRowGroups - 1) / (16 * kRowGroups) : a.groups;
   if (blocks > 0x7fffffffLL) return -2;
   if (block_rows == 1) {
     if (vec)

@@ -80,11 +80,52 @@ __device__ __forceinline__ typename Raw<T, V>::type pack(const float (&f)[V]) {
   }
 }
 
-__device__ __forceinline__ float silu(float v) { return v / (1.f + expf(-v)); }
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+constexpr float kLog2e = 1.4426950408889634f;
 
+// v / (1 + exp(-v)).  fp32 results take expf and a rounded division.  For bf16 results,
+// whose half step is 2^-8 of the value, ex2 and a reciprocal (2 ulp each; the exponent's
+// rounding adds |v| 2^-24) stay below 2^-19 for |v| up to 16, where the result or exp(-v)
+// is beyond bf16's reach; 5 instructions instead of about 30.  Both give NaN for
+// v = -infinity, as the formula does.
+template <typename T>
+__device__ __forceinline__ float silu(float v) {
+  if constexpr (sizeof(T) == 4)
+    return v / (1.f + expf(-v));
+  else
+    return v * rcp(1.f + ex2(-kLog2e * v));
+}
+
+// log(1 + exp(v)) = max(v, 0) + log1p(e) with e = exp(-|v|) <= 1, and the series
+//   log1p(e) = 2 (s + s^3/3 + s^5/5 + ...),  s = e / (2 + e) <= 1/3,
+// which has no cancellation for small e (a step's relative error goes into the decay of
+// every state).  Cut after s^17: the rest is below (1/9)^9 / 19 = 1.4e-10 of the first
+// term.  Relative error: ex2 4 u, its argument 2 |v| u, the reciprocal 2 u, about 6 u for
+// the sums (u = 2^-24).
 __device__ __forceinline__ float softplus(float v) {
-  // above 20 exp(-v) is below half a step of v
-  return v > 20.f ? v : log1pf(expf(v));
+  const float e = ex2(-kLog2e * fabsf(v));
+  const float s = e * rcp(2.f + e);
+  const float q = s * s;
+  float p = 1.f / 17;
+  p = fmaf(p, q, 1.f / 15);
+  p = fmaf(p, q, 1.f / 13);
+  p = fmaf(p, q, 1.f / 11);
+  p = fmaf(p, q, 1.f / 9);
+  p = fmaf(p, q, 1.f / 7);
+  p = fmaf(p, q, 1.f / 5);
+  p = fmaf(p, q, 1.f / 3);
+  p = fmaf(p, q, 1.f);
+  const float r = fmaf(2.f * s, p, fmaxf(v, 0.f));
+  return v != v ? v : r;  // fmaxf would drop a NaN
 }
 
 // First b in [0, n) with s[b] >= v (n if none); ends for any contents of s.

@@ -19,22 +19,14 @@ using namespace seq;
 
 __device__ unsigned int g_ssm_status;
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kS = 4;    // states per lane
 constexpr int kTT = 32;  // tokens per tile of the prompt kernel
-
-__device__ __forceinline__ float ex2(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
 
 struct Args {
   cwg_ssm p;
   int per;      // channels per group
   int cblocks;  // CTAs along one group's channels
-  int run;      // rows per CTA (steps)
-  bool vec_state;
+  bool vec_state, vec_a;  // the state's and A's rows are whole 16-byte vectors
 };
 
 // A lane's four states of one cache line, or zeros.
@@ -231,7 +223,7 @@ __global__ void __launch_bounds__(Geo<L>::kThreads) ssm_prompt(const Args a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           y[e] = fmaf(p.D && c + e < nch ? p.D[c0 + c + e] : 0.f, u[e], s_y[t][c + e]);
-          if (p.z) y[e] *= silu(z[e]);
+          if (p.z) y[e] *= silu<T>(z[e]);
         }
         Piece<T, VEC>::store(static_cast<T *>(p.y) + (size_t)(t0 + t) * p.ldy + c0 + c, y,
                              nch - c);
@@ -242,63 +234,78 @@ __global__ void __launch_bounds__(Geo<L>::kThreads) ssm_prompt(const Args a) {
 }
 
 // ---- one token of each sequence ----------------------------------------------------
-// Bound by the states, 8 N bytes per channel in and out; the lanes of a channel
-// compute its step together, a CTA's rows share A.
-template <typename T, int L>
+// Bound by the states, 8 N bytes per channel in and out.  A CTA takes RR rows of one
+// channel block: the rows share A, and all their states are loaded before the first is
+// used.  Which lines may be written is found out meanwhile.
+template <typename T, int L, int RR>
 __global__ void __launch_bounds__(Geo<L>::kThreads) ssm_token(const Args a) {
   constexpr int CH = Geo<L>::kCH;
   const cwg_ssm &p = a.p;
   const int tid = threadIdx.x;
   const int cblk = blockIdx.x % a.cblocks;
   const int group = (blockIdx.x / a.cblocks) % p.groups;
-  const int run = blockIdx.x / (a.cblocks * p.groups);
+  const int r0 = blockIdx.x / (a.cblocks * p.groups) * RR;
   const int ch = tid / L, l = tid % L, i0 = l * kS;
   const int in = cblk * CH + ch, c = group * a.per + in;
   const bool mine = in < a.per;
-  float A2[kS];
+  float h[RR][kS], bv[RR][kS], cv[RR][kS], u[RR], d[RR], z[RR];
+  float *line[RR];
 #pragma unroll
-  for (int i = 0; i < kS; ++i)
-    A2[i] = mine && i0 + i < p.states ? p.A[(size_t)c * p.states + i0 + i] * kLog2e : 0.f;
+  for (int k = 0; k < RR; ++k) {
+    const int r = r0 + k;
+    const bool row = r < p.tokens;
+    const int slot = !row ? -1 : p.slots ? p.slots[r] : r;
+    const bool in_range = slot >= 0 && slot < p.n_slots;
+    line[k] = in_range && mine ? p.state + ((size_t)slot * p.channels + c) * p.states : nullptr;
+#pragma unroll
+    for (int i = 0; i < kS; ++i) h[k][i] = 0.f;
+    if (line[k]) load_states(line[k], i0, p.states, a.vec_state, h[k]);
+    const size_t at = (size_t)(row ? r : 0);
+    u[k] = d[k] = z[k] = 0.f;
+    if (mine && row) {
+      u[k] = to_f32(static_cast<const T *>(p.u)[at * p.ldu + c]);
+      d[k] = to_f32(static_cast<const T *>(p.dt)[at * p.lddt + c]);
+      if (p.z) z[k] = to_f32(static_cast<const T *>(p.z)[at * p.ldz + c]);
+    }
+#pragma unroll
+    for (int i = 0; i < kS; ++i) {
+      const bool ok = row && i0 + i < p.states;
+      const size_t col = (size_t)group * p.states + i0 + i;
+      bv[k][i] = ok ? to_f32(static_cast<const T *>(p.B)[at * p.ldb + col]) : 0.f;
+      cv[k][i] = ok ? to_f32(static_cast<const T *>(p.C)[at * p.ldc + col]) : 0.f;
+    }
+  }
+  float A2[kS] = {0.f, 0.f, 0.f, 0.f};
+  if (mine) load_states(p.A + (size_t)c * p.states, i0, p.states, a.vec_a, A2);
+#pragma unroll
+  for (int i = 0; i < kS; ++i) A2[i] *= kLog2e;
   const float bias = mine && p.dt_bias ? p.dt_bias[c] : 0.f;
   const float skip = mine && p.D ? p.D[c] : 0.f;
   bool bad = false;
-  const int r1 = min((run + 1) * a.run, p.tokens);
-  for (int r = run * a.run; r < r1; ++r) {
-    const int slot = line_of(p.slots, r, p.n_slots, bad);
-    float *line = p.state + ((size_t)(slot < 0 ? 0 : slot) * p.channels + c) * p.states;
-    const size_t row = (size_t)r;
-    float h[kS] = {0.f, 0.f, 0.f, 0.f}, bv[kS], cv[kS];
-    float u = 0.f, d = 0.f, z = 0.f;
-    if (mine) {
-      if (slot >= 0) load_states(line, i0, p.states, a.vec_state, h);
-      u = to_f32(static_cast<const T *>(p.u)[row * p.ldu + c]);
-      d = to_f32(static_cast<const T *>(p.dt)[row * p.lddt + c]) + bias;
-      if (p.z) z = to_f32(static_cast<const T *>(p.z)[row * p.ldz + c]);
-    }
 #pragma unroll
-    for (int i = 0; i < kS; ++i) {
-      const bool ok = i0 + i < p.states;
-      const size_t col = (size_t)group * p.states + i0 + i;
-      bv[i] = ok ? to_f32(static_cast<const T *>(p.B)[row * p.ldb + col]) : 0.f;
-      cv[i] = ok ? to_f32(static_cast<const T *>(p.C)[row * p.ldc + col]) : 0.f;
+  for (int k = 0; k < RR; ++k) {
+    if (r0 + k >= p.tokens) break;
+    if (line_of(p.slots, r0 + k, p.n_slots, bad) < 0) {  // a line given twice counts as none
+      line[k] = nullptr;
+#pragma unroll
+      for (int i = 0; i < kS; ++i) h[k][i] = 0.f;
     }
-    if (p.flags & CWG_SOFTPLUS) d = softplus(d);
-    const float du = d * u;
+    float step = d[k] + bias;
+    if (p.flags & CWG_SOFTPLUS) step = softplus(step);
+    const float du = step * u[k];
     float y = 0.f;
 #pragma unroll
     for (int i = 0; i < kS; ++i) {
-      h[i] = fmaf(ex2(d * A2[i]), h[i], du * bv[i]);
-      y = fmaf(h[i], cv[i], y);
+      h[k][i] = fmaf(ex2(step * A2[i]), h[k][i], du * bv[k][i]);
+      y = fmaf(h[k][i], cv[k][i], y);
     }
 #pragma unroll
     for (int o = L / 2; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-    if (mine) {
-      if (slot >= 0) store_states(line, i0, p.states, a.vec_state, h);
-      if (l == 0) {
-        y = fmaf(skip, u, y);
-        if (p.z) y *= silu(z);
-        static_cast<T *>(p.y)[row * p.ldy + c] = pack1<T>(y);
-      }
+    if (line[k]) store_states(line[k], i0, p.states, a.vec_state, h[k]);
+    if (mine && l == 0) {
+      y = fmaf(skip, u[k], y);
+      if (p.z) y *= silu<T>(z[k]);
+      static_cast<T *>(p.y)[(size_t)(r0 + k) * p.ldy + c] = pack1<T>(y);
     }
   }
   if (bad && tid == 0 && cblk == 0 && group == 0) atomicOr(&g_ssm_status, CWGK_STATUS_INDEX);
@@ -325,12 +332,17 @@ static int launch(const cwg_ssm *op, bool step, cudaStream_t s) {
   a.per = op->channels / op->groups;
   a.cblocks = (a.per + G::kCH - 1) / G::kCH;
   a.vec_state = op->states == G::kNP && aligned16(op->state);
-  a.run = 1;
-  const long long rows = step ? (op->tokens + a.run - 1) / a.run : op->n_seq;
-  const long long blocks = rows * a.cblocks * op->groups;
-  if (blocks > 0x7fffffffLL) return -2;
+  a.vec_a = op->states == G::kNP && aligned16(op->A);
+  const long long blocks = (long long)op->n_seq * a.cblocks * op->groups;
+  const long long step_blocks = (long long)op->tokens * a.cblocks * op->groups;
+  if ((step ? step_blocks : blocks) > 0x7fffffffLL) return -2;
   if (step) {
-    ssm_token<T, L><<<(unsigned)blocks, G::kThreads, 0, s>>>(a);
+    // rows that share A as soon as every SM has work all the same
+    if (step_blocks >= 4 * 4 * 148)
+      ssm_token<T, L, 4><<<(unsigned)((long long)((op->tokens + 3) / 4) * a.cblocks * op->groups),
+                           G::kThreads, 0, s>>>(a);
+    else
+      ssm_token<T, L, 1><<<(unsigned)step_blocks, G::kThreads, 0, s>>>(a);
     return done();
   }
   constexpr int E = 16 / (int)sizeof(T);

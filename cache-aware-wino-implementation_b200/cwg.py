@@ -276,62 +276,33 @@ def version() -> str:
 # These take torch tensors: sizes and row distances come from the tensors (a column range
 # of a wider matrix is passed as it is), and every tensor is checked before the call, since
 # a wrong type, device or size would otherwise only show as wrong memory accesses.
-# ValueError names the argument; what the library itself refuses is a CwgError.
-def _arg(t, name: str, dtype, shape, device, none_ok: bool = False) -> int | None:
-    """Device address of a contiguous tensor of the given type and shape (None: any size)."""
-    if t is None:
-        if none_ok:
-            return None
-        raise ValueError(f"{name} is missing")
-    if t.dtype is not dtype:
-        raise ValueError(f"{name} is {t.dtype}, not {dtype}")
-    if t.get_device() != device:
-        raise ValueError(f"{name} is not on the call's device cuda:{device}")
-    got = t.shape
-    if len(got) != len(shape) or any(w is not None and g != w for g, w in zip(got, shape)):
-        raise ValueError(f"{name} has shape {tuple(got)}, not {tuple(shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} is not contiguous")
-    return t.data_ptr()
+# ValueError names the argument; what the library itself refuses is a CwgError.  The checks
+# are compiled (csrc/cwg_torch.cpp): a decoding step's kernels are shorter than they would
+# take in Python.
+_torch_ext = None
 
 
-def _rows(t, name: str, dtype, rows: int, cols: int, device) -> tuple[int, int]:
-    """(address, row distance) of a [rows][cols] tensor whose rows are contiguous."""
-    if t is None:
-        raise ValueError(f"{name} is missing")
-    if t.dtype is not dtype:
-        raise ValueError(f"{name} is {t.dtype}, not {dtype}")
-    if t.get_device() != device:
-        raise ValueError(f"{name} is not on the call's device cuda:{device}")
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {(rows, cols)}")
-    ld, one = t.stride()
-    if (one != 1 and cols > 1) or (ld < cols and rows > 1):
-        raise ValueError(f"{name} has strides {(ld, one)}: rows of {cols} neighbouring elements "
-                         "are needed")
-    return t.data_ptr(), ld
+def _ext():
+    """Loads lib/cwg_torch.so once and gives it libcwg's entry points."""
+    global _torch_ext
+    if _torch_ext is None:
+        import importlib.util
 
+        import torch  # noqa: F401  (its libraries are the module's)
 
-def _call(first, name: str, stream) -> int:
-    """The device of a call: the current one, which `first` and the stream have to be on."""
-    import torch
-
-    if first is None or first.dim() != 2:
-        raise ValueError(f"{name} is not a matrix of [rows][columns]")
-    if not first.is_cuda:
-        raise ValueError(f"{name} is not on a CUDA device")
-    device = first.get_device()
-    if device != torch.cuda.current_device():
-        raise ValueError(f"{name} is on cuda:{device}, not on the current device")
-    if stream is not None and not isinstance(stream, int) and stream.device_index != device:
-        raise ValueError("the stream belongs to another device")
-    return device
-
-
-def _io(flags: int):
-    import torch
-
-    return torch.bfloat16 if flags & BF16 else torch.float32
+        path = os.path.join(HERE, "lib", "cwg_torch.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"cwg_torch.so not found at {path}: build it with "
+                               "`python -c 'import __graft_entry__ as g; g.build()'`")
+        spec = importlib.util.spec_from_file_location("cwg_torch", path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        L = lib()
+        mod.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+            L.cwg_conv1d_causal, L.cwg_conv1d_causal_step, L.cwg_ssm_scan, L.cwg_ssm_step,
+            L.cwg_fp8_quantize, L.cwg_fp8_matmul)))
+        _torch_ext = mod
+    return _torch_ext
 
 
 def conv1d_causal(x, w, bias, y, state, starts, slots=None, resume=None, flags: int = 0,
@@ -340,77 +311,22 @@ def conv1d_causal(x, w, bias, y, state, starts, slots=None, resume=None, flags: 
     bias (channels,) or None, state (lines, width - 1, channels) or None, starts (sequences + 1,)
     int32, slots (sequences,) int32 or None, resume (sequences,) uint8 or None.  `state` is
     updated in place.  flags: BF16, SILU or RELU."""
-    import torch
-
-    dev, dt = _call(x, "x", stream), _io(flags)
-    tokens, ch = x.shape
-    if w is None or w.dim() != 2:
-        raise ValueError("w is not (channels, width)")
-    width = w.shape[1]
-    if starts is None or starts.dim() != 1 or starts.shape[0] < 1:
-        raise ValueError("starts is not (sequences + 1,)")
-    n_seq = starts.shape[0] - 1
-    n_slots = 0 if state is None else state.shape[0]
-    xp, ldx = _rows(x, "x", dt, tokens, ch, dev)
-    yp, ldy = _rows(y, "y", dt, tokens, ch, dev)
-    _check(lib().cwg_conv1d_causal(
-        xp, ldx, _arg(w, "w", torch.float32, (ch, width), dev),
-        _arg(bias, "bias", torch.float32, (ch,), dev, True), yp, ldy,
-        _arg(state, "state", dt, (None, width - 1, ch), dev, True),
-        _arg(starts, "starts", torch.int32, (None,), dev),
-        _arg(slots, "slots", torch.int32, (n_seq,), dev, True),
-        _arg(resume, "resume", torch.uint8, (n_seq,), dev, True),
-        tokens, n_seq, n_slots, ch, width, flags, _stream(stream)), "cwg_conv1d_causal")
+    st = (_torch_ext or _ext()).conv1d_causal(x, w, bias, y, state, starts, slots, resume, flags,
+                                              stream)
+    if st:
+        _check(st, "cwg_conv1d_causal")
 
 
 def conv1d_causal_step(x, w, bias, y, state, slots=None, flags: int = 0, stream=None) -> None:
     """One token of each sequence: x and y (sequences, channels), the rest as for
     conv1d_causal.  `state` is updated in place."""
-    import torch
-
-    dev, dt = _call(x, "x", stream), _io(flags)
-    n, ch = x.shape
-    if w is None or w.dim() != 2:
-        raise ValueError("w is not (channels, width)")
-    width = w.shape[1]
-    xp, ldx = _rows(x, "x", dt, n, ch, dev)
-    yp, ldy = _rows(y, "y", dt, n, ch, dev)
-    _check(lib().cwg_conv1d_causal_step(
-        xp, ldx, _arg(w, "w", torch.float32, (ch, width), dev),
-        _arg(bias, "bias", torch.float32, (ch,), dev, True), yp, ldy,
-        _arg(state, "state", dt, (None, width - 1, ch), dev),
-        _arg(slots, "slots", torch.int32, (n,), dev, True), n, state.shape[0], ch, width, flags,
-        _stream(stream)), "cwg_conv1d_causal_step")
+    st = (_torch_ext or _ext()).conv1d_causal_step(x, w, bias, y, state, slots, flags, stream)
+    if st:
+        _check(st, "cwg_conv1d_causal_step")
 
 
 def ssm_workspace_bytes(tokens: int, n_seq: int, channels: int, states: int) -> int:
     return int(lib().cwg_ssm_workspace_bytes(tokens, n_seq, channels, states))
-
-
-def _ssm(u, dt, A, B, C, D, dt_bias, z, y, state, slots, n_seq, flags, stream) -> cwg_ssm:
-    import torch
-
-    dev, io = _call(u, "u", stream), _io(flags)
-    rows, ch = u.shape
-    if A is None or A.dim() != 2 or A.shape[1] < 1:
-        raise ValueError("A is not (channels, states)")
-    n = A.shape[1]
-    if B is None or B.dim() != 2 or B.shape[1] < n or B.shape[1] % n:
-        raise ValueError("B is not (tokens, groups * states)")
-    cols = B.shape[1]
-    up, ldu = _rows(u, "u", io, rows, ch, dev)
-    dp, lddt = _rows(dt, "dt", io, rows, ch, dev)
-    bp, ldb = _rows(B, "B", io, rows, cols, dev)
-    cp, ldc = _rows(C, "C", io, rows, cols, dev)
-    zp, ldz = (None, 0) if z is None else _rows(z, "z", io, rows, ch, dev)
-    yp, ldy = _rows(y, "y", io, rows, ch, dev)
-    f32 = torch.float32
-    return cwg_ssm(
-        up, dp, bp, cp, zp, yp, ldu, lddt, ldb, ldc, ldz, ldy, _arg(A, "A", f32, (ch, n), dev),
-        _arg(D, "D", f32, (ch,), dev, True), _arg(dt_bias, "dt_bias", f32, (ch,), dev, True),
-        _arg(state, "state", f32, (None, ch, n), dev, True), None,
-        _arg(slots, "slots", torch.int32, (n_seq,), dev, True), None, rows, n_seq,
-        0 if state is None else state.shape[0], ch, cols // n, n, flags)
 
 
 def ssm_scan(u, dt, A, B, C, D, dt_bias, z, y, state, starts, slots=None, resume=None,
@@ -420,66 +336,37 @@ def ssm_scan(u, dt, A, B, C, D, dt_bias, z, y, state, starts, slots=None, resume
     state (lines, channels, states) fp32 or None, starts, slots and resume as for
     conv1d_causal.  workspace: uint8, ssm_workspace_bytes(...) of them, or None (sequences are
     then never cut).  `state` is updated in place.  flags: BF16, SOFTPLUS."""
-    import torch
-
-    if starts is None or starts.dim() != 1 or starts.shape[0] < 1:
-        raise ValueError("starts is not (sequences + 1,)")
-    n_seq = starts.shape[0] - 1
-    op = _ssm(u, dt, A, B, C, D, dt_bias, z, y, state, slots, n_seq, flags, stream)
-    dev = u.get_device()
-    op.starts = _arg(starts, "starts", torch.int32, (None,), dev)
-    op.resume = _arg(resume, "resume", torch.uint8, (n_seq,), dev, True)
-    ws = _arg(workspace, "workspace", torch.uint8, (None,), dev, True)
-    size = 0 if workspace is None else workspace.shape[0]
-    _check(lib().cwg_ssm_scan(ctypes.byref(op), ws, size, _stream(stream)), "cwg_ssm_scan")
+    st = (_torch_ext or _ext()).ssm_scan(u, dt, A, B, C, D, dt_bias, z, y, state, starts, slots,
+                                         resume, workspace, flags, stream)
+    if st:
+        _check(st, "cwg_ssm_scan")
 
 
 def ssm_step(u, dt, A, B, C, D, dt_bias, z, y, state, slots=None, flags: int = 0,
              stream=None) -> None:
     """One token of each sequence: rows are sequences, the rest as for ssm_scan.  `state` is
     updated in place."""
-    if state is None:
-        raise ValueError("state is missing")
-    n = 0 if u is None or u.dim() != 2 else u.shape[0]
-    op = _ssm(u, dt, A, B, C, D, dt_bias, z, y, state, slots, n, flags, stream)
-    _check(lib().cwg_ssm_step(ctypes.byref(op), _stream(stream)), "cwg_ssm_step")
+    st = (_torch_ext or _ext()).ssm_step(u, dt, A, B, C, D, dt_bias, z, y, state, slots, flags,
+                                         stream)
+    if st:
+        _check(st, "cwg_ssm_step")
 
 
 def fp8_quantize(x, q, scale, block_rows: int, flags: int = 0, stream=None) -> None:
     """e4m3 values q (rows, cols) and scales (ceil(rows / block_rows), ceil(cols / 128)) of x
     (rows, cols), per block_rows (1 or 128) x 128 elements.  flags: BF16."""
-    import torch
-
-    dev = _call(x, "x", stream)
-    rows, cols = x.shape
-    if block_rows not in (1, 128):
-        raise ValueError("block_rows is 1 or 128")
-    xp, ldx = _rows(x, "x", _io(flags), rows, cols, dev)
-    qp, ldq = _rows(q, "q", torch.float8_e4m3fn, rows, cols, dev)
-    sp, lds = _rows(scale, "scale", torch.float32, -(-rows // block_rows), -(-cols // 128), dev)
-    _check(lib().cwg_fp8_quantize(xp, ldx, qp, ldq, sp, lds, rows, cols, block_rows, flags,
-                                  _stream(stream)), "cwg_fp8_quantize")
+    st = (_torch_ext or _ext()).fp8_quantize(x, q, scale, block_rows, flags, stream)
+    if st:
+        _check(st, "cwg_fp8_quantize")
 
 
 def fp8_matmul(a, a_scale, w, w_scale, bias, y, flags: int = 0, stream=None) -> None:
     """y (m, n) = a (m, k) w (n, k)^T + bias, a and w e4m3 with the scales that fp8_quantize
     gives them with block_rows 1 and 128; rows of a and w start on 16-byte boundaries.
     flags: BF16 (y), RELU."""
-    import torch
-
-    dev, fp8, f32 = _call(a, "a", stream), torch.float8_e4m3fn, torch.float32
-    m, k = a.shape
-    if w is None or w.dim() != 2:
-        raise ValueError("w is not (n, k)")
-    n, kb = w.shape[0], -(-k // 128)
-    ap, lda = _rows(a, "a", fp8, m, k, dev)
-    wp, ldw = _rows(w, "w", fp8, n, k, dev)
-    asp, ldas = _rows(a_scale, "a_scale", f32, m, kb, dev)
-    wsp, ldws = _rows(w_scale, "w_scale", f32, -(-n // 128), kb, dev)
-    yp, ldy = _rows(y, "y", _io(flags), m, n, dev)
-    _check(lib().cwg_fp8_matmul(ap, lda, asp, ldas, wp, ldw, wsp, ldws,
-                                _arg(bias, "bias", f32, (n,), dev, True), yp, ldy, m, n, k, flags,
-                                _stream(stream)), "cwg_fp8_matmul")
+    st = (_torch_ext or _ext()).fp8_matmul(a, a_scale, w, w_scale, bias, y, flags, stream)
+    if st:
+        _check(st, "cwg_fp8_matmul")
 
 
 # ---- host-pointer per-tile API ----------------------------------------------------

@@ -19,12 +19,17 @@ def silu(v):
     return v * torch.sigmoid(v)
 
 
-def act(v, err, kind):
-    """An activation of values that carry an error, and its error: silu' stays below 1.1;
-    exp (4 u), 1 + e (u), the division (u) and the product rounding make 6 u of the result."""
+def silu_error(v, dtype):
+    """Relative: exp (4 u), 1 + e (u), the division (u); for bf16 results the exponent's two
+    roundings add 2 |v| u, and a reciprocal of 2 u with its product replaces the division."""
+    return (8 + 2 * v.abs() if dtype == torch.bfloat16 else torch.full_like(v, 6)) * U
+
+
+def act(v, err, kind, dtype):
+    """An activation of values that carry an error, and its error: silu' stays below 1.1."""
     if kind == "silu":
         y = silu(v)
-        return y, 1.1 * err + 6 * U * y.abs()
+        return y, 1.1 * err + silu_error(v, dtype) * y.abs()
     if kind == "relu":
         return v.clamp_min(0), err
     return v, err
@@ -46,7 +51,7 @@ def conv1d(x, w, bias, line, kind):
     for j in range(k):
         v += past[j:j + len(x)] * w[:, j]
         size += (past[j:j + len(x)] * w[:, j]).abs()
-    y, err = act(v, k * U * size, kind)
+    y, err = act(v, k * U * size, kind, x.dtype)
     return rounded(y, err, x.dtype), past[len(past) - (k - 1):]
 
 
@@ -58,11 +63,14 @@ def ssm(u, dt, A, B, C, D, dt_bias, z, h, softplus):
     of = torch.arange(ch) // (ch // B.shape[1])
     u, A, B, C = u.to(F64), A.to(F64), B.to(F64), C.to(F64)
     v = dt.to(F64) + (0 if dt_bias is None else dt_bias.to(F64))
-    # dt + bias rounds once; log(1 + exp) is 1-Lipschitz, exp's 4 u of e^v / (1 + e^v) <= step
-    # and log1p's 4 u come on top
+    # dt + bias rounds once (log(1 + exp) is 1-Lipschitz); exp is off by (4 + 2 |v|) u of
+    # itself, which moves log(1 + exp) by no more than that of itself (it is at least e / (1 +
+    # e) times as large where e <= 1); reciprocal, series and sums add 8 u.  The larger of v
+    # and 0 is exact: for v > 0 only log1p(e) <= 0.7 carries these
     if softplus:
         step = torch.nn.functional.softplus(v, threshold=60)
-        dstep = U * v.abs() + 8 * U * step
+        small = torch.nn.functional.softplus(-v.abs(), threshold=60)
+        dstep = U * v.abs() + (12 + 2 * v.abs()) * U * small + U * step
     else:
         step, dstep = v, U * v.abs()
     h = h.to(F64).clone()
@@ -85,7 +93,7 @@ def ssm(u, dt, A, B, C, D, dt_bias, z, h, softplus):
         ey = ey + U * y.abs() + U * (D.to(F64) * u).abs()
     if z is not None:
         g = silu(z.to(F64))
-        y, ey = y * g, ey * g.abs() + 7 * U * (y * g).abs()
+        y, ey = y * g, ey * g.abs() + (U + silu_error(z.to(F64), dtype)) * (y * g).abs()
     return rounded(y, 1.01 * ey, dtype), (h, 1.01 * eh + 1e-37)
 
 

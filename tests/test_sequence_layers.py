@@ -391,3 +391,35 @@ def check_matmul(dev, m, n, k, dtype, relu, with_bias, seed=15):
 ])
 def test_fp8_matmul(cuda_dev, dtype, m, n, k):
     check_matmul(cuda_dev, m, n, k, dtype, relu=(m + n) % 2 == 0, with_bias=m != 16)
+
+
+# ---- the Python mirror's checks ------------------------------------------------------------
+def test_tensors_that_do_not_fit_are_named(cuda_dev):
+    dev = cuda_dev
+    x, y = torch.zeros(4, 64, device=dev), torch.zeros(4, 64, device=dev)
+    w, st = torch.zeros(64, 4, device=dev), torch.zeros(5, 3, 64, device=dev)
+    sl = torch.zeros(4, dtype=torch.int32, device=dev)
+    for bad, what in (
+        (dict(x=x.bfloat16()), "x is BFloat16"), (dict(x=x.t()), "x has strides"),
+        (dict(y=y[:3]), "y has shape"), (dict(y=y.cpu()), "y is not on the call's device"),
+        (dict(y=None), "y is missing"), (dict(w=w.double()), "w is Double"),
+        (dict(y=torch.zeros(4, 128, device=dev)[:, ::2]), "y has strides"),
+        (dict(x=x[:1].expand(4, 64)), "x has strides"), (dict(state=st[:, :2]), "state has shape"),
+        (dict(state=st.transpose(0, 1).contiguous().transpose(0, 1)), "state is not contiguous"),
+        (dict(slots=sl.long()), "slots is Long"), (dict(slots=sl[:2]), "slots has shape"),
+        (dict(bias=w), "bias has shape"), (dict(x=3), "x is not a matrix"),
+    ):
+        a = dict(x=x, w=w, bias=None, y=y, state=st, slots=sl)
+        a.update(bad)
+        with pytest.raises(ValueError, match=what):
+            cwg.conv1d_causal_step(**a)
+    with pytest.raises(AttributeError):
+        cwg.conv1d_causal_step(x, w, None, y, st, sl, 0, "stream")
+    with pytest.raises(cwg.CwgError) as e:
+        cwg.conv1d_causal_step(x, w, None, x, st, sl)
+    assert e.value.status == cwg.EINVAL
+    q = torch.zeros(4, 100, device=dev).to(torch.float8_e4m3fn)
+    s1 = torch.zeros(4, 1, device=dev)
+    with pytest.raises(cwg.CwgError) as e:  # rows that do not start on 16 bytes
+        cwg.fp8_matmul(q, s1, q, s1[:1], None, torch.zeros(4, 4, device=dev))
+    assert e.value.status == cwg.EINVAL
