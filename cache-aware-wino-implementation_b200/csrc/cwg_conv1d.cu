@@ -6,7 +6,7 @@
 // 2K flops and one exponential per element against 4 bytes (bf16) or 8 (fp32) in
 // and out: bound by memory.
 //
-// Prompts: a thread owns one 16-byte vector of channels and a run of consecutive
+// Prompts: a thread owns four channels and a run of consecutive
 // rows, so that a row is read once (plus K - 1 rows of halo per run) and the
 // window slides through registers while the next four rows are loaded.
 // The K - 1 first rows of a sequence, which need the cache line, are all computed
@@ -27,13 +27,6 @@ constexpr int kConvThreads = 128;
 constexpr int kAhead = 4;          // rows per step; the next step's are loaded meanwhile
 constexpr int kStartsInSmem = 1024;
 
-template <typename T, int ACT>
-__device__ __forceinline__ float activate(float v) {
-  if (ACT == CWGK_ACT_RELU) return v < 0.f ? 0.f : v;  // NaN stays
-  if (ACT == CWGK_ACT_SILU) return silu<T>(v);
-  return v;
-}
-
 struct ConvArgs {
   const void *x;
   const float *w, *bias;
@@ -48,51 +41,87 @@ struct ConvArgs {
   int runs;
 };
 
-template <int V, int K>
-__device__ __forceinline__ void load_weights(const ConvArgs &a, int c, bool active,
-                                             float (&w)[V][K], float (&b)[V]) {
+// V channels as pairs (one channel: the second half of its pair is idle).
+template <int V>
+struct Chan {
+  static constexpr int N = (V + 1) / 2;
+  F2 p[N];
+  __device__ __forceinline__ void set(const float (&f)[V]) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    b[v] = active && a.bias ? a.bias[c + v] : 0.f;
-    if (V > 1 && K == 4) {  // 16-byte aligned: the host checked w for the vector path
-      const float4 f = active ? *reinterpret_cast<const float4 *>(a.w + (size_t)(c + v) * K)
-                              : make_float4(0, 0, 0, 0);
-      w[v][0] = f.x;
-      w[v][1] = f.y;
-      w[v][K > 2 ? 2 : 0] = f.z;
-      w[v][K - 1] = f.w;
-    } else {
+    for (int i = 0; i < N; ++i) p[i] = f2(f[2 * i], V > 1 ? f[(2 * i + 1) % V] : 0.f);
+  }
+  __device__ __forceinline__ void get(float (&f)[V]) const {
 #pragma unroll
-      for (int j = 0; j < K; ++j) w[v][j] = active ? a.w[(size_t)(c + v) * K + j] : 0.f;
+    for (int i = 0; i < N; ++i) {
+      const float2 h = halves(p[i]);
+      f[2 * i] = h.x;
+      if (V > 1) f[(2 * i + 1) % V] = h.y;
     }
   }
+  template <typename R>
+  __device__ __forceinline__ void from(R raw) {
+    float f[V];
+    unpack(raw, f);
+    set(f);
+  }
+};
+
+template <int V, int K>
+__device__ __forceinline__ void load_weights(const ConvArgs &a, int c, bool active,
+                                             Chan<V> (&w)[K], Chan<V> &b) {
+  float f[K][V], g[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    g[v] = active && a.bias ? a.bias[c + v] : 0.f;
+    if (V > 1 && K == 4) {  // 16-byte aligned: the host checked w for the vector path
+      const float4 q = active ? *reinterpret_cast<const float4 *>(a.w + (size_t)(c + v) * K)
+                              : make_float4(0, 0, 0, 0);
+      f[0][v] = q.x;
+      f[1][v] = q.y;
+      f[K > 2 ? 2 : 0][v] = q.z;
+      f[K - 1][v] = q.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < K; ++j) f[j][v] = active ? a.w[(size_t)(c + v) * K + j] : 0.f;
+    }
+  }
+  b.set(g);
+#pragma unroll
+  for (int j = 0; j < K; ++j) w[j].set(f[j]);
 }
 
 // act(b + sum_j w[j] h[j]) with h the window's rows, oldest first, x the newest.
 template <typename T, int V, int K, int ACT>
-__device__ __forceinline__ void window_row(const float (&w)[V][K], const float (&b)[V],
-                                           const float (&h)[K - 1][V], const float (&x)[V],
-                                           float (&y)[V]) {
+__device__ __forceinline__ typename Raw<T, V>::type window_row(const Chan<V> (&w)[K],
+                                                               const Chan<V> &b,
+                                                               const Chan<V> (&h)[K - 1],
+                                                               const Chan<V> &x) {
+  Chan<V> s = b;
+#pragma unroll
+  for (int i = 0; i < Chan<V>::N; ++i) {
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) s.p[i] = fma2(w[j].p[i], h[j].p[i], s.p[i]);
+    s.p[i] = fma2(w[K - 1].p[i], x.p[i], s.p[i]);
+    if (ACT == CWGK_ACT_SILU && sizeof(T) == 2) s.p[i] = silu_bf16x2(s.p[i]);
+  }
+  float y[V];
+  s.get(y);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    float s = b[v];
-#pragma unroll
-    for (int j = 0; j < K - 1; ++j) s = fmaf(w[v][j], h[j][v], s);
-    y[v] = activate<T, ACT>(fmaf(w[v][K - 1], x[v], s));
+    if (ACT == CWGK_ACT_RELU && y[v] < 0.f) y[v] = 0.f;  // NaN stays
+    if (ACT == CWGK_ACT_SILU && sizeof(T) == 4) y[v] = silu<float>(y[v]);
   }
+  return pack<T, V>(y);
 }
 template <int V, int K>
-__device__ __forceinline__ void slide(float (&h)[K - 1][V], const float (&x)[V]) {
+__device__ __forceinline__ void slide(Chan<V> (&h)[K - 1], const Chan<V> &x) {
 #pragma unroll
-  for (int j = 0; j < K - 2; ++j)
-#pragma unroll
-    for (int v = 0; v < V; ++v) h[j][v] = h[j + 1][v];
-#pragma unroll
-  for (int v = 0; v < V; ++v) h[K - 2][v] = x[v];
+  for (int j = 0; j < K - 2; ++j) h[j] = h[j + 1];
+  h[K - 2] = x;
 }
 
 template <typename T, int V, int K, int ACT>
-__global__ void __launch_bounds__(kConvThreads, 4) conv1d_prompt(const ConvArgs a) {
+__global__ void __launch_bounds__(kConvThreads) conv1d_prompt(const ConvArgs a) {
   __shared__ int s_starts[kStartsInSmem + 1];
   const T *x = static_cast<const T *>(a.x);
   T *y = static_cast<T *>(a.y);
@@ -112,7 +141,7 @@ __global__ void __launch_bounds__(kConvThreads, 4) conv1d_prompt(const ConvArgs 
   const int t0 = run * a.run;
   const int t1 = min(t0 + a.run, a.tokens);
 
-  float w[V][K], b[V], h[K - 1][V];
+  Chan<V> w[K], b, h[K - 1];
   load_weights<V, K>(a, c, active, w, b);
 
   // Sequences that begin in this run (the first run also has those that begin
@@ -132,24 +161,27 @@ __global__ void __launch_bounds__(kConvThreads, 4) conv1d_prompt(const ConvArgs 
     T *line = state + ((size_t)(slot < 0 ? 0 : slot) * (K - 1)) * a.channels + c;
 #pragma unroll
     for (int j = 0; j < K - 1; ++j)
-      unpack(carry ? load_raw<T, V>(line + (size_t)j * a.channels) : zero_raw<T, V>(), h[j]);
+      h[j].from(carry ? load_raw<T, V>(line + (size_t)j * a.channels) : zero_raw<T, V>());
     const int len = end - begin;
 #pragma unroll
     for (int i = 0; i < K - 1; ++i) {
       if (i < len) {
-        float xv[V], yv[V];
-        unpack(load_raw<T, V>(x + (size_t)(begin + i) * a.ldx + c), xv);
-        window_row<T, V, K, ACT>(w, b, h, xv, yv);
-        store_raw<T, V>(y + (size_t)(begin + i) * a.ldy + c, pack<T, V>(yv));
+        Chan<V> xv;
+        xv.from(load_raw<T, V>(x + (size_t)(begin + i) * a.ldx + c));
+        store_raw<T, V>(y + (size_t)(begin + i) * a.ldy + c,
+                        window_row<T, V, K, ACT>(w, b, h, xv));
         slide<V, K>(h, xv);
       }
     }
     if (slot >= 0) {
 #pragma unroll
-      for (int j = 0; j < K - 1; ++j)
+      for (int j = 0; j < K - 1; ++j) {
+        float f[V];
+        h[j].get(f);
         store_raw<T, V>(line + (size_t)j * a.channels,
                         len >= K - 1 ? load_raw<T, V>(x + (size_t)(end - (K - 1) + j) * a.ldx + c)
-                                     : pack<T, V>(h[j]));
+                                     : pack<T, V>(f));
+      }
     }
   }
   if (bad && lane == 0 && c == 0) atomicOr(&g_seq_status, CWGK_STATUS_INDEX);
@@ -163,8 +195,8 @@ __global__ void __launch_bounds__(kConvThreads, 4) conv1d_prompt(const ConvArgs 
 #pragma unroll
   for (int j = 0; j < K - 1; ++j) {
     const int t = t0 - (K - 1) + j;
-    unpack(t >= 0 && t < a.tokens ? load_raw<T, V>(x + (size_t)t * a.ldx + c) : zero_raw<T, V>(),
-           h[j]);
+    h[j].from(t >= 0 && t < a.tokens ? load_raw<T, V>(x + (size_t)t * a.ldx + c)
+                                     : zero_raw<T, V>());
   }
   typename Raw<T, V>::type raw[kAhead], next[kAhead];
   auto fetch = [&](int t) {
@@ -180,10 +212,9 @@ __global__ void __launch_bounds__(kConvThreads, 4) conv1d_prompt(const ConvArgs 
     if (t - begin >= K - 1 && t + kAhead <= end) {  // all of one sequence, as nearly always
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        float xv[V], yv[V];
-        unpack(raw[i], xv);
-        window_row<T, V, K, ACT>(w, b, h, xv, yv);
-        store_raw<T, V>(y + (size_t)(t + i) * a.ldy + c, pack<T, V>(yv));
+        Chan<V> xv;
+        xv.from(raw[i]);
+        store_raw<T, V>(y + (size_t)(t + i) * a.ldy + c, window_row<T, V, K, ACT>(w, b, h, xv));
         slide<V, K>(h, xv);
       }
       continue;
@@ -197,21 +228,18 @@ __global__ void __launch_bounds__(kConvThreads, 4) conv1d_prompt(const ConvArgs 
         end = starts[s + 1];
         if (begin < 0 || end > a.tokens) end = begin = 0;
       }
-      float xv[V];
-      unpack(i == 0 ? raw[0] : i == 1 ? raw[1] : i == 2 ? raw[2] : raw[3], xv);
-      if (t + i < end && t + i - begin >= K - 1) {
-        float yv[V];
-        window_row<T, V, K, ACT>(w, b, h, xv, yv);
-        store_raw<T, V>(y + (size_t)(t + i) * a.ldy + c, pack<T, V>(yv));
-      }
+      Chan<V> xv;
+      xv.from(i == 0 ? raw[0] : i == 1 ? raw[1] : i == 2 ? raw[2] : raw[3]);
+      if (t + i < end && t + i - begin >= K - 1)
+        store_raw<T, V>(y + (size_t)(t + i) * a.ldy + c, window_row<T, V, K, ACT>(w, b, h, xv));
       slide<V, K>(h, xv);
     }
   }
 }
 
-// One token of each sequence: a thread owns a vector of channels and `run` rows,
-// which share the weights; per row K vectors in and K out (x and the line, y and
-// the line moved by one).
+// One token of each sequence: a thread owns a vector of channels of one row; K vectors
+// in (x and the line) and K out (y and the line moved by one).  The loads are issued
+// before the search for an earlier row with the same line.
 template <typename T, int V, int K, int ACT>
 __global__ void __launch_bounds__(kConvThreads) conv1d_step(const ConvArgs a) {
   const T *x = static_cast<const T *>(a.x);
@@ -219,39 +247,42 @@ __global__ void __launch_bounds__(kConvThreads) conv1d_step(const ConvArgs a) {
   T *state = static_cast<T *>(a.state);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cb = blockIdx.x % a.cblocks;
-  const int run = (blockIdx.x / a.cblocks) * (4 / a.wc) + warp / a.wc;
-  if (run >= a.runs) return;
+  const int r = (blockIdx.x / a.cblocks) * (4 / a.wc) + warp / a.wc;
+  if (r >= a.runs) return;
   const int c = ((cb * a.wc + warp % a.wc) * 32 + lane) * V;
   const bool active = c < a.channels;
-  float w[V][K], b[V];
+  int slot = a.slots ? a.slots[r] : r;
+  bool bad = slot >= a.n_slots;
+  if (bad) slot = -1;
+  T *line = state + ((size_t)(slot < 0 ? 0 : slot) * (K - 1)) * a.channels + c;
+  typename Raw<T, V>::type raw[K];
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j)
+    raw[j] = slot >= 0 && active ? load_raw<T, V>(line + (size_t)j * a.channels)
+                                 : zero_raw<T, V>();
+  raw[K - 1] = active ? load_raw<T, V>(x + (size_t)r * a.ldx + c) : zero_raw<T, V>();
+  Chan<V> w[K], b, h[K - 1], xv;
   load_weights<V, K>(a, c, active, w, b);
-  bool bad = false;
-  const int r1 = min((run + 1) * a.run, a.n_seq);
-  for (int r = run * a.run; r < r1; ++r) {
-    const int slot = line_of(a.slots, r, a.n_slots, bad);
-    if (!active) continue;
-    T *line = state + ((size_t)(slot < 0 ? 0 : slot) * (K - 1)) * a.channels + c;
-    typename Raw<T, V>::type raw[K];
+  if (slot >= 0 && a.slots && taken_before(a.slots, r, slot)) {
+    slot = -1;
+    bad = true;
 #pragma unroll
-    for (int j = 0; j < K - 1; ++j)
-      raw[j] = slot >= 0 ? load_raw<T, V>(line + (size_t)j * a.channels) : zero_raw<T, V>();
-    raw[K - 1] = load_raw<T, V>(x + (size_t)r * a.ldx + c);
-    float h[K - 1][V], xv[V], yv[V];
-#pragma unroll
-    for (int j = 0; j < K - 1; ++j) unpack(raw[j], h[j]);
-    unpack(raw[K - 1], xv);
-    window_row<T, V, K, ACT>(w, b, h, xv, yv);
-    store_raw<T, V>(y + (size_t)r * a.ldy + c, pack<T, V>(yv));
-    if (slot >= 0) {
-#pragma unroll
-      for (int j = 0; j < K - 1; ++j)
-        store_raw<T, V>(line + (size_t)j * a.channels, raw[j + 1]);
-    }
+    for (int j = 0; j < K - 1; ++j) raw[j] = zero_raw<T, V>();
   }
   if (bad && lane == 0 && c == 0) atomicOr(&g_seq_status, CWGK_STATUS_INDEX);
+  if (!active) return;
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j) h[j].from(raw[j]);
+  xv.from(raw[K - 1]);
+  store_raw<T, V>(y + (size_t)r * a.ldy + c, window_row<T, V, K, ACT>(w, b, h, xv));
+  if (slot >= 0) {
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j)
+      store_raw<T, V>(line + (size_t)j * a.channels, raw[j + 1]);
+  }
 }
 
-static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+static bool aligned(const void *p, size_t n) { return (uintptr_t)p % n == 0; }
 
 template <typename T, int V, int K, int ACT>
 static int launch_conv1d(const cwgk_conv1d *op, bool step, cudaStream_t stream) {
@@ -310,10 +341,11 @@ static int conv1d_width(const cwgk_conv1d *op, bool step, cudaStream_t s) {
 }
 template <typename T>
 static int conv1d(const cwgk_conv1d *op, bool step, cudaStream_t s) {
-  constexpr int V = 16 / (int)sizeof(T);
+  constexpr int V = 4;  // 8 or 16 bytes: with 8 bf16 channels a thread needs 128 registers
   const bool one = (step ? op->n_seq : op->tokens) <= 1;  // no second row: ld says nothing
-  const bool vec = op->channels % V == 0 && aligned16(op->x) && aligned16(op->y) &&
-                   aligned16(op->state) && aligned16(op->w) &&
+  constexpr size_t B = V * sizeof(T);
+  const bool vec = op->channels % V == 0 && aligned(op->x, B) && aligned(op->y, B) &&
+                   aligned(op->state, B) && aligned(op->w, 16) &&
                    (one || (op->ldx % V == 0 && op->ldy % V == 0));
   return vec ? conv1d_width<T, V>(op, step, s) : conv1d_width<T, 1>(op, step, s);
 }

@@ -39,12 +39,28 @@ __device__ __forceinline__ float scale_of(uint32_t amax) {
   const float s = __fdiv_rn(__uint_as_float(amax), kE4m3Max);
   return s < kScaleMin ? kScaleMin : s;  // NaN stays
 }
-__device__ __forceinline__ uint32_t e4m3x4(const float *v, float s) {
-  const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(
-      make_float2(__fdiv_rn(v[0], s), __fdiv_rn(v[1], s)), __NV_SATFINITE, __NV_E4M3);
-  const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(
-      make_float2(__fdiv_rn(v[2], s), __fdiv_rn(v[3], s)), __NV_SATFINITE, __NV_E4M3);
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  const __nv_fp8x2_storage_t lo =
+      __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const __nv_fp8x2_storage_t hi =
+      __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
   return (uint32_t)lo | (uint32_t)hi << 16;
+}
+// Codes of v / s without a division per element.  t = v r with r = 1 / s rounded is off
+// the quotient by at most 2^-23 of it, so the rounded quotient lies between
+// t (1 - 2^-22) and t (1 + 2^-22), themselves rounded; rounding to e4m3 is monotone, so
+// where both ends have the same code that is the quotient's.  Otherwise (about one in
+// 2^17 values) the division decides.
+__device__ __forceinline__ uint32_t codes4(const float *v, float s, float r) {
+  using namespace seq;
+  const F2 rr = f2(r, r), down = f2(1.f - 0x1p-22f, 1.f - 0x1p-22f),
+           up = f2(1.f + 0x1p-22f, 1.f + 0x1p-22f);
+  const F2 t0 = mul2(f2(v[0], v[1]), rr), t1 = mul2(f2(v[2], v[3]), rr);
+  const float2 a = halves(mul2(t0, down)), b = halves(mul2(t1, down));
+  const float2 c = halves(mul2(t0, up)), d = halves(mul2(t1, up));
+  const uint32_t q = e4m3x4(a.x, a.y, b.x, b.y);
+  if (q == e4m3x4(c.x, c.y, d.x, d.y)) return q;
+  return e4m3x4(__fdiv_rn(v[0], s), __fdiv_rn(v[1], s), __fdiv_rn(v[2], s), __fdiv_rn(v[3], s));
 }
 
 struct QuantArgs {
@@ -75,7 +91,8 @@ __device__ __forceinline__ void load8(const T *p, int n, float (&v)[8]) {
 }
 template <bool VEC>
 __device__ __forceinline__ void store8(uint8_t *q, const float (&v)[8], float s, int n) {
-  const uint32_t a = e4m3x4(v, s), b = e4m3x4(v + 4, s);
+  const float r = __frcp_rn(s);
+  const uint32_t a = codes4(v, s, r), b = codes4(v + 4, s, r);
   if (VEC && n >= 8) {
     *reinterpret_cast<uint2 *>(q) = make_uint2(a, b);
   } else {
@@ -90,16 +107,16 @@ __device__ __forceinline__ void store8(uint8_t *q, const float (&v)[8], float s,
 constexpr int kRowGroups = 4;
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quantize_rows(const QuantArgs a) {
-  const long long first = (long long)blockIdx.x * (16 * kRowGroups) + (threadIdx.x >> 4);
+  const unsigned first = blockIdx.x * (16 * kRowGroups) + (threadIdx.x >> 4);
   const int lane = threadIdx.x & 15;
   float v[kRowGroups][8];
   int row[kRowGroups], kb[kRowGroups], n[kRowGroups];
 #pragma unroll
   for (int k = 0; k < kRowGroups; ++k) {
-    const long long g = first + k * 16;
-    row[k] = (int)(g / a.kblocks);
-    kb[k] = (int)(g - (long long)row[k] * a.kblocks);
-    n[k] = g < a.groups ? a.cols - (kb[k] * 128 + lane * 8) : 0;
+    const unsigned g = first + k * 16;
+    row[k] = (int)(g / (unsigned)a.kblocks);
+    kb[k] = (int)(g % (unsigned)a.kblocks);
+    n[k] = g < (unsigned)a.groups ? a.cols - (kb[k] * 128 + lane * 8) : 0;
     load8<T, VEC>(static_cast<const T *>(a.x) + (n[k] > 0 ? (size_t)row[k] * a.ldx : 0) +
                       kb[k] * 128 + lane * 8,
                   n[k], v[k]);
@@ -158,7 +175,7 @@ static int quantize(QuantArgs a, int block_rows, cudaStream_t s) {
   const bool vec = ((uintptr_t)a.x & 15) == 0 && ((uintptr_t)a.q & 7) == 0 &&
                    a.cols % E == 0 && (one || (a.ldx % E == 0 && a.ldq % 8 == 0));
   const long long blocks = block_rows == 1 ? (a.groups + 16 * kRowGroups - 1) / (16 * kRowGroups) : a.groups;
-  if (blocks > 0x7fffffffLL) return -2;
+  if (a.groups > 0x7fffffffLL - 16 * kRowGroups) return -2;  // 32-bit group numbers
   if (block_rows == 1) {
     if (vec)
       quantize_rows<T, true><<<(unsigned)blocks, 256, 0, s>>>(a);

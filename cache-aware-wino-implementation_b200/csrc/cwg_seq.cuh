@@ -10,11 +10,15 @@
 namespace cwg {
 namespace seq {
 
-// V elements of T, moved as one 16-byte vector (or one element, V = 1).
+// V elements of T, moved as one 16-byte vector (or 8 bytes, or one element, V = 1).
 template <typename T, int V>
 struct Raw {
-  static_assert(V == 1 || V * sizeof(T) == 16, "one element or one 16-byte vector");
+  static_assert(V * sizeof(T) == 16, "one element, 8 bytes or 16 bytes");
   using type = uint4;
+};
+template <>
+struct Raw<__nv_bfloat16, 4> {
+  using type = uint2;
 };
 template <>
 struct Raw<float, 1> {
@@ -37,6 +41,8 @@ template <typename T, int V>
 __device__ __forceinline__ typename Raw<T, V>::type zero_raw() {
   if constexpr (V == 1)
     return from_f32<T>(0.f);
+  else if constexpr (V * sizeof(T) == 8)
+    return make_uint2(0, 0);
   else
     return make_uint4(0, 0, 0, 0);
 }
@@ -48,6 +54,12 @@ __device__ __forceinline__ void unpack(uint4 v, float (&f)[4]) {
   f[1] = __uint_as_float(v.y);
   f[2] = __uint_as_float(v.z);
   f[3] = __uint_as_float(v.w);
+}
+__device__ __forceinline__ void unpack(uint2 v, float (&f)[4]) {
+  f[0] = __uint_as_float(v.x << 16);
+  f[1] = __uint_as_float(v.x & 0xFFFF0000u);
+  f[2] = __uint_as_float(v.y << 16);
+  f[3] = __uint_as_float(v.y & 0xFFFF0000u);
 }
 __device__ __forceinline__ void unpack(uint4 v, float (&f)[8]) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -66,6 +78,11 @@ template <typename T, int V>
 __device__ __forceinline__ typename Raw<T, V>::type pack(const float (&f)[V]) {
   if constexpr (V == 1) {
     return from_f32<T>(f[0]);
+  } else if constexpr (V * sizeof(T) == 8) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(f[0], f[1]);
+    const __nv_bfloat162 b = __floats2bfloat162_rn(f[2], f[3]);
+    return make_uint2(*reinterpret_cast<const uint32_t *>(&a),
+                      *reinterpret_cast<const uint32_t *>(&b));
   } else if constexpr (V == 4) {
     return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
                       __float_as_uint(f[3]));
@@ -78,6 +95,37 @@ __device__ __forceinline__ typename Raw<T, V>::type pack(const float (&f)[V]) {
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
+}
+
+// Two fp32 values in one 64-bit register: one instruction works on both, each half
+// rounded as the scalar instruction rounds.
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 halves(F2 p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
 }
 
 __device__ __forceinline__ float ex2(float v) {
@@ -103,6 +151,12 @@ __device__ __forceinline__ float silu(float v) {
     return v / (1.f + expf(-v));
   else
     return v * rcp(1.f + ex2(-kLog2e * v));
+}
+
+__device__ __forceinline__ F2 silu_bf16x2(F2 v) {
+  const float2 t = halves(mul2(v, f2(-kLog2e, -kLog2e)));
+  const float2 e = halves(add2(f2(ex2(t.x), ex2(t.y)), f2(1.f, 1.f)));
+  return mul2(v, f2(rcp(e.x), rcp(e.y)));
 }
 
 // log(1 + exp(v)) = max(v, 0) + log1p(e) with e = exp(-|v|) <= 1, and the series
@@ -145,7 +199,13 @@ __device__ __forceinline__ int lower_bound(const int *s, int n, int v) {
 // together, and all of them get the answer.
 __device__ __forceinline__ bool taken_before(const int *slots, int b, int slot) {
   bool hit = false;
-  for (int i = (int)(threadIdx.x & 31); i < b; i += 32) hit |= slots[i] == slot;
+  for (int i0 = (int)(threadIdx.x & 31); i0 < b; i0 += 128) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {  // four loads in flight
+      const int i = i0 + 32 * k;
+      hit |= i < b && slots[i] == slot;
+    }
+  }
   return __any_sync(0xffffffffu, hit) != 0;
 }
 

@@ -27,6 +27,7 @@ struct Args {
   int per;      // channels per group
   int cblocks;  // CTAs along one group's channels
   bool vec_state, vec_a;  // the state's and A's rows are whole 16-byte vectors
+  bool vec_bc;            // B and C can be read four states at a time
 };
 
 // A lane's four states of one cache line, or zeros.
@@ -236,10 +237,26 @@ __global__ void __launch_bounds__(Geo<L>::kThreads) ssm_prompt(const Args a) {
 // ---- one token of each sequence ----------------------------------------------------
 // Bound by the states, 8 N bytes per channel in and out.  A CTA takes RR rows of one
 // channel block: the rows share A, and all their states are loaded before the first is
-// used.  Which lines may be written is found out meanwhile.
+// used.  Meanwhile the CTA's threads look together for lines that an earlier row has too.
+template <typename T>
+__device__ __forceinline__ void load4(const T *p, int i0, int n, bool vec, float (&f)[4]) {
+  if (vec) {
+    if constexpr (sizeof(T) == 4) {
+      unpack(*reinterpret_cast<const uint4 *>(p + i0), f);
+    } else {
+      const uint2 v = *reinterpret_cast<const uint2 *>(p + i0);
+      f[0] = __uint_as_float(v.x << 16), f[1] = __uint_as_float(v.x & 0xFFFF0000u);
+      f[2] = __uint_as_float(v.y << 16), f[3] = __uint_as_float(v.y & 0xFFFF0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = i0 + i < n ? to_f32(p[i0 + i]) : 0.f;
+  }
+}
+
 template <typename T, int L, int RR>
 __global__ void __launch_bounds__(Geo<L>::kThreads) ssm_token(const Args a) {
-  constexpr int CH = Geo<L>::kCH;
+  constexpr int CH = Geo<L>::kCH, NT = Geo<L>::kThreads;
   const cwg_ssm &p = a.p;
   const int tid = threadIdx.x;
   const int cblk = blockIdx.x % a.cblocks;
@@ -248,63 +265,100 @@ __global__ void __launch_bounds__(Geo<L>::kThreads) ssm_token(const Args a) {
   const int ch = tid / L, l = tid % L, i0 = l * kS;
   const int in = cblk * CH + ch, c = group * a.per + in;
   const bool mine = in < a.per;
-  float h[RR][kS], bv[RR][kS], cv[RR][kS], u[RR], d[RR], z[RR];
-  float *line[RR];
+  const size_t width = (size_t)p.channels * p.states, at = (size_t)c * p.states;
+  // Rows r0 + l, r0 + l + L, ... of the channel are lane l's: it computes their steps and
+  // finishes their outputs (with more lanes than rows, lane l takes row l % RR too, which
+  // only lane l = row stores).
+  constexpr int E = L < RR ? RR / L : 1;
+  float h[RR][kS], u[E], d[E], z[E];
+  int slot[RR];
+  bool bad = false;
 #pragma unroll
   for (int k = 0; k < RR; ++k) {
     const int r = r0 + k;
-    const bool row = r < p.tokens;
-    const int slot = !row ? -1 : p.slots ? p.slots[r] : r;
-    const bool in_range = slot >= 0 && slot < p.n_slots;
-    line[k] = in_range && mine ? p.state + ((size_t)slot * p.channels + c) * p.states : nullptr;
+    slot[k] = r >= p.tokens ? -1 : p.slots ? p.slots[r] : r;
+    if (slot[k] >= p.n_slots) slot[k] = -1, bad = true;
+  }
+#pragma unroll
+  for (int k = 0; k < RR; ++k) {
 #pragma unroll
     for (int i = 0; i < kS; ++i) h[k][i] = 0.f;
-    if (line[k]) load_states(line[k], i0, p.states, a.vec_state, h[k]);
-    const size_t at = (size_t)(row ? r : 0);
-    u[k] = d[k] = z[k] = 0.f;
-    if (mine && row) {
-      u[k] = to_f32(static_cast<const T *>(p.u)[at * p.ldu + c]);
-      d[k] = to_f32(static_cast<const T *>(p.dt)[at * p.lddt + c]);
-      if (p.z) z[k] = to_f32(static_cast<const T *>(p.z)[at * p.ldz + c]);
-    }
+    if (mine && slot[k] >= 0)
+      load_states(p.state + (size_t)slot[k] * width + at, i0, p.states, a.vec_state, h[k]);
+  }
 #pragma unroll
-    for (int i = 0; i < kS; ++i) {
-      const bool ok = row && i0 + i < p.states;
-      const size_t col = (size_t)group * p.states + i0 + i;
-      bv[k][i] = ok ? to_f32(static_cast<const T *>(p.B)[at * p.ldb + col]) : 0.f;
-      cv[k][i] = ok ? to_f32(static_cast<const T *>(p.C)[at * p.ldc + col]) : 0.f;
+  for (int e = 0; e < E; ++e) {
+    const int r = r0 + (L < RR ? e * L + l : l % RR);
+    const size_t rr = (size_t)(r < p.tokens ? r : 0);
+    u[e] = d[e] = z[e] = 0.f;
+    if (mine) {
+      u[e] = to_f32(static_cast<const T *>(p.u)[rr * p.ldu + c]);
+      d[e] = to_f32(static_cast<const T *>(p.dt)[rr * p.lddt + c]);
+      if (p.z) z[e] = to_f32(static_cast<const T *>(p.z)[rr * p.ldz + c]);
     }
   }
   float A2[kS] = {0.f, 0.f, 0.f, 0.f};
-  if (mine) load_states(p.A + (size_t)c * p.states, i0, p.states, a.vec_a, A2);
+  if (mine) load_states(p.A + at, i0, p.states, a.vec_a, A2);
 #pragma unroll
   for (int i = 0; i < kS; ++i) A2[i] *= kLog2e;
   const float bias = mine && p.dt_bias ? p.dt_bias[c] : 0.f;
   const float skip = mine && p.D ? p.D[c] : 0.f;
-  bool bad = false;
+  if (p.slots) {
+    int taken = 0;
+    for (int i = tid; i < r0 + RR - 1 && i < p.tokens; i += NT) {
+      const int other = p.slots[i];
+#pragma unroll
+      for (int k = 0; k < RR; ++k) taken |= (i < r0 + k && other == slot[k]) << k;
+    }
+    if (__syncthreads_or(taken)) {
+#pragma unroll
+      for (int k = 0; k < RR; ++k)
+        if (__syncthreads_or(taken & (1 << k)) && slot[k] >= 0) {
+          slot[k] = -1;
+          bad = true;
+#pragma unroll
+          for (int i = 0; i < kS; ++i) h[k][i] = 0.f;
+        }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    d[e] += bias;
+    if (p.flags & CWG_SOFTPLUS) d[e] = softplus(d[e]);
+    z[e] = p.z ? silu<T>(z[e]) : 1.f;
+  }
+  const T *Brow = static_cast<const T *>(p.B) + (size_t)r0 * p.ldb + (size_t)group * p.states;
+  const T *Crow = static_cast<const T *>(p.C) + (size_t)r0 * p.ldc + (size_t)group * p.states;
+  float out[E] = {};
 #pragma unroll
   for (int k = 0; k < RR; ++k) {
-    if (r0 + k >= p.tokens) break;
-    if (line_of(p.slots, r0 + k, p.n_slots, bad) < 0) {  // a line given twice counts as none
-      line[k] = nullptr;
-#pragma unroll
-      for (int i = 0; i < kS; ++i) h[k][i] = 0.f;
-    }
-    float step = d[k] + bias;
-    if (p.flags & CWG_SOFTPLUS) step = softplus(step);
-    const float du = step * u[k];
+    if (RR > 1 && r0 + k >= p.tokens) break;
+    // lane and piece that hold row k's step
+    constexpr unsigned kAll = 0xffffffffu;
+    const int from = L < RR ? k % L : k, e = L < RR ? k / L : 0;
+    const float step = L > 1 && RR > 1 ? __shfl_sync(kAll, d[e], from, L) : d[e];
+    const float uk = L > 1 && RR > 1 ? __shfl_sync(kAll, u[e], from, L) : u[e];
+    float bv[4], cv[4];
+    load4(Brow + (size_t)k * p.ldb, i0, p.states, a.vec_bc, bv);
+    load4(Crow + (size_t)k * p.ldc, i0, p.states, a.vec_bc, cv);
+    const float du = step * uk;
     float y = 0.f;
 #pragma unroll
     for (int i = 0; i < kS; ++i) {
-      h[k][i] = fmaf(ex2(step * A2[i]), h[k][i], du * bv[k][i]);
-      y = fmaf(h[k][i], cv[k][i], y);
+      h[k][i] = fmaf(ex2(step * A2[i]), h[k][i], du * bv[i]);
+      y = fmaf(h[k][i], cv[i], y);
     }
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-    if (line[k]) store_states(line[k], i0, p.states, a.vec_state, h[k]);
-    if (mine && l == 0) {
-      y = fmaf(skip, u[k], y);
-      if (p.z) y *= silu<T>(z[k]);
+    for (int o = L / 2; o > 0; o >>= 1) y += __shfl_xor_sync(kAll, y, o);
+    if (mine && slot[k] >= 0)
+      store_states(p.state + (size_t)slot[k] * width + at, i0, p.states, a.vec_state, h[k]);
+    if (l == from || RR == 1) out[e] = y;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int k = L < RR ? e * L + l : l;
+    if (mine && k < RR && r0 + k < p.tokens) {
+      const float y = fmaf(skip, u[e], out[e]) * z[e];
       static_cast<T *>(p.y)[(size_t)(r0 + k) * p.ldy + c] = pack1<T>(y);
     }
   }
@@ -333,6 +387,8 @@ static int launch(const cwg_ssm *op, bool step, cudaStream_t s) {
   a.cblocks = (a.per + G::kCH - 1) / G::kCH;
   a.vec_state = op->states == G::kNP && aligned16(op->state);
   a.vec_a = op->states == G::kNP && aligned16(op->A);
+  a.vec_bc = op->states == G::kNP && ((uintptr_t)op->B % (4 * sizeof(T))) == 0 &&
+             ((uintptr_t)op->C % (4 * sizeof(T))) == 0 && a.p.ldb % 4 == 0 && a.p.ldc % 4 == 0;
   const long long blocks = (long long)op->n_seq * a.cblocks * op->groups;
   const long long step_blocks = (long long)op->tokens * a.cblocks * op->groups;
   if ((step ? step_blocks : blocks) > 0x7fffffffLL) return -2;
