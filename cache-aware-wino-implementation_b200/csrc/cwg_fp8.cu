@@ -33,8 +33,6 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 constexpr float kE4m3Max = 448.f;
 constexpr float kScaleMin = 1.17549435e-38f;  // 2^-126
 
-// max |x| by its bits: NaN is larger than infinity, infinity than any number
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 __device__ __forceinline__ float scale_of(uint32_t amax) {
   const float s = __fdiv_rn(__uint_as_float(amax), kE4m3Max);
   return s < kScaleMin ? kScaleMin : s;  // NaN stays
@@ -72,99 +70,110 @@ struct QuantArgs {
   long long groups;
 };
 
-// 8 consecutive elements of a row (zeros past the end), and their codes back.
+// 8 consecutive elements of a row, zeros past the end, as they are in memory.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T *p, int n, float (&v)[8]) {
-  if constexpr (VEC) {
-    constexpr int E = 16 / (int)sizeof(T);
+struct Eight {
+  static constexpr int E = VEC ? 16 / (int)sizeof(T) : 1;
+  typename seq::Raw<T, E>::type raw[8 / E];
+  __device__ __forceinline__ void load(const T *p, int n) {
+#pragma unroll
+    for (int i = 0; i < 8; i += E)  // VEC: cols is a multiple of E
+      raw[i / E] = i < n ? seq::load_raw<T, E>(p + i) : seq::zero_raw<T, E>();
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
 #pragma unroll
     for (int i = 0; i < 8; i += E) {
       float f[E];
-      seq::unpack(i < n ? seq::load_raw<T, E>(p + i) : seq::zero_raw<T, E>(), f);
+      seq::unpack(raw[i / E], f);
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[i + e] = i + e < n ? f[e] : 0.f;
+      for (int e = 0; e < E; ++e) v[i + e] = f[e];
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.f;
   }
-}
-template <bool VEC>
-__device__ __forceinline__ void store8(uint8_t *q, const float (&v)[8], float s, int n) {
-  const float r = __frcp_rn(s);
-  const uint32_t a = codes4(v, s, r), b = codes4(v + 4, s, r);
-  if (VEC && n >= 8) {
-    *reinterpret_cast<uint2 *>(q) = make_uint2(a, b);
-  } else {
+  // Largest magnitude, by its bits: NaN is above infinity, infinity above any number.
+  __device__ __forceinline__ uint32_t amax() const {
+    if constexpr (VEC && sizeof(T) == 2) {
+      const uint32_t k = 0x7fff7fffu;
+      const uint32_t m = __vmaxu2(__vmaxu2(raw[0].x & k, raw[0].y & k),
+                                  __vmaxu2(raw[0].z & k, raw[0].w & k));
+      return max(m << 16, m & 0xffff0000u);
+    } else {
+      float v[8];
+      get(v);
+      uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) q[i] = (uint8_t)((i < 4 ? a >> 8 * i : b >> 8 * (i - 4)) & 0xff);
+      for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+      return m;
+    }
   }
-}
+  __device__ __forceinline__ void store(uint8_t *q, float s, float r, int n) const {
+    float v[8];
+    get(v);
+    const uint32_t a = codes4(v, s, r), b = codes4(v + 4, s, r);
+    if (VEC && n >= 8) {
+      *reinterpret_cast<uint2 *>(q) = make_uint2(a, b);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < n) q[i] = (uint8_t)((i < 4 ? a >> 8 * i : b >> 8 * (i - 4)) & 0xff);
+    }
+  }
+};
 
-// A half-warp per group of 1 x 128, 8 elements a lane; it takes kRowGroups groups, whose
-// loads are all in flight before the first is used.
-constexpr int kRowGroups = 4;
+// Four lanes per group of 1 x 128, 32 elements a lane, all loaded before the first is
+// used; per group one division, one reciprocal and one index division then serve 32
+// elements of each lane.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quantize_rows(const QuantArgs a) {
-  const unsigned first = blockIdx.x * (16 * kRowGroups) + (threadIdx.x >> 4);
-  const int lane = threadIdx.x & 15;
-  float v[kRowGroups][8];
-  int row[kRowGroups], kb[kRowGroups], n[kRowGroups];
+  const unsigned g = blockIdx.x * 64 + (threadIdx.x >> 2);
+  const int lane = threadIdx.x & 3;
+  const bool ok = g < (unsigned)a.groups;
+  const int row = ok ? (int)(g / (unsigned)a.kblocks) : 0;
+  const int kb = ok ? (int)g - row * a.kblocks : 0;
+  const int c = kb * 128 + lane * 8, n = ok ? a.cols - c : 0;
+  const T *x = static_cast<const T *>(a.x) + (size_t)row * a.ldx + c;
+  Eight<T, VEC> v[4];
 #pragma unroll
-  for (int k = 0; k < kRowGroups; ++k) {
-    const unsigned g = first + k * 16;
-    row[k] = (int)(g / (unsigned)a.kblocks);
-    kb[k] = (int)(g % (unsigned)a.kblocks);
-    n[k] = g < (unsigned)a.groups ? a.cols - (kb[k] * 128 + lane * 8) : 0;
-    load8<T, VEC>(static_cast<const T *>(a.x) + (n[k] > 0 ? (size_t)row[k] * a.ldx : 0) +
-                      kb[k] * 128 + lane * 8,
-                  n[k], v[k]);
-  }
-#pragma unroll
-  for (int k = 0; k < kRowGroups; ++k) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[k][i]));
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float s = scale_of(m);
-    if (n[k] > 0) {
-      if (lane == 0) a.scale[(size_t)row[k] * a.lds + kb[k]] = s;
-      store8<VEC>(a.q + (size_t)row[k] * a.ldq + kb[k] * 128 + lane * 8, v[k], s, n[k]);
-    }
-  }
-}
-
-// One CTA per block of 128 x 128, 64 elements a thread held in registers.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) quantize_blocks(const QuantArgs a) {
-  __shared__ uint32_t s_max[8];
-  const int kb = blockIdx.x % a.kblocks, rb = blockIdx.x / a.kblocks;
-  const int c = kb * 128 + (threadIdx.x & 15) * 8, r0 = rb * 128 + (threadIdx.x >> 4);
-  float v[8][8];
+  for (int k = 0; k < 4; ++k) v[k].load(x + k * 32, n - k * 32);
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = r0 + i * 16;
-    const int n = r < a.rows ? a.cols - c : 0;
-    load8<T, VEC>(static_cast<const T *>(a.x) + (size_t)(r < a.rows ? r : 0) * a.ldx + c, n,
-                  v[i]);
+  for (int k = 0; k < 4; ++k) m = max(m, v[k].amax());
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  const float s = scale_of(m), r = __frcp_rn(s);
+  if (ok && lane == 0) a.scale[(size_t)row * a.lds + kb] = s;
+  uint8_t *q = a.q + (size_t)row * a.ldq + c;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) m = max(m, abs_bits(v[i][e]));
+  for (int k = 0; k < 4; ++k)
+    if (n > k * 32) v[k].store(q + k * 32, s, r, n - k * 32);
+}
+
+// One CTA per block of 128 x 128, 32 elements a thread held in registers.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(512) quantize_blocks(const QuantArgs a) {
+  __shared__ uint32_t s_max[16];
+  const int kb = blockIdx.x % a.kblocks, rb = blockIdx.x / a.kblocks;
+  const int c = kb * 128 + (threadIdx.x & 15) * 8, r0 = rb * 128 + (threadIdx.x >> 4);
+  Eight<T, VEC> v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = r0 + i * 32;
+    v[i].load(static_cast<const T *>(a.x) + (size_t)(r < a.rows ? r : 0) * a.ldx + c,
+              r < a.rows ? a.cols - c : 0);
   }
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = max(m, v[i].amax());
   m = __reduce_max_sync(0xffffffffu, m);
   if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, s_max[i]);
-  const float s = scale_of(m);
+  for (int i = 0; i < 16; ++i) m = max(m, s_max[i]);
+  const float s = scale_of(m), r = __frcp_rn(s);
   if (threadIdx.x == 0) a.scale[(size_t)rb * a.lds + kb] = s;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = r0 + i * 16;
-    if (r < a.rows && c < a.cols) store8<VEC>(a.q + (size_t)r * a.ldq + c, v[i], s, a.cols - c);
-  }
+  for (int i = 0; i < 4; ++i)
+    if (r0 + i * 32 < a.rows && c < a.cols)
+      v[i].store(a.q + (size_t)(r0 + i * 32) * a.ldq + c, s, r, a.cols - c);
 }
 
 template <typename T>
@@ -174,8 +183,8 @@ static int quantize(QuantArgs a, int block_rows, cudaStream_t s) {
   // a whole vector at a row's end may reach past cols only if the row does
   const bool vec = ((uintptr_t)a.x & 15) == 0 && ((uintptr_t)a.q & 7) == 0 &&
                    a.cols % E == 0 && (one || (a.ldx % E == 0 && a.ldq % 8 == 0));
-  const long long blocks = block_rows == 1 ? (a.groups + 16 * kRowGroups - 1) / (16 * kRowGroups) : a.groups;
-  if (a.groups > 0x7fffffffLL - 16 * kRowGroups) return -2;  // 32-bit group numbers
+  const long long blocks = block_rows == 1 ? (a.groups + 63) / 64 : a.groups;
+  if (a.groups > 0x7fffffffLL - 64) return -2;  // 32-bit group numbers
   if (block_rows == 1) {
     if (vec)
       quantize_rows<T, true><<<(unsigned)blocks, 256, 0, s>>>(a);
@@ -183,9 +192,9 @@ static int quantize(QuantArgs a, int block_rows, cudaStream_t s) {
       quantize_rows<T, false><<<(unsigned)blocks, 256, 0, s>>>(a);
   } else {
     if (vec)
-      quantize_blocks<T, true><<<(unsigned)blocks, 256, 0, s>>>(a);
+      quantize_blocks<T, true><<<(unsigned)blocks, 512, 0, s>>>(a);
     else
-      quantize_blocks<T, false><<<(unsigned)blocks, 256, 0, s>>>(a);
+      quantize_blocks<T, false><<<(unsigned)blocks, 512, 0, s>>>(a);
   }
   cwgk_count_launch();
   const cudaError_t e = cudaGetLastError();

@@ -52,20 +52,47 @@ __device__ __forceinline__ void store_states(float *line, int i0, int n, bool ve
   }
 }
 
+// Four values of one row of B or C as fp32; those at and past n read as zero.
+template <typename T>
+__device__ __forceinline__ void load4(const T *p, int i0, int n, bool vec, float (&f)[4]) {
+  if (vec) {
+    if constexpr (sizeof(T) == 4) {
+      unpack(*reinterpret_cast<const uint4 *>(p + i0), f);
+    } else {
+      const uint2 v = *reinterpret_cast<const uint2 *>(p + i0);
+      f[0] = __uint_as_float(v.x << 16), f[1] = __uint_as_float(v.x & 0xFFFF0000u);
+      f[2] = __uint_as_float(v.y << 16), f[3] = __uint_as_float(v.y & 0xFFFF0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = i0 + i < n ? to_f32(p[i0 + i]) : 0.f;
+  }
+}
+
 // ---- prompts --------------------------------------------------------------------
-// One CTA per (sequence, block of CH channels of one group): it walks the sequence
-// in tiles of kTT tokens.  Per tile the CTA turns dt and u into (d, d u) pairs and
-// B, C into fp32 in shared memory, the lanes run the recurrence over the tile, and
-// the CTA finishes y with full-width row accesses.  The next tile's operands are
-// loaded into registers while the recurrence runs.
+// One CTA per (sequence, block of kCH channels of one group) walks the sequence in tiles
+// of kTT tokens, its warps in two roles that work on neighbouring tiles at the same time:
+//   * scan warps hold the states and run the recurrence over tile i, reading the pairs
+//     (d, d u) and B, C from shared memory; a channel's L lanes reduce L tokens' sums
+//     together, so that each lane ends up with one token's (L - 1 shuffles per L tokens);
+//   * element warps finish tile i - 1 (skip, gate, full-width row stores), prepare tile
+//     i + 1 (step, d u, B and C next to one another) and load tile i + 2.
+// One barrier per tile.  Bound by the exponentials: N per token and channel at 16 a clock
+// and SM; the elementwise part adds 4 more, and the shared-memory reads of B and C (kept
+// in the input's type) come next.
 template <int L>
-struct Geo {
-  static constexpr int kCH = L <= 4 ? 64 : 256 / L;
-  static constexpr int kThreads = kCH * L;
-  static constexpr int kNP = kS * L;
-  static constexpr int kTasks = kTT * kCH / 8;  // 8-channel pieces of a tile
-  static constexpr int kPer = (kTasks + kThreads - 1) / kThreads;
-  static constexpr int kPerB = kTT * kNP / kThreads;
+struct Prompt {
+  static constexpr int kCH = L <= 4 ? 32 : 128 / L;
+  static constexpr int kScan = kCH * L;             // scan threads
+  static constexpr int kElem = 128;                 // element threads
+  static constexpr int kThreads = kScan + kElem;
+  static constexpr int kTasks = kTT * kCH / 8;      // 8-channel pieces of a tile
+  static constexpr int kPieces = (kTT * L + kElem - 1) / kElem;  // 4-state pieces of B, C
+  // y rows: the L tokens x 32 / L channels of one store fall in all 32 banks (L = 16: in
+  // half of them); read as 16-byte vectors
+  static constexpr int kPitch = kCH + (L <= 8 ? 32 / L : 4);
+  static_assert(kPitch % 4 == 0 && kCH % 8 == 0, "rows of whole vectors");
+  static_assert(kTasks <= kElem, "one piece per element thread");
 };
 
 // 8 consecutive channels of one row as fp32; channels past `n` read as zero.
@@ -103,20 +130,44 @@ struct Piece {
   }
 };
 
+// Four states' B and C of one token, in the input's type.
+template <typename T>
+struct alignas(8 * sizeof(T)) States4 {
+  T b[4], c[4];
+};
+__device__ __forceinline__ void get_bc(const States4<float> &s, F2 (&b)[2], F2 (&c)[2]) {
+  const float4 x = *reinterpret_cast<const float4 *>(s.b);
+  const float4 y = *reinterpret_cast<const float4 *>(s.c);
+  b[0] = f2(x.x, x.y), b[1] = f2(x.z, x.w);
+  c[0] = f2(y.x, y.y), c[1] = f2(y.z, y.w);
+}
+__device__ __forceinline__ void get_bc(const States4<__nv_bfloat16> &s, F2 (&b)[2], F2 (&c)[2]) {
+  float f[8];
+  unpack(*reinterpret_cast<const uint4 *>(&s), f);
+  b[0] = f2(f[0], f[1]), b[1] = f2(f[2], f[3]);
+  c[0] = f2(f[4], f[5]), c[1] = f2(f[6], f[7]);
+}
+
+// Where the pairs (d, d u) of channels 2 j, 2 j + 1 of an 8-channel piece are kept in
+// their row: turned so that 8 threads' 16-byte stores fall in all banks.
+__device__ __forceinline__ int turned(int t, int c8, int j) {
+  return c8 * 4 + ((j + (c8 >> 1) + 2 * (t & 1)) & 3);
+}
+
 template <typename T, int L, bool VEC>
-__global__ void __launch_bounds__(Geo<L>::kThreads) ssm_prompt(const Args a) {
-  using G = Geo<L>;
-  constexpr int CH = G::kCH, NT = G::kThreads, NP = G::kNP, PER = G::kPer, PERB = G::kPerB;
-  __shared__ __align__(16) float2 s_dx[kTT][CH];
-  __shared__ __align__(16) float s_b[kTT][NP], s_c[kTT][NP];
-  __shared__ __align__(16) float s_y[kTT][CH];
+__global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) {
+  using G = Prompt<L>;
+  constexpr int CH = G::kCH;
+  __shared__ __align__(16) float4 s_dx[2][kTT][CH / 2];
+  __shared__ States4<T> s_bc[2][kTT][L];
+  __shared__ __align__(16) float s_y[2][kTT][G::kPitch];
   const cwg_ssm &p = a.p;
   const int tid = threadIdx.x;
   const int cblk = blockIdx.x % a.cblocks;
   const int group = (blockIdx.x / a.cblocks) % p.groups;
   const int b = blockIdx.x / (a.cblocks * p.groups);
-  const int in0 = cblk * CH;                // first channel within the group
-  const int c0 = group * a.per + in0;       // first channel
+  const int in0 = cblk * CH;            // first channel within the group
+  const int c0 = group * a.per + in0;   // first channel
   const int nch = min(CH, a.per - in0);
   const int begin = p.starts[b], end = p.starts[b + 1];
   const bool report = tid == 0 && cblk == 0 && group == 0;
@@ -128,131 +179,189 @@ __global__ void __launch_bounds__(Geo<L>::kThreads) ssm_prompt(const Args a) {
   const int slot = p.state ? line_of(p.slots, b, p.n_slots, bad) : -1;
   if (bad && report) atomicOr(&g_ssm_status, CWGK_STATUS_INDEX);
   const bool carry = slot >= 0 && p.resume && p.resume[b];
+  const int tiles = (end - begin + kTT - 1) / kTT;
 
-  // the recurrence's view: lane `l` of channel `ch`, states i0 .. i0 + 3
-  const int ch = tid / L, l = tid % L, i0 = l * kS;
-  const bool mine = ch < nch;
-  float A2[kS], h[kS];
-  float *line = p.state + ((size_t)(slot < 0 ? 0 : slot) * p.channels + c0 + ch) * p.states;
-#pragma unroll
-  for (int i = 0; i < kS; ++i) {
-    A2[i] = mine && i0 + i < p.states ? p.A[(size_t)(c0 + ch) * p.states + i0 + i] * kLog2e : 0.f;
-    h[i] = 0.f;
-  }
-  if (carry && mine) load_states(line, i0, p.states, a.vec_state, h);
-
-  // the tile's view: 8-channel pieces
-  Piece<T, VEC> ru[PER], rd[PER], rz[PER], cu[PER], cz[PER];
-  float rb[PERB], rc[PERB];
-  auto fetch = [&](int t0) {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int task = tid + i * NT;
-      const int t = t0 + task / (CH / 8), c = (task % (CH / 8)) * 8;
-      const int n = task < G::kTasks && t < end ? nch - c : 0;
-      const size_t at = (size_t)t;
-      ru[i].load(static_cast<const T *>(p.u) + at * p.ldu + c0 + c, n);
-      rd[i].load(static_cast<const T *>(p.dt) + at * p.lddt + c0 + c, n);
-      rz[i].load(static_cast<const T *>(p.z) + at * p.ldz + c0 + c, p.z ? n : 0);
+  if (tid < G::kScan) {
+    // ---- lane l of channel ch, states i0 .. i0 + 3
+    const int ch = tid / L, l = tid % L, i0 = l * kS;
+    const bool mine = ch < nch;
+    float A2[kS] = {0.f, 0.f, 0.f, 0.f}, h[kS] = {0.f, 0.f, 0.f, 0.f};
+    const size_t at = (size_t)(c0 + ch) * p.states;
+    float *line = p.state + (size_t)(slot < 0 ? 0 : slot) * p.channels * p.states + at;
+    if (mine) {
+      load_states(p.A + at, i0, p.states, a.vec_a, A2);
+      if (carry) load_states(line, i0, p.states, a.vec_state, h);
     }
+    const F2 a01 = f2(A2[0] * kLog2e, A2[1] * kLog2e), a23 = f2(A2[2] * kLog2e, A2[3] * kLog2e);
+    F2 h01 = f2(h[0], h[1]), h23 = f2(h[2], h[3]);
+    const int at0 = turned(0, ch >> 3, (ch & 7) >> 1) * 4 + (ch & 1) * 2;
+    const int at1 = turned(1, ch >> 3, (ch & 7) >> 1) * 4 + (ch & 1) * 2;
+    __syncthreads();
+    for (int i = 0; i < tiles; ++i) {
+      const float(*dx)[CH * 2] = reinterpret_cast<const float(*)[CH * 2]>(s_dx[i & 1]);
+      const States4<T>(*bc)[L] = s_bc[i & 1];
+      float(*ys)[G::kPitch] = s_y[i & 1];
+#pragma unroll 1
+      for (int t0 = 0; t0 < kTT; t0 += (L < 4 ? 4 : L)) {
+        constexpr int TG = L < 4 ? 4 : L;
+        float y[TG];
 #pragma unroll
-    for (int i = 0; i < PERB; ++i) {
-      const int e = tid + i * NT;
-      const int t = t0 + e / NP, s = e % NP;
-      const bool ok = t < end && s < p.states;
-      const size_t col = (size_t)group * p.states + s;
-      rb[i] = ok ? to_f32(static_cast<const T *>(p.B)[(size_t)t * p.ldb + col]) : 0.f;
-      rc[i] = ok ? to_f32(static_cast<const T *>(p.C)[(size_t)t * p.ldc + col]) : 0.f;
+        for (int t = 0; t < TG; ++t) {
+          const float2 v = *reinterpret_cast<const float2 *>(&dx[t0 + t][t & 1 ? at1 : at0]);
+          F2 bv[2], cv[2];
+          get_bc(bc[t0 + t][l], bv, cv);
+          const F2 dd = f2(v.x, v.x), uu = f2(v.y, v.y);
+          const float2 x01 = halves(mul2(dd, a01)), x23 = halves(mul2(dd, a23));
+          h01 = fma2(f2(ex2(x01.x), ex2(x01.y)), h01, mul2(uu, bv[0]));
+          h23 = fma2(f2(ex2(x23.x), ex2(x23.y)), h23, mul2(uu, bv[1]));
+          const float2 s = halves(fma2(h01, cv[0], mul2(h23, cv[1])));
+          y[t] = s.x + s.y;
+        }
+#pragma unroll
+        for (int g = 0; g < TG; g += L) {  // L tokens' sums over the channel's L lanes
+#pragma unroll
+          for (int o = L / 2; o > 0; o >>= 1) {
+            const bool up = l & o;
+#pragma unroll
+            for (int k = 0; k < o; ++k) {
+              const float give = up ? y[g + k] : y[g + k + o];
+              const float keep = up ? y[g + k + o] : y[g + k];
+              y[g + k] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+            }
+          }
+          ys[t0 + g + l][ch] = y[g];
+        }
+      }
+      __syncthreads();
     }
-  };
-
-  fetch(begin);
-  for (int t0 = begin; t0 < end; t0 += kTT) {
-    // (d, d u) of every (token, channel); rows past the end have d = 0, which
-    // leaves the states as they are
+    if (slot >= 0 && mine) {
+      const float2 x = halves(h01), y = halves(h23);
+      const float out[kS] = {x.x, x.y, y.x, y.y};
+      store_states(line, i0, p.states, a.vec_state, out);
+    }
+  } else {
+    // ---- 8-channel pieces of the tiles' rows
+    const int e = tid - G::kScan;
+    const int tt = e / (CH / 8), c8 = e % (CH / 8), c = c8 * 8;
+    const bool task = e < G::kTasks && c < nch;
+    struct Row {
+      Piece<T, VEC> u, z;
+    } last, now, next;
+    Piece<T, VEC> step;
+    struct {
+      float b[4], c[4];
+    } bc[G::kPieces];
+    float bias[8], skip[8];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int task = tid + i * NT;
-      const int t = task / (CH / 8), c = (task % (CH / 8)) * 8;
-      if (task < G::kTasks) {
+    for (int k = 0; k < 8; ++k) {
+      const bool ok = task && c + k < nch;
+      bias[k] = ok && p.dt_bias ? p.dt_bias[c0 + c + k] : 0.f;
+      skip[k] = ok && p.D ? p.D[c0 + c + k] : 0.f;
+    }
+    auto load = [&](int i) {
+      const int t = begin + i * kTT + tt;
+      const int n = task && t < end ? nch - c : 0;
+      const size_t at = (size_t)(n > 0 ? t : 0);
+      next.u.load(static_cast<const T *>(p.u) + at * p.ldu + c0 + c, n);
+      step.load(static_cast<const T *>(p.dt) + at * p.lddt + c0 + c, n);
+      next.z.load(static_cast<const T *>(p.z) + at * p.ldz + c0 + c, p.z ? n : 0);
+#pragma unroll
+      for (int k = 0; k < G::kPieces; ++k) {
+        const int q = e + k * G::kElem, s = q % L, tq = begin + i * kTT + q / L;
+        const bool ok = q < kTT * L && tq < end;
+        const size_t row = (size_t)(ok ? tq : 0);
+        const int n4 = ok ? p.states : 0;
+        const T *bp = static_cast<const T *>(p.B) + row * p.ldb + (size_t)group * p.states;
+        const T *cp = static_cast<const T *>(p.C) + row * p.ldc + (size_t)group * p.states;
+        load4(bp, s * 4, n4, a.vec_bc && ok, bc[k].b);
+        load4(cp, s * 4, n4, a.vec_bc && ok, bc[k].c);
+      }
+    };
+    // pairs (d, d u); rows past the end have d = 0, which leaves the states as they are
+    auto prepare = [&](int i) {
+      const bool row = begin + i * kTT + tt < end;
+      if (e < G::kTasks) {
         float u[8], d[8];
-        ru[i].get(u);
-        rd[i].get(d);
-        const bool row = t0 + t < end;
+        next.u.get(u);
+        step.get(d);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const bool ok = row && c + e < nch;
-          float v = d[e] + (ok && p.dt_bias ? p.dt_bias[c0 + c + e] : 0.f);
+        for (int k = 0; k < 8; ++k) {
+          float v = d[k] + bias[k];
           if (p.flags & CWG_SOFTPLUS) v = softplus(v);
-          s_dx[t][c + e] = ok ? make_float2(v, v * u[e]) : make_float2(0.f, 0.f);
+          d[k] = row && c + k < nch ? v : 0.f;
+          u[k] = row && c + k < nch ? v * u[k] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          s_dx[i & 1][tt][turned(tt, c8, k)] =
+              make_float4(d[2 * k], u[2 * k], d[2 * k + 1], u[2 * k + 1]);
+      }
+#pragma unroll
+      for (int k = 0; k < G::kPieces; ++k) {
+        const int q = e + k * G::kElem;
+        if (q < kTT * L) {
+          States4<T> &s = s_bc[i & 1][q / L][q % L];
+          if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float4 *>(s.b) =
+                make_float4(bc[k].b[0], bc[k].b[1], bc[k].b[2], bc[k].b[3]);
+            *reinterpret_cast<float4 *>(s.c) =
+                make_float4(bc[k].c[0], bc[k].c[1], bc[k].c[2], bc[k].c[3]);
+          } else {  // exact: they came from bf16
+            const float f[8] = {bc[k].b[0], bc[k].b[1], bc[k].b[2], bc[k].b[3],
+                                bc[k].c[0], bc[k].c[1], bc[k].c[2], bc[k].c[3]};
+            *reinterpret_cast<uint4 *>(&s) = pack<T, 8>(f);
+          }
         }
       }
-      cu[i] = ru[i];
-      cz[i] = rz[i];
-    }
+    };
+    auto finish = [&](int i) {
+      const int t = begin + i * kTT + tt;
+      if (!task || t >= end) return;
+      float u[8], z[8], y[8];
+      last.u.get(u);
+      last.z.get(z);
+      const float4 lo = *reinterpret_cast<const float4 *>(&s_y[i & 1][tt][c]);
+      const float4 hi = *reinterpret_cast<const float4 *>(&s_y[i & 1][tt][c + 4]);
+      y[0] = lo.x, y[1] = lo.y, y[2] = lo.z, y[3] = lo.w;
+      y[4] = hi.x, y[5] = hi.y, y[6] = hi.z, y[7] = hi.w;
 #pragma unroll
-    for (int i = 0; i < PERB; ++i) {
-      const int e = tid + i * NT;
-      s_b[e / NP][e % NP] = rb[i];
-      s_c[e / NP][e % NP] = rc[i];
-    }
-    __syncthreads();
-    if (t0 + kTT < end) fetch(t0 + kTT);
-#pragma unroll 4
-    for (int t = 0; t < kTT; ++t) {
-      const float2 dx = s_dx[t][ch];
-      const float4 bv = *reinterpret_cast<const float4 *>(&s_b[t][i0]);
-      const float4 cv = *reinterpret_cast<const float4 *>(&s_c[t][i0]);
-      h[0] = fmaf(ex2(dx.x * A2[0]), h[0], dx.y * bv.x);
-      h[1] = fmaf(ex2(dx.x * A2[1]), h[1], dx.y * bv.y);
-      h[2] = fmaf(ex2(dx.x * A2[2]), h[2], dx.y * bv.z);
-      h[3] = fmaf(ex2(dx.x * A2[3]), h[3], dx.y * bv.w);
-      float y = fmaf(h[0], cv.x, h[1] * cv.y) + fmaf(h[2], cv.z, h[3] * cv.w);
-#pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-      if (l == 0) s_y[t][ch] = y;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int task = tid + i * NT;
-      const int t = task / (CH / 8), c = (task % (CH / 8)) * 8;
-      if (task < G::kTasks && t0 + t < end && c < nch) {
-        float u[8], z[8], y[8];
-        cu[i].get(u);
-        cz[i].get(z);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          y[e] = fmaf(p.D && c + e < nch ? p.D[c0 + c + e] : 0.f, u[e], s_y[t][c + e]);
-          if (p.z) y[e] *= silu<T>(z[e]);
-        }
-        Piece<T, VEC>::store(static_cast<T *>(p.y) + (size_t)(t0 + t) * p.ldy + c0 + c, y,
-                             nch - c);
+      for (int k = 0; k < 8; ++k) {
+        y[k] = fmaf(skip[k], u[k], y[k]);
+        if (p.z) y[k] *= silu<T>(z[k]);
       }
+      Piece<T, VEC>::store(static_cast<T *>(p.y) + (size_t)t * p.ldy + c0 + c, y, nch - c);
+    };
+    if (tiles > 0) {
+      load(0);
+      prepare(0);
+      now = next;
+      load(1);
     }
+    __syncthreads();
+    for (int i = 0; i < tiles; ++i) {
+      if (i > 0) finish(i - 1);
+      last = now;
+      if (i + 1 < tiles) {
+        prepare(i + 1);
+        now = next;
+        load(i + 2);
+      }
+      __syncthreads();
+    }
+    if (tiles > 0) finish(tiles - 1);
   }
-  if (slot >= 0 && mine) store_states(line, i0, p.states, a.vec_state, h);
 }
 
 // ---- one token of each sequence ----------------------------------------------------
 // Bound by the states, 8 N bytes per channel in and out.  A CTA takes RR rows of one
 // channel block: the rows share A, and all their states are loaded before the first is
 // used.  Meanwhile the CTA's threads look together for lines that an earlier row has too.
-template <typename T>
-__device__ __forceinline__ void load4(const T *p, int i0, int n, bool vec, float (&f)[4]) {
-  if (vec) {
-    if constexpr (sizeof(T) == 4) {
-      unpack(*reinterpret_cast<const uint4 *>(p + i0), f);
-    } else {
-      const uint2 v = *reinterpret_cast<const uint2 *>(p + i0);
-      f[0] = __uint_as_float(v.x << 16), f[1] = __uint_as_float(v.x & 0xFFFF0000u);
-      f[2] = __uint_as_float(v.y << 16), f[3] = __uint_as_float(v.y & 0xFFFF0000u);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = i0 + i < n ? to_f32(p[i0 + i]) : 0.f;
-  }
-}
+template <int L>
+struct Geo {
+  static constexpr int kCH = L <= 4 ? 64 : 256 / L;
+  static constexpr int kThreads = kCH * L;
+  static constexpr int kNP = kS * L;
+};
 
 template <typename T, int L, int RR>
 __global__ void __launch_bounds__(Geo<L>::kThreads) ssm_token(const Args a) {
@@ -384,7 +493,8 @@ static int launch(const cwg_ssm *op, bool step, cudaStream_t s) {
   a.p = *op;
   if (op->tokens <= 1) a.p.ldu = a.p.lddt = a.p.ldz = a.p.ldy = 0, a.p.ldb = a.p.ldc = 0;
   a.per = op->channels / op->groups;
-  a.cblocks = (a.per + G::kCH - 1) / G::kCH;
+  const int ch = step ? G::kCH : Prompt<L>::kCH;
+  a.cblocks = (a.per + ch - 1) / ch;
   a.vec_state = op->states == G::kNP && aligned16(op->state);
   a.vec_a = op->states == G::kNP && aligned16(op->A);
   a.vec_bc = op->states == G::kNP && ((uintptr_t)op->B % (4 * sizeof(T))) == 0 &&
@@ -406,9 +516,9 @@ static int launch(const cwg_ssm *op, bool step, cudaStream_t s) {
                    aligned16(op->y) && a.p.ldu % E == 0 && a.p.lddt % E == 0 &&
                    a.p.ldy % E == 0 && (!op->z || a.p.ldz % E == 0);
   if (vec)
-    ssm_prompt<T, L, true><<<(unsigned)blocks, G::kThreads, 0, s>>>(a);
+    ssm_prompt<T, L, true><<<(unsigned)blocks, Prompt<L>::kThreads, 0, s>>>(a);
   else
-    ssm_prompt<T, L, false><<<(unsigned)blocks, G::kThreads, 0, s>>>(a);
+    ssm_prompt<T, L, false><<<(unsigned)blocks, Prompt<L>::kThreads, 0, s>>>(a);
   return done();
 }
 
