@@ -76,7 +76,7 @@ __device__ __forceinline__ void load4(const T *p, int i0, int n, bool vec, float
 //     (d, d u) and B, C from shared memory; a channel's L lanes reduce L tokens' sums
 //     together, so that each lane ends up with one token's (L - 1 shuffles per L tokens);
 //   * element warps finish tile i - 1 (skip, gate, full-width row stores), prepare tile
-//     i + 1 (step, d u, B and C next to one another) and load tile i + 2.
+//     i + 1 (step, d u, B and C next to one another) and load tile i + 3.
 // One barrier per tile.  Bound by the exponentials: N per token and channel at 16 a clock
 // and SM; the elementwise part adds 4 more, and the shared-memory reads of B and C (kept
 // in the input's type) come next.
@@ -93,6 +93,8 @@ struct Prompt {
   static constexpr int kPitch = kCH + (L <= 8 ? 32 / L : 4);
   static_assert(kPitch % 4 == 0 && kCH % 8 == 0, "rows of whole vectors");
   static_assert(kTasks <= kElem, "one piece per element thread");
+  template <typename T>  // tokens a scan warp takes at a time
+  static constexpr int kGroup = L > 8 ? L : sizeof(T) == 2 ? 8 : (L > 4 ? L : 4);
 };
 
 // 8 consecutive channels of one row as fp32; channels past `n` read as zero.
@@ -132,18 +134,45 @@ struct Piece {
 
 // Four states' B and C of one token, in the input's type.
 template <typename T>
-struct alignas(8 * sizeof(T)) States4 {
-  T b[4], c[4];
+struct States4 {
+  uint4 raw[sizeof(T) / 2];
+  // n: how many of the four states there are; vec: all of them, aligned
+  __device__ __forceinline__ void load(const T *b, const T *c, int n, bool vec) {
+    if (vec && n > 0) {
+      if constexpr (sizeof(T) == 4) {
+        raw[0] = load_raw<T, 4>(b);
+        raw[1] = load_raw<T, 4>(c);
+      } else {
+        const uint2 x = load_raw<T, 4>(b), y = load_raw<T, 4>(c);
+        raw[0] = make_uint4(x.x, x.y, y.x, y.y);
+      }
+    } else {
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f[i] = i < n ? to_f32(b[i]) : 0.f;
+        f[4 + i] = i < n ? to_f32(c[i]) : 0.f;
+      }
+      if constexpr (sizeof(T) == 4) {
+        const float x[4] = {f[0], f[1], f[2], f[3]}, y[4] = {f[4], f[5], f[6], f[7]};
+        raw[0] = pack<T, 4>(x);
+        raw[1] = pack<T, 4>(y);
+      } else {  // exact: they came from bf16
+        raw[0] = pack<T, 8>(f);
+      }
+    }
+  }
 };
 __device__ __forceinline__ void get_bc(const States4<float> &s, F2 (&b)[2], F2 (&c)[2]) {
-  const float4 x = *reinterpret_cast<const float4 *>(s.b);
-  const float4 y = *reinterpret_cast<const float4 *>(s.c);
-  b[0] = f2(x.x, x.y), b[1] = f2(x.z, x.w);
-  c[0] = f2(y.x, y.y), c[1] = f2(y.z, y.w);
+  float x[4], y[4];
+  unpack(s.raw[0], x);
+  unpack(s.raw[1], y);
+  b[0] = f2(x[0], x[1]), b[1] = f2(x[2], x[3]);
+  c[0] = f2(y[0], y[1]), c[1] = f2(y[2], y[3]);
 }
 __device__ __forceinline__ void get_bc(const States4<__nv_bfloat16> &s, F2 (&b)[2], F2 (&c)[2]) {
   float f[8];
-  unpack(*reinterpret_cast<const uint4 *>(&s), f);
+  unpack(s.raw[0], f);
   b[0] = f2(f[0], f[1]), b[1] = f2(f[2], f[3]);
   c[0] = f2(f[4], f[5]), c[1] = f2(f[6], f[7]);
 }
@@ -198,19 +227,36 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) 
     const int at1 = turned(1, ch >> 3, (ch & 7) >> 1) * 4 + (ch & 1) * 2;
     __syncthreads();
     for (int i = 0; i < tiles; ++i) {
-      const float(*dx)[CH * 2] = reinterpret_cast<const float(*)[CH * 2]>(s_dx[i & 1]);
+      const float *dx = reinterpret_cast<const float *>(s_dx[i & 1]);
       const States4<T>(*bc)[L] = s_bc[i & 1];
       float(*ys)[G::kPitch] = s_y[i & 1];
-#pragma unroll 1
-      for (int t0 = 0; t0 < kTT; t0 += (L < 4 ? 4 : L)) {
-        constexpr int TG = L < 4 ? 4 : L;
+      // TG tokens at a time; where registers allow, the next ones' operands are read
+      // while these are worked on
+      constexpr int TG = G::template kGroup<T>;
+      constexpr bool kPrefetch = TG * (2 + 2 * (int)sizeof(T)) <= 48;
+      float2 v[TG];
+      States4<T> w[TG];
+      auto fetch = [&](int t0) {
+#pragma unroll
+        for (int t = 0; t < TG; ++t) {
+          v[t] = *reinterpret_cast<const float2 *>(dx + (t0 + t) * (CH * 2) + (t & 1 ? at1 : at0));
+          w[t] = bc[t0 + t][l];
+        }
+      };
+      fetch(0);
+#pragma unroll
+      for (int t0 = 0; t0 < kTT; t0 += TG) {
+        float2 dv[TG];
+        States4<T> sv[TG];
+#pragma unroll
+        for (int t = 0; t < TG; ++t) dv[t] = v[t], sv[t] = w[t];
+        if (kPrefetch && t0 + TG < kTT) fetch(t0 + TG);
         float y[TG];
 #pragma unroll
         for (int t = 0; t < TG; ++t) {
-          const float2 v = *reinterpret_cast<const float2 *>(&dx[t0 + t][t & 1 ? at1 : at0]);
           F2 bv[2], cv[2];
-          get_bc(bc[t0 + t][l], bv, cv);
-          const F2 dd = f2(v.x, v.x), uu = f2(v.y, v.y);
+          get_bc(sv[t], bv, cv);
+          const F2 dd = f2(dv[t].x, dv[t].x), uu = f2(dv[t].y, dv[t].y);
           const float2 x01 = halves(mul2(dd, a01)), x23 = halves(mul2(dd, a23));
           h01 = fma2(f2(ex2(x01.x), ex2(x01.y)), h01, mul2(uu, bv[0]));
           h23 = fma2(f2(ex2(x23.x), ex2(x23.y)), h23, mul2(uu, bv[1]));
@@ -218,19 +264,20 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) 
           y[t] = s.x + s.y;
         }
 #pragma unroll
-        for (int g = 0; g < TG; g += L) {  // L tokens' sums over the channel's L lanes
+        for (int o = L / 2; o > 0; o >>= 1) {  // L tokens' sums over the channel's L lanes
+          const bool up = l & o;
 #pragma unroll
-          for (int o = L / 2; o > 0; o >>= 1) {
-            const bool up = l & o;
+          for (int g = 0; g < TG; g += L)
 #pragma unroll
             for (int k = 0; k < o; ++k) {
               const float give = up ? y[g + k] : y[g + k + o];
               const float keep = up ? y[g + k + o] : y[g + k];
               y[g + k] = keep + __shfl_xor_sync(0xffffffffu, give, o);
             }
-          }
-          ys[t0 + g + l][ch] = y[g];
         }
+#pragma unroll
+        for (int g = 0; g < TG; g += L) ys[t0 + g + l][ch] = y[g];
+        if (!kPrefetch && t0 + TG < kTT) fetch(t0 + TG);
       }
       __syncthreads();
     }
@@ -244,13 +291,14 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) 
     const int e = tid - G::kScan;
     const int tt = e / (CH / 8), c8 = e % (CH / 8), c = c8 * 8;
     const bool task = e < G::kTasks && c < nch;
-    struct Row {
-      Piece<T, VEC> u, z;
-    } last, now, next;
-    Piece<T, VEC> step;
+    // what a tile needs, on its way from memory for two tiles' time
+    struct Stage {
+      Piece<T, VEC> u, d, z;
+      States4<T> bc[G::kPieces];
+    } even, odd;
     struct {
-      float b[4], c[4];
-    } bc[G::kPieces];
+      Piece<T, VEC> u, z;
+    } last, now;
     float bias[8], skip[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -258,32 +306,30 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) 
       bias[k] = ok && p.dt_bias ? p.dt_bias[c0 + c + k] : 0.f;
       skip[k] = ok && p.D ? p.D[c0 + c + k] : 0.f;
     }
-    auto load = [&](int i) {
+    auto load = [&](int i, Stage &st) {
       const int t = begin + i * kTT + tt;
       const int n = task && t < end ? nch - c : 0;
       const size_t at = (size_t)(n > 0 ? t : 0);
-      next.u.load(static_cast<const T *>(p.u) + at * p.ldu + c0 + c, n);
-      step.load(static_cast<const T *>(p.dt) + at * p.lddt + c0 + c, n);
-      next.z.load(static_cast<const T *>(p.z) + at * p.ldz + c0 + c, p.z ? n : 0);
+      st.u.load(static_cast<const T *>(p.u) + at * p.ldu + c0 + c, n);
+      st.d.load(static_cast<const T *>(p.dt) + at * p.lddt + c0 + c, n);
+      st.z.load(static_cast<const T *>(p.z) + at * p.ldz + c0 + c, p.z ? n : 0);
 #pragma unroll
       for (int k = 0; k < G::kPieces; ++k) {
         const int q = e + k * G::kElem, s = q % L, tq = begin + i * kTT + q / L;
         const bool ok = q < kTT * L && tq < end;
-        const size_t row = (size_t)(ok ? tq : 0);
-        const int n4 = ok ? p.states : 0;
-        const T *bp = static_cast<const T *>(p.B) + row * p.ldb + (size_t)group * p.states;
-        const T *cp = static_cast<const T *>(p.C) + row * p.ldc + (size_t)group * p.states;
-        load4(bp, s * 4, n4, a.vec_bc && ok, bc[k].b);
-        load4(cp, s * 4, n4, a.vec_bc && ok, bc[k].c);
+        const size_t row = (size_t)(ok ? tq : 0), col = (size_t)group * p.states + s * 4;
+        st.bc[k].load(static_cast<const T *>(p.B) + row * p.ldb + col,
+                      static_cast<const T *>(p.C) + row * p.ldc + col, ok ? p.states - s * 4 : 0,
+                      a.vec_bc);
       }
     };
     // pairs (d, d u); rows past the end have d = 0, which leaves the states as they are
-    auto prepare = [&](int i) {
+    auto prepare = [&](int i, const Stage &st) {
       const bool row = begin + i * kTT + tt < end;
       if (e < G::kTasks) {
         float u[8], d[8];
-        next.u.get(u);
-        step.get(d);
+        st.u.get(u);
+        st.d.get(d);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           float v = d[k] + bias[k];
@@ -299,19 +345,7 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) 
 #pragma unroll
       for (int k = 0; k < G::kPieces; ++k) {
         const int q = e + k * G::kElem;
-        if (q < kTT * L) {
-          States4<T> &s = s_bc[i & 1][q / L][q % L];
-          if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<float4 *>(s.b) =
-                make_float4(bc[k].b[0], bc[k].b[1], bc[k].b[2], bc[k].b[3]);
-            *reinterpret_cast<float4 *>(s.c) =
-                make_float4(bc[k].c[0], bc[k].c[1], bc[k].c[2], bc[k].c[3]);
-          } else {  // exact: they came from bf16
-            const float f[8] = {bc[k].b[0], bc[k].b[1], bc[k].b[2], bc[k].b[3],
-                                bc[k].c[0], bc[k].c[1], bc[k].c[2], bc[k].c[3]};
-            *reinterpret_cast<uint4 *>(&s) = pack<T, 8>(f);
-          }
-        }
+        if (q < kTT * L) s_bc[i & 1][q / L][q % L] = st.bc[k];
       }
     };
     auto finish = [&](int i) {
@@ -331,22 +365,30 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) 
       }
       Piece<T, VEC>::store(static_cast<T *>(p.y) + (size_t)t * p.ldy + c0 + c, y, nch - c);
     };
-    if (tiles > 0) {
-      load(0);
-      prepare(0);
-      now = next;
-      load(1);
-    }
-    __syncthreads();
-    for (int i = 0; i < tiles; ++i) {
+    // step i: tile i + 1 is in `st`, which then takes tile i + 3
+    auto advance = [&](int i, Stage &st) {
       if (i > 0) finish(i - 1);
       last = now;
       if (i + 1 < tiles) {
-        prepare(i + 1);
-        now = next;
-        load(i + 2);
+        prepare(i + 1, st);
+        now.u = st.u;
+        now.z = st.z;
+        load(i + 3, st);
       }
       __syncthreads();
+    };
+    if (tiles > 0) {
+      load(0, even);
+      load(1, odd);
+      prepare(0, even);
+      now.u = even.u;
+      now.z = even.z;
+      load(2, even);
+    }
+    __syncthreads();
+    for (int i = 0; i < tiles; i += 2) {
+      advance(i, odd);
+      if (i + 1 < tiles) advance(i + 1, even);
     }
     if (tiles > 0) finish(tiles - 1);
   }
