@@ -97,71 +97,71 @@ struct Prompt {
   static constexpr int kGroup = L > 8 ? L : sizeof(T) == 2 ? 8 : (L > 4 ? L : 4);
 };
 
-// 8 consecutive channels of one row as fp32; channels past `n` read as zero.
+// Asynchronous copy of B bytes into shared memory; zeros where !ok.
+template <int B>
+__device__ __forceinline__ void copy_async(void *dst, const void *src, bool ok) {
+  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+  if constexpr (B == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src),
+                 "r"(ok ? 16 : 0)
+                 : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(src), "n"(B),
+                 "r"(ok ? B : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void copy_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void copy_wait() {  // all but the N newest groups have landed
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// W elements of a row, of which n exist (VEC: all of them aligned and n whole vectors).
+// Elements of two bytes that are not aligned cannot be copied asynchronously.
+template <typename T, int W, bool VEC>
+__device__ __forceinline__ void copy_row(T *dst, const T *src, int n, const T *safe) {
+  if constexpr (VEC) {
+    constexpr int B = W * (int)sizeof(T) < 16 ? W * (int)sizeof(T) : 16, E = B / (int)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < W; i += E) copy_async<B>(dst + i, i < n ? src + i : safe, i < n);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) copy_async<4>(dst + i, i < n ? src + i : safe, i < n);
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; ++i) dst[i] = i < n ? src[i] : from_f32<T>(0.f);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void read8(const T *p, float (&f)[8]) {
+  constexpr int E = 16 / (int)sizeof(T);
+#pragma unroll
+  for (int i = 0; i < 8; i += E) {
+    float g[E];
+    unpack(load_raw<T, E>(p + i), g);
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[i + e] = g[e];
+  }
+}
 template <typename T, bool VEC>
-struct Piece {
-  static constexpr int kRaw = VEC ? (int)sizeof(T) * 8 / 16 : 8;
-  using R = typename Raw<T, VEC ? 16 / (int)sizeof(T) : 1>::type;
-  R raw[kRaw];
-  __device__ __forceinline__ void load(const T *p, int n) {
+__device__ __forceinline__ void write8(T *p, const float (&f)[8], int n) {
+  constexpr int E = VEC ? 16 / (int)sizeof(T) : 1;
 #pragma unroll
-    for (int i = 0; i < kRaw; ++i) {
-      constexpr int E = 8 / kRaw;
-      raw[i] = i * E < n ? load_raw<T, E>(p + i * E) : zero_raw<T, E>();
-    }
+  for (int i = 0; i < 8; i += E) {
+    float g[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) g[e] = f[i + e];
+    if (i < n) store_raw<T, E>(p + i, pack<T, E>(g));
   }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
-    constexpr int E = 8 / kRaw;
-#pragma unroll
-    for (int i = 0; i < kRaw; ++i) {
-      float g[E];
-      unpack(raw[i], g);
-#pragma unroll
-      for (int e = 0; e < E; ++e) f[i * E + e] = g[e];
-    }
-  }
-  __device__ static __forceinline__ void store(T *p, const float (&f)[8], int n) {
-    constexpr int E = 8 / kRaw;
-#pragma unroll
-    for (int i = 0; i < kRaw; ++i) {
-      float g[E];
-#pragma unroll
-      for (int e = 0; e < E; ++e) g[e] = f[i * E + e];
-      if (i * E < n) store_raw<T, E>(p + i * E, pack<T, E>(g));
-    }
-  }
-};
+}
 
 // Four states' B and C of one token, in the input's type.
 template <typename T>
 struct States4 {
   uint4 raw[sizeof(T) / 2];
-  // n: how many of the four states there are; vec: all of them, aligned
-  __device__ __forceinline__ void load(const T *b, const T *c, int n, bool vec) {
-    if (vec && n > 0) {
-      if constexpr (sizeof(T) == 4) {
-        raw[0] = load_raw<T, 4>(b);
-        raw[1] = load_raw<T, 4>(c);
-      } else {
-        const uint2 x = load_raw<T, 4>(b), y = load_raw<T, 4>(c);
-        raw[0] = make_uint4(x.x, x.y, y.x, y.y);
-      }
-    } else {
-      float f[8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f[i] = i < n ? to_f32(b[i]) : 0.f;
-        f[4 + i] = i < n ? to_f32(c[i]) : 0.f;
-      }
-      if constexpr (sizeof(T) == 4) {
-        const float x[4] = {f[0], f[1], f[2], f[3]}, y[4] = {f[4], f[5], f[6], f[7]};
-        raw[0] = pack<T, 4>(x);
-        raw[1] = pack<T, 4>(y);
-      } else {  // exact: they came from bf16
-        raw[0] = pack<T, 8>(f);
-      }
-    }
-  }
+  __device__ __forceinline__ T *b() { return reinterpret_cast<T *>(raw); }
+  __device__ __forceinline__ T *c() { return reinterpret_cast<T *>(raw) + 4; }
 };
 __device__ __forceinline__ void get_bc(const States4<float> &s, F2 (&b)[2], F2 (&c)[2]) {
   float x[4], y[4];
@@ -183,13 +183,24 @@ __device__ __forceinline__ int turned(int t, int c8, int j) {
   return c8 * 4 + ((j + (c8 >> 1) + 2 * (t & 1)) & 3);
 }
 
-template <typename T, int L, bool VEC>
+// Shared memory of a CTA: the rows of four tiles, the pairs and sums of two.
+template <typename T, int L>
+struct PromptSmem {
+  using G = Prompt<L>;
+  static constexpr int kStages = 4;
+  float4 dx[2][kTT][G::kCH / 2];
+  float y[2][kTT][G::kPitch];
+  States4<T> bc[kStages][kTT][L];
+  T u[kStages][kTT][G::kCH], d[kStages][kTT][G::kCH], z[kStages][kTT][G::kCH];
+};
+
+template <typename T, int L, bool VEC, bool VBC>
 __global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) {
   using G = Prompt<L>;
   constexpr int CH = G::kCH;
-  __shared__ __align__(16) float4 s_dx[2][kTT][CH / 2];
-  __shared__ States4<T> s_bc[2][kTT][L];
-  __shared__ __align__(16) float s_y[2][kTT][G::kPitch];
+  constexpr int NS = PromptSmem<T, L>::kStages;
+  extern __shared__ __align__(16) unsigned char smem[];
+  PromptSmem<T, L> &sh = *reinterpret_cast<PromptSmem<T, L> *>(smem);
   const cwg_ssm &p = a.p;
   const int tid = threadIdx.x;
   const int cblk = blockIdx.x % a.cblocks;
@@ -227,9 +238,9 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) 
     const int at1 = turned(1, ch >> 3, (ch & 7) >> 1) * 4 + (ch & 1) * 2;
     __syncthreads();
     for (int i = 0; i < tiles; ++i) {
-      const float *dx = reinterpret_cast<const float *>(s_dx[i & 1]);
-      const States4<T>(*bc)[L] = s_bc[i & 1];
-      float(*ys)[G::kPitch] = s_y[i & 1];
+      const float *dx = reinterpret_cast<const float *>(sh.dx[i & 1]);
+      const States4<T>(*bc)[L] = sh.bc[i % NS];
+      float(*ys)[G::kPitch] = sh.y[i & 1];
       // TG tokens at a time; where registers allow, the next ones' operands are read
       // while these are worked on
       constexpr int TG = G::template kGroup<T>;
@@ -291,14 +302,6 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) 
     const int e = tid - G::kScan;
     const int tt = e / (CH / 8), c8 = e % (CH / 8), c = c8 * 8;
     const bool task = e < G::kTasks && c < nch;
-    // what a tile needs, on its way from memory for two tiles' time
-    struct Stage {
-      Piece<T, VEC> u, d, z;
-      States4<T> bc[G::kPieces];
-    } even, odd;
-    struct {
-      Piece<T, VEC> u, z;
-    } last, now;
     float bias[8], skip[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -306,30 +309,38 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) 
       bias[k] = ok && p.dt_bias ? p.dt_bias[c0 + c + k] : 0.f;
       skip[k] = ok && p.D ? p.D[c0 + c + k] : 0.f;
     }
-    auto load = [&](int i, Stage &st) {
-      const int t = begin + i * kTT + tt;
+    const T *gu = static_cast<const T *>(p.u), *gd = static_cast<const T *>(p.dt);
+    const T *gz = static_cast<const T *>(p.z);
+    const T *gb = static_cast<const T *>(p.B), *gc = static_cast<const T *>(p.C);
+    auto load = [&](int i) {
+      const int t = begin + i * kTT + tt, st = i % NS;
       const int n = task && t < end ? nch - c : 0;
       const size_t at = (size_t)(n > 0 ? t : 0);
-      st.u.load(static_cast<const T *>(p.u) + at * p.ldu + c0 + c, n);
-      st.d.load(static_cast<const T *>(p.dt) + at * p.lddt + c0 + c, n);
-      st.z.load(static_cast<const T *>(p.z) + at * p.ldz + c0 + c, p.z ? n : 0);
+      if (e < G::kTasks) {
+        copy_row<T, 8, VEC>(&sh.u[st][tt][c], gu + at * p.ldu + c0 + c, n, gu);
+        copy_row<T, 8, VEC>(&sh.d[st][tt][c], gd + at * p.lddt + c0 + c, n, gd);
+        if (p.z) copy_row<T, 8, VEC>(&sh.z[st][tt][c], gz + at * p.ldz + c0 + c, n, gz);
+      }
 #pragma unroll
       for (int k = 0; k < G::kPieces; ++k) {
         const int q = e + k * G::kElem, s = q % L, tq = begin + i * kTT + q / L;
-        const bool ok = q < kTT * L && tq < end;
-        const size_t row = (size_t)(ok ? tq : 0), col = (size_t)group * p.states + s * 4;
-        st.bc[k].load(static_cast<const T *>(p.B) + row * p.ldb + col,
-                      static_cast<const T *>(p.C) + row * p.ldc + col, ok ? p.states - s * 4 : 0,
-                      a.vec_bc);
+        if (q < kTT * L) {
+          const int n4 = tq < end ? p.states - s * 4 : 0;
+          const size_t row = (size_t)(n4 > 0 ? tq : 0), col = (size_t)group * p.states + s * 4;
+          copy_row<T, 4, VBC>(sh.bc[st][q / L][s].b(), gb + row * p.ldb + col, n4, gb);
+          copy_row<T, 4, VBC>(sh.bc[st][q / L][s].c(), gc + row * p.ldc + col, n4, gc);
+        }
       }
+      copy_commit();
     };
-    // pairs (d, d u); rows past the end have d = 0, which leaves the states as they are
-    auto prepare = [&](int i, const Stage &st) {
+    // pairs (d, d u) of the thread's own piece; rows past the end have d = 0, which leaves
+    // the states as they are
+    auto prepare = [&](int i) {
       const bool row = begin + i * kTT + tt < end;
       if (e < G::kTasks) {
         float u[8], d[8];
-        st.u.get(u);
-        st.d.get(d);
+        read8(&sh.u[i % NS][tt][c], u);
+        read8(&sh.d[i % NS][tt][c], d);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           float v = d[k] + bias[k];
@@ -339,58 +350,43 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) 
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          s_dx[i & 1][tt][turned(tt, c8, k)] =
+          sh.dx[i & 1][tt][turned(tt, c8, k)] =
               make_float4(d[2 * k], u[2 * k], d[2 * k + 1], u[2 * k + 1]);
-      }
-#pragma unroll
-      for (int k = 0; k < G::kPieces; ++k) {
-        const int q = e + k * G::kElem;
-        if (q < kTT * L) s_bc[i & 1][q / L][q % L] = st.bc[k];
       }
     };
     auto finish = [&](int i) {
       const int t = begin + i * kTT + tt;
       if (!task || t >= end) return;
       float u[8], z[8], y[8];
-      last.u.get(u);
-      last.z.get(z);
-      const float4 lo = *reinterpret_cast<const float4 *>(&s_y[i & 1][tt][c]);
-      const float4 hi = *reinterpret_cast<const float4 *>(&s_y[i & 1][tt][c + 4]);
-      y[0] = lo.x, y[1] = lo.y, y[2] = lo.z, y[3] = lo.w;
-      y[4] = hi.x, y[5] = hi.y, y[6] = hi.z, y[7] = hi.w;
+      read8(&sh.u[i % NS][tt][c], u);
+      read8(&sh.y[i & 1][tt][c], y);
+      if (p.z) read8(&sh.z[i % NS][tt][c], z);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         y[k] = fmaf(skip[k], u[k], y[k]);
         if (p.z) y[k] *= silu<T>(z[k]);
       }
-      Piece<T, VEC>::store(static_cast<T *>(p.y) + (size_t)t * p.ldy + c0 + c, y, nch - c);
-    };
-    // step i: tile i + 1 is in `st`, which then takes tile i + 3
-    auto advance = [&](int i, Stage &st) {
-      if (i > 0) finish(i - 1);
-      last = now;
-      if (i + 1 < tiles) {
-        prepare(i + 1, st);
-        now.u = st.u;
-        now.z = st.z;
-        load(i + 3, st);
-      }
-      __syncthreads();
+      write8<T, VEC>(static_cast<T *>(p.y) + (size_t)t * p.ldy + c0 + c, y, nch - c);
     };
     if (tiles > 0) {
-      load(0, even);
-      load(1, odd);
-      prepare(0, even);
-      now.u = even.u;
-      now.z = even.z;
-      load(2, even);
+      load(0);
+      load(1);
+      load(2);
+      copy_wait<2>();
+      prepare(0);
     }
     __syncthreads();
-    for (int i = 0; i < tiles; i += 2) {
-      advance(i, odd);
-      if (i + 1 < tiles) advance(i + 1, even);
+    for (int i = 0; i < tiles; ++i) {
+      if (i > 0) finish(i - 1);
+      if (i + 1 < tiles) {
+        load(i + 3);  // where tile i - 1 was
+        copy_wait<2>();
+        prepare(i + 1);
+      }
+      __syncthreads();
     }
     if (tiles > 0) finish(tiles - 1);
+    copy_wait<0>();
   }
 }
 
@@ -528,6 +524,18 @@ static int done() {
   return 0;
 }
 
+template <typename T, int L, bool VEC, bool VBC>
+static int launch_prompt(const Args &a, unsigned blocks, cudaStream_t s) {
+  constexpr int bytes = (int)sizeof(PromptSmem<T, L>);
+  const cudaError_t e = smem_attr_once<ssm_prompt<T, L, VEC, VBC>>(bytes);
+  if (e != cudaSuccess) {
+    cwgk_set_cuda_error((int)e);
+    return -3;
+  }
+  ssm_prompt<T, L, VEC, VBC><<<blocks, Prompt<L>::kThreads, bytes, s>>>(a);
+  return done();
+}
+
 template <typename T, int L>
 static int launch(const cwg_ssm *op, bool step, cudaStream_t s) {
   using G = Geo<L>;
@@ -557,11 +565,10 @@ static int launch(const cwg_ssm *op, bool step, cudaStream_t s) {
   const bool vec = a.per % 8 == 0 && aligned16(op->u) && aligned16(op->dt) && aligned16(op->z) &&
                    aligned16(op->y) && a.p.ldu % E == 0 && a.p.lddt % E == 0 &&
                    a.p.ldy % E == 0 && (!op->z || a.p.ldz % E == 0);
-  if (vec)
-    ssm_prompt<T, L, true><<<(unsigned)blocks, Prompt<L>::kThreads, 0, s>>>(a);
-  else
-    ssm_prompt<T, L, false><<<(unsigned)blocks, Prompt<L>::kThreads, 0, s>>>(a);
-  return done();
+  if (vec && a.vec_bc) return launch_prompt<T, L, true, true>(a, (unsigned)blocks, s);
+  if (vec) return launch_prompt<T, L, true, false>(a, (unsigned)blocks, s);
+  if (a.vec_bc) return launch_prompt<T, L, false, true>(a, (unsigned)blocks, s);
+  return launch_prompt<T, L, false, false>(a, (unsigned)blocks, s);
 }
 
 template <typename T>
