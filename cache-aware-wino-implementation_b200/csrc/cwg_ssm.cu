@@ -76,7 +76,7 @@ __device__ __forceinline__ void load4(const T *p, int i0, int n, bool vec, float
 //     (d, d u) and B, C from shared memory; a channel's L lanes reduce L tokens' sums
 //     together, so that each lane ends up with one token's (L - 1 shuffles per L tokens);
 //   * element warps finish tile i - 1 (skip, gate, full-width row stores), prepare tile
-//     i + 1 (step, d u, B and C next to one another) and load tile i + 3.
+//     i + 1 (step, d u) and start the asynchronous copies of tile i + 3.
 // One barrier per tile.  Bound by the exponentials: N per token and channel at 16 a clock
 // and SM; the elementwise part adds 4 more, and the shared-memory reads of B and C (kept
 // in the input's type) come next.
@@ -84,15 +84,13 @@ template <int L>
 struct Prompt {
   static constexpr int kCH = L <= 4 ? 32 : 128 / L;
   static constexpr int kScan = kCH * L;             // scan threads
-  static constexpr int kElem = 128;                 // element threads
+  static constexpr int kTasks = kTT * kCH / 4;      // 4-channel pieces of a tile
+  static constexpr int kElem = kTasks < 128 ? 128 : kTasks;  // element threads
   static constexpr int kThreads = kScan + kElem;
-  static constexpr int kTasks = kTT * kCH / 8;      // 8-channel pieces of a tile
-  static constexpr int kPieces = (kTT * L + kElem - 1) / kElem;  // 4-state pieces of B, C
   // y rows: the L tokens x 32 / L channels of one store fall in all 32 banks (L = 16: in
   // half of them); read as 16-byte vectors
   static constexpr int kPitch = kCH + (L <= 8 ? 32 / L : 4);
   static_assert(kPitch % 4 == 0 && kCH % 8 == 0, "rows of whole vectors");
-  static_assert(kTasks <= kElem, "one piece per element thread");
   template <typename T>  // tokens a scan warp takes at a time
   static constexpr int kGroup = L > 8 ? L : sizeof(T) == 2 ? 8 : (L > 4 ? L : 4);
 };
@@ -117,42 +115,44 @@ template <int N>
 __device__ __forceinline__ void copy_wait() {  // all but the N newest groups have landed
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-// W elements of a row, of which n exist (VEC: all of them aligned and n whole vectors).
-// Elements of two bytes that are not aligned cannot be copied asynchronously.
-template <typename T, int W, bool VEC>
-__device__ __forceinline__ void copy_row(T *dst, const T *src, int n, const T *safe) {
-  if constexpr (VEC) {
-    constexpr int B = W * (int)sizeof(T) < 16 ? W * (int)sizeof(T) : 16, E = B / (int)sizeof(T);
+// Part of a tile that the element threads copy: W elements at a time of rows of `width`,
+// of which n exist and `rows` hold tokens; consecutive threads take neighbouring
+// pieces.  VEC: pieces of 16 bytes (or W elements if that is less), all aligned and n
+// whole pieces.  Two-byte elements that are not aligned cannot be copied asynchronously.
+template <typename T, int NT, int WIDTH, int W, bool VEC, typename Dst>
+__device__ __forceinline__ void copy_rows(int e, const T *src, size_t ld, int n, int rows,
+                                          Dst dst) {
+  constexpr int B = W * (int)sizeof(T) < 16 ? W * (int)sizeof(T) : 16;
+  constexpr int E = VEC ? B / (int)sizeof(T) : 1, per = WIDTH / E;
 #pragma unroll
-    for (int i = 0; i < W; i += E) copy_async<B>(dst + i, i < n ? src + i : safe, i < n);
-  } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < W; ++i) copy_async<4>(dst + i, i < n ? src + i : safe, i < n);
-  } else {
-#pragma unroll
-    for (int i = 0; i < W; ++i) dst[i] = i < n ? src[i] : from_f32<T>(0.f);
+  for (int q0 = 0; q0 < kTT * per; q0 += NT) {
+    const int q = q0 + e, t = q / per, c = q % per * E;
+    if (kTT * per % NT && q >= kTT * per) break;
+    const bool ok = t < rows && c < n;
+    const T *from = ok ? src + (size_t)t * ld + c : src;
+    if constexpr (E * sizeof(T) >= 4)
+      copy_async<E * (int)sizeof(T)>(dst(t, c), from, ok);
+    else
+      *dst(t, c) = ok ? *from : from_f32<T>(0.f);
   }
+}
+// Barrier of the element warps alone.
+template <int N>
+__device__ __forceinline__ void named_bar() {
+  asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory");
 }
 template <typename T>
-__device__ __forceinline__ void read8(const T *p, float (&f)[8]) {
-  constexpr int E = 16 / (int)sizeof(T);
-#pragma unroll
-  for (int i = 0; i < 8; i += E) {
-    float g[E];
-    unpack(load_raw<T, E>(p + i), g);
-#pragma unroll
-    for (int e = 0; e < E; ++e) f[i + e] = g[e];
-  }
+__device__ __forceinline__ void read4(const T *p, float (&f)[4]) {
+  unpack(load_raw<T, 4>(p), f);
 }
 template <typename T, bool VEC>
-__device__ __forceinline__ void write8(T *p, const float (&f)[8], int n) {
-  constexpr int E = VEC ? 16 / (int)sizeof(T) : 1;
+__device__ __forceinline__ void write4(T *p, const float (&f)[4], int n) {
+  if constexpr (VEC) {
+    store_raw<T, 4>(p, pack<T, 4>(f));
+  } else {
 #pragma unroll
-  for (int i = 0; i < 8; i += E) {
-    float g[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) g[e] = f[i + e];
-    if (i < n) store_raw<T, E>(p + i, pack<T, E>(g));
+    for (int i = 0; i < 4; ++i)
+      if (i < n) p[i] = pack1<T>(f[i]);
   }
 }
 
@@ -161,7 +161,7 @@ template <typename T>
 struct States4 {
   uint4 raw[sizeof(T) / 2];
   __device__ __forceinline__ T *b() { return reinterpret_cast<T *>(raw); }
-  __device__ __forceinline__ T *c() { return reinterpret_cast<T *>(raw) + 4; }
+  __device__ __forceinline__ T *c() { return b() + 4; }
 };
 __device__ __forceinline__ void get_bc(const States4<float> &s, F2 (&b)[2], F2 (&c)[2]) {
   float x[4], y[4];
@@ -183,11 +183,12 @@ __device__ __forceinline__ int turned(int t, int c8, int j) {
   return c8 * 4 + ((j + (c8 >> 1) + 2 * (t & 1)) & 3);
 }
 
-// Shared memory of a CTA: the rows of four tiles, the pairs and sums of two.
+// Shared memory of a CTA: the rows of five tiles (three ahead of the one in work, one
+// behind it), the pairs and sums of two.
 template <typename T, int L>
 struct PromptSmem {
   using G = Prompt<L>;
-  static constexpr int kStages = 4;
+  static constexpr int kStages = 5;
   float4 dx[2][kTT][G::kCH / 2];
   float y[2][kTT][G::kPitch];
   States4<T> bc[kStages][kTT][L];
@@ -298,90 +299,87 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) 
       store_states(line, i0, p.states, a.vec_state, out);
     }
   } else {
-    // ---- 8-channel pieces of the tiles' rows
+    // ---- 4-channel pieces of the tiles' rows
     const int e = tid - G::kScan;
-    const int tt = e / (CH / 8), c8 = e % (CH / 8), c = c8 * 8;
+    const int tt = e / (CH / 4), c4 = e % (CH / 4), c = c4 * 4;
     const bool task = e < G::kTasks && c < nch;
-    float bias[8], skip[8];
+    float bias[4], skip[4];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < 4; ++k) {
       const bool ok = task && c + k < nch;
       bias[k] = ok && p.dt_bias ? p.dt_bias[c0 + c + k] : 0.f;
       skip[k] = ok && p.D ? p.D[c0 + c + k] : 0.f;
     }
-    const T *gu = static_cast<const T *>(p.u), *gd = static_cast<const T *>(p.dt);
-    const T *gz = static_cast<const T *>(p.z);
-    const T *gb = static_cast<const T *>(p.B), *gc = static_cast<const T *>(p.C);
     auto load = [&](int i) {
-      const int t = begin + i * kTT + tt, st = i % NS;
-      const int n = task && t < end ? nch - c : 0;
-      const size_t at = (size_t)(n > 0 ? t : 0);
-      if (e < G::kTasks) {
-        copy_row<T, 8, VEC>(&sh.u[st][tt][c], gu + at * p.ldu + c0 + c, n, gu);
-        copy_row<T, 8, VEC>(&sh.d[st][tt][c], gd + at * p.lddt + c0 + c, n, gd);
-        if (p.z) copy_row<T, 8, VEC>(&sh.z[st][tt][c], gz + at * p.ldz + c0 + c, n, gz);
-      }
-#pragma unroll
-      for (int k = 0; k < G::kPieces; ++k) {
-        const int q = e + k * G::kElem, s = q % L, tq = begin + i * kTT + q / L;
-        if (q < kTT * L) {
-          const int n4 = tq < end ? p.states - s * 4 : 0;
-          const size_t row = (size_t)(n4 > 0 ? tq : 0), col = (size_t)group * p.states + s * 4;
-          copy_row<T, 4, VBC>(sh.bc[st][q / L][s].b(), gb + row * p.ldb + col, n4, gb);
-          copy_row<T, 4, VBC>(sh.bc[st][q / L][s].c(), gc + row * p.ldc + col, n4, gc);
-        }
-      }
+      const int st = i % NS, t0 = begin + i * kTT, rows = end - t0;
+      const size_t at = (size_t)(rows > 0 ? t0 : begin), col = (size_t)group * p.states;
+      auto part = [&](const void *src, long long ld, T(*to)[CH]) {
+        copy_rows<T, G::kElem, CH, 8, VEC>(e, static_cast<const T *>(src) + at * ld + c0,
+                                           (size_t)ld, nch, rows,
+                                           [&](int t, int k) { return &to[t][k]; });
+      };
+      part(p.u, p.ldu, sh.u[st]);
+      part(p.dt, p.lddt, sh.d[st]);
+      if (p.z) part(p.z, p.ldz, sh.z[st]);
+      copy_rows<T, G::kElem, kS * L, 4, VBC>(
+          e, static_cast<const T *>(p.B) + at * p.ldb + col, (size_t)p.ldb, p.states, rows,
+          [&](int t, int k) { return sh.bc[st][t][k / kS].b() + k % kS; });
+      copy_rows<T, G::kElem, kS * L, 4, VBC>(
+          e, static_cast<const T *>(p.C) + at * p.ldc + col, (size_t)p.ldc, p.states, rows,
+          [&](int t, int k) { return sh.bc[st][t][k / kS].c() + k % kS; });
       copy_commit();
     };
-    // pairs (d, d u) of the thread's own piece; rows past the end have d = 0, which leaves
-    // the states as they are
+    // pairs (d, d u); rows past the end have d = 0, which leaves the states as they are
     auto prepare = [&](int i) {
       const bool row = begin + i * kTT + tt < end;
       if (e < G::kTasks) {
-        float u[8], d[8];
-        read8(&sh.u[i % NS][tt][c], u);
-        read8(&sh.d[i % NS][tt][c], d);
+        float u[4], d[4];
+        read4(&sh.u[i % NS][tt][c], u);
+        read4(&sh.d[i % NS][tt][c], d);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < 4; ++k) {
           float v = d[k] + bias[k];
           if (p.flags & CWG_SOFTPLUS) v = softplus(v);
           d[k] = row && c + k < nch ? v : 0.f;
           u[k] = row && c + k < nch ? v * u[k] : 0.f;
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          sh.dx[i & 1][tt][turned(tt, c8, k)] =
+        for (int k = 0; k < 2; ++k)
+          sh.dx[i & 1][tt][turned(tt, c4 >> 1, (c4 & 1) * 2 + k)] =
               make_float4(d[2 * k], u[2 * k], d[2 * k + 1], u[2 * k + 1]);
       }
     };
     auto finish = [&](int i) {
       const int t = begin + i * kTT + tt;
       if (!task || t >= end) return;
-      float u[8], z[8], y[8];
-      read8(&sh.u[i % NS][tt][c], u);
-      read8(&sh.y[i & 1][tt][c], y);
-      if (p.z) read8(&sh.z[i % NS][tt][c], z);
+      float u[4], z[4], y[4];
+      read4(&sh.u[i % NS][tt][c], u);
+      read4(&sh.y[i & 1][tt][c], y);
+      if (p.z) read4(&sh.z[i % NS][tt][c], z);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < 4; ++k) {
         y[k] = fmaf(skip[k], u[k], y[k]);
         if (p.z) y[k] *= silu<T>(z[k]);
       }
-      write8<T, VEC>(static_cast<T *>(p.y) + (size_t)t * p.ldy + c0 + c, y, nch - c);
+      write4<T, VEC>(static_cast<T *>(p.y) + (size_t)t * p.ldy + c0 + c, y, nch - c);
     };
+    // All element threads' copies of a tile have landed when the barrier behind their
+    // waits is passed; the scan warps need B and C, the element threads each other's rows.
     if (tiles > 0) {
       load(0);
       load(1);
       load(2);
-      copy_wait<2>();
-      prepare(0);
+      copy_wait<1>();
     }
+    named_bar<G::kElem>();
+    if (tiles > 0) prepare(0);
     __syncthreads();
     for (int i = 0; i < tiles; ++i) {
       if (i > 0) finish(i - 1);
       if (i + 1 < tiles) {
-        load(i + 3);  // where tile i - 1 was
-        copy_wait<2>();
+        load(i + 3);  // where tile i - 2 was
         prepare(i + 1);
+        copy_wait<1>();  // tile i + 2
       }
       __syncthreads();
     }
@@ -390,10 +388,6 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) 
   }
 }
 
-// ---- one token of each sequence ----------------------------------------------------
-// Bound by the states, 8 N bytes per channel in and out.  A CTA takes RR rows of one
-// channel block: the rows share A, and all their states are loaded before the first is
-// used.  Meanwhile the CTA's threads look together for lines that an earlier row has too.
 template <int L>
 struct Geo {
   static constexpr int kCH = L <= 4 ? 64 : 256 / L;
