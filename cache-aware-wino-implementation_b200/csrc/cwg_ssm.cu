@@ -30,7 +30,7 @@ struct Args {
   bool vec_bc;            // B and C can be read four states at a time
 };
 
-// A lane's four states of one cache line, or zeros.
+// A lane's four states of one cache line (or four values of A's row).
 __device__ __forceinline__ void load_states(const float *line, int i0, int n, bool vec,
                                             float (&h)[kS]) {
   if (vec) {
@@ -87,12 +87,9 @@ struct Prompt {
   static constexpr int kTasks = kTT * kCH / 4;      // 4-channel pieces of a tile
   static constexpr int kElem = kTasks < 128 ? 128 : kTasks;  // element threads
   static constexpr int kThreads = kScan + kElem;
-  // y rows: the L tokens x 32 / L channels of one store fall in all 32 banks (L = 16: in
-  // half of them); read as 16-byte vectors
+  // y rows: the L tokens x 32 / L channels of one store fall in (nearly) all banks
   static constexpr int kPitch = kCH + (L <= 8 ? 32 / L : 4);
   static_assert(kPitch % 4 == 0 && kCH % 8 == 0, "rows of whole vectors");
-  template <typename T>  // tokens a scan warp takes at a time
-  static constexpr int kGroup = L > 8 ? L : sizeof(T) == 2 ? 8 : (L > 4 ? L : 4);
 };
 
 // Asynchronous copy of B bytes into shared memory; zeros where !ok.
@@ -156,26 +153,41 @@ __device__ __forceinline__ void write4(T *p, const float (&f)[4], int n) {
   }
 }
 
-// Four states' B and C of one token, in the input's type.
+__device__ __forceinline__ void unpack_word(uint2 v, float (&f)[2]) {
+  f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y);
+}
+__device__ __forceinline__ void unpack_word(uint2 v, float (&f)[4]) { unpack(v, f); }
+// A lane's four states' B and C of one token, in the input's type.
 template <typename T>
-struct States4 {
-  uint4 raw[sizeof(T) / 2];
-  __device__ __forceinline__ T *b() { return reinterpret_cast<T *>(raw); }
-  __device__ __forceinline__ T *c() { return b() + 4; }
+struct alignas(16) LaneBC {
+  static constexpr int kWords = 2 * kS * (int)sizeof(T) / 8;
+  uint2 raw[kWords];
+  __device__ __forceinline__ T *at(int i) { return reinterpret_cast<T *>(raw) + i; }
+  __device__ __forceinline__ void read(const LaneBC &from) {  // in 16-byte vectors
+#pragma unroll
+    for (int i = 0; i < kWords; i += 2) {
+      const uint4 q = *reinterpret_cast<const uint4 *>(from.raw + i);
+      raw[i] = make_uint2(q.x, q.y);
+      raw[i + 1] = make_uint2(q.z, q.w);
+    }
+  }
+  __device__ __forceinline__ void get(F2 (&b)[kS / 2], F2 (&c)[kS / 2]) const {
+    constexpr int E = 8 / (int)sizeof(T);  // values per word
+    float f[2 * kS];
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      float g[E];
+      unpack_word(raw[i], g);
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[i * E + e] = g[e];
+    }
+#pragma unroll
+    for (int i = 0; i < kS / 2; ++i) {
+      b[i] = f2(f[2 * i], f[2 * i + 1]);
+      c[i] = f2(f[kS + 2 * i], f[kS + 2 * i + 1]);
+    }
+  }
 };
-__device__ __forceinline__ void get_bc(const States4<float> &s, F2 (&b)[2], F2 (&c)[2]) {
-  float x[4], y[4];
-  unpack(s.raw[0], x);
-  unpack(s.raw[1], y);
-  b[0] = f2(x[0], x[1]), b[1] = f2(x[2], x[3]);
-  c[0] = f2(y[0], y[1]), c[1] = f2(y[2], y[3]);
-}
-__device__ __forceinline__ void get_bc(const States4<__nv_bfloat16> &s, F2 (&b)[2], F2 (&c)[2]) {
-  float f[8];
-  unpack(s.raw[0], f);
-  b[0] = f2(f[0], f[1]), b[1] = f2(f[2], f[3]);
-  c[0] = f2(f[4], f[5]), c[1] = f2(f[6], f[7]);
-}
 
 // Where the pairs (d, d u) of channels 2 j, 2 j + 1 of an 8-channel piece are kept in
 // their row: turned so that 8 threads' 16-byte stores fall in all banks.
@@ -191,7 +203,7 @@ struct PromptSmem {
   static constexpr int kStages = 5;
   float4 dx[2][kTT][G::kCH / 2];
   float y[2][kTT][G::kPitch];
-  States4<T> bc[kStages][kTT][L];
+  LaneBC<T> bc[kStages][kTT][L];
   T u[kStages][kTT][G::kCH], d[kStages][kTT][G::kCH], z[kStages][kTT][G::kCH];
 };
 
@@ -226,53 +238,59 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) 
     // ---- lane l of channel ch, states i0 .. i0 + 3
     const int ch = tid / L, l = tid % L, i0 = l * kS;
     const bool mine = ch < nch;
-    float A2[kS] = {0.f, 0.f, 0.f, 0.f}, h[kS] = {0.f, 0.f, 0.f, 0.f};
+    float A2[kS] = {}, h[kS] = {};
     const size_t at = (size_t)(c0 + ch) * p.states;
     float *line = p.state + (size_t)(slot < 0 ? 0 : slot) * p.channels * p.states + at;
     if (mine) {
       load_states(p.A + at, i0, p.states, a.vec_a, A2);
       if (carry) load_states(line, i0, p.states, a.vec_state, h);
     }
-    const F2 a01 = f2(A2[0] * kLog2e, A2[1] * kLog2e), a23 = f2(A2[2] * kLog2e, A2[3] * kLog2e);
-    F2 h01 = f2(h[0], h[1]), h23 = f2(h[2], h[3]);
+    F2 a2[kS / 2], hh[kS / 2];
+#pragma unroll
+    for (int k = 0; k < kS / 2; ++k) {
+      a2[k] = f2(A2[2 * k] * kLog2e, A2[2 * k + 1] * kLog2e);
+      hh[k] = f2(h[2 * k], h[2 * k + 1]);
+    }
     const int at0 = turned(0, ch >> 3, (ch & 7) >> 1) * 4 + (ch & 1) * 2;
     const int at1 = turned(1, ch >> 3, (ch & 7) >> 1) * 4 + (ch & 1) * 2;
     __syncthreads();
     for (int i = 0; i < tiles; ++i) {
       const float *dx = reinterpret_cast<const float *>(sh.dx[i & 1]);
-      const States4<T>(*bc)[L] = sh.bc[i % NS];
+      const LaneBC<T>(*bc)[L] = sh.bc[i % NS];
       float(*ys)[G::kPitch] = sh.y[i & 1];
-      // TG tokens at a time; where registers allow, the next ones' operands are read
+      // TG tokens at a time, their sums reduced together; the next ones' operands are read
       // while these are worked on
-      constexpr int TG = G::template kGroup<T>;
-      constexpr bool kPrefetch = TG * (2 + 2 * (int)sizeof(T)) <= 48;
+      constexpr int TG = L > 8 ? L : 8;
       float2 v[TG];
-      States4<T> w[TG];
+      LaneBC<T> w[TG];
       auto fetch = [&](int t0) {
 #pragma unroll
         for (int t = 0; t < TG; ++t) {
           v[t] = *reinterpret_cast<const float2 *>(dx + (t0 + t) * (CH * 2) + (t & 1 ? at1 : at0));
-          w[t] = bc[t0 + t][l];
+          w[t].read(bc[t0 + t][l]);
         }
       };
       fetch(0);
 #pragma unroll
       for (int t0 = 0; t0 < kTT; t0 += TG) {
+        float y[TG];
         float2 dv[TG];
-        States4<T> sv[TG];
+        LaneBC<T> sv[TG];
 #pragma unroll
         for (int t = 0; t < TG; ++t) dv[t] = v[t], sv[t] = w[t];
-        if (kPrefetch && t0 + TG < kTT) fetch(t0 + TG);
-        float y[TG];
+        if (t0 + TG < kTT) fetch(t0 + TG);
 #pragma unroll
         for (int t = 0; t < TG; ++t) {
-          F2 bv[2], cv[2];
-          get_bc(sv[t], bv, cv);
+          F2 bv[kS / 2], cv[kS / 2], sum;
+          sv[t].get(bv, cv);
           const F2 dd = f2(dv[t].x, dv[t].x), uu = f2(dv[t].y, dv[t].y);
-          const float2 x01 = halves(mul2(dd, a01)), x23 = halves(mul2(dd, a23));
-          h01 = fma2(f2(ex2(x01.x), ex2(x01.y)), h01, mul2(uu, bv[0]));
-          h23 = fma2(f2(ex2(x23.x), ex2(x23.y)), h23, mul2(uu, bv[1]));
-          const float2 s = halves(fma2(h01, cv[0], mul2(h23, cv[1])));
+#pragma unroll
+          for (int k = 0; k < kS / 2; ++k) {
+            const float2 x = halves(mul2(dd, a2[k]));
+            hh[k] = fma2(f2(ex2(x.x), ex2(x.y)), hh[k], mul2(uu, bv[k]));
+            sum = k ? fma2(hh[k], cv[k], sum) : mul2(hh[k], cv[k]);
+          }
+          const float2 s = halves(sum);
           y[t] = s.x + s.y;
         }
 #pragma unroll
@@ -289,13 +307,16 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) 
         }
 #pragma unroll
         for (int g = 0; g < TG; g += L) ys[t0 + g + l][ch] = y[g];
-        if (!kPrefetch && t0 + TG < kTT) fetch(t0 + TG);
       }
       __syncthreads();
     }
     if (slot >= 0 && mine) {
-      const float2 x = halves(h01), y = halves(h23);
-      const float out[kS] = {x.x, x.y, y.x, y.y};
+      float out[kS];
+#pragma unroll
+      for (int k = 0; k < kS / 2; ++k) {
+        const float2 x = halves(hh[k]);
+        out[2 * k] = x.x, out[2 * k + 1] = x.y;
+      }
       store_states(line, i0, p.states, a.vec_state, out);
     }
   } else {
@@ -321,12 +342,12 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) 
       part(p.u, p.ldu, sh.u[st]);
       part(p.dt, p.lddt, sh.d[st]);
       if (p.z) part(p.z, p.ldz, sh.z[st]);
-      copy_rows<T, G::kElem, kS * L, 4, VBC>(
+      copy_rows<T, G::kElem, kS * L, kS, VBC>(
           e, static_cast<const T *>(p.B) + at * p.ldb + col, (size_t)p.ldb, p.states, rows,
-          [&](int t, int k) { return sh.bc[st][t][k / kS].b() + k % kS; });
-      copy_rows<T, G::kElem, kS * L, 4, VBC>(
+          [&](int t, int k) { return sh.bc[st][t][k / kS].at(k % kS); });
+      copy_rows<T, G::kElem, kS * L, kS, VBC>(
           e, static_cast<const T *>(p.C) + at * p.ldc + col, (size_t)p.ldc, p.states, rows,
-          [&](int t, int k) { return sh.bc[st][t][k / kS].c() + k % kS; });
+          [&](int t, int k) { return sh.bc[st][t][k / kS].at(kS + k % kS); });
       copy_commit();
     };
     // pairs (d, d u); rows past the end have d = 0, which leaves the states as they are
@@ -530,31 +551,25 @@ static int launch_prompt(const Args &a, unsigned blocks, cudaStream_t s) {
   return done();
 }
 
-template <typename T, int L>
-static int launch(const cwg_ssm *op, bool step, cudaStream_t s) {
-  using G = Geo<L>;
+static Args make_args(const cwg_ssm *op, int np, size_t esz) {
   Args a;
   a.p = *op;
   if (op->tokens <= 1) a.p.ldu = a.p.lddt = a.p.ldz = a.p.ldy = 0, a.p.ldb = a.p.ldc = 0;
   a.per = op->channels / op->groups;
-  const int ch = step ? G::kCH : Prompt<L>::kCH;
-  a.cblocks = (a.per + ch - 1) / ch;
-  a.vec_state = op->states == G::kNP && aligned16(op->state);
-  a.vec_a = op->states == G::kNP && aligned16(op->A);
-  a.vec_bc = op->states == G::kNP && ((uintptr_t)op->B % (4 * sizeof(T))) == 0 &&
-             ((uintptr_t)op->C % (4 * sizeof(T))) == 0 && a.p.ldb % 4 == 0 && a.p.ldc % 4 == 0;
+  a.cblocks = 0;
+  a.vec_state = op->states == np && aligned16(op->state);
+  a.vec_a = op->states == np && aligned16(op->A);
+  a.vec_bc = op->states == np && ((uintptr_t)op->B % (4 * esz)) == 0 &&
+             ((uintptr_t)op->C % (4 * esz)) == 0 && a.p.ldb % 4 == 0 && a.p.ldc % 4 == 0;
+  return a;
+}
+
+template <typename T, int L>
+static int prompts(const cwg_ssm *op, cudaStream_t s) {
+  Args a = make_args(op, kS * L, sizeof(T));
+  a.cblocks = (a.per + Prompt<L>::kCH - 1) / Prompt<L>::kCH;
   const long long blocks = (long long)op->n_seq * a.cblocks * op->groups;
-  const long long step_blocks = (long long)op->tokens * a.cblocks * op->groups;
-  if ((step ? step_blocks : blocks) > 0x7fffffffLL) return -2;
-  if (step) {
-    // rows that share A as soon as every SM has work all the same
-    if (step_blocks >= 4 * 4 * 148)
-      ssm_token<T, L, 4><<<(unsigned)((long long)((op->tokens + 3) / 4) * a.cblocks * op->groups),
-                           G::kThreads, 0, s>>>(a);
-    else
-      ssm_token<T, L, 1><<<(unsigned)step_blocks, G::kThreads, 0, s>>>(a);
-    return done();
-  }
+  if (blocks > 0x7fffffffLL) return -2;
   constexpr int E = 16 / (int)sizeof(T);
   const bool vec = a.per % 8 == 0 && aligned16(op->u) && aligned16(op->dt) && aligned16(op->z) &&
                    aligned16(op->y) && a.p.ldu % E == 0 && a.p.lddt % E == 0 &&
@@ -563,6 +578,27 @@ static int launch(const cwg_ssm *op, bool step, cudaStream_t s) {
   if (vec) return launch_prompt<T, L, true, false>(a, (unsigned)blocks, s);
   if (a.vec_bc) return launch_prompt<T, L, false, true>(a, (unsigned)blocks, s);
   return launch_prompt<T, L, false, false>(a, (unsigned)blocks, s);
+}
+
+template <typename T, int L>
+static int steps(const cwg_ssm *op, cudaStream_t s) {
+  using G = Geo<L>;
+  Args a = make_args(op, G::kNP, sizeof(T));
+  a.cblocks = (a.per + G::kCH - 1) / G::kCH;
+  const long long blocks = (long long)op->tokens * a.cblocks * op->groups;
+  if (blocks > 0x7fffffffLL) return -2;
+  // rows that share A as soon as every SM has work all the same
+  if (blocks >= 4 * 4 * 148)
+    ssm_token<T, L, 4><<<(unsigned)((long long)((op->tokens + 3) / 4) * a.cblocks * op->groups),
+                         G::kThreads, 0, s>>>(a);
+  else
+    ssm_token<T, L, 1><<<(unsigned)blocks, G::kThreads, 0, s>>>(a);
+  return done();
+}
+
+template <typename T, int L>
+static int launch(const cwg_ssm *op, bool step, cudaStream_t s) {
+  return step ? steps<T, L>(op, s) : prompts<T, L>(op, s);
 }
 
 template <typename T>
