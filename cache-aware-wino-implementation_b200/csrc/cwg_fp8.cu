@@ -243,6 +243,7 @@ struct MatArgs {
   size_t lda_scale, ldw_scale, ldy;
   int m, n, kblocks, per;  // per: k blocks of one cluster rank
   int splits, relu, bf16;
+  int vec_y;               // rows of y are 16-byte aligned
 };
 
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, int x, int y,
@@ -519,6 +520,282 @@ __global__ void __launch_bounds__(Cfg<TN>::kThreads, Cfg<TN>::kMinBlocks)
   }
 }
 
+// ---- many rows: two SMs on one tile ---------------------------------------------------
+// A CTA pair computes 256 rows of a x 256 outputs with tcgen05.mma.cta_group::2: each CTA
+// loads its 128 rows of a and 128 of the 256 rows of w per block of 128 k (32 KB for
+// 512 cycles of MMA; one CTA with a 128 x 256 tile would need 48 KB, which is above what
+// L2 feeds an SM). A block's products fill one of two accumulators of 128 rows x 256
+// columns; the eight promoting warps of each CTA, 32 rows x 128 columns each, read it
+// back, multiply by the row's as[kb] and the 128 columns' ws[kb], and add it to 128 fp32
+// registers a thread, while the other accumulator is being filled: 64 two-column FMAs and
+// 8 loads of 16 columns per thread and block, about half of the block's 512 cycles on two
+// warps per scheduler.  Persistent: a pair walks over tiles, and the rings run on.
+// Rank 0 issues all MMAs; rank 1's MMA warp relays its landed stages to it.
+struct PairCfg {
+  static constexpr int kTile = 256;
+  static constexpr int kPromote = 8;
+  static constexpr int kThreads = (kPromote + 2) * 32;
+  static constexpr int kAcc = 2;
+  static constexpr int kTmem = 512;
+  static constexpr int kStageBytes = 2 * 128 * kTileK;
+  static constexpr int kStages = 6;
+  static constexpr int kBarOff = kStages * kStageBytes;
+  // full[], peer[], empty[], acc_full[2], acc_empty[2], drain
+  static constexpr int kBars = 3 * kStages + 2 * kAcc + 1;
+  static constexpr int kSmem = kBarOff + 8 * kBars + 16 + 1024;
+};
+
+__device__ __forceinline__ void mma_fp8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                             uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Tiles in the order a pair's neighbours take them: bands of 8 tile rows, column by
+// column, so that pairs that run together share rows of a and of w in L2.
+__device__ __forceinline__ void pair_tile(const MatArgs &p, int t, int &m0, int &n0) {
+  const int mt = (p.m + 255) / 256, nt = (p.n + 255) / 256;
+  const int band = t / (8 * nt), rows = min(8, mt - band * 8), r = t - band * 8 * nt;
+  m0 = (band * 8 + r % rows) * 256;
+  n0 = r / rows * 256;
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1)
+    fp8_matmul_pair(const __grid_constant__ CUtensorMap map_a,
+                    const __grid_constant__ CUtensorMap map_w, const MatArgs p, int tiles) {
+  using C = PairCfg;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t sbase = (smem_u32(smem_raw) + 1023) & ~1023u;
+  uint8_t *smem = smem_raw + (sbase - smem_u32(smem_raw));
+  const uint32_t full = sbase + C::kBarOff, peer = full + 8 * C::kStages;
+  const uint32_t empty = peer + 8 * C::kStages, acc_full = empty + 8 * C::kStages;
+  const uint32_t acc_empty = acc_full + 8 * C::kAcc, drain = acc_empty + 8 * C::kAcc;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + C::kBarOff + 8 * C::kBars);
+  volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int mine = pair < tiles ? (tiles - 1 - pair) / pairs + 1 : 0;  // tiles of this pair
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(peer + 8 * i, 1);
+      mbar_init(empty + 8 * i, 1);
+    }
+    for (int i = 0; i < C::kAcc; ++i) {
+      mbar_init(acc_full + 8 * i, 1);
+      mbar_init(acc_empty + 8 * i, 2 * C::kPromote);  // both CTAs' warps, at rank 0
+    }
+    mbar_init(drain, 1);
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == C::kPromote) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)),
+                 "r"(C::kTmem));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    tc_fence_before();
+  }
+  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers exist before any remote arrival
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int total = mine * p.kblocks;  // blocks this pair works through
+
+  if (warp == C::kPromote) {
+    if (rank == 0) {
+      // ---- MMAs of the pair
+      constexpr uint32_t idesc = idesc_fp8(256, 256);
+      bool ok = true;
+      for (int i = 0; i < total; ++i) {
+        const int st = i % C::kStages, ac = i % C::kAcc;
+        const uint32_t ph = (i / C::kStages) & 1;
+        ok = __all_sync(0xffffffffu,
+                        mbar_wait(acc_empty + 8 * ac, ((i / C::kAcc) & 1) ^ 1, abort) &&
+                            mbar_wait(full + 8 * st, ph, abort) &&
+                            mbar_wait(peer + 8 * st, ph, abort));
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t a = desc_sw128(sbase + st * C::kStageBytes);
+        const uint64_t w = desc_sw128(sbase + st * C::kStageBytes + 128 * kTileK);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (elect_one()) mma_fp8_pair(tmem + ac * 256, a + 2 * k, w + 2 * k, idesc, k > 0);
+        __syncwarp();
+        if (elect_one()) tc_commit_pair(empty + 8 * st, 3);
+        if (elect_one()) tc_commit_pair(acc_full + 8 * ac, 3);
+        __syncwarp();
+      }
+      if (!ok) {  // what was issued finishes before anything is freed
+        if (elect_one()) tc_commit_pair(drain, 1);
+        __syncwarp();
+        const unsigned long long t0 = globaltimer();
+        while (!mbar_try(drain, 0) && globaltimer() - t0 < kTimeoutNs) {
+        }
+      }
+    } else {
+      const uint32_t peer0 = mapa_shared(peer, 0);
+      for (int i = 0; i < total; ++i) {
+        const int st = i % C::kStages;
+        if (!__all_sync(0xffffffffu, mbar_wait(full + 8 * st, (i / C::kStages) & 1, abort)))
+          break;
+        if (elect_one()) mbar_arrive_cluster(peer0 + 8 * st);
+        __syncwarp();
+      }
+    }
+  } else if (warp == C::kPromote + 1) {
+    // ---- this CTA's rows of a and of w
+    int i = 0;
+    bool ok = true;
+    for (int j = 0; ok && j < mine; ++j) {
+      int m0, n0;
+      pair_tile(p, pair + j * pairs, m0, n0);
+      for (int kb = 0; kb < p.kblocks; ++kb, ++i) {
+        const int st = i % C::kStages;
+        ok = __all_sync(0xffffffffu,
+                        mbar_wait(empty + 8 * st, ((i / C::kStages) & 1) ^ 1, abort));
+        if (!ok) break;
+        if (elect_one()) {
+          const uint32_t dst = sbase + st * C::kStageBytes;
+          mbar_expect_tx(full + 8 * st, C::kStageBytes);
+          tma_2d(dst, &map_a, kb * kTileK, m0 + (int)rank * 128, full + 8 * st);
+          tma_2d(dst + 128 * kTileK, &map_w, kb * kTileK, n0 + (int)rank * 128, full + 8 * st);
+        }
+        __syncwarp();
+      }
+    }
+    // never leave the CTA with a copy still writing shared memory
+    for (int q = i - C::kStages > 0 ? i - C::kStages : 0; q < i; ++q) {
+      const unsigned long long t0 = globaltimer();
+      while (!mbar_try(full + 8 * (q % C::kStages), (q / C::kStages) & 1) &&
+             globaltimer() - t0 < kTimeoutNs) {
+      }
+    }
+  } else {
+    // ---- promotion
+    using seq::F2;
+    const int quad = warp & 3, half = warp >> 2;
+    const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16) + half * 128;
+    const uint32_t empty0 = mapa_shared(acc_empty, 0);
+    constexpr int kGroup = 4;  // blocks whose scales are read together, one group ahead
+    float as[kGroup], ws[kGroup];
+    int m0 = 0, n0 = 0;
+    const float *asp = p.a_scale, *wsp = p.w_scale;
+    auto locate = [&](int j) {
+      pair_tile(p, pair + j * pairs, m0, n0);
+      const int row = m0 + (int)rank * 128 + quad * 32 + lane, nb = n0 / 128 + half;
+      asp = p.a_scale + (size_t)(row < p.m ? row : p.m - 1) * p.lda_scale;
+      wsp = p.w_scale + (size_t)(nb < (p.n + 127) / 128 ? nb : 0) * p.ldw_scale;
+    };
+    auto fetch = [&](int kb) {
+#pragma unroll
+      for (int k = 0; k < kGroup; ++k) {
+        const bool in = kb + k < p.kblocks;
+        as[k] = in ? asp[kb + k] : 0.f;
+        ws[k] = in ? wsp[kb + k] : 0.f;
+      }
+    };
+    bool ok = true;
+    int i = 0;
+    if (mine > 0) {
+      locate(0);
+      fetch(0);
+    }
+    for (int j = 0; ok && j < mine; ++j) {
+      F2 acc[64];
+#pragma unroll
+      for (int q = 0; q < 64; ++q) acc[q] = seq::f2(0.f, 0.f);
+      for (int kb = 0; ok && kb < p.kblocks; kb += kGroup) {
+        float sc[kGroup];
+#pragma unroll
+        for (int k = 0; k < kGroup; ++k) sc[k] = as[k] * ws[k];
+        if (kb + kGroup < p.kblocks) fetch(kb + kGroup);
+#pragma unroll
+        for (int k = 0; k < kGroup; ++k) {
+          if (kb + k >= p.kblocks) break;
+          const int ac = i % C::kAcc;
+          ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * ac, (i / C::kAcc) & 1, abort));
+          if (!ok) break;
+          tc_fence_after();
+          const F2 s2 = seq::f2(sc[k], sc[k]);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            float v[16];
+            tmem_ld16(trow + ac * 256 + c * 16, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              acc[c * 8 + q] = seq::fma2(seq::f2(v[2 * q], v[2 * q + 1]), s2, acc[c * 8 + q]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (rank == 0)
+              mbar_arrive(acc_empty + 8 * ac);
+            else
+              mbar_arrive_cluster(empty0 + 8 * ac);
+          }
+          ++i;
+        }
+      }
+      const int row = m0 + (int)rank * 128 + quad * 32 + lane, col = n0 + half * 128;
+      if (j + 1 < mine) {  // the next tile's scales come while this one is stored
+        locate(j + 1);
+        fetch(0);
+      }
+      if (!ok || row >= p.m || col >= p.n) continue;
+      const int ncol = min(128, p.n - col);
+      const size_t at = (size_t)row * p.ldy + col;
+      const bool vec = ncol == 128 && p.vec_y;
+#pragma unroll
+      for (int q = 0; q < 64; q += 4) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 h = seq::halves(acc[q + e]);
+          v[2 * e] = h.x, v[2 * e + 1] = h.y;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (p.bias && 2 * q + e < ncol) v[e] += p.bias[col + 2 * q + e];
+          if (p.relu && v[e] < 0.f) v[e] = 0.f;  // NaN stays
+        }
+        if (vec && p.bf16) {
+          *reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(p.y) + at + 2 * q) =
+              seq::pack<__nv_bfloat16, 8>(v);
+        } else if (vec) {
+          float4 *to = reinterpret_cast<float4 *>(static_cast<float *>(p.y) + at + 2 * q);
+          to[0] = make_float4(v[0], v[1], v[2], v[3]);
+          to[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (2 * q + e < ncol) {
+              if (p.bf16)
+                static_cast<__nv_bfloat16 *>(p.y)[at + 2 * q + e] = pack1<__nv_bfloat16>(v[e]);
+              else
+                static_cast<float *>(p.y)[at + 2 * q + e] = v[e];
+            }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // rank 0's MMAs read both CTAs' shared memory and tensor memory
+  if (warp == C::kPromote) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(C::kTmem));
+  }
+}
+
 // Row-major e4m3 matrix [rows][k], rows ld bytes apart, as tiles of box_rows x 128.
 // Reads outside [rows][k] give zeros.
 static int make_map(CUtensorMap *map, const void *base, long long ld, int rows, int k,
@@ -555,13 +832,7 @@ static int make_map(CUtensorMap *map, const void *base, long long ld, int rows, 
   return 0;
 }
 
-template <int TN>
-static int launch(const cwgk_fp8 *op, cudaStream_t s) {
-  using C = Cfg<TN>;
-  CUtensorMap map_a, map_w;
-  int rc = make_map(&map_a, op->a, op->lda, op->m, op->k, TN);
-  if (!rc) rc = make_map(&map_w, op->w, op->ldw, op->n, op->k, 128);
-  if (rc) return rc;
+static MatArgs make_args(const cwgk_fp8 *op) {
   MatArgs p;
   p.a_scale = op->a_scale;
   p.w_scale = op->w_scale;
@@ -573,8 +844,75 @@ static int launch(const cwgk_fp8 *op, cudaStream_t s) {
   p.m = op->m;
   p.n = op->n;
   p.kblocks = (op->k + kTileK - 1) / kTileK;
+  p.per = p.kblocks;
+  p.splits = 1;
   p.relu = op->relu;
   p.bf16 = op->bf16;
+  const long long esz = op->bf16 ? 2 : 4;
+  p.vec_y = ((uintptr_t)op->y & 15) == 0 && (op->m <= 1 || op->ldy * esz % 16 == 0);
+  return p;
+}
+
+// Co-resident pairs of the current device (one CTA per SM; a cluster needs two SMs that
+// can form one), asked once per device.
+static int resident_pairs() {
+  static std::atomic<int> cache[64];
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  int n = cache[dev].load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(sms / 2 * 2));
+  cfg.blockDim = dim3(PairCfg::kThreads);
+  cfg.dynamicSmemBytes = PairCfg::kSmem;
+  if (cudaOccupancyMaxActiveClusters(&n, (const void *)fp8_matmul_pair, &cfg) != cudaSuccess ||
+      n <= 0) {
+    (void)cudaGetLastError();
+    n = sms / 2;
+  }
+  cache[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// The pair kernel where its tiles fill at least half of the pairs.
+static bool pair_pays(const cwgk_fp8 *op) {
+  const long long tiles = (long long)((op->m + 255) / 256) * ((op->n + 255) / 256);
+  return op->m > 128 && tiles >= 37;
+}
+
+static int launch_pair(const cwgk_fp8 *op, cudaStream_t s) {
+  CUtensorMap map_a, map_w;
+  int rc = make_map(&map_a, op->a, op->lda, op->m, op->k, 128);
+  if (!rc) rc = make_map(&map_w, op->w, op->ldw, op->n, op->k, 128);
+  if (rc) return rc;
+  const MatArgs p = make_args(op);
+  const long long tiles = (long long)((op->m + 255) / 256) * ((op->n + 255) / 256);
+  if (tiles * p.kblocks > 0x7fffffffLL) return -2;
+  cudaError_t e = smem_attr_once<fp8_matmul_pair>(PairCfg::kSmem);
+  if (e == cudaSuccess) {
+    const int most = resident_pairs(), pairs = (int)(tiles < most ? tiles : most);
+    if (pairs <= 0) return -3;
+    fp8_matmul_pair<<<(unsigned)(2 * pairs), PairCfg::kThreads, PairCfg::kSmem, s>>>(
+        map_a, map_w, p, (int)tiles);
+    cwgk_count_launch();
+    e = cudaGetLastError();
+  }
+  if (e != cudaSuccess) {
+    cwgk_set_cuda_error((int)e);
+    return -3;
+  }
+  return 0;
+}
+
+template <int TN>
+static int launch(const cwgk_fp8 *op, cudaStream_t s) {
+  using C = Cfg<TN>;
+  CUtensorMap map_a, map_w;
+  int rc = make_map(&map_a, op->a, op->lda, op->m, op->k, TN);
+  if (!rc) rc = make_map(&map_w, op->w, op->ldw, op->n, op->k, 128);
+  if (rc) return rc;
+  MatArgs p = make_args(op);
   const long long tiles = (long long)((op->n + 127) / 128) * ((op->m + TN - 1) / TN);
   int splits = 1;
   while (splits < 8 && tiles * splits * 2 <= 148 * C::kMinBlocks && p.kblocks >= splits * 4)
@@ -633,6 +971,7 @@ int cwgk_fp8_matmul(const cwgk_fp8 *op, void *stream) {
   if (op->m <= 16) return cwg::fp8::launch<16>(op, s);
   if (op->m <= 32) return cwg::fp8::launch<32>(op, s);
   if (op->m <= 64) return cwg::fp8::launch<64>(op, s);
+  if (cwg::fp8::pair_pays(op)) return cwg::fp8::launch_pair(op, s);
   return cwg::fp8::launch<128>(op, s);
 }
 

@@ -393,6 +393,14 @@ def test_fp8_matmul(cuda_dev, dtype, m, n, k):
     check_matmul(cuda_dev, m, n, k, dtype, relu=(m + n) % 2 == 0, with_bias=m != 16)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("m,n,k", [(1300, 1700, 384), (2560, 1024, 129), (2600, 2304, 1000),
+                                   (160, 9500, 100), (4864, 4300, 256)])
+def test_fp8_matmul_pairs(cuda_dev, dtype, m, n, k):
+    """Tiles of 256 x 256, more of them than pairs, cut at every edge."""
+    check_matmul(cuda_dev, m, n, k, dtype, relu=dtype == "fp32", with_bias=True)
+
+
 # ---- the Python mirror's checks ------------------------------------------------------------
 def test_tensors_that_do_not_fit_are_named(cuda_dev):
     dev = cuda_dev
