@@ -243,7 +243,7 @@ struct MatArgs {
   size_t lda_scale, ldw_scale, ldy;
   int m, n, kblocks, per;  // per: k blocks of one cluster rank
   int splits, relu, bf16;
-  int vec_y;               // rows of y are 16-byte aligned
+  int vec_y, vec_scale;    // rows of y and of a_scale are 16-byte aligned
 };
 
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, int x, int y,
@@ -525,23 +525,32 @@ __global__ void __launch_bounds__(Cfg<TN>::kThreads, Cfg<TN>::kMinBlocks)
 // loads its 128 rows of a and 128 of the 256 rows of w per block of 128 k (32 KB for
 // 512 cycles of MMA; one CTA with a 128 x 256 tile would need 48 KB, which is above what
 // L2 feeds an SM). A block's products fill one of two accumulators of 128 rows x 256
-// columns; the eight promoting warps of each CTA, 32 rows x 128 columns each, read it
-// back, multiply by the row's as[kb] and the 128 columns' ws[kb], and add it to 128 fp32
-// registers a thread, while the other accumulator is being filled: 64 two-column FMAs and
-// 8 loads of 16 columns per thread and block, about half of the block's 512 cycles on two
-// warps per scheduler.  Persistent: a pair walks over tiles, and the rings run on.
-// Rank 0 issues all MMAs; rank 1's MMA warp relays its landed stages to it.
+// columns; the sixteen promoting warps of each CTA, 32 rows x 64 columns each, read it
+// back, multiply by the row's as[kb] and the columns' ws[kb], and add it to 64 fp32
+// registers a thread, while the other accumulator is being filled: 32 two-column FMAs and
+// 4 loads of 16 columns per thread and block, which four warps per scheduler overlap.  Persistent: a pair walks over tiles, and the rings run on.
+// Rank 0 issues all MMAs; rank 1's MMA warp relays its landed stages to it.  One warp per
+// CTA keeps the scales of its 128 rows and of the tile's two blocks of w in shared memory,
+// a group of eight blocks ahead: read by every promoting warp from global memory (four of
+// them need the same rows, 32 sectors a load) they cost more than the FMAs, 383 us
+// instead of @@ for 8192 x 8192 x 4096.
 struct PairCfg {
   static constexpr int kTile = 256;
-  static constexpr int kPromote = 8;
-  static constexpr int kThreads = (kPromote + 2) * 32;
+  static constexpr int kPromote = 16;
+  static constexpr int kCols = 4 * kTile / kPromote;  // columns per promoting thread
+  static_assert(kCols == 64, "two biases a lane");
+  static constexpr int kThreads = (kPromote + 3) * 32;
   static constexpr int kAcc = 2;
   static constexpr int kTmem = 512;
   static constexpr int kStageBytes = 2 * 128 * kTileK;
-  static constexpr int kStages = 6;
-  static constexpr int kBarOff = kStages * kStageBytes;
-  // full[], peer[], empty[], acc_full[2], acc_empty[2], drain
-  static constexpr int kBars = 3 * kStages + 2 * kAcc + 1;
+  static constexpr int kStages = 5;
+  static constexpr int kPatchOff = kStages * kStageBytes;  // 32 rows x 64 bytes per warp
+  // scales of kGroupK blocks, twice: [block][128 rows], then [block] of two w blocks
+  static constexpr int kScaleOff = kPatchOff + kPromote * 2048;
+  static constexpr int kScaleBytes = kGroupK * (128 + 2) * 4;
+  static constexpr int kBarOff = kScaleOff + 2 * kScaleBytes;
+  // full[], peer[], empty[], acc_full[2], acc_empty[2], s_full[2], s_empty[2], drain
+  static constexpr int kBars = 3 * kStages + 2 * kAcc + 5;
   static constexpr int kSmem = kBarOff + 8 * kBars + 16 + 1024;
 };
 
@@ -572,7 +581,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
   uint8_t *smem = smem_raw + (sbase - smem_u32(smem_raw));
   const uint32_t full = sbase + C::kBarOff, peer = full + 8 * C::kStages;
   const uint32_t empty = peer + 8 * C::kStages, acc_full = empty + 8 * C::kStages;
-  const uint32_t acc_empty = acc_full + 8 * C::kAcc, drain = acc_empty + 8 * C::kAcc;
+  const uint32_t acc_empty = acc_full + 8 * C::kAcc, s_full = acc_empty + 8 * C::kAcc;
+  const uint32_t s_empty = s_full + 16, drain = s_empty + 16;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + C::kBarOff + 8 * C::kBars);
   volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
@@ -590,6 +600,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
     for (int i = 0; i < C::kAcc; ++i) {
       mbar_init(acc_full + 8 * i, 1);
       mbar_init(acc_empty + 8 * i, 2 * C::kPromote);  // both CTAs' warps, at rank 0
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + 8 * i, 1);
+      mbar_init(s_empty + 8 * i, C::kPromote);
     }
     mbar_init(drain, 1);
     *abort = 0;
@@ -677,111 +691,168 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
              globaltimer() - t0 < kTimeoutNs) {
       }
     }
+  } else if (warp == C::kPromote + 2) {
+    // ---- scales, the next group's in registers while the ring is full
+    float as[4][kGroupK], ws = 0.f;
+    auto fetch = [&](int j, int kb) {
+      int m0, n0;
+      pair_tile(p, pair + j * pairs, m0, n0);
+      m0 += (int)rank * 128;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = m0 + r * 32 + lane;
+        const float *from = p.a_scale + (size_t)(row < p.m ? row : 0) * p.lda_scale + kb;
+#pragma unroll
+        for (int k = 0; k < kGroupK; k += 4) {
+          if (p.vec_scale && kb + k + 4 <= p.kblocks) {
+            const float4 v = *reinterpret_cast<const float4 *>(from + k);
+            as[r][k] = v.x, as[r][k + 1] = v.y, as[r][k + 2] = v.z, as[r][k + 3] = v.w;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) as[r][k + e] = kb + k + e < p.kblocks ? from[k + e] : 0.f;
+          }
+        }
+      }
+      // lanes 0 .. 7: the first block of w, 8 .. 15: the second
+      const int nb = n0 / 128 + lane / kGroupK, b = kb + lane % kGroupK;
+      ws = lane < 2 * kGroupK && nb < (p.n + 127) / 128 && b < p.kblocks
+               ? p.w_scale[(size_t)nb * p.ldw_scale + b]
+               : 0.f;
+    };
+    if (mine > 0) fetch(0, 0);
+    bool ok = true;
+    for (int j = 0, g = 0; ok && j < mine; ++j)
+      for (int kb = 0; kb < p.kblocks; kb += kGroupK, ++g) {
+        ok = __all_sync(0xffffffffu, mbar_wait(s_empty + 8 * (g & 1), ((g >> 1) & 1) ^ 1, abort));
+        if (!ok) break;
+        float *dst = reinterpret_cast<float *>(smem + C::kScaleOff + (g & 1) * C::kScaleBytes);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int k = 0; k < kGroupK; ++k) dst[k * 128 + r * 32 + lane] = as[r][k];
+        if (lane < 2 * kGroupK) dst[kGroupK * 128 + lane] = ws;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_full + 8 * (g & 1));
+        if (kb + kGroupK < p.kblocks)
+          fetch(j, kb + kGroupK);
+        else if (j + 1 < mine)
+          fetch(j + 1, 0);
+      }
   } else {
     // ---- promotion
     using seq::F2;
-    const int quad = warp & 3, half = warp >> 2;
-    const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16) + half * 128;
+    const int quad = warp & 3, part = warp >> 2;
+    const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16) + part * C::kCols;
     const uint32_t empty0 = mapa_shared(acc_empty, 0);
-    constexpr int kGroup = 4;  // blocks whose scales are read together, one group ahead
-    float as[kGroup], ws[kGroup];
-    int m0 = 0, n0 = 0;
-    const float *asp = p.a_scale, *wsp = p.w_scale;
-    auto locate = [&](int j) {
-      pair_tile(p, pair + j * pairs, m0, n0);
-      const int row = m0 + (int)rank * 128 + quad * 32 + lane, nb = n0 / 128 + half;
-      asp = p.a_scale + (size_t)(row < p.m ? row : p.m - 1) * p.lda_scale;
-      wsp = p.w_scale + (size_t)(nb < (p.n + 127) / 128 ? nb : 0) * p.ldw_scale;
-    };
-    auto fetch = [&](int kb) {
-#pragma unroll
-      for (int k = 0; k < kGroup; ++k) {
-        const bool in = kb + k < p.kblocks;
-        as[k] = in ? asp[kb + k] : 0.f;
-        ws[k] = in ? wsp[kb + k] : 0.f;
-      }
-    };
     bool ok = true;
-    int i = 0;
-    if (mine > 0) {
-      locate(0);
-      fetch(0);
-    }
+    int i = 0, g = 0;
     for (int j = 0; ok && j < mine; ++j) {
-      F2 acc[64];
+      F2 acc[C::kCols / 2];
 #pragma unroll
-      for (int q = 0; q < 64; ++q) acc[q] = seq::f2(0.f, 0.f);
-      for (int kb = 0; ok && kb < p.kblocks; kb += kGroup) {
-        float sc[kGroup];
+      for (int q = 0; q < C::kCols / 2; ++q) acc[q] = seq::f2(0.f, 0.f);
+      for (int kb = 0; kb < p.kblocks; ++kb, ++i) {
+        const int ac = i % C::kAcc, k = kb % kGroupK;
+        if (k == 0) ok = mbar_wait(s_full + 8 * (g & 1), (g >> 1) & 1, abort);
+        ok = ok && mbar_wait(acc_full + 8 * ac, (i / C::kAcc) & 1, abort);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const float *sc =
+            reinterpret_cast<const float *>(smem + C::kScaleOff + (g & 1) * C::kScaleBytes);
+        const float scale = sc[k * 128 + quad * 32 + lane] *
+                            sc[kGroupK * 128 + (part * C::kCols / 128) * kGroupK + k];
+        const F2 s2 = seq::f2(scale, scale);
 #pragma unroll
-        for (int k = 0; k < kGroup; ++k) sc[k] = as[k] * ws[k];
-        if (kb + kGroup < p.kblocks) fetch(kb + kGroup);
+        for (int c = 0; c < C::kCols / 16; ++c) {
+          float v[16];
+          tmem_ld16(trow + ac * 256 + c * 16, v);
+          tmem_wait_ld();
 #pragma unroll
-        for (int k = 0; k < kGroup; ++k) {
-          if (kb + k >= p.kblocks) break;
-          const int ac = i % C::kAcc;
-          ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * ac, (i / C::kAcc) & 1, abort));
-          if (!ok) break;
-          tc_fence_after();
-          const F2 s2 = seq::f2(sc[k], sc[k]);
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            float v[16];
-            tmem_ld16(trow + ac * 256 + c * 16, v);
-            tmem_wait_ld();
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-              acc[c * 8 + q] = seq::fma2(seq::f2(v[2 * q], v[2 * q + 1]), s2, acc[c * 8 + q]);
-          }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            if (rank == 0)
-              mbar_arrive(acc_empty + 8 * ac);
-            else
-              mbar_arrive_cluster(empty0 + 8 * ac);
-          }
-          ++i;
+          for (int q = 0; q < 8; ++q)
+            acc[c * 8 + q] = seq::fma2(seq::f2(v[2 * q], v[2 * q + 1]), s2, acc[c * 8 + q]);
         }
+        tc_fence_before();
+        __syncwarp();
+        const bool last = k == kGroupK - 1 || kb == p.kblocks - 1;  // of the group
+        if (lane == 0) {
+          if (rank == 0)
+            mbar_arrive(acc_empty + 8 * ac);
+          else
+            mbar_arrive_cluster(empty0 + 8 * ac);
+          if (last) mbar_arrive(s_empty + 8 * (g & 1));
+        }
+        g += last;
       }
-      const int row = m0 + (int)rank * 128 + quad * 32 + lane, col = n0 + half * 128;
-      if (j + 1 < mine) {  // the next tile's scales come while this one is stored
-        locate(j + 1);
-        fetch(0);
-      }
-      if (!ok || row >= p.m || col >= p.n) continue;
-      const int ncol = min(128, p.n - col);
+      int m0, n0;
+      pair_tile(p, pair + j * pairs, m0, n0);
+      const int row = m0 + (int)rank * 128 + quad * 32 + lane, col = n0 + part * C::kCols;
+      if (!ok || col >= p.n) continue;  // whole warps
+      const int ncol = min(C::kCols, p.n - col);
       const size_t at = (size_t)row * p.ldy + col;
-      const bool vec = ncol == 128 && p.vec_y;
+      const bool vec = ncol == C::kCols && p.vec_y;
+      // the columns' biases, two a lane, handed round by shuffles
+      float bias[2];
 #pragma unroll
-      for (int q = 0; q < 64; q += 4) {
-        float v[8];
+      for (int e = 0; e < 2; ++e)
+        bias[e] = p.bias && e * 32 + lane < ncol ? p.bias[col + e * 32 + lane] : 0.f;
+      auto out = [&](int c) {  // column c of this row, finished
+        const float2 h = seq::halves(acc[c / 2]);
+        float v = c % 2 ? h.y : h.x;
+        if (p.bias) v += __shfl_sync(0xffffffffu, bias[c / 32], c % 32);
+        return p.relu && v < 0.f ? 0.f : v;  // NaN stays
+      };
+      if (vec) {
+        // 64 bytes of each row at a time through a patch of the warp's own, its 16-byte
+        // pieces turned by the row so that neither side has bank conflicts: a store
+        // instruction then writes 8 rows x 64 contiguous bytes instead of 32 rows x 16
+        uint8_t *patch = smem + C::kPatchOff + warp * 2048;
+        const size_t esz = p.bf16 ? 2 : 4;
+        uint8_t *to = static_cast<uint8_t *>(p.y) +
+                      ((size_t)(row - lane) * p.ldy + col) * esz;
+        const int step = p.bf16 ? 32 : 16;  // columns per 64 bytes
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 h = seq::halves(acc[q + e]);
-          v[2 * e] = h.x, v[2 * e + 1] = h.y;
-        }
+        for (int q = 0; q < C::kCols; q += 16) {
+          // 16 columns: two pieces in bf16, four in fp32
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (p.bias && 2 * q + e < ncol) v[e] += p.bias[col + 2 * q + e];
-          if (p.relu && v[e] < 0.f) v[e] = 0.f;  // NaN stays
-        }
-        if (vec && p.bf16) {
-          *reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(p.y) + at + 2 * q) =
-              seq::pack<__nv_bfloat16, 8>(v);
-        } else if (vec) {
-          float4 *to = reinterpret_cast<float4 *>(static_cast<float *>(p.y) + at + 2 * q);
-          to[0] = make_float4(v[0], v[1], v[2], v[3]);
-          to[1] = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
+          for (int k = 0; k < 16; k += 8) {
+            float v[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (2 * q + e < ncol) {
-              if (p.bf16)
-                static_cast<__nv_bfloat16 *>(p.y)[at + 2 * q + e] = pack1<__nv_bfloat16>(v[e]);
-              else
-                static_cast<float *>(p.y)[at + 2 * q + e] = v[e];
+            for (int e = 0; e < 8; ++e) v[e] = out(q + k + e);
+            const int piece = p.bf16 ? (q % 32 + k) / 8 : k / 4;
+            auto put = [&](int c, uint4 w) {
+              *reinterpret_cast<uint4 *>(patch + lane * 64 + ((c ^ (lane >> 1)) & 3) * 16) = w;
+            };
+            if (p.bf16) {
+              put(piece, seq::pack<__nv_bfloat16, 8>(v));
+            } else {
+              const float lo[4] = {v[0], v[1], v[2], v[3]}, hi[4] = {v[4], v[5], v[6], v[7]};
+              put(piece, seq::pack<float, 4>(lo));
+              put(piece + 1, seq::pack<float, 4>(hi));
             }
+          }
+          if ((q + 16) % step) continue;
+          __syncwarp();
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int r = g * 8 + lane / 4, c = lane % 4;
+            const uint4 w =
+                *reinterpret_cast<const uint4 *>(patch + r * 64 + ((c ^ (r >> 1)) & 3) * 16);
+            if (row - lane + r < p.m)
+              *reinterpret_cast<uint4 *>(to + (size_t)r * p.ldy * esz + (q + 16 - step) * esz +
+                                         c * 16) = w;
+          }
+          __syncwarp();
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < C::kCols; ++c) {
+          const float v = out(c);
+          if (row < p.m && c < ncol) {
+            if (p.bf16)
+              static_cast<__nv_bfloat16 *>(p.y)[at + c] = pack1<__nv_bfloat16>(v);
+            else
+              static_cast<float *>(p.y)[at + c] = v;
+          }
         }
       }
     }
@@ -849,6 +920,7 @@ static MatArgs make_args(const cwgk_fp8 *op) {
   p.relu = op->relu;
   p.bf16 = op->bf16;
   const long long esz = op->bf16 ? 2 : 4;
+  p.vec_scale = ((uintptr_t)op->a_scale & 15) == 0 && (op->m <= 1 || op->lda_scale % 4 == 0);
   p.vec_y = ((uintptr_t)op->y & 15) == 0 && (op->m <= 1 || op->ldy * esz % 16 == 0);
   return p;
 }

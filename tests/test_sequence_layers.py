@@ -371,16 +371,17 @@ def on_dev(q, dev):
     return t[:, :q.shape[1]]
 
 
-def check_matmul(dev, m, n, k, dtype, relu, with_bias, seed=15):
+def check_matmul(dev, m, n, k, dtype, relu, with_bias, seed=15, pad=(3, 2)):
     a, a_s, w, w_s, bias = matmul_case(m, n, k, seed)
-    ym, y = wide(torch.zeros(m, n, dtype=DT[dtype]), dev, 3, 2)
+    left, right = pad
+    ym, y = wide(torch.zeros(m, n, dtype=DT[dtype]), dev, left, right)
     flags = (cwg.BF16 if dtype == "bf16" else 0) | (cwg.RELU if relu else 0)
     cwg.fp8_matmul(on_dev(a, dev), a_s.to(dev), on_dev(w, dev), w_s.to(dev),
                    bias.to(dev) if with_bias else None, y, flags)
     cwg.device_status()
     R.close(y, R.matmul(a, a_s, w, w_s, bias if with_bias else None, relu, DT[dtype]),
             f"{m}x{n}x{k}")
-    assert (ym[:, :3] == GUARD).all() and (ym[:, 3 + n:] == GUARD).all()
+    assert (ym[:, :left] == GUARD).all() and (ym[:, left + n:] == GUARD).all()
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
@@ -399,6 +400,8 @@ def test_fp8_matmul(cuda_dev, dtype, m, n, k):
 def test_fp8_matmul_pairs(cuda_dev, dtype, m, n, k):
     """Tiles of 256 x 256, more of them than pairs, cut at every edge."""
     check_matmul(cuda_dev, m, n, k, dtype, relu=dtype == "fp32", with_bias=True)
+    check_matmul(cuda_dev, m, n, k, dtype, relu=False, with_bias=m % 3 == 0,
+                 pad=(8, 24 - n % 8))
 
 
 # ---- the Python mirror's checks ------------------------------------------------------------
