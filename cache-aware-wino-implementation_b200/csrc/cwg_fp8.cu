@@ -630,10 +630,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
       for (int i = 0; i < total; ++i) {
         const int st = i % C::kStages, ac = i % C::kAcc;
         const uint32_t ph = (i / C::kStages) & 1;
-        ok = __all_sync(0xffffffffu,
-                        mbar_wait(acc_empty + 8 * ac, ((i / C::kAcc) & 1) ^ 1, abort) &&
-                            mbar_wait(full + 8 * st, ph, abort) &&
-                            mbar_wait(peer + 8 * st, ph, abort));
+        // the lanes wait for the three barriers side by side: a look at one takes about 100
+        // cycles
+        const uint32_t bar = lane % 3 == 0   ? acc_empty + 8 * ac
+                             : lane % 3 == 1 ? full + 8 * st
+                                             : peer + 8 * st;
+        const uint32_t par = lane % 3 == 0 ? ((i / C::kAcc) & 1) ^ 1 : ph;
+        ok = __all_sync(0xffffffffu, mbar_wait(bar, par, abort));
         if (!ok) break;
         tc_fence_after();
         const uint64_t a = desc_sw128(sbase + st * C::kStageBytes);
@@ -767,21 +770,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
           float v[16];
           tmem_ld16(trow + ac * 256 + c * 16, v);
           tmem_wait_ld();
+          if (c == C::kCols / 16 - 1) {  // all read: the accumulator may be filled again
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if (rank == 0)
+                mbar_arrive(acc_empty + 8 * ac);
+              else
+                mbar_arrive_cluster(empty0 + 8 * ac);
+            }
+          }
 #pragma unroll
           for (int q = 0; q < 8; ++q)
             acc[c * 8 + q] = seq::fma2(seq::f2(v[2 * q], v[2 * q + 1]), s2, acc[c * 8 + q]);
         }
-        tc_fence_before();
-        __syncwarp();
-        const bool last = k == kGroupK - 1 || kb == p.kblocks - 1;  // of the group
-        if (lane == 0) {
-          if (rank == 0)
-            mbar_arrive(acc_empty + 8 * ac);
-          else
-            mbar_arrive_cluster(empty0 + 8 * ac);
-          if (last) mbar_arrive(s_empty + 8 * (g & 1));
+        if (k == kGroupK - 1 || kb == p.kblocks - 1) {  // the group's last block
+          __syncwarp();
+          if (lane == 0) mbar_arrive(s_empty + 8 * (g & 1));
+          ++g;
         }
-        g += last;
       }
       int m0, n0;
       pair_tile(p, pair + j * pairs, m0, n0);
