@@ -522,36 +522,46 @@ __global__ void __launch_bounds__(Cfg<TN>::kThreads, Cfg<TN>::kMinBlocks)
 
 // ---- many rows: two SMs on one tile ---------------------------------------------------
 // A CTA pair computes 256 rows of a x 256 outputs with tcgen05.mma.cta_group::2: each CTA
-// loads its 128 rows of a and 128 of the 256 rows of w per block of 128 k (32 KB for
-// 512 cycles of MMA; one CTA with a 128 x 256 tile would need 48 KB, which is above what
-// L2 feeds an SM). A block's products fill one of two accumulators of 128 rows x 256
-// columns; the sixteen promoting warps of each CTA, 32 rows x 64 columns each, read it
-// back, multiply by the row's as[kb] and the columns' ws[kb], and add it to 64 fp32
-// registers a thread, while the other accumulator is being filled: 32 two-column FMAs and
-// 4 loads of 16 columns per thread and block, which four warps per scheduler overlap.  Persistent: a pair walks over tiles, and the rings run on.
-// Rank 0 issues all MMAs; rank 1's MMA warp relays its landed stages to it.  One warp per
-// CTA keeps the scales of its 128 rows and of the tile's two blocks of w in shared memory,
-// a group of eight blocks ahead: read by every promoting warp from global memory (four of
-// them need the same rows, 32 sectors a load) they cost more than the FMAs, 383 us
-// instead of @@ for 8192 x 8192 x 4096.
+// loads its 128 rows of a and 128 of the 256 rows of w per block of 128 k (32 KB for the
+// 512 cycles of its MMAs; one CTA with a 128 x 256 tile would need 48 KB).  A block's
+// products fill one of two accumulators of 128 rows x 256 columns; the eight promoting
+// warps of each CTA, 32 rows x 128 columns each, read it back, multiply by the row's
+// as[kb] and the 128 columns' ws[kb], and add it to 128 fp32 registers a thread while the
+// other accumulator is being filled.
+//
+// What bounds it is the promoting warps' chain of latencies per block (barrier, tensor
+// memory, hand-over), not their arithmetic, so that chain is what the code shortens: a
+// chunk of 32 columns is always on its way from tensor memory while the one before it is
+// added, the next block's first chunk too; that takes 64 more registers a thread, which
+// the warps that only issue give up.
+//
+// Persistent: a pair walks over tiles, and the rings run on.  Rank 0 issues all MMAs; rank
+// 1's MMA warp relays its landed stages to it.  One warp per CTA keeps the scales of its
+// 128 rows, those of the tile's two blocks of w, and the biases in shared memory, a group
+// of eight blocks ahead.
 struct PairCfg {
-  static constexpr int kTile = 256;
-  static constexpr int kPromote = 16;
-  static constexpr int kCols = 4 * kTile / kPromote;  // columns per promoting thread
-  static_assert(kCols == 64, "two biases a lane");
-  static constexpr int kThreads = (kPromote + 3) * 32;
+  static constexpr int kN = 256;
+  static constexpr int kPromote = 8;               // warps 4 .. 11
+  static constexpr int kCols = 4 * kN / kPromote;  // columns per promoting thread
+  static constexpr int kThreads = 4 * 32 + kPromote * 32;
+  // registers: 168 a thread at launch, 384 threads; 72 x 128 + 216 x 256 are as many
+  static constexpr int kRegsFew = 72, kRegsMany = 216;
   static constexpr int kAcc = 2;
   static constexpr int kTmem = 512;
-  static constexpr int kStageBytes = 2 * 128 * kTileK;
-  static constexpr int kStages = 5;
+  static constexpr int kStageBytes = (128 + kN / 2) * kTileK;
+  static constexpr int kStages = 6;
   static constexpr int kPatchOff = kStages * kStageBytes;  // 32 rows x 64 bytes per warp
   // scales of kGroupK blocks, twice: [block][128 rows], then [block] of two w blocks
-  static constexpr int kScaleOff = kPatchOff + kPromote * 2048;
+  static constexpr int kScaleOff = kPatchOff + kPromote * 32 * 64;
   static constexpr int kScaleBytes = kGroupK * (128 + 2) * 4;
-  static constexpr int kBarOff = kScaleOff + 2 * kScaleBytes;
-  // full[], peer[], empty[], acc_full[2], acc_empty[2], s_full[2], s_empty[2], drain
+  // biases of three tiles: the scale warp may be two tiles ahead of a promoting warp's stores
+  static constexpr int kBiasOff = kScaleOff + 2 * kScaleBytes;
+  static constexpr int kBarOff = kBiasOff + 3 * kN * 4;
+  // full[], peer[], empty[], acc_full[], acc_empty[], s_full[2], s_empty[2], drain
   static constexpr int kBars = 3 * kStages + 2 * kAcc + 5;
   static constexpr int kSmem = kBarOff + 8 * kBars + 16 + 1024;
+  static_assert(kAcc == 2, "the promoting warps take the accumulators in turn");
+  static_assert(kRegsFew * 128 + kRegsMany * 256 <= 168 * kThreads, "registers at launch");
 };
 
 __device__ __forceinline__ void mma_fp8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
@@ -563,13 +573,69 @@ __device__ __forceinline__ void mma_fp8_pair(uint32_t d_tmem, uint64_t a_desc, u
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// 32 columns of one lane; valid after tmem_wait_ld.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
+      "%28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // Tiles in the order a pair's neighbours take them: bands of 8 tile rows, column by
 // column, so that pairs that run together share rows of a and of w in L2.
 __device__ __forceinline__ void pair_tile(const MatArgs &p, int t, int &m0, int &n0) {
-  const int mt = (p.m + 255) / 256, nt = (p.n + 255) / 256;
+  const int mt = (p.m + 255) / 256, nt = (p.n + PairCfg::kN - 1) / PairCfg::kN;
   const int band = t / (8 * nt), rows = min(8, mt - band * 8), r = t - band * 8 * nt;
   m0 = (band * 8 + r % rows) * 256;
-  n0 = r / rows * 256;
+  n0 = r / rows * PairCfg::kN;
+}
+
+// A warp's 32 rows x COLS columns, 64 bytes of each row at a time through a patch of its
+// own, whose 16-byte pieces are turned by the row so that neither side has bank conflicts:
+// a store instruction then writes 64 bytes of 8 rows instead of 16 bytes of 32.
+template <typename T, int COLS>
+__device__ __forceinline__ void store_rows(uint8_t *patch, const seq::F2 (&acc)[COLS / 2],
+                                           const MatArgs &p, int row, int col, int lane) {
+  constexpr int E = 16 / (int)sizeof(T), kRound = 4 * E;  // columns per 64 bytes
+#pragma unroll
+  for (int c0 = 0; c0 < COLS; c0 += kRound) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float v[E];
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        const float2 f = seq::halves(acc[(c0 + k * E + e) / 2]);
+        v[e] = f.x, v[e + 1] = f.y;
+      }
+      *reinterpret_cast<uint4 *>(patch + lane * 64 + ((k ^ (lane >> 1)) & 3) * 16) =
+          seq::pack<T, E>(v);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int r = g * 8 + lane / 4, c = lane % 4;
+      const uint4 w = *reinterpret_cast<const uint4 *>(patch + r * 64 + ((c ^ (r >> 1)) & 3) * 16);
+      if (row - lane + r < p.m)
+        *reinterpret_cast<uint4 *>(static_cast<T *>(p.y) + (size_t)(row - lane + r) * p.ldy + col +
+                                   c0 + c * E) = w;
+    }
+    __syncwarp();
+  }
 }
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1)
@@ -609,7 +675,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == C::kPromote) {
+  if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(tmem_slot)),
                  "r"(C::kTmem));
@@ -622,10 +688,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
   const uint32_t tmem = *tmem_slot;
   const int total = mine * p.kblocks;  // blocks this pair works through
 
-  if (warp == C::kPromote) {
+  if (warp < 4) {
+  regs_dec<C::kRegsFew>();
+  if (warp == 0) {
     if (rank == 0) {
       // ---- MMAs of the pair
-      constexpr uint32_t idesc = idesc_fp8(256, 256);
+      constexpr uint32_t idesc = idesc_fp8(256, C::kN);
       bool ok = true;
       for (int i = 0; i < total; ++i) {
         const int st = i % C::kStages, ac = i % C::kAcc;
@@ -643,7 +711,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
         const uint64_t w = desc_sw128(sbase + st * C::kStageBytes + 128 * kTileK);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (elect_one()) mma_fp8_pair(tmem + ac * 256, a + 2 * k, w + 2 * k, idesc, k > 0);
+          if (elect_one()) mma_fp8_pair(tmem + ac * C::kN, a + 2 * k, w + 2 * k, idesc, k > 0);
         __syncwarp();
         if (elect_one()) tc_commit_pair(empty + 8 * st, 3);
         if (elect_one()) tc_commit_pair(acc_full + 8 * ac, 3);
@@ -666,7 +734,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
         __syncwarp();
       }
     }
-  } else if (warp == C::kPromote + 1) {
+  } else if (warp == 1) {
     // ---- this CTA's rows of a and of w
     int i = 0;
     bool ok = true;
@@ -682,7 +750,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
           const uint32_t dst = sbase + st * C::kStageBytes;
           mbar_expect_tx(full + 8 * st, C::kStageBytes);
           tma_2d(dst, &map_a, kb * kTileK, m0 + (int)rank * 128, full + 8 * st);
-          tma_2d(dst + 128 * kTileK, &map_w, kb * kTileK, n0 + (int)rank * 128, full + 8 * st);
+          tma_2d(dst + 128 * kTileK, &map_w, kb * kTileK, n0 + (int)rank * (C::kN / 2), full + 8 * st);
         }
         __syncwarp();
       }
@@ -694,9 +762,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
              globaltimer() - t0 < kTimeoutNs) {
       }
     }
-  } else if (warp == C::kPromote + 2) {
+  } else if (warp == 2) {
     // ---- scales, the next group's in registers while the ring is full
-    float as[4][kGroupK], ws = 0.f;
+    float as[4][kGroupK], ws = 0.f, bias[C::kN / 32] = {};
     auto fetch = [&](int j, int kb) {
       int m0, n0;
       pair_tile(p, pair + j * pairs, m0, n0);
@@ -721,6 +789,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
       ws = lane < 2 * kGroupK && nb < (p.n + 127) / 128 && b < p.kblocks
                ? p.w_scale[(size_t)nb * p.ldw_scale + b]
                : 0.f;
+      if (kb == 0 && p.bias) {
+#pragma unroll
+        for (int e = 0; e < C::kN / 32; ++e)
+          bias[e] = n0 + e * 32 + lane < p.n ? p.bias[n0 + e * 32 + lane] : 0.f;
+      }
     };
     if (mine > 0) fetch(0, 0);
     bool ok = true;
@@ -734,6 +807,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
 #pragma unroll
           for (int k = 0; k < kGroupK; ++k) dst[k * 128 + r * 32 + lane] = as[r][k];
         if (lane < 2 * kGroupK) dst[kGroupK * 128 + lane] = ws;
+        if (kb == 0) {
+          float *to = reinterpret_cast<float *>(smem + C::kBiasOff) + j % 3 * C::kN;
+#pragma unroll
+          for (int e = 0; e < C::kN / 32; ++e) to[e * 32 + lane] = bias[e];
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(s_full + 8 * (g & 1));
         if (kb + kGroupK < p.kblocks)
@@ -741,120 +819,105 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
         else if (j + 1 < mine)
           fetch(j + 1, 0);
       }
+  }
   } else {
     // ---- promotion
+    regs_inc<C::kRegsMany>();
     using seq::F2;
-    const int quad = warp & 3, part = warp >> 2;
-    const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16) + part * C::kCols;
-    const uint32_t empty0 = mapa_shared(acc_empty, 0);
+    const int quad = warp & 3, half = (warp - 4) >> 2;
+    const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16) + half * C::kCols;
+    const uint32_t free_at = mapa_shared(acc_empty, 0);  // rank 0 waits for both CTAs' warps
+    uint8_t *patch = smem + C::kPatchOff + (warp - 4) * (32 * 64);
+    constexpr int kChunks = C::kCols / 32;
+    static_assert(kChunks % 2 == 0, "a block begins with the first buffer");
+    uint32_t buf[2][32];
     bool ok = true;
-    int i = 0, g = 0;
+    int ac = 0, par = 0, g = 0;  // accumulator, parity of its round, group of scales
     for (int j = 0; ok && j < mine; ++j) {
+      int m0, n0;
+      pair_tile(p, pair + j * pairs, m0, n0);
       F2 acc[C::kCols / 2];
 #pragma unroll
       for (int q = 0; q < C::kCols / 2; ++q) acc[q] = seq::f2(0.f, 0.f);
-      for (int kb = 0; kb < p.kblocks; ++kb, ++i) {
-        const int ac = i % C::kAcc, k = kb % kGroupK;
+      bool begun = false;  // the block's first chunk is on its way already
+      for (int kb = 0; kb < p.kblocks; ++kb) {
+        const int k = kb % kGroupK;
         if (k == 0) ok = mbar_wait(s_full + 8 * (g & 1), (g >> 1) & 1, abort);
-        ok = ok && mbar_wait(acc_full + 8 * ac, (i / C::kAcc) & 1, abort);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after();
         const float *sc =
             reinterpret_cast<const float *>(smem + C::kScaleOff + (g & 1) * C::kScaleBytes);
-        const float scale = sc[k * 128 + quad * 32 + lane] *
-                            sc[kGroupK * 128 + (part * C::kCols / 128) * kGroupK + k];
+        const float scale =
+            sc[k * 128 + quad * 32 + lane] * sc[kGroupK * 128 + half * kGroupK + k];
+        if (!begun) {
+          ok = __all_sync(0xffffffffu, ok && mbar_wait(acc_full + 8 * ac, par, abort));
+          if (!ok) break;
+          tc_fence_after();
+          tmem_ld32(trow + ac * C::kN, buf[0]);
+        }
         const F2 s2 = seq::f2(scale, scale);
+        const int next = ac ^ 1, next_par = par ^ ac;
 #pragma unroll
-        for (int c = 0; c < C::kCols / 16; ++c) {
-          float v[16];
-          tmem_ld16(trow + ac * 256 + c * 16, v);
+        for (int c = 0; c < kChunks; ++c) {
+          bool ready = false;  // a look at the next block, while this one's last chunk comes
+          if (c + 1 == kChunks && kb + 1 < p.kblocks)
+            ready = mbar_test(acc_full + 8 * next, next_par);
           tmem_wait_ld();
-          if (c == C::kCols / 16 - 1) {  // all read: the accumulator may be filled again
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-              if (rank == 0)
-                mbar_arrive(acc_empty + 8 * ac);
-              else
-                mbar_arrive_cluster(empty0 + 8 * ac);
+          if (c + 1 < kChunks) {
+            tmem_ld32(trow + ac * C::kN + (c + 1) * 32, buf[(c + 1) & 1]);
+          } else {
+            tc_fence_before();  // all read: the accumulator may be filled again
+            begun = __all_sync(0xffffffffu, ready);
+            if (elect_one()) mbar_arrive_cluster(free_at + 8 * ac);
+            if (begun) {
+              tc_fence_after();
+              tmem_ld32(trow + next * C::kN, buf[0]);
             }
           }
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
-            acc[c * 8 + q] = seq::fma2(seq::f2(v[2 * q], v[2 * q + 1]), s2, acc[c * 8 + q]);
+          for (int q = 0; q < 16; ++q)
+            acc[c * 16 + q] = seq::fma2(seq::f2(__uint_as_float(buf[c & 1][2 * q]),
+                                                __uint_as_float(buf[c & 1][2 * q + 1])),
+                                        s2, acc[c * 16 + q]);
         }
         if (k == kGroupK - 1 || kb == p.kblocks - 1) {  // the group's last block
           __syncwarp();
           if (lane == 0) mbar_arrive(s_empty + 8 * (g & 1));
           ++g;
         }
+        par = next_par;
+        ac = next;
       }
-      int m0, n0;
-      pair_tile(p, pair + j * pairs, m0, n0);
-      const int row = m0 + (int)rank * 128 + quad * 32 + lane, col = n0 + part * C::kCols;
+      const int row = m0 + (int)rank * 128 + quad * 32 + lane, col = n0 + half * C::kCols;
       if (!ok || col >= p.n) continue;  // whole warps
       const int ncol = min(C::kCols, p.n - col);
-      const size_t at = (size_t)row * p.ldy + col;
-      const bool vec = ncol == C::kCols && p.vec_y;
-      // the columns' biases, two a lane, handed round by shuffles
-      float bias[2];
+      if (p.bias) {
+        const float *bias = reinterpret_cast<const float *>(smem + C::kBiasOff) +
+                            j % 3 * C::kN + half * C::kCols;
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        bias[e] = p.bias && e * 32 + lane < ncol ? p.bias[col + e * 32 + lane] : 0.f;
-      auto out = [&](int c) {  // column c of this row, finished
-        const float2 h = seq::halves(acc[c / 2]);
-        float v = c % 2 ? h.y : h.x;
-        if (p.bias) v += __shfl_sync(0xffffffffu, bias[c / 32], c % 32);
-        return p.relu && v < 0.f ? 0.f : v;  // NaN stays
-      };
-      if (vec) {
-        // 64 bytes of each row at a time through a patch of the warp's own, its 16-byte
-        // pieces turned by the row so that neither side has bank conflicts: a store
-        // instruction then writes 8 rows x 64 contiguous bytes instead of 32 rows x 16
-        uint8_t *patch = smem + C::kPatchOff + warp * 2048;
-        const size_t esz = p.bf16 ? 2 : 4;
-        uint8_t *to = static_cast<uint8_t *>(p.y) +
-                      ((size_t)(row - lane) * p.ldy + col) * esz;
-        const int step = p.bf16 ? 32 : 16;  // columns per 64 bytes
-#pragma unroll
-        for (int q = 0; q < C::kCols; q += 16) {
-          // 16 columns: two pieces in bf16, four in fp32
-#pragma unroll
-          for (int k = 0; k < 16; k += 8) {
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = out(q + k + e);
-            const int piece = p.bf16 ? (q % 32 + k) / 8 : k / 4;
-            auto put = [&](int c, uint4 w) {
-              *reinterpret_cast<uint4 *>(patch + lane * 64 + ((c ^ (lane >> 1)) & 3) * 16) = w;
-            };
-            if (p.bf16) {
-              put(piece, seq::pack<__nv_bfloat16, 8>(v));
-            } else {
-              const float lo[4] = {v[0], v[1], v[2], v[3]}, hi[4] = {v[4], v[5], v[6], v[7]};
-              put(piece, seq::pack<float, 4>(lo));
-              put(piece + 1, seq::pack<float, 4>(hi));
-            }
-          }
-          if ((q + 16) % step) continue;
-          __syncwarp();
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const int r = g * 8 + lane / 4, c = lane % 4;
-            const uint4 w =
-                *reinterpret_cast<const uint4 *>(patch + r * 64 + ((c ^ (r >> 1)) & 3) * 16);
-            if (row - lane + r < p.m)
-              *reinterpret_cast<uint4 *>(to + (size_t)r * p.ldy * esz + (q + 16 - step) * esz +
-                                         c * 16) = w;
-          }
-          __syncwarp();
+        for (int c = 0; c < C::kCols; c += 4) {
+          const float4 f = *reinterpret_cast<const float4 *>(bias + c);
+          acc[c / 2] = seq::add2(acc[c / 2], seq::f2(f.x, f.y));
+          acc[c / 2 + 1] = seq::add2(acc[c / 2 + 1], seq::f2(f.z, f.w));
         }
-      } else {
+      }
+      if (p.relu) {
+#pragma unroll
+        for (int c = 0; c < C::kCols / 2; ++c) {
+          const float2 f = seq::halves(acc[c]);
+          acc[c] = seq::f2(f.x < 0.f ? 0.f : f.x, f.y < 0.f ? 0.f : f.y);  // NaN stays
+        }
+      }
+      if (ncol == C::kCols && p.vec_y) {
+        if (p.bf16)
+          store_rows<__nv_bfloat16, C::kCols>(patch, acc, p, row, col, lane);
+        else
+          store_rows<float, C::kCols>(patch, acc, p, row, col, lane);
+      } else if (row < p.m) {
+        const size_t at = (size_t)row * p.ldy + col;
 #pragma unroll
         for (int c = 0; c < C::kCols; ++c) {
-          const float v = out(c);
-          if (row < p.m && c < ncol) {
+          const float2 f = seq::halves(acc[c / 2]);
+          const float v = c % 2 ? f.y : f.x;
+          if (c < ncol) {
             if (p.bf16)
               static_cast<__nv_bfloat16 *>(p.y)[at + c] = pack1<__nv_bfloat16>(v);
             else
@@ -867,7 +930,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();  // rank 0's MMAs read both CTAs' shared memory and tensor memory
-  if (warp == C::kPromote) {
+  if (warp == 0) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                  "r"(C::kTmem));
@@ -956,17 +1019,19 @@ static int resident_pairs() {
 
 // The pair kernel where its tiles fill at least half of the pairs.
 static bool pair_pays(const cwgk_fp8 *op) {
-  const long long tiles = (long long)((op->m + 255) / 256) * ((op->n + 255) / 256);
+  const long long tiles =
+      (long long)((op->m + 255) / 256) * ((op->n + PairCfg::kN - 1) / PairCfg::kN);
   return op->m > 128 && tiles >= 37;
 }
 
 static int launch_pair(const cwgk_fp8 *op, cudaStream_t s) {
   CUtensorMap map_a, map_w;
   int rc = make_map(&map_a, op->a, op->lda, op->m, op->k, 128);
-  if (!rc) rc = make_map(&map_w, op->w, op->ldw, op->n, op->k, 128);
+  if (!rc) rc = make_map(&map_w, op->w, op->ldw, op->n, op->k, PairCfg::kN / 2);
   if (rc) return rc;
   const MatArgs p = make_args(op);
-  const long long tiles = (long long)((op->m + 255) / 256) * ((op->n + 255) / 256);
+  const long long tiles =
+      (long long)((op->m + 255) / 256) * ((op->n + PairCfg::kN - 1) / PairCfg::kN);
   if (tiles * p.kblocks > 0x7fffffffLL) return -2;
   cudaError_t e = smem_attr_once<fp8_matmul_pair>(PairCfg::kSmem);
   if (e == cudaSuccess) {
