@@ -52,23 +52,6 @@ __device__ __forceinline__ void store_states(float *line, int i0, int n, bool ve
   }
 }
 
-// Four values of one row of B or C as fp32; those at and past n read as zero.
-template <typename T>
-__device__ __forceinline__ void load4(const T *p, int i0, int n, bool vec, float (&f)[4]) {
-  if (vec) {
-    if constexpr (sizeof(T) == 4) {
-      unpack(*reinterpret_cast<const uint4 *>(p + i0), f);
-    } else {
-      const uint2 v = *reinterpret_cast<const uint2 *>(p + i0);
-      f[0] = __uint_as_float(v.x << 16), f[1] = __uint_as_float(v.x & 0xFFFF0000u);
-      f[2] = __uint_as_float(v.y << 16), f[3] = __uint_as_float(v.y & 0xFFFF0000u);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = i0 + i < n ? to_f32(p[i0 + i]) : 0.f;
-  }
-}
-
 // ---- prompts --------------------------------------------------------------------
 // One CTA per (sequence, block of kCH channels of one group) walks the sequence in tiles
 // of kTT tokens, its warps in two roles that work on neighbouring tiles at the same time:
@@ -416,7 +399,32 @@ struct Geo {
   static constexpr int kNP = kS * L;
 };
 
-template <typename T, int L, int RR>
+// One row's B or C of a lane: four values, as they are in memory.
+template <typename T, bool VEC>
+struct Four {
+  typename Raw<T, VEC ? 4 : 1>::type raw[VEC ? 1 : 4];
+  __device__ __forceinline__ void load(const T *p, int n) {  // n of them exist
+    if constexpr (VEC) {
+      raw[0] = n > 0 ? load_raw<T, 4>(p) : zero_raw<T, 4>();
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[i] = i < n ? p[i] : from_f32<T>(0.f);
+    }
+  }
+  __device__ __forceinline__ void get(F2 (&v)[2]) const {
+    float f[4];
+    if constexpr (VEC) {
+      unpack(raw[0], f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = to_f32(raw[i]);
+    }
+    v[0] = f2(f[0], f[1]), v[1] = f2(f[2], f[3]);
+  }
+};
+
+// VEC: states == 4 L, and state, A, B and C can be read four states at a time.
+template <typename T, int L, int RR, bool VEC>
 __global__ void __launch_bounds__(Geo<L>::kThreads) ssm_token(const Args a) {
   constexpr int CH = Geo<L>::kCH, NT = Geo<L>::kThreads;
   const cwg_ssm &p = a.p;
@@ -427,47 +435,57 @@ __global__ void __launch_bounds__(Geo<L>::kThreads) ssm_token(const Args a) {
   const int ch = tid / L, l = tid % L, i0 = l * kS;
   const int in = cblk * CH + ch, c = group * a.per + in;
   const bool mine = in < a.per;
-  const size_t width = (size_t)p.channels * p.states, at = (size_t)c * p.states;
+  const int rows = min(RR, p.tokens - r0);
+  const size_t width = (size_t)p.channels * p.states;
+  float *state = p.state + (size_t)c * p.states;
   // Rows r0 + l, r0 + l + L, ... of the channel are lane l's: it computes their steps and
   // finishes their outputs (with more lanes than rows, lane l takes row l % RR too, which
   // only lane l = row stores).
   constexpr int E = L < RR ? RR / L : 1;
-  float h[RR][kS], u[E], d[E], z[E];
   int slot[RR];
   bool bad = false;
 #pragma unroll
   for (int k = 0; k < RR; ++k) {
-    const int r = r0 + k;
-    slot[k] = r >= p.tokens ? -1 : p.slots ? p.slots[r] : r;
+    slot[k] = k >= rows ? -1 : p.slots ? p.slots[r0 + k] : r0 + k;
     if (slot[k] >= p.n_slots) slot[k] = -1, bad = true;
   }
+  float h[RR][kS], A2[kS] = {0.f, 0.f, 0.f, 0.f}, u[E], d[E], z[E];
+  Four<T, VEC> bv[RR], cv[RR];
 #pragma unroll
   for (int k = 0; k < RR; ++k) {
 #pragma unroll
     for (int i = 0; i < kS; ++i) h[k][i] = 0.f;
     if (mine && slot[k] >= 0)
-      load_states(p.state + (size_t)slot[k] * width + at, i0, p.states, a.vec_state, h[k]);
+      load_states(state + (size_t)slot[k] * width, i0, p.states, VEC, h[k]);
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const int r = r0 + (L < RR ? e * L + l : l % RR);
-    const size_t rr = (size_t)(r < p.tokens ? r : 0);
+    const int k = L < RR ? e * L + l : l % RR;
+    const size_t r = (size_t)(r0 + (k < rows ? k : 0));
     u[e] = d[e] = z[e] = 0.f;
     if (mine) {
-      u[e] = to_f32(static_cast<const T *>(p.u)[rr * p.ldu + c]);
-      d[e] = to_f32(static_cast<const T *>(p.dt)[rr * p.lddt + c]);
-      if (p.z) z[e] = to_f32(static_cast<const T *>(p.z)[rr * p.ldz + c]);
+      u[e] = to_f32(static_cast<const T *>(p.u)[r * p.ldu + c]);
+      d[e] = to_f32(static_cast<const T *>(p.dt)[r * p.lddt + c]);
+      if (p.z) z[e] = to_f32(static_cast<const T *>(p.z)[r * p.ldz + c]);
     }
   }
-  float A2[kS] = {0.f, 0.f, 0.f, 0.f};
-  if (mine) load_states(p.A + at, i0, p.states, a.vec_a, A2);
+  const T *Brow =
+      static_cast<const T *>(p.B) + (size_t)r0 * p.ldb + (size_t)group * p.states + i0;
+  const T *Crow =
+      static_cast<const T *>(p.C) + (size_t)r0 * p.ldc + (size_t)group * p.states + i0;
 #pragma unroll
-  for (int i = 0; i < kS; ++i) A2[i] *= kLog2e;
+  for (int k = 0; k < RR; ++k) {
+    bv[k].load(Brow + (size_t)k * p.ldb, k < rows ? p.states - i0 : 0);
+    cv[k].load(Crow + (size_t)k * p.ldc, k < rows ? p.states - i0 : 0);
+  }
+  if (mine) load_states(p.A + (size_t)c * p.states, i0, p.states, VEC, A2);
+  const F2 a01 = f2(A2[0] * kLog2e, A2[1] * kLog2e), a23 = f2(A2[2] * kLog2e, A2[3] * kLog2e);
   const float bias = mine && p.dt_bias ? p.dt_bias[c] : 0.f;
   const float skip = mine && p.D ? p.D[c] : 0.f;
   if (p.slots) {
     int taken = 0;
-    for (int i = tid; i < r0 + RR - 1 && i < p.tokens; i += NT) {
+    const int upto = min(r0 + RR - 1, p.tokens);
+    for (int i = tid; i < upto; i += NT) {
       const int other = p.slots[i];
 #pragma unroll
       for (int k = 0; k < RR; ++k) taken |= (i < r0 + k && other == slot[k]) << k;
@@ -489,37 +507,37 @@ __global__ void __launch_bounds__(Geo<L>::kThreads) ssm_token(const Args a) {
     if (p.flags & CWG_SOFTPLUS) d[e] = softplus(d[e]);
     z[e] = p.z ? silu<T>(z[e]) : 1.f;
   }
-  const T *Brow = static_cast<const T *>(p.B) + (size_t)r0 * p.ldb + (size_t)group * p.states;
-  const T *Crow = static_cast<const T *>(p.C) + (size_t)r0 * p.ldc + (size_t)group * p.states;
   float out[E] = {};
 #pragma unroll
   for (int k = 0; k < RR; ++k) {
-    if (RR > 1 && r0 + k >= p.tokens) break;
     // lane and piece that hold row k's step
     constexpr unsigned kAll = 0xffffffffu;
     const int from = L < RR ? k % L : k, e = L < RR ? k / L : 0;
     const float step = L > 1 && RR > 1 ? __shfl_sync(kAll, d[e], from, L) : d[e];
     const float uk = L > 1 && RR > 1 ? __shfl_sync(kAll, u[e], from, L) : u[e];
-    float bv[4], cv[4];
-    load4(Brow + (size_t)k * p.ldb, i0, p.states, a.vec_bc, bv);
-    load4(Crow + (size_t)k * p.ldc, i0, p.states, a.vec_bc, cv);
     const float du = step * uk;
-    float y = 0.f;
-#pragma unroll
-    for (int i = 0; i < kS; ++i) {
-      h[k][i] = fmaf(ex2(step * A2[i]), h[k][i], du * bv[i]);
-      y = fmaf(h[k][i], cv[i], y);
-    }
+    F2 b[2], q[2];
+    bv[k].get(b);
+    cv[k].get(q);
+    const F2 ss = f2(step, step), dd = f2(du, du);
+    const float2 x01 = halves(mul2(ss, a01)), x23 = halves(mul2(ss, a23));
+    const F2 h01 = fma2(f2(ex2(x01.x), ex2(x01.y)), f2(h[k][0], h[k][1]), mul2(dd, b[0]));
+    const F2 h23 = fma2(f2(ex2(x23.x), ex2(x23.y)), f2(h[k][2], h[k][3]), mul2(dd, b[1]));
+    const float2 s = halves(fma2(h01, q[0], mul2(h23, q[1])));
+    float y = s.x + s.y;
 #pragma unroll
     for (int o = L / 2; o > 0; o >>= 1) y += __shfl_xor_sync(kAll, y, o);
-    if (mine && slot[k] >= 0)
-      store_states(p.state + (size_t)slot[k] * width + at, i0, p.states, a.vec_state, h[k]);
+    if (mine && slot[k] >= 0) {
+      const float2 lo = halves(h01), hi = halves(h23);
+      const float w[kS] = {lo.x, lo.y, hi.x, hi.y};
+      store_states(state + (size_t)slot[k] * width, i0, p.states, VEC, w);
+    }
     if (l == from || RR == 1) out[e] = y;
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int k = L < RR ? e * L + l : l;
-    if (mine && k < RR && r0 + k < p.tokens) {
+    if (mine && k < rows) {
       const float y = fmaf(skip, u[e], out[e]) * z[e];
       static_cast<T *>(p.y)[(size_t)(r0 + k) * p.ldy + c] = pack1<T>(y);
     }
@@ -588,11 +606,18 @@ static int steps(const cwg_ssm *op, cudaStream_t s) {
   const long long blocks = (long long)op->tokens * a.cblocks * op->groups;
   if (blocks > 0x7fffffffLL) return -2;
   // rows that share A as soon as every SM has work all the same
-  if (blocks >= 4 * 4 * 148)
-    ssm_token<T, L, 4><<<(unsigned)((long long)((op->tokens + 3) / 4) * a.cblocks * op->groups),
-                         G::kThreads, 0, s>>>(a);
+  const bool four = blocks >= 4 * 4 * 148, vec = a.vec_state && a.vec_a && a.vec_bc;
+  const unsigned grid =
+      four ? (unsigned)((long long)((op->tokens + 3) / 4) * a.cblocks * op->groups)
+           : (unsigned)blocks;
+  if (four && vec)
+    ssm_token<T, L, 4, true><<<grid, G::kThreads, 0, s>>>(a);
+  else if (four)
+    ssm_token<T, L, 4, false><<<grid, G::kThreads, 0, s>>>(a);
+  else if (vec)
+    ssm_token<T, L, 1, true><<<grid, G::kThreads, 0, s>>>(a);
   else
-    ssm_token<T, L, 1><<<(unsigned)blocks, G::kThreads, 0, s>>>(a);
+    ssm_token<T, L, 1, false><<<grid, G::kThreads, 0, s>>>(a);
   return done();
 }
 
