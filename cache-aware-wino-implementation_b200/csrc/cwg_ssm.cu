@@ -392,47 +392,46 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) 
   }
 }
 
-template <int L>
+template <int V, int L>
 struct Geo {
-  static constexpr int kCH = L <= 4 ? 64 : 256 / L;
+  static constexpr int kCH = V * L <= 4 ? 64 : 256 / (V * L);
   static constexpr int kThreads = kCH * L;
-  static constexpr int kNP = kS * L;
+  static constexpr int kNP = 4 * V * L;
 };
 
-// One row's B or C of a lane: four values, as they are in memory.
-template <typename T, bool VEC>
-struct Four {
-  typename Raw<T, VEC ? 4 : 1>::type raw[VEC ? 1 : 4];
+// One row's B or C of a lane: 4 V values, as they are in memory.
+template <typename T, int V, bool VEC>
+struct Row4 {
+  static constexpr int E = !VEC ? 1 : V * 4 * (int)sizeof(T) >= 16 ? 16 / (int)sizeof(T) : 4;
+  typename Raw<T, E>::type raw[4 * V / E];
   __device__ __forceinline__ void load(const T *p, int n) {  // n of them exist
-    if constexpr (VEC) {
-      raw[0] = n > 0 ? load_raw<T, 4>(p) : zero_raw<T, 4>();
-    } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) raw[i] = i < n ? p[i] : from_f32<T>(0.f);
-    }
+    for (int i = 0; i < 4 * V; i += E) raw[i / E] = i < n ? load_raw<T, E>(p + i) : zero_raw<T, E>();
   }
-  __device__ __forceinline__ void get(F2 (&v)[2]) const {
-    float f[4];
-    if constexpr (VEC) {
-      unpack(raw[0], f);
-    } else {
+  __device__ __forceinline__ void get(F2 (&v)[2 * V]) const {
+    float f[4 * V];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) f[i] = to_f32(raw[i]);
+    for (int i = 0; i < 4 * V; i += E) {
+      float g[E];
+      unpack(raw[i / E], g);
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[i + e] = g[e];
     }
-    v[0] = f2(f[0], f[1]), v[1] = f2(f[2], f[3]);
+#pragma unroll
+    for (int i = 0; i < 2 * V; ++i) v[i] = f2(f[2 * i], f[2 * i + 1]);
   }
 };
 
-// VEC: states == 4 L, and state, A, B and C can be read four states at a time.
-template <typename T, int L, int RR, bool VEC>
-__global__ void __launch_bounds__(Geo<L>::kThreads) ssm_token(const Args a) {
-  constexpr int CH = Geo<L>::kCH, NT = Geo<L>::kThreads;
+// 4 V states per lane: 8 where there are that many, since what a row costs besides its
+// states (step, shuffles, addresses) is then paid by half as many threads.
+// VEC: states == 4 V L, and state, A, B and C can be read in whole vectors.
+template <typename T, int V, int L, int RR, bool VEC>
+__global__ void __launch_bounds__(Geo<V, L>::kThreads) ssm_token(const Args a) {
+  constexpr int CH = Geo<V, L>::kCH, NT = Geo<V, L>::kThreads;
   const cwg_ssm &p = a.p;
   const int tid = threadIdx.x;
-  const int cblk = blockIdx.x % a.cblocks;
-  const int group = (blockIdx.x / a.cblocks) % p.groups;
-  const int r0 = blockIdx.x / (a.cblocks * p.groups) * RR;
-  const int ch = tid / L, l = tid % L, i0 = l * kS;
+  const int cblk = blockIdx.x, group = blockIdx.y, r0 = (int)blockIdx.z * RR;
+  const int ch = tid / L, l = tid % L, i0 = l * 4 * V;
   const int in = cblk * CH + ch, c = group * a.per + in;
   const bool mine = in < a.per;
   const int rows = min(RR, p.tokens - r0);
@@ -449,14 +448,17 @@ __global__ void __launch_bounds__(Geo<L>::kThreads) ssm_token(const Args a) {
     slot[k] = k >= rows ? -1 : p.slots ? p.slots[r0 + k] : r0 + k;
     if (slot[k] >= p.n_slots) slot[k] = -1, bad = true;
   }
-  float h[RR][kS], A2[kS] = {0.f, 0.f, 0.f, 0.f}, u[E], d[E], z[E];
-  Four<T, VEC> bv[RR], cv[RR];
+  float h[RR][V][kS], u[E], d[E], z[E];
+  Row4<T, V, VEC> bv[RR], cv[RR];
 #pragma unroll
   for (int k = 0; k < RR; ++k) {
 #pragma unroll
-    for (int i = 0; i < kS; ++i) h[k][i] = 0.f;
-    if (mine && slot[k] >= 0)
-      load_states(state + (size_t)slot[k] * width, i0, p.states, VEC, h[k]);
+    for (int v = 0; v < V; ++v) {
+#pragma unroll
+      for (int i = 0; i < kS; ++i) h[k][v][i] = 0.f;
+      if (mine && slot[k] >= 0)
+        load_states(state + (size_t)slot[k] * width, i0 + 4 * v, p.states, VEC, h[k][v]);
+    }
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) {
@@ -478,8 +480,14 @@ __global__ void __launch_bounds__(Geo<L>::kThreads) ssm_token(const Args a) {
     bv[k].load(Brow + (size_t)k * p.ldb, k < rows ? p.states - i0 : 0);
     cv[k].load(Crow + (size_t)k * p.ldc, k < rows ? p.states - i0 : 0);
   }
-  if (mine) load_states(p.A + (size_t)c * p.states, i0, p.states, VEC, A2);
-  const F2 a01 = f2(A2[0] * kLog2e, A2[1] * kLog2e), a23 = f2(A2[2] * kLog2e, A2[3] * kLog2e);
+  F2 a2[2 * V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    float f[kS] = {0.f, 0.f, 0.f, 0.f};
+    if (mine) load_states(p.A + (size_t)c * p.states, i0 + 4 * v, p.states, VEC, f);
+    a2[2 * v] = f2(f[0] * kLog2e, f[1] * kLog2e);
+    a2[2 * v + 1] = f2(f[2] * kLog2e, f[3] * kLog2e);
+  }
   const float bias = mine && p.dt_bias ? p.dt_bias[c] : 0.f;
   const float skip = mine && p.D ? p.D[c] : 0.f;
   if (p.slots) {
@@ -497,7 +505,9 @@ __global__ void __launch_bounds__(Geo<L>::kThreads) ssm_token(const Args a) {
           slot[k] = -1;
           bad = true;
 #pragma unroll
-          for (int i = 0; i < kS; ++i) h[k][i] = 0.f;
+          for (int v = 0; v < V; ++v)
+#pragma unroll
+            for (int i = 0; i < kS; ++i) h[k][v][i] = 0.f;
         }
     }
   }
@@ -516,21 +526,27 @@ __global__ void __launch_bounds__(Geo<L>::kThreads) ssm_token(const Args a) {
     const float step = L > 1 && RR > 1 ? __shfl_sync(kAll, d[e], from, L) : d[e];
     const float uk = L > 1 && RR > 1 ? __shfl_sync(kAll, u[e], from, L) : u[e];
     const float du = step * uk;
-    F2 b[2], q[2];
+    F2 b[2 * V], q[2 * V], sum;
     bv[k].get(b);
     cv[k].get(q);
     const F2 ss = f2(step, step), dd = f2(du, du);
-    const float2 x01 = halves(mul2(ss, a01)), x23 = halves(mul2(ss, a23));
-    const F2 h01 = fma2(f2(ex2(x01.x), ex2(x01.y)), f2(h[k][0], h[k][1]), mul2(dd, b[0]));
-    const F2 h23 = fma2(f2(ex2(x23.x), ex2(x23.y)), f2(h[k][2], h[k][3]), mul2(dd, b[1]));
-    const float2 s = halves(fma2(h01, q[0], mul2(h23, q[1])));
+#pragma unroll
+    for (int i = 0; i < 2 * V; ++i) {
+      float *hh = h[k][i / 2] + i % 2 * 2;
+      const float2 x = halves(mul2(ss, a2[i]));
+      const F2 w = fma2(f2(ex2(x.x), ex2(x.y)), f2(hh[0], hh[1]), mul2(dd, b[i]));
+      sum = i ? fma2(w, q[i], sum) : mul2(w, q[i]);
+      const float2 f = halves(w);
+      hh[0] = f.x, hh[1] = f.y;
+    }
+    const float2 s = halves(sum);
     float y = s.x + s.y;
 #pragma unroll
     for (int o = L / 2; o > 0; o >>= 1) y += __shfl_xor_sync(kAll, y, o);
     if (mine && slot[k] >= 0) {
-      const float2 lo = halves(h01), hi = halves(h23);
-      const float w[kS] = {lo.x, lo.y, hi.x, hi.y};
-      store_states(state + (size_t)slot[k] * width, i0, p.states, VEC, w);
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        store_states(state + (size_t)slot[k] * width, i0 + 4 * v, p.states, VEC, h[k][v]);
     }
     if (l == from || RR == 1) out[e] = y;
   }
@@ -569,7 +585,8 @@ static int launch_prompt(const Args &a, unsigned blocks, cudaStream_t s) {
   return done();
 }
 
-static Args make_args(const cwg_ssm *op, int np, size_t esz) {
+// lane: values of B and C that are read at a time.
+static Args make_args(const cwg_ssm *op, int np, int lane, size_t esz) {
   Args a;
   a.p = *op;
   if (op->tokens <= 1) a.p.ldu = a.p.lddt = a.p.ldz = a.p.ldy = 0, a.p.ldb = a.p.ldc = 0;
@@ -577,14 +594,15 @@ static Args make_args(const cwg_ssm *op, int np, size_t esz) {
   a.cblocks = 0;
   a.vec_state = op->states == np && aligned16(op->state);
   a.vec_a = op->states == np && aligned16(op->A);
-  a.vec_bc = op->states == np && ((uintptr_t)op->B % (4 * esz)) == 0 &&
-             ((uintptr_t)op->C % (4 * esz)) == 0 && a.p.ldb % 4 == 0 && a.p.ldc % 4 == 0;
+  a.vec_bc = op->states == np && ((uintptr_t)op->B % (lane * esz)) == 0 &&
+             ((uintptr_t)op->C % (lane * esz)) == 0 && a.p.ldb % lane == 0 &&
+             a.p.ldc % lane == 0;
   return a;
 }
 
 template <typename T, int L>
 static int prompts(const cwg_ssm *op, cudaStream_t s) {
-  Args a = make_args(op, kS * L, sizeof(T));
+  Args a = make_args(op, kS * L, 4, sizeof(T));
   a.cblocks = (a.per + Prompt<L>::kCH - 1) / Prompt<L>::kCH;
   const long long blocks = (long long)op->n_seq * a.cblocks * op->groups;
   if (blocks > 0x7fffffffLL) return -2;
@@ -598,32 +616,33 @@ static int prompts(const cwg_ssm *op, cudaStream_t s) {
   return launch_prompt<T, L, false, false>(a, (unsigned)blocks, s);
 }
 
-template <typename T, int L>
+template <typename T, int V, int L>
 static int steps(const cwg_ssm *op, cudaStream_t s) {
-  using G = Geo<L>;
-  Args a = make_args(op, G::kNP, sizeof(T));
+  using G = Geo<V, L>;
+  Args a = make_args(op, G::kNP, V * 4 * sizeof(T) >= 16 ? 16 / (int)sizeof(T) : 4, sizeof(T));
   a.cblocks = (a.per + G::kCH - 1) / G::kCH;
+  if (op->groups > 65535 || op->tokens > 65535) return -2;
+  // two rows that share A as soon as every SM has work all the same (256 rows of 4096 x 16:
+  // 38.4 us with four)
   const long long blocks = (long long)op->tokens * a.cblocks * op->groups;
-  if (blocks > 0x7fffffffLL) return -2;
-  // rows that share A as soon as every SM has work all the same
-  const bool four = blocks >= 4 * 4 * 148, vec = a.vec_state && a.vec_a && a.vec_bc;
-  const unsigned grid =
-      four ? (unsigned)((long long)((op->tokens + 3) / 4) * a.cblocks * op->groups)
-           : (unsigned)blocks;
-  if (four && vec)
-    ssm_token<T, L, 4, true><<<grid, G::kThreads, 0, s>>>(a);
-  else if (four)
-    ssm_token<T, L, 4, false><<<grid, G::kThreads, 0, s>>>(a);
+  const bool two = blocks >= 4 * 2 * 148, vec = a.vec_state && a.vec_a && a.vec_bc;
+  const dim3 grid((unsigned)a.cblocks, (unsigned)op->groups,
+                  (unsigned)(two ? (op->tokens + 1) / 2 : op->tokens));
+  if (two && vec)
+    ssm_token<T, V, L, 2, true><<<grid, G::kThreads, 0, s>>>(a);
+  else if (two)
+    ssm_token<T, V, L, 2, false><<<grid, G::kThreads, 0, s>>>(a);
   else if (vec)
-    ssm_token<T, L, 1, true><<<grid, G::kThreads, 0, s>>>(a);
+    ssm_token<T, V, L, 1, true><<<grid, G::kThreads, 0, s>>>(a);
   else
-    ssm_token<T, L, 1, false><<<grid, G::kThreads, 0, s>>>(a);
+    ssm_token<T, V, L, 1, false><<<grid, G::kThreads, 0, s>>>(a);
   return done();
 }
 
 template <typename T, int L>
 static int launch(const cwg_ssm *op, bool step, cudaStream_t s) {
-  return step ? steps<T, L>(op, s) : prompts<T, L>(op, s);
+  constexpr int V = L > 1 ? 2 : 1;
+  return step ? steps<T, V, L / V>(op, s) : prompts<T, L>(op, s);
 }
 
 template <typename T>

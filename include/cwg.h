@@ -275,7 +275,8 @@ typedef struct cwg_ssm {
 size_t cwg_ssm_workspace_bytes(int tokens, int n_seq, int channels, int states);
 int cwg_ssm_scan(const cwg_ssm *op, void *workspace, size_t workspace_bytes, void *stream);
 
-/* One token of each of op->tokens sequences: row i, line slots[i], updated in place. */
+/* One token of each of op->tokens sequences (at most 65535): row i, line slots[i], updated
+ * in place. */
 int cwg_ssm_step(const cwg_ssm *op, void *stream);
 
 /* ---- 8-bit matrix product with scales per block of 128 (DEVICE pointers) ------- */
