@@ -8,7 +8,7 @@
 //
 // Prompts: a thread owns four channels and a run of consecutive
 // rows, so that a row is read once (plus K - 1 rows of halo per run) and the
-// window slides through registers while the next four rows are loaded.
+// window slides through registers while the next eight rows are loaded.
 // The K - 1 first rows of a sequence, which need the cache line, are all computed
 // by the thread whose run holds the sequence's first row, and that thread stores
 // the new line after it: no other thread reads a line, so the old line can be
@@ -24,7 +24,7 @@ namespace seq {
 __device__ unsigned int g_seq_status;
 
 constexpr int kConvThreads = 128;
-constexpr int kAhead = 4;          // rows per step; the next step's are loaded meanwhile
+constexpr int kAhead = 8;          // rows per step; the next step's are loaded meanwhile
 constexpr int kStartsInSmem = 1024;
 
 struct ConvArgs {
@@ -198,42 +198,53 @@ __global__ void __launch_bounds__(kConvThreads) conv1d_prompt(const ConvArgs a) 
     h[j].from(t >= 0 && t < a.tokens ? load_raw<T, V>(x + (size_t)t * a.ldx + c)
                                      : zero_raw<T, V>());
   }
+  const T *px = x + (size_t)t0 * a.ldx + c;  // of row t
+  T *py = y + (size_t)t0 * a.ldy + c;
   typename Raw<T, V>::type raw[kAhead], next[kAhead];
-  auto fetch = [&](int t) {
+  auto fetch = [&](const T *from, int left) {  // kAhead rows, of which `left` are the run's
+    if (left >= kAhead) {
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i)
-      next[i] = t + i < t1 ? load_raw<T, V>(x + (size_t)(t + i) * a.ldx + c) : zero_raw<T, V>();
+      for (int i = 0; i < kAhead; ++i) next[i] = load_raw<T, V>(from + i * a.ldx);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        next[i] = i < left ? load_raw<T, V>(from + i * a.ldx) : zero_raw<T, V>();
+    }
   };
-  fetch(t0);
+  fetch(px, t1 - t0);
   for (int t = t0; t < t1; t += kAhead) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) raw[i] = next[i];
-    fetch(t + kAhead);
-    if (t - begin >= K - 1 && t + kAhead <= end) {  // all of one sequence, as nearly always
+    px += kAhead * a.ldx;
+    fetch(px, t1 - t - kAhead);
+    if (t - begin >= K - 1 && t + kAhead <= end && t + kAhead <= t1) {
+      // all of one sequence, as nearly always
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         Chan<V> xv;
         xv.from(raw[i]);
-        store_raw<T, V>(y + (size_t)(t + i) * a.ldy + c, window_row<T, V, K, ACT>(w, b, h, xv));
+        store_raw<T, V>(py + i * a.ldy, window_row<T, V, K, ACT>(w, b, h, xv));
         slide<V, K>(h, xv);
       }
-      continue;
-    }
-#pragma unroll 1
-    for (int i = 0; i < kAhead; ++i) {
-      if (t + i >= t1) break;
-      while (s + 1 < a.n_seq && starts[s + 1] <= t + i) {
-        ++s;
-        begin = starts[s];
-        end = starts[s + 1];
-        if (begin < 0 || end > a.tokens) end = begin = 0;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (t + i < t1) {
+          while (s + 1 < a.n_seq && starts[s + 1] <= t + i) {
+            ++s;
+            begin = starts[s];
+            end = starts[s + 1];
+            if (begin < 0 || end > a.tokens) end = begin = 0;
+          }
+          Chan<V> xv;
+          xv.from(raw[i]);
+          if (t + i < end && t + i - begin >= K - 1)
+            store_raw<T, V>(py + i * a.ldy, window_row<T, V, K, ACT>(w, b, h, xv));
+          slide<V, K>(h, xv);
+        }
       }
-      Chan<V> xv;
-      xv.from(i == 0 ? raw[0] : i == 1 ? raw[1] : i == 2 ? raw[2] : raw[3]);
-      if (t + i < end && t + i - begin >= K - 1)
-        store_raw<T, V>(y + (size_t)(t + i) * a.ldy + c, window_row<T, V, K, ACT>(w, b, h, xv));
-      slide<V, K>(h, xv);
     }
+    py += kAhead * a.ldy;
   }
 }
 
@@ -302,10 +313,15 @@ static int launch_conv1d(const cwgk_conv1d *op, bool step, cudaStream_t stream) 
   a.n_slots = op->n_slots;
   a.channels = op->channels;
   const int warps = (op->channels + 32 * V - 1) / (32 * V);
+  const int rows = step ? op->n_seq : op->tokens;
   a.wc = warps >= 3 ? 4 : warps;
   a.cblocks = (warps + a.wc - 1) / a.wc;
-  const int rows = step ? op->n_seq : op->tokens;
-  a.run = step ? 1 : 32;
+  // Long runs share the weights and the first rows' halo; the run is halved until every SM
+  // has 16 warps (16384 x 4096 bf16: 58 us with 128 or 64 rows, 61 with 32; 1237 x 1001
+  // fp32: 17, 11.5, 9.3 us with 128, 64, 32).
+  a.run = step ? 1 : 128;
+  while (!step && a.run > kAhead && (long long)warps * ((rows + a.run - 1) / a.run) < 148 * 16)
+    a.run /= 2;
   a.runs = rows > 0 ? (rows + a.run - 1) / a.run : 1;
   const int per = 4 / a.wc;
   const long long blocks = (long long)a.cblocks * ((a.runs + per - 1) / per);
