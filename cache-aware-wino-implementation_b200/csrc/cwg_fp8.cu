@@ -44,21 +44,25 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
       __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
   return (uint32_t)lo | (uint32_t)hi << 16;
 }
-// Codes of v / s without a division per element.  t = v r with r = 1 / s rounded is off
-// the quotient by at most 2^-23 of it, so the rounded quotient lies between
-// t (1 - 2^-22) and t (1 + 2^-22), themselves rounded; rounding to e4m3 is monotone, so
-// where both ends have the same code that is the quotient's.  Otherwise (about one in
-// 2^17 values) the division decides.
+// Codes of v / s, the quotients rounded to fp32 first.  With r = 1 / s correctly rounded
+// and q = v r, one correction q + (v - q s) r gives the correctly rounded quotient
+// (Markstein 1990) as long as v - q s is exact: 1.5 two-wide instructions per element
+// instead of a division.  A test of the interval around v r, with the division only where
+// two codes are possible, does not pay for bf16 data: its quotients are often exactly
+// between two codes (30.5 against 16.9 us for 8192 x 4096).
 __device__ __forceinline__ uint32_t codes4(const float *v, float s, float r) {
   using namespace seq;
-  const F2 rr = f2(r, r), down = f2(1.f - 0x1p-22f, 1.f - 0x1p-22f),
-           up = f2(1.f + 0x1p-22f, 1.f + 0x1p-22f);
-  const F2 t0 = mul2(f2(v[0], v[1]), rr), t1 = mul2(f2(v[2], v[3]), rr);
-  const float2 a = halves(mul2(t0, down)), b = halves(mul2(t1, down));
-  const float2 c = halves(mul2(t0, up)), d = halves(mul2(t1, up));
-  const uint32_t q = e4m3x4(a.x, a.y, b.x, b.y);
-  if (q == e4m3x4(c.x, c.y, d.x, d.y)) return q;
-  return e4m3x4(__fdiv_rn(v[0], s), __fdiv_rn(v[1], s), __fdiv_rn(v[2], s), __fdiv_rn(v[3], s));
+  const F2 rr = f2(r, r), minus = f2(-s, -s);
+  float2 c[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const F2 x = f2(v[2 * i], v[2 * i + 1]), q = mul2(x, rr);
+    c[i] = halves(fma2(fma2(q, minus, x), rr, q));
+  }
+  return e4m3x4(c[0].x, c[0].y, c[1].x, c[1].y);
+}
+__device__ __noinline__ uint32_t divided4(float a, float b, float c, float d, float s) {
+  return e4m3x4(__fdiv_rn(a, s), __fdiv_rn(b, s), __fdiv_rn(c, s), __fdiv_rn(d, s));
 }
 
 struct QuantArgs {
@@ -105,19 +109,41 @@ struct Eight {
       return m;
     }
   }
-  __device__ __forceinline__ void store(uint8_t *q, float s, float r, int n) const {
+  __device__ __forceinline__ uint2 codes(float s, float r) const {
     float v[8];
     get(v);
-    const uint32_t a = codes4(v, s, r), b = codes4(v + 4, s, r);
-    if (VEC && n >= 8) {
-      *reinterpret_cast<uint2 *>(q) = make_uint2(a, b);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < n) q[i] = (uint8_t)((i < 4 ? a >> 8 * i : b >> 8 * (i - 4)) & 0xff);
-    }
+    return make_uint2(codes4(v, s, r), codes4(v + 4, s, r));
+  }
+  __device__ __forceinline__ uint2 divided(float s) const {
+    float v[8];
+    get(v);
+    return make_uint2(divided4(v[0], v[1], v[2], v[3], s), divided4(v[4], v[5], v[6], v[7], s));
   }
 };
+// 8 codes of a row, of which n are the matrix's.
+template <bool VEC>
+__device__ __forceinline__ void store8(uint8_t *q, uint2 w, int n) {
+  if (VEC && n >= 8) {
+    *reinterpret_cast<uint2 *>(q) = w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) q[i] = (uint8_t)((i < 4 ? w.x >> 8 * i : w.y >> 8 * (i - 4)) & 0xff);
+  }
+}
+// The codes of four pieces of a thread.  Scales near the end of the range, where the
+// correction's remainder would underflow, and infinite or NaN ones take the division.
+template <typename T, bool VEC>
+__device__ __forceinline__ void codes_of(const Eight<T, VEC> (&v)[4], float s, uint2 (&w)[4]) {
+  if (s > 0x1p-90f && s < 0x1p127f) {
+    const float r = __frcp_rn(s);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = v[k].codes(s, r);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = v[k].divided(s);
+  }
+}
 
 // Four lanes per group of 1 x 128, 32 elements a lane, all loaded before the first is
 // used; per group one division, one reciprocal and one index division then serve 32
@@ -139,12 +165,14 @@ __global__ void __launch_bounds__(256) quantize_rows(const QuantArgs a) {
   for (int k = 0; k < 4; ++k) m = max(m, v[k].amax());
   m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
   m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-  const float s = scale_of(m), r = __frcp_rn(s);
+  const float s = scale_of(m);
   if (ok && lane == 0) a.scale[(size_t)row * a.lds + kb] = s;
+  uint2 w[4];
+  codes_of(v, s, w);
   uint8_t *q = a.q + (size_t)row * a.ldq + c;
 #pragma unroll
   for (int k = 0; k < 4; ++k)
-    if (n > k * 32) v[k].store(q + k * 32, s, r, n - k * 32);
+    if (n > k * 32) store8<VEC>(q + k * 32, w[k], n - k * 32);
 }
 
 // One CTA per block of 128 x 128, 32 elements a thread held in registers.
@@ -168,12 +196,14 @@ __global__ void __launch_bounds__(512) quantize_blocks(const QuantArgs a) {
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 16; ++i) m = max(m, s_max[i]);
-  const float s = scale_of(m), r = __frcp_rn(s);
+  const float s = scale_of(m);
+  uint2 w[4];
+  codes_of(v, s, w);
   if (threadIdx.x == 0) a.scale[(size_t)rb * a.lds + kb] = s;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (r0 + i * 32 < a.rows && c < a.cols)
-      v[i].store(a.q + (size_t)(r0 + i * 32) * a.ldq + c, s, r, a.cols - c);
+      store8<VEC>(a.q + (size_t)(r0 + i * 32) * a.ldq + c, w[i], a.cols - c);
 }
 
 template <typename T>

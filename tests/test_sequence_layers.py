@@ -345,6 +345,25 @@ def test_fp8_quantize(cuda_dev, dtype, block_rows, rows, cols, pad):
     assert (qm[:, cols:].float() == 1.0).all()
 
 
+def test_fp8_quantize_rounds_as_the_division(cuda_dev):
+    """Every bf16 magnitude of three binades under scales of many mantissas, among them
+    quotients that lie between two codes, and groups near the ends of the range."""
+    m = torch.arange(128, 512, dtype=torch.int32)
+    x = (m << 16 | 0x3c000000).view(torch.float32)  # bf16 bit patterns as fp32
+    rows = []
+    for top in list(range(128, 256)) + [511]:
+        big = torch.tensor((top << 16) | 0x3f000000, dtype=torch.int32).view(torch.float32)
+        for part in x.split(127):
+            rows.append(torch.cat((part, big.repeat(128 - len(part)))))
+    x = torch.stack(rows)
+    x = torch.cat((x, x * 2.0 ** -118, x * 2.0 ** 122, -x * 3.0 ** -40))
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=cuda_dev)
+    s = torch.empty(len(x), 1, device=cuda_dev)
+    cwg.fp8_quantize(x.to(cuda_dev), q, s, 1)
+    want, scale = R.quantize(x, 1)
+    assert torch.equal(s.cpu(), scale) and torch.equal(q.float().cpu(), want.float())
+
+
 def test_fp8_quantize_infinity_and_nan(cuda_dev):
     x = torch.ones(3, 256)
     x[0, 5], x[1, 130], x[2, 7] = float("inf"), float("nan"), -float("inf")
