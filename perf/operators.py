@@ -21,13 +21,11 @@ GROUP = 128  # columns (and, for weights, rows) that share a scale
 
 
 def _cwg():
-    pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
-                       "cache-aware-wino-implementation_b200")
-    if pkg not in sys.path:
-        sys.path.insert(0, pkg)
-    import cwg
-
-    return cwg
+    if "cwg" not in sys.modules:  # as any program, once
+        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(
+            os.path.abspath(__file__))), "cache-aware-wino-implementation_b200"))
+        import cwg  # noqa: F401
+    return sys.modules["cwg"]
 
 
 # ---- cases ------------------------------------------------------------------------
