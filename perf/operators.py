@@ -241,32 +241,31 @@ def _own(s):
     c = s["case"]
     op = c["op"]
     flags = cwg.BF16 if c["dtype"] == "bf16" else 0
-    stream = torch.cuda.current_stream()
     if op == "conv":
         cwg.conv1d_causal(s["x"], s["w"], s["bias"], s["y"], s["state"], s["starts"], s["slots"],
-                          s["resume"], flags | cwg.SILU, stream)
+                          s["resume"], flags | cwg.SILU)
         return s["y"], s["state"]
     if op == "conv_step":
         cwg.conv1d_causal_step(s["x"], s["w"], s["bias"], s["y"], s["state"], s["slots"],
-                               flags | cwg.SILU, stream)
+                               flags | cwg.SILU)
         return s["y"], s["state"]
     if op == "scan":
         need = cwg.ssm_workspace_bytes(c["tokens"], c["seqs"], c["channels"], c["states"])
         workspace = torch.empty(need, dtype=torch.uint8, device="cuda")
         cwg.ssm_scan(s["u"], s["dt"], s["A"], s["B"], s["C"], s["D"], s["dt_bias"], s["z"],
                      s["y"], s["state"], s["starts"], s["slots"], s["resume"], workspace,
-                     flags | cwg.SOFTPLUS, stream)
+                     flags | cwg.SOFTPLUS)
         return s["y"], s["state"]
     if op == "scan_step":
         cwg.ssm_step(s["u"], s["dt"], s["A"], s["B"], s["C"], s["D"], s["dt_bias"], s["z"],
-                     s["y"], s["state"], s["slots"], flags | cwg.SOFTPLUS, stream)
+                     s["y"], s["state"], s["slots"], flags | cwg.SOFTPLUS)
         return s["y"], s["state"]
     if op == "quantize":
-        cwg.fp8_quantize(s["x"], s["q"], s["scale"], c["block_rows"], flags, stream)
+        cwg.fp8_quantize(s["x"], s["q"], s["scale"], c["block_rows"], flags)
         return s["q"], s["scale"]
     if c["relu"]:
         flags |= cwg.RELU
-    cwg.fp8_matmul(s["a"], s["a_scale"], s["w"], s["w_scale"], s["bias"], s["y"], flags, stream)
+    cwg.fp8_matmul(s["a"], s["a_scale"], s["w"], s["w_scale"], s["bias"], s["y"], flags)
     return s["y"]
 
 
