@@ -11,7 +11,8 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
-#include <c10/core/impl/VirtualGuardImpl.h>
+#include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <stdexcept>
@@ -49,7 +50,7 @@ const at::Tensor &tensor(PyObject *o, const char *name) {
 // What all of a call's tensors have to agree on, taken from its first one.
 struct Call {
   int device;
-  void *stream;
+  void *stream = nullptr;
   at::ScalarType io;
   unsigned flags;
 
@@ -63,12 +64,13 @@ struct Call {
     const at::Tensor &t = THPVariable_Unpack(first);
     if (!t.is_cuda()) refuse(name, "is not on a CUDA device");
     device = t.get_device();
-    if (device != c10::impl::VirtualGuardImpl(c10::DeviceType::CUDA).getDevice().index())
+    if (device != c10::cuda::current_device())
       refuse(name, "is on cuda:" + std::to_string(device) + ", not on the current device");
-    stream = nullptr;
-    if (PyLong_Check(stream_)) {
+    if (stream_ == Py_None) {  // the stream that torch's own operators would use
+      stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+    } else if (PyLong_Check(stream_)) {
       stream = PyLong_AsVoidPtr(stream_);
-    } else if (stream_ != Py_None) {
+    } else {
       PyObject *h = PyObject_GetAttrString(stream_, "cuda_stream");
       PyObject *d = h ? PyObject_GetAttrString(stream_, "device_index") : nullptr;
       if (!d) {

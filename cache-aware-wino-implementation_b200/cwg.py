@@ -276,7 +276,9 @@ def version() -> str:
 # These take torch tensors: sizes and row distances come from the tensors (a column range
 # of a wider matrix is passed as it is), and every tensor is checked before the call, since
 # a wrong type, device or size would otherwise only show as wrong memory accesses.
-# ValueError names the argument; what the library itself refuses is a CwgError.  The checks
+# ValueError names the argument; what the library itself refuses is a CwgError.  Without a
+# stream a call runs on torch's current stream, as an operator of torch's on the same tensors
+# would (the calls above, which take addresses, run on the default stream then).  The checks
 # are compiled (csrc/cwg_torch.cpp): a decoding step's kernels are shorter than they would
 # take in Python.
 _torch_ext = None

@@ -453,3 +453,62 @@ def test_tensors_that_do_not_fit_are_named(cuda_dev):
     with pytest.raises(cwg.CwgError) as e:  # rows that do not start on 16 bytes
         cwg.fp8_matmul(q, s1, q, s1[:1], None, torch.zeros(4, 4, device=dev))
     assert e.value.status == cwg.EINVAL
+
+
+# ---- streams and graphs --------------------------------------------------------------------
+def decode_calls(dev, seed=21):
+    """A decoding step's calls on buffers of their own: quantise, product, convolution, scan."""
+    g = gen(seed)
+    n, ch, k = 5, 64, 200
+    x = randn(g, n, k, dtype=torch.bfloat16).to(dev)
+    q = on_dev(torch.zeros(n, k).to(torch.float8_e4m3fn), dev)
+    s = torch.empty(n, 2, device=dev)
+    w, w_s = R.quantize(randn(g, 2 * ch, k, std=0.1), 128)
+    w, w_s = on_dev(w, dev), w_s.to(dev)
+    xz = torch.empty(n, 2 * ch, dtype=torch.bfloat16, device=dev)
+    cw, cb = randn(g, ch, 4).to(dev), randn(g, ch).to(dev)
+    cst = randn(g, n, 3, ch, dtype=torch.bfloat16).to(dev)
+    u = torch.empty(n, ch, dtype=torch.bfloat16, device=dev)
+    dt, bc = (randn(g, n, m, dtype=torch.bfloat16).to(dev) for m in (ch, 32))
+    A, D, db = -torch.rand(ch, 16, generator=g).to(dev), randn(g, ch).to(dev), randn(g, ch).to(dev)
+    h, y = randn(g, n, ch, 16).to(dev), torch.empty_like(u)
+
+    def calls():
+        cwg.fp8_quantize(x, q, s, 1, cwg.BF16)
+        cwg.fp8_matmul(q, s, w, w_s, None, xz, cwg.BF16)
+        cwg.conv1d_causal_step(xz[:, :ch], cw, cb, u, cst, None, cwg.BF16 | cwg.SILU)
+        cwg.ssm_step(u, dt, A, bc[:, :16], bc[:, 16:], D, db, xz[:, ch:], y, h, None,
+                     cwg.BF16 | cwg.SOFTPLUS)
+    return calls, (x, xz, cst, u, h, y)
+
+
+def test_calls_follow_the_current_stream_and_replay(cuda_dev):
+    """The same steps eagerly on a side stream, and captured there and replayed on another
+    graph's heels, give what they give on the default stream, bit for bit."""
+    plain, want = decode_calls(cuda_dev)
+    for _ in range(3):
+        plain()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    eager, got = decode_calls(cuda_dev)
+    other, got2 = decode_calls(cuda_dev)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)  # what runs on the wrong stream would run too early
+        got[0].mul_(2)
+        got[0].div_(2)
+        for _ in range(3):
+            eager()
+    side.synchronize()
+    graph, graph2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        other()
+    with torch.cuda.graph(graph2):
+        other()
+    graph.replay()
+    graph2.replay()
+    graph.replay()
+    torch.cuda.synchronize()
+    cwg.device_status()
+    for a, b, c in zip(want, got, got2):
+        assert torch.equal(a, b) and torch.equal(a, c)
