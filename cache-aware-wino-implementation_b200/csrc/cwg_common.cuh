@@ -32,6 +32,37 @@ inline cudaError_t smem_attr_once(int bytes) {
   return smem_attr_once(done, (const void *)Kernel, bytes);
 }
 
+// Launch of one of the kernels that begin with griddep_wait(): a programmatic dependent
+// launch (its CTAs may start while the previous kernel of the stream drains, and wait for
+// that kernel's completion before they touch global memory) unless `pdl` is 0.
+// cluster > 1: CTAs per cluster.
+template <typename... K, typename... A>
+inline cudaError_t launch_dependent(void (*kernel)(K...), dim3 grid, unsigned threads, size_t smem,
+                                    cudaStream_t stream, int pdl, unsigned cluster, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  unsigned n = 0;
+  if (pdl) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) (void)cudaGetLastError();
+  return e;
+}
+
 // Reads a translation unit's status word and clears it when it is set.
 inline int read_clear_status(unsigned &word, unsigned *status) {
   unsigned v = 0;

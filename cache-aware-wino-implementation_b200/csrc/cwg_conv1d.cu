@@ -123,6 +123,8 @@ __device__ __forceinline__ void slide(Chan<V> (&h)[K - 1], const Chan<V> &x) {
 template <typename T, int V, int K, int ACT>
 __global__ void __launch_bounds__(kConvThreads) conv1d_prompt(const ConvArgs a) {
   __shared__ int s_starts[kStartsInSmem + 1];
+  griddep_wait();
+  griddep_launch_dependents();
   const T *x = static_cast<const T *>(a.x);
   T *y = static_cast<T *>(a.y);
   T *state = static_cast<T *>(a.state);
@@ -253,6 +255,8 @@ __global__ void __launch_bounds__(kConvThreads) conv1d_prompt(const ConvArgs a) 
 // before the search for an earlier row with the same line.
 template <typename T, int V, int K, int ACT>
 __global__ void __launch_bounds__(kConvThreads) conv1d_step(const ConvArgs a) {
+  griddep_wait();
+  griddep_launch_dependents();
   const T *x = static_cast<const T *>(a.x);
   T *y = static_cast<T *>(a.y);
   T *state = static_cast<T *>(a.state);
@@ -326,12 +330,10 @@ static int launch_conv1d(const cwgk_conv1d *op, bool step, cudaStream_t stream) 
   const int per = 4 / a.wc;
   const long long blocks = (long long)a.cblocks * ((a.runs + per - 1) / per);
   if (blocks > 0x7fffffffLL) return -2;
-  if (step)
-    conv1d_step<T, V, K, ACT><<<(unsigned)blocks, kConvThreads, 0, stream>>>(a);
-  else
-    conv1d_prompt<T, V, K, ACT><<<(unsigned)blocks, kConvThreads, 0, stream>>>(a);
+  const auto kernel = step ? conv1d_step<T, V, K, ACT> : conv1d_prompt<T, V, K, ACT>;
+  const cudaError_t e = launch_dependent(kernel, dim3((unsigned)blocks), kConvThreads, 0, stream,
+                                         op->pdl, 1, a);
   cwgk_count_launch();
-  const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) {
     cwgk_set_cuda_error((int)e);
     return -3;

@@ -150,6 +150,8 @@ __device__ __forceinline__ void codes_of(const Eight<T, VEC> (&v)[4], float s, u
 // elements of each lane.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quantize_rows(const QuantArgs a) {
+  griddep_wait();
+  griddep_launch_dependents();
   const unsigned g = blockIdx.x * 64 + (threadIdx.x >> 2);
   const int lane = threadIdx.x & 3;
   const bool ok = g < (unsigned)a.groups;
@@ -178,6 +180,8 @@ __global__ void __launch_bounds__(256) quantize_rows(const QuantArgs a) {
 // One CTA per block of 128 x 128, 32 elements a thread held in registers.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(512) quantize_blocks(const QuantArgs a) {
+  griddep_wait();
+  griddep_launch_dependents();
   __shared__ uint32_t s_max[16];
   const int kb = blockIdx.x % a.kblocks, rb = blockIdx.x / a.kblocks;
   const int c = kb * 128 + (threadIdx.x & 15) * 8, r0 = rb * 128 + (threadIdx.x >> 4);
@@ -207,7 +211,7 @@ __global__ void __launch_bounds__(512) quantize_blocks(const QuantArgs a) {
 }
 
 template <typename T>
-static int quantize(QuantArgs a, int block_rows, cudaStream_t s) {
+static int quantize(QuantArgs a, int block_rows, int pdl, cudaStream_t s) {
   constexpr int E = 16 / (int)sizeof(T);
   const bool one = a.rows <= 1;
   // a whole vector at a row's end may reach past cols only if the row does
@@ -215,19 +219,12 @@ static int quantize(QuantArgs a, int block_rows, cudaStream_t s) {
                    a.cols % E == 0 && (one || (a.ldx % E == 0 && a.ldq % 8 == 0));
   const long long blocks = block_rows == 1 ? (a.groups + 63) / 64 : a.groups;
   if (a.groups > 0x7fffffffLL - 64) return -2;  // 32-bit group numbers
-  if (block_rows == 1) {
-    if (vec)
-      quantize_rows<T, true><<<(unsigned)blocks, 256, 0, s>>>(a);
-    else
-      quantize_rows<T, false><<<(unsigned)blocks, 256, 0, s>>>(a);
-  } else {
-    if (vec)
-      quantize_blocks<T, true><<<(unsigned)blocks, 512, 0, s>>>(a);
-    else
-      quantize_blocks<T, false><<<(unsigned)blocks, 512, 0, s>>>(a);
-  }
+  const bool one_row = block_rows == 1;
+  const auto kernel = one_row ? (vec ? quantize_rows<T, true> : quantize_rows<T, false>)
+                              : (vec ? quantize_blocks<T, true> : quantize_blocks<T, false>);
+  const cudaError_t e = launch_dependent(kernel, dim3((unsigned)blocks), one_row ? 256 : 512, 0, s,
+                                         pdl, 1, a);
   cwgk_count_launch();
-  const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) {
     cwgk_set_cuda_error((int)e);
     return -3;
@@ -371,6 +368,9 @@ __global__ void __launch_bounds__(Cfg<TN>::kThreads, Cfg<TN>::kMinBlocks)
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  // Nothing above touched global memory.  Tensor memory is taken only now: the previous
+  // kernel's CTAs may still have to allocate theirs, and this one waits for them.
+  griddep_wait();
   if (warp == C::kPromote) {  // the MMA warp owns the tensor memory
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(tmem_slot)),
@@ -380,6 +380,7 @@ __global__ void __launch_bounds__(Cfg<TN>::kThreads, Cfg<TN>::kMinBlocks)
   }
   __syncthreads();
   tc_fence_after();
+  griddep_launch_dependents();
   const uint32_t tmem = *tmem_slot;
 
   float acc[C::kCols];
@@ -705,6 +706,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  griddep_wait();  // before tensor memory is taken, as above
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(tmem_slot)),
@@ -715,6 +717,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
   __syncthreads();
   cluster_sync_all();  // both CTAs' barriers exist before any remote arrival
   tc_fence_after();
+  griddep_launch_dependents();
   const uint32_t tmem = *tmem_slot;
   const int total = mine * p.kblocks;  // blocks this pair works through
 
@@ -1067,10 +1070,9 @@ static int launch_pair(const cwgk_fp8 *op, cudaStream_t s) {
   if (e == cudaSuccess) {
     const int most = resident_pairs(), pairs = (int)(tiles < most ? tiles : most);
     if (pairs <= 0) return -3;
-    fp8_matmul_pair<<<(unsigned)(2 * pairs), PairCfg::kThreads, PairCfg::kSmem, s>>>(
-        map_a, map_w, p, (int)tiles);
+    e = launch_dependent(fp8_matmul_pair, dim3((unsigned)(2 * pairs)), PairCfg::kThreads,
+                         PairCfg::kSmem, s, op->pdl, 1, map_a, map_w, p, (int)tiles);
     cwgk_count_launch();
-    e = cudaGetLastError();
   }
   if (e != cudaSuccess) {
     cwgk_set_cuda_error((int)e);
@@ -1096,18 +1098,8 @@ static int launch(const cwgk_fp8 *op, cudaStream_t s) {
   if (tiles * splits > 0x7fffffffLL) return -2;
   cudaError_t e = smem_attr_once<fp8_matmul<TN>>(C::kSmem);
   if (e == cudaSuccess) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * splits));
-    cfg.blockDim = dim3(C::kThreads);
-    cfg.dynamicSmemBytes = C::kSmem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)splits;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, fp8_matmul<TN>, map_a, map_w, p);
+    e = launch_dependent(fp8_matmul<TN>, dim3((unsigned)(tiles * splits)), C::kThreads, C::kSmem,
+                         s, op->pdl, (unsigned)splits, map_a, map_w, p);
     cwgk_count_launch();
   }
   if (e != cudaSuccess) {
@@ -1124,7 +1116,8 @@ static int launch(const cwgk_fp8 *op, cudaStream_t s) {
 extern "C" {
 
 int cwgk_fp8_quantize(const void *x, long long ldx, void *q, long long ldq, float *scale,
-                      long long lds, int rows, int cols, int block_rows, int bf16, void *stream) {
+                      long long lds, int rows, int cols, int block_rows, int bf16, int pdl,
+                      void *stream) {
   cwg::fp8::QuantArgs a;
   a.x = x;
   a.q = static_cast<uint8_t *>(q);
@@ -1136,8 +1129,8 @@ int cwgk_fp8_quantize(const void *x, long long ldx, void *q, long long ldq, floa
   a.cols = cols;
   a.kblocks = (cols + 127) / 128;
   a.groups = (long long)((rows + block_rows - 1) / block_rows) * a.kblocks;
-  return bf16 ? cwg::fp8::quantize<__nv_bfloat16>(a, block_rows, (cudaStream_t)stream)
-              : cwg::fp8::quantize<float>(a, block_rows, (cudaStream_t)stream);
+  return bf16 ? cwg::fp8::quantize<__nv_bfloat16>(a, block_rows, pdl, (cudaStream_t)stream)
+              : cwg::fp8::quantize<float>(a, block_rows, pdl, (cudaStream_t)stream);
 }
 
 int cwgk_fp8_matmul(const cwgk_fp8 *op, void *stream) {

@@ -38,7 +38,7 @@ static int overlaps(const void *a, long long lda, long long wa, const void *b, l
 
 static int act_of(unsigned flags, unsigned allowed) {
   const unsigned act = flags & (CWG_RELU | CWG_SILU);
-  if (flags & ~(allowed | CWG_BF16)) return -1;
+  if (flags & ~(allowed | CWG_BF16 | CWG_NO_PDL)) return -1;
   if (act == (CWG_RELU | CWG_SILU)) return -1;
   return act == CWG_RELU ? CWGK_ACT_RELU : act == CWG_SILU ? CWGK_ACT_SILU : CWGK_ACT_NONE;
 }
@@ -75,7 +75,7 @@ int cwg_conv1d_causal(const void *x, long long ldx, const float *w, const float 
   if (act < 0) return CWG_EINVAL;
   const cwgk_conv1d op = {x,      ldx,    w,      bias,  y,       ldy,      state, starts,
                           slots,  resume, tokens, n_seq, n_slots, channels, width, act,
-                          (flags & CWG_BF16) != 0};
+                          (flags & CWG_BF16) != 0, !(flags & CWG_NO_PDL)};
   const int rc = conv1d_check(&op, tokens, flags);
   if (rc) return rc;
   if (n_seq == 0) return CWG_OK;
@@ -90,7 +90,8 @@ int cwg_conv1d_causal_step(const void *x, long long ldx, const float *w, const f
   const int act = act_of(flags, CWG_RELU | CWG_SILU);
   if (act < 0) return CWG_EINVAL;
   const cwgk_conv1d op = {x,    ldx, w, bias, y,       ldy,      state, 0,  slots,
-                          0,    n,   n, n_slots, channels, width, act, (flags & CWG_BF16) != 0};
+                          0,    n,   n, n_slots, channels, width, act, (flags & CWG_BF16) != 0,
+                          !(flags & CWG_NO_PDL)};
   const int rc = conv1d_check(&op, n, flags);
   if (rc) return rc;
   if (n == 0) return CWG_OK;
@@ -100,7 +101,7 @@ int cwg_conv1d_causal_step(const void *x, long long ldx, const float *w, const f
 
 static int ssm_check(const cwg_ssm *p, int n_seq) {
   if (!p) return CWG_EINVAL;
-  if (p->flags & ~(CWG_BF16 | CWG_SOFTPLUS)) return CWG_EINVAL;
+  if (p->flags & ~(CWG_BF16 | CWG_SOFTPLUS | CWG_NO_PDL)) return CWG_EINVAL;
   const size_t esz = (p->flags & CWG_BF16) ? 2 : 4;
   if (p->tokens < 0 || p->tokens > kMaxRows || n_seq < 0 || p->channels <= 0 || p->groups <= 0 || p->states <= 0)
     return CWG_EINVAL;
@@ -157,7 +158,7 @@ int cwg_ssm_step(const cwg_ssm *op, void *stream) {
 int cwg_fp8_quantize(const void *x, long long ldx, void *q, long long ldq, float *scale,
                      long long lds, int rows, int cols, int block_rows, unsigned flags,
                      void *stream) {
-  if (flags & ~CWG_BF16) return CWG_EINVAL;
+  if (flags & ~(CWG_BF16 | CWG_NO_PDL)) return CWG_EINVAL;
   if (rows < 0 || cols <= 0 || (block_rows != 1 && block_rows != 128)) return CWG_EINVAL;
   if (rows == 0) return CWG_OK;
   const size_t esz = (flags & CWG_BF16) ? 2 : 4;
@@ -167,14 +168,14 @@ int cwg_fp8_quantize(const void *x, long long ldx, void *q, long long ldq, float
       !rows_ok(scale, lds, rb, kb, 4))
     return CWG_EINVAL;
   return cwgk_fp8_quantize(x, ldx, q, ldq, scale, lds, rows, cols, block_rows,
-                           (flags & CWG_BF16) != 0, stream);
+                           (flags & CWG_BF16) != 0, !(flags & CWG_NO_PDL), stream);
 }
 
 int cwg_fp8_matmul(const void *a, long long lda, const float *a_scale, long long lda_scale,
                    const void *w, long long ldw, const float *w_scale, long long ldw_scale,
                    const float *bias, void *y, long long ldy, int m, int n, int k,
                    unsigned flags, void *stream) {
-  if (flags & ~(CWG_BF16 | CWG_RELU)) return CWG_EINVAL;
+  if (flags & ~(CWG_BF16 | CWG_RELU | CWG_NO_PDL)) return CWG_EINVAL;
   if (m < 0 || n <= 0 || k <= 0) return CWG_EINVAL;
   if (m == 0) return CWG_OK;
   const size_t esz = (flags & CWG_BF16) ? 2 : 4;
@@ -186,6 +187,7 @@ int cwg_fp8_matmul(const void *a, long long lda, const float *a_scale, long long
   if ((m > 1 && (lda & 15)) || (n > 1 && (ldw & 15))) return CWG_EINVAL;
   const cwgk_fp8 op = {a,       w,         lda,       ldw, a_scale, w_scale, bias,
                        lda_scale, ldw_scale, y,         ldy, m,       n,       k,
-                       (flags & CWG_RELU) != 0, (flags & CWG_BF16) != 0};
+                       (flags & CWG_RELU) != 0, (flags & CWG_BF16) != 0,
+                       !(flags & CWG_NO_PDL)};
   return cwgk_fp8_matmul(&op, stream);
 }

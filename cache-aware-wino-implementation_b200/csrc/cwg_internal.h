@@ -148,7 +148,7 @@ typedef struct cwgk_conv1d {
   void *state;
   const int *starts, *slots;
   const unsigned char *resume;
-  int tokens, n_seq, n_slots, channels, width, act, bf16;
+  int tokens, n_seq, n_slots, channels, width, act, bf16, pdl;
 } cwgk_conv1d;
 int cwgk_conv1d_prompt(const cwgk_conv1d *op, void *stream);
 int cwgk_conv1d_step(const cwgk_conv1d *op, void *stream); /* n_seq rows */
@@ -162,7 +162,8 @@ int cwgk_ssm_step(const struct cwg_ssm *op, void *stream);
 
 /* 8-bit product (csrc/cwg_fp8.cu), arguments checked by the host entry. */
 int cwgk_fp8_quantize(const void *x, long long ldx, void *q, long long ldq, float *scale,
-                      long long lds, int rows, int cols, int block_rows, int bf16, void *stream);
+                      long long lds, int rows, int cols, int block_rows, int bf16, int pdl,
+                      void *stream);
 typedef struct cwgk_fp8 {
   const void *a, *w;
   long long lda, ldw;
@@ -170,7 +171,7 @@ typedef struct cwgk_fp8 {
   long long lda_scale, ldw_scale;
   void *y;
   long long ldy;
-  int m, n, k, relu, bf16;
+  int m, n, k, relu, bf16, pdl;
 } cwgk_fp8;
 int cwgk_fp8_matmul(const cwgk_fp8 *op, void *stream);
 

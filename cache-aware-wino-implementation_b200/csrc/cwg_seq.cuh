@@ -6,9 +6,13 @@
 #include <stdint.h>
 
 #include "cwg_common.cuh"
+#include "cwg_tcgen05.cuh"
 
 namespace cwg {
 namespace seq {
+
+using tc::griddep_launch_dependents;
+using tc::griddep_wait;
 
 // V elements of T, moved as one 16-byte vector (or 8 bytes, or one element, V = 1).
 template <typename T, int V>

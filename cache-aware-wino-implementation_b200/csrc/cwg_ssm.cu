@@ -192,6 +192,8 @@ struct PromptSmem {
 
 template <typename T, int L, bool VEC, bool VBC>
 __global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) {
+  griddep_wait();
+  griddep_launch_dependents();
   using G = Prompt<L>;
   constexpr int CH = G::kCH;
   constexpr int NS = PromptSmem<T, L>::kStages;
@@ -427,6 +429,8 @@ struct Row4 {
 // VEC: states == 4 V L, and state, A, B and C can be read in whole vectors.
 template <typename T, int V, int L, int RR, bool VEC>
 __global__ void __launch_bounds__(Geo<V, L>::kThreads) ssm_token(const Args a) {
+  griddep_wait();
+  griddep_launch_dependents();
   constexpr int CH = Geo<V, L>::kCH, NT = Geo<V, L>::kThreads;
   const cwg_ssm &p = a.p;
   const int tid = threadIdx.x;
@@ -563,9 +567,12 @@ __global__ void __launch_bounds__(Geo<V, L>::kThreads) ssm_token(const Args a) {
 
 static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
-static int done() {
+template <typename K>
+static int start(K kernel, dim3 grid, unsigned threads, size_t smem, cudaStream_t s,
+                 const Args &a) {
+  const cudaError_t e =
+      launch_dependent(kernel, grid, threads, smem, s, !(a.p.flags & CWG_NO_PDL), 1, a);
   cwgk_count_launch();
-  const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) {
     cwgk_set_cuda_error((int)e);
     return -3;
@@ -581,8 +588,7 @@ static int launch_prompt(const Args &a, unsigned blocks, cudaStream_t s) {
     cwgk_set_cuda_error((int)e);
     return -3;
   }
-  ssm_prompt<T, L, VEC, VBC><<<blocks, Prompt<L>::kThreads, bytes, s>>>(a);
-  return done();
+  return start(ssm_prompt<T, L, VEC, VBC>, dim3(blocks), Prompt<L>::kThreads, bytes, s, a);
 }
 
 // lane: values of B and C that are read at a time.
@@ -628,15 +634,9 @@ static int steps(const cwg_ssm *op, cudaStream_t s) {
   const bool two = blocks >= 4 * 2 * 148, vec = a.vec_state && a.vec_a && a.vec_bc;
   const dim3 grid((unsigned)a.cblocks, (unsigned)op->groups,
                   (unsigned)(two ? (op->tokens + 1) / 2 : op->tokens));
-  if (two && vec)
-    ssm_token<T, V, L, 2, true><<<grid, G::kThreads, 0, s>>>(a);
-  else if (two)
-    ssm_token<T, V, L, 2, false><<<grid, G::kThreads, 0, s>>>(a);
-  else if (vec)
-    ssm_token<T, V, L, 1, true><<<grid, G::kThreads, 0, s>>>(a);
-  else
-    ssm_token<T, V, L, 1, false><<<grid, G::kThreads, 0, s>>>(a);
-  return done();
+  const auto kernel = two ? (vec ? ssm_token<T, V, L, 2, true> : ssm_token<T, V, L, 2, false>)
+                          : (vec ? ssm_token<T, V, L, 1, true> : ssm_token<T, V, L, 1, false>);
+  return start(kernel, grid, G::kThreads, 0, s, a);
 }
 
 template <typename T, int L>

@@ -231,7 +231,8 @@ int cwg_conv3x3_nonfused(const float *x, const float *U, const float *bias, floa
  *
  * y must not overlap the inputs (disjoint columns of one matrix do not overlap):
  * CWG_EINVAL.  All calls are asynchronous on `stream`, allocate nothing and can be
- * captured into a graph. */
+ * captured into a graph; they are programmatic dependent launches (see CWG_NO_PDL, which
+ * they take too). */
 
 /* y[t][c] = act(bias[c] + sum_j w[c][j] x[t - width + 1 + j][c]); rows before the
  * sequence come from its line.  w fp32 [channels][width], width 2 .. 4, bias fp32
