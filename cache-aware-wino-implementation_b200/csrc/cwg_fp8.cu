@@ -74,14 +74,17 @@ struct QuantArgs {
   long long groups;
 };
 
-// 8 consecutive elements of a row, zeros past the end, as they are in memory.
-template <typename T, bool VEC>
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// 8 consecutive elements of a row, zeros past the end, as they are in memory: whole 16-byte
+// vectors, of which a row has a whole number.
+template <typename T>
 struct Eight {
-  static constexpr int E = VEC ? 16 / (int)sizeof(T) : 1;
-  typename seq::Raw<T, E>::type raw[8 / E];
+  static constexpr int E = 16 / (int)sizeof(T);
+  uint4 raw[8 / E];
   __device__ __forceinline__ void load(const T *p, int n) {
 #pragma unroll
-    for (int i = 0; i < 8; i += E)  // VEC: cols is a multiple of E
+    for (int i = 0; i < 8; i += E)
       raw[i / E] = i < n ? seq::load_raw<T, E>(p + i) : seq::zero_raw<T, E>();
   }
   __device__ __forceinline__ void get(float (&v)[8]) const {
@@ -95,7 +98,7 @@ struct Eight {
   }
   // Largest magnitude, by its bits: NaN is above infinity, infinity above any number.
   __device__ __forceinline__ uint32_t amax() const {
-    if constexpr (VEC && sizeof(T) == 2) {
+    if constexpr (sizeof(T) == 2) {
       const uint32_t k = 0x7fff7fffu;
       const uint32_t m = __vmaxu2(__vmaxu2(raw[0].x & k, raw[0].y & k),
                                   __vmaxu2(raw[0].z & k, raw[0].w & k));
@@ -105,119 +108,177 @@ struct Eight {
       get(v);
       uint32_t m = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+      for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i]));
       return m;
     }
   }
-  __device__ __forceinline__ uint2 codes(float s, float r) const {
-    float v[8];
-    get(v);
-    return make_uint2(codes4(v, s, r), codes4(v + 4, s, r));
-  }
-  __device__ __forceinline__ uint2 divided(float s) const {
-    float v[8];
-    get(v);
-    return make_uint2(divided4(v[0], v[1], v[2], v[3], s), divided4(v[4], v[5], v[6], v[7], s));
-  }
 };
-// 8 codes of a row, of which n are the matrix's.
-template <bool VEC>
-__device__ __forceinline__ void store8(uint8_t *q, uint2 w, int n) {
-  if (VEC && n >= 8) {
-    *reinterpret_cast<uint2 *>(q) = w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) q[i] = (uint8_t)((i < 4 ? w.x >> 8 * i : w.y >> 8 * (i - 4)) & 0xff);
-  }
-}
-// The codes of four pieces of a thread.  Scales near the end of the range, where the
-// correction's remainder would underflow, and infinite or NaN ones take the division.
-template <typename T, bool VEC>
-__device__ __forceinline__ void codes_of(const Eight<T, VEC> (&v)[4], float s, uint2 (&w)[4]) {
+// Codes of N values.  Scales near the end of the range, where the correction's remainder
+// would underflow, and infinite or NaN ones take the division.
+template <int N>
+__device__ __forceinline__ void codes_of(const float (&v)[N], float s, uint32_t (&w)[N / 4]) {
   if (s > 0x1p-90f && s < 0x1p127f) {
     const float r = __frcp_rn(s);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) w[k] = v[k].codes(s, r);
+    for (int k = 0; k < N; k += 4) w[k / 4] = codes4(v + k, s, r);
   } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) w[k] = v[k].divided(s);
+    for (int k = 0; k < N; k += 4) w[k / 4] = divided4(v[k], v[k + 1], v[k + 2], v[k + 3], s);
+  }
+}
+// The same of four pieces, which are unpacked one at a time (all at once they take 60
+// registers a thread instead of 40: 18.8 against 16.8 us for 8192 x 4096 bf16).
+template <typename T>
+__device__ __forceinline__ void codes_of(const Eight<T> (&v)[4], float s, uint32_t (&w)[8]) {
+  if (s > 0x1p-90f && s < 0x1p127f) {
+    const float r = __frcp_rn(s);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float f[8];
+      v[k].get(f);
+      w[2 * k] = codes4(f, s, r);
+      w[2 * k + 1] = codes4(f + 4, s, r);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float f[8];
+      v[k].get(f);
+      w[2 * k] = divided4(f[0], f[1], f[2], f[3], s);
+      w[2 * k + 1] = divided4(f[4], f[5], f[6], f[7], s);
+    }
+  }
+}
+// The codes of 8 elements of a row, of which n are the matrix's.
+__device__ __forceinline__ void store8(uint8_t *q, uint32_t a, uint32_t b, int n) {
+  if (n >= 8) {
+    *reinterpret_cast<uint2 *>(q) = make_uint2(a, b);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) q[i] = (uint8_t)((i < 4 ? a >> 8 * i : b >> 8 * (i - 4)) & 0xff);
   }
 }
 
-// Four lanes per group of 1 x 128, 32 elements a lane, all loaded before the first is
-// used; per group one division, one reciprocal and one index division then serve 32
-// elements of each lane.
+// Groups of 1 x 128.  VEC: four lanes per group, 32 elements a lane, all loaded before the
+// first is used; per group one division, one reciprocal and one index division then serve
+// 32 elements of each lane.  Else a warp per group, neighbouring lanes on neighbouring
+// elements.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quantize_rows(const QuantArgs a) {
   griddep_wait();
   griddep_launch_dependents();
-  const unsigned g = blockIdx.x * 64 + (threadIdx.x >> 2);
-  const int lane = threadIdx.x & 3;
+  constexpr int kLanes = VEC ? 4 : 32;
+  const unsigned g = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  const int lane = threadIdx.x % kLanes;
   const bool ok = g < (unsigned)a.groups;
   const int row = ok ? (int)(g / (unsigned)a.kblocks) : 0;
   const int kb = ok ? (int)g - row * a.kblocks : 0;
-  const int c = kb * 128 + lane * 8, n = ok ? a.cols - c : 0;
-  const T *x = static_cast<const T *>(a.x) + (size_t)row * a.ldx + c;
-  Eight<T, VEC> v[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) v[k].load(x + k * 32, n - k * 32);
+  const T *x = static_cast<const T *>(a.x) + (size_t)row * a.ldx + kb * 128;
+  uint8_t *q = a.q + (size_t)row * a.ldq + kb * 128;
+  const int n = ok ? a.cols - kb * 128 : 0;  // the group's elements, and those behind it
   uint32_t m = 0;
+  auto scale_group = [&]() {  // from the lanes' largest magnitudes
 #pragma unroll
-  for (int k = 0; k < 4; ++k) m = max(m, v[k].amax());
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-  const float s = scale_of(m);
-  if (ok && lane == 0) a.scale[(size_t)row * a.lds + kb] = s;
-  uint2 w[4];
-  codes_of(v, s, w);
-  uint8_t *q = a.q + (size_t)row * a.ldq + c;
+    for (int o = kLanes / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float s = scale_of(m);
+    if (ok && lane == 0) a.scale[(size_t)row * a.lds + kb] = s;
+    return s;
+  };
+  if constexpr (VEC) {
+    Eight<T> v[4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (n > k * 32) store8<VEC>(q + k * 32, w[k], n - k * 32);
+    for (int k = 0; k < 4; ++k) v[k].load(x + k * 32 + lane * 8, n - k * 32 - lane * 8);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m = max(m, v[k].amax());
+    uint32_t w[8];
+    codes_of(v, scale_group(), w);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int c = k * 32 + lane * 8;
+      if (c < n) store8(q + c, w[2 * k], w[2 * k + 1], n - c);
+    }
+  } else {
+    float f[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      f[k] = k * 32 + lane < n ? to_f32(x[k * 32 + lane]) : 0.f;
+      m = max(m, abs_bits(f[k]));
+    }
+    uint32_t w[1];
+    codes_of(f, scale_group(), w);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k * 32 + lane < n) q[k * 32 + lane] = (uint8_t)(w[0] >> 8 * k);
+  }
 }
 
-// One CTA per block of 128 x 128, 32 elements a thread held in registers.
+// One CTA per block of 128 x 128, 32 elements a thread held in registers: four pieces of 8
+// columns (VEC), or one column of 32 rows, so that neighbouring threads read and write
+// neighbouring elements (1000 x 1543 fp32: 7.4 us with pieces of 8 there too, 5.2 so).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(512) quantize_blocks(const QuantArgs a) {
   griddep_wait();
   griddep_launch_dependents();
   __shared__ uint32_t s_max[16];
   const int kb = blockIdx.x % a.kblocks, rb = blockIdx.x / a.kblocks;
-  const int c = kb * 128 + (threadIdx.x & 15) * 8, r0 = rb * 128 + (threadIdx.x >> 4);
-  Eight<T, VEC> v[4];
+  const int tid = threadIdx.x;
+  const int c = kb * 128 + (VEC ? tid % 16 * 8 : tid % 128);
+  const int r0 = rb * 128 + (VEC ? tid / 16 : tid / 128);
+  const int n = a.cols - c;
+  const T *x = static_cast<const T *>(a.x) + c;
+  uint8_t *q = a.q + c;
+  uint32_t m = 0, w[8];
+  auto scale_block = [&]() {  // from the threads' largest magnitudes
+    m = __reduce_max_sync(0xffffffffu, m);
+    if ((tid & 31) == 0) s_max[tid >> 5] = m;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = r0 + i * 32;
-    v[i].load(static_cast<const T *>(a.x) + (size_t)(r < a.rows ? r : 0) * a.ldx + c,
-              r < a.rows ? a.cols - c : 0);
+    for (int i = 0; i < 16; ++i) m = max(m, s_max[i]);
+    const float s = scale_of(m);
+    if (tid == 0) a.scale[(size_t)rb * a.lds + kb] = s;
+    return s;
+  };
+  if constexpr (VEC) {
+    Eight<T> v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = r0 + i * 32;
+      v[i].load(x + (size_t)(r < a.rows ? r : 0) * a.ldx, r < a.rows ? n : 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = max(m, v[i].amax());
+    codes_of(v, scale_block(), w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = r0 + i * 32;
+      if (r < a.rows && n > 0) store8(q + (size_t)r * a.ldq, w[2 * i], w[2 * i + 1], n);
+    }
+  } else {
+    float f[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const int r = r0 + i * 4;
+      f[i] = r < a.rows && n > 0 ? to_f32(x[(size_t)r * a.ldx]) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 32; ++i) m = max(m, abs_bits(f[i]));
+    codes_of(f, scale_block(), w);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const int r = r0 + i * 4;
+      if (r < a.rows && n > 0) q[(size_t)r * a.ldq] = (uint8_t)(w[i / 4] >> 8 * (i % 4));
+    }
   }
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) m = max(m, v[i].amax());
-  m = __reduce_max_sync(0xffffffffu, m);
-  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 16; ++i) m = max(m, s_max[i]);
-  const float s = scale_of(m);
-  uint2 w[4];
-  codes_of(v, s, w);
-  if (threadIdx.x == 0) a.scale[(size_t)rb * a.lds + kb] = s;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (r0 + i * 32 < a.rows && c < a.cols)
-      store8<VEC>(a.q + (size_t)(r0 + i * 32) * a.ldq + c, w[i], a.cols - c);
 }
 
 template <typename T>
 static int quantize(QuantArgs a, int block_rows, int pdl, cudaStream_t s) {
   constexpr int E = 16 / (int)sizeof(T);
   const bool one = a.rows <= 1;
-  // a whole vector at a row's end may reach past cols only if the row does
   const bool vec = ((uintptr_t)a.x & 15) == 0 && ((uintptr_t)a.q & 7) == 0 &&
                    a.cols % E == 0 && (one || (a.ldx % E == 0 && a.ldq % 8 == 0));
-  const long long blocks = block_rows == 1 ? (a.groups + 63) / 64 : a.groups;
+  const long long blocks = block_rows != 1 ? a.groups : vec ? (a.groups + 63) / 64 : (a.groups + 7) / 8;
   if (a.groups > 0x7fffffffLL - 64) return -2;  // 32-bit group numbers
   const bool one_row = block_rows == 1;
   const auto kernel = one_row ? (vec ? quantize_rows<T, true> : quantize_rows<T, false>)
