@@ -26,6 +26,8 @@ struct Args {
   cwg_ssm p;
   int per;      // channels per group
   int cblocks;  // CTAs along one group's channels
+  int chunk;    // prompts: tokens per chunk of a cut sequence, 0: not cut
+  float *ends, *sums;  // cut sequences: see ssm_prompt
   bool vec_state, vec_a;  // the state's and A's rows are whole 16-byte vectors
   bool vec_bc;            // B and C can be read four states at a time
 };
@@ -190,8 +192,31 @@ struct PromptSmem {
   T u[kStages][kTT][G::kCH], d[kStages][kTT][G::kCH], z[kStages][kTT][G::kCH];
 };
 
-template <typename T, int L, bool VEC, bool VBC>
-__global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) {
+// Cut sequences.  A recurrence is serial, so one sequence alone keeps n_seq x channels / 32
+// CTAs busy; when that is few, sequences are cut into chunks of a.chunk tokens.  A first
+// launch (SUMMARY) runs the recurrence of every chunk but a sequence's last, from zeros
+// (the first chunk: from the sequence's state), without outputs, and keeps each chunk's
+// end states and sum of steps.  In the second launch a chunk finds its initial state
+// from those of the chunks before it,
+//   h = end_0;  h = exp(A sum_j d) h + end_j,  j = 1 .. k - 1,
+// and runs as a whole sequence does.  Exponentials are computed about 1.8 times.
+//
+// Chunk k of sequence b has index starts[b] / chunk + b + k: ascending offsets give every
+// chunk an index of its own below tokens / chunk + n_seq.  `ends` and `sums` are kept by
+// that index; the entry of a sequence's last chunk, which has no summary, keeps the state
+// that the sequence begins with, since the last chunk may replace the cache line before the
+// first one of the second launch has started.
+//
+// kRoomy is the whole kernel compiled for one CTA per SM: with 100 to 150 registers the scan
+// warps' operands are read further ahead, which shortens a tile when a CTA has its SM for
+// itself (nine fp32 sequences, 288 CTAs: 30 us, 40 dense; one of 4096 tokens x 2048 channels
+// x 64 states: 233, 324), and costs occupancy when there are many CTAs (eight sequences of
+// 1024 x 4096: 272 us, 232 dense).
+enum { kDense = 0, kRoomy = 1, kSummary = 2 };
+template <typename T, int L, bool VEC, bool VBC, int MODE>
+__global__ void __launch_bounds__(Prompt<L>::kThreads, MODE == kRoomy ? 1 : 0)
+    ssm_prompt(const Args a) {
+  constexpr bool SUMMARY = MODE == kSummary;
   griddep_wait();
   griddep_launch_dependents();
   using G = Prompt<L>;
@@ -203,15 +228,43 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) 
   const int tid = threadIdx.x;
   const int cblk = blockIdx.x % a.cblocks;
   const int group = (blockIdx.x / a.cblocks) % p.groups;
-  const int b = blockIdx.x / (a.cblocks * p.groups);
+  const int index = blockIdx.x / (a.cblocks * p.groups);
   const int in0 = cblk * CH;            // first channel within the group
   const int c0 = group * a.per + in0;   // first channel
   const int nch = min(CH, a.per - in0);
-  const int begin = p.starts[b], end = p.starts[b + 1];
   const bool report = tid == 0 && cblk == 0 && group == 0;
+  int b = index, part = 0, parts = 1, head = index;  // sequence, its chunks, its first index
+  if (a.chunk) {
+    auto base = [&](int q) { return min(max(p.starts[q], 0), p.tokens) / a.chunk + q; };
+    int hi = p.n_seq;
+    b = 0;  // after the search: the first sequence with a base above `index`
+    while (b < hi) {
+      const int mid = (b + hi) >> 1;
+      if (base(mid) <= index)
+        b = mid + 1;
+      else
+        hi = mid;
+    }
+    if (blockIdx.x == 0 && !SUMMARY) {  // a sequence with bad offsets may have no index
+      bool wrong = false;
+      for (int q = tid; q < p.n_seq; q += G::kThreads)
+        wrong |= p.starts[q] < 0 || p.starts[q + 1] < p.starts[q] || p.starts[q + 1] > p.tokens;
+      if (wrong) atomicOr(&g_ssm_status, CWGK_STATUS_INDEX);
+    }
+    if (--b < 0) return;
+    head = base(b);
+    part = index - head;
+  }
+  int begin = p.starts[b], end = p.starts[b + 1];
   if (begin < 0 || end < begin || end > p.tokens) {
     if (report) atomicOr(&g_ssm_status, CWGK_STATUS_INDEX);
     return;
+  }
+  if (a.chunk) {
+    parts = max(1, (end - begin + a.chunk - 1) / a.chunk);
+    if (part >= parts || (SUMMARY && part == parts - 1)) return;
+    begin += part * a.chunk;
+    end = min(end, begin + a.chunk);
   }
   bool bad = false;
   const int slot = p.state ? line_of(p.slots, b, p.n_slots, bad) : -1;
@@ -225,11 +278,30 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) 
     const bool mine = ch < nch;
     float A2[kS] = {}, h[kS] = {};
     const size_t at = (size_t)(c0 + ch) * p.states;
-    float *line = p.state + (size_t)(slot < 0 ? 0 : slot) * p.channels * p.states + at;
+    const size_t width = (size_t)p.channels * p.states;
+    float *line = p.state + (size_t)(slot < 0 ? 0 : slot) * width + at;
     if (mine) {
       load_states(p.A + at, i0, p.states, a.vec_a, A2);
-      if (carry) load_states(line, i0, p.states, a.vec_state, h);
+      float *ends = a.ends + (size_t)head * width + at;  // of the sequence's first chunk
+      const bool vec = p.states == kS * L;
+      if (part == 0 && (SUMMARY || parts == 1)) {
+        if (carry) load_states(line, i0, p.states, a.vec_state, h);
+        if (SUMMARY) store_states(ends + (size_t)(parts - 1) * width, i0, p.states, vec, h);
+      } else if (part == 0) {
+        load_states(ends + (size_t)(parts - 1) * width, i0, p.states, vec, h);
+      } else if (!SUMMARY) {
+        load_states(ends, i0, p.states, vec, h);
+#pragma unroll 4
+        for (int j = 1; j < part; ++j) {
+          float e[kS];
+          load_states(ends + (size_t)j * width, i0, p.states, vec, e);
+          const float d = a.sums[(size_t)(head + j) * p.channels + c0 + ch];
+#pragma unroll
+          for (int k = 0; k < kS; ++k) h[k] = fmaf(ex2(d * (A2[k] * kLog2e)), h[k], e[k]);
+        }
+      }
     }
+    float sum_d = 0.f, lost_d = 0.f;  // of the steps, with what its additions lost
     F2 a2[kS / 2], hh[kS / 2];
 #pragma unroll
     for (int k = 0; k < kS / 2; ++k) {
@@ -273,37 +345,55 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) 
           for (int k = 0; k < kS / 2; ++k) {
             const float2 x = halves(mul2(dd, a2[k]));
             hh[k] = fma2(f2(ex2(x.x), ex2(x.y)), hh[k], mul2(uu, bv[k]));
-            sum = k ? fma2(hh[k], cv[k], sum) : mul2(hh[k], cv[k]);
+            if (!SUMMARY) sum = k ? fma2(hh[k], cv[k], sum) : mul2(hh[k], cv[k]);
           }
-          const float2 s = halves(sum);
-          y[t] = s.x + s.y;
+          if (SUMMARY) {
+            y[t] = dv[t].x;
+          } else {
+            const float2 s = halves(sum);
+            y[t] = s.x + s.y;
+          }
         }
+        if constexpr (SUMMARY) {  // the steps pairwise, then with compensation: a sum's rounding enters
+                        // the decay of everything before this chunk
 #pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) {  // L tokens' sums over the channel's L lanes
-          const bool up = l & o;
+          for (int o = 1; o < TG; o *= 2)
 #pragma unroll
-          for (int g = 0; g < TG; g += L)
+            for (int t = 0; t < TG; t += 2 * o) y[t] += y[t + o];
+          const float to = sum_d + y[0], back = to - sum_d;
+          lost_d += (sum_d - (to - back)) + (y[0] - back);
+          sum_d = to;
+        } else {
 #pragma unroll
-            for (int k = 0; k < o; ++k) {
-              const float give = up ? y[g + k] : y[g + k + o];
-              const float keep = up ? y[g + k + o] : y[g + k];
-              y[g + k] = keep + __shfl_xor_sync(0xffffffffu, give, o);
-            }
+          for (int o = L / 2; o > 0; o >>= 1) {  // L tokens' sums over the channel's L lanes
+            const bool up = l & o;
+#pragma unroll
+            for (int g = 0; g < TG; g += L)
+#pragma unroll
+              for (int k = 0; k < o; ++k) {
+                const float give = up ? y[g + k] : y[g + k + o];
+                const float keep = up ? y[g + k + o] : y[g + k];
+                y[g + k] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+              }
+          }
+#pragma unroll
+          for (int g = 0; g < TG; g += L) ys[t0 + g + l][ch] = y[g];
         }
-#pragma unroll
-        for (int g = 0; g < TG; g += L) ys[t0 + g + l][ch] = y[g];
       }
       __syncthreads();
     }
-    if (slot >= 0 && mine) {
-      float out[kS];
+    float out[kS];
 #pragma unroll
-      for (int k = 0; k < kS / 2; ++k) {
-        const float2 x = halves(hh[k]);
-        out[2 * k] = x.x, out[2 * k + 1] = x.y;
-      }
-      store_states(line, i0, p.states, a.vec_state, out);
+    for (int k = 0; k < kS / 2; ++k) {
+      const float2 x = halves(hh[k]);
+      out[2 * k] = x.x, out[2 * k + 1] = x.y;
     }
+    if (SUMMARY && mine) {
+      store_states(a.ends + (size_t)index * width + at, i0, p.states, p.states == kS * L, out);
+      if (l == 0) a.sums[(size_t)index * p.channels + c0 + ch] = sum_d + lost_d;
+    }
+    if (!SUMMARY && slot >= 0 && mine && part == parts - 1)
+      store_states(line, i0, p.states, a.vec_state, out);
   } else {
     // ---- 4-channel pieces of the tiles' rows
     const int e = tid - G::kScan;
@@ -319,18 +409,19 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) 
     auto load = [&](int i) {
       const int st = i % NS, t0 = begin + i * kTT, rows = end - t0;
       const size_t at = (size_t)(rows > 0 ? t0 : begin), col = (size_t)group * p.states;
-      auto part = [&](const void *src, long long ld, T(*to)[CH]) {
+      auto rows_of = [&](const void *src, long long ld, T(*to)[CH]) {
         copy_rows<T, G::kElem, CH, 8, VEC>(e, static_cast<const T *>(src) + at * ld + c0,
                                            (size_t)ld, nch, rows,
                                            [&](int t, int k) { return &to[t][k]; });
       };
-      part(p.u, p.ldu, sh.u[st]);
-      part(p.dt, p.lddt, sh.d[st]);
-      if (p.z) part(p.z, p.ldz, sh.z[st]);
+      rows_of(p.u, p.ldu, sh.u[st]);
+      rows_of(p.dt, p.lddt, sh.d[st]);
+      if (p.z && !SUMMARY) rows_of(p.z, p.ldz, sh.z[st]);
       copy_rows<T, G::kElem, kS * L, kS, VBC>(
           e, static_cast<const T *>(p.B) + at * p.ldb + col, (size_t)p.ldb, p.states, rows,
           [&](int t, int k) { return sh.bc[st][t][k / kS].at(k % kS); });
-      copy_rows<T, G::kElem, kS * L, kS, VBC>(
+      if (!SUMMARY)
+        copy_rows<T, G::kElem, kS * L, kS, VBC>(
           e, static_cast<const T *>(p.C) + at * p.ldc + col, (size_t)p.ldc, p.states, rows,
           [&](int t, int k) { return sh.bc[st][t][k / kS].at(kS + k % kS); });
       copy_commit();
@@ -381,7 +472,7 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) 
     if (tiles > 0) prepare(0);
     __syncthreads();
     for (int i = 0; i < tiles; ++i) {
-      if (i > 0) finish(i - 1);
+      if (i > 0 && !SUMMARY) finish(i - 1);
       if (i + 1 < tiles) {
         load(i + 3);  // where tile i - 2 was
         prepare(i + 1);
@@ -389,7 +480,7 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads) ssm_prompt(const Args a) 
       }
       __syncthreads();
     }
-    if (tiles > 0) finish(tiles - 1);
+    if (tiles > 0 && !SUMMARY) finish(tiles - 1);
     copy_wait<0>();
   }
 }
@@ -582,13 +673,37 @@ static int start(K kernel, dim3 grid, unsigned threads, size_t smem, cudaStream_
 
 template <typename T, int L, bool VEC, bool VBC>
 static int launch_prompt(const Args &a, unsigned blocks, cudaStream_t s) {
-  constexpr int bytes = (int)sizeof(PromptSmem<T, L>);
-  const cudaError_t e = smem_attr_once<ssm_prompt<T, L, VEC, VBC>>(bytes);
+  constexpr int bytes = (int)sizeof(PromptSmem<T, L>), threads = Prompt<L>::kThreads;
+  cudaError_t e = smem_attr_once<ssm_prompt<T, L, VEC, VBC, kDense>>(bytes);
+  if (e == cudaSuccess) e = smem_attr_once<ssm_prompt<T, L, VEC, VBC, kRoomy>>(bytes);
+  if (e == cudaSuccess) e = smem_attr_once<ssm_prompt<T, L, VEC, VBC, kSummary>>(bytes);
   if (e != cudaSuccess) {
     cwgk_set_cuda_error((int)e);
     return -3;
   }
-  return start(ssm_prompt<T, L, VEC, VBC>, dim3(blocks), Prompt<L>::kThreads, bytes, s, a);
+  if (a.chunk) {
+    const int rc = start(ssm_prompt<T, L, VEC, VBC, kSummary>, dim3(blocks), threads, bytes, s, a);
+    if (rc) return rc;
+  }
+  const auto kernel = blocks <= 2 * 148 ? ssm_prompt<T, L, VEC, VBC, kRoomy>
+                                        : ssm_prompt<T, L, VEC, VBC, kDense>;
+  return start(kernel, dim3(blocks), threads, bytes, s, a);
+}
+
+// Tokens per chunk when a call's sequences are cut, else 0.  `ctas`: CTAs along the
+// channels.  Cut where at most half of the SMs would have a CTA and sequences are at least
+// four chunks long on average; chunks of 256 tokens or more (8 tiles), as many as make
+// three CTAs per SM (one sequence of 1024 tokens, 1024 channels: 32 us, 41 uncut; of 600: 31
+// and 26; of 8192 tokens and 256, 1024, 2048 channels: 47, 130, 254 us, 300 uncut).
+static int chunk_of(int tokens, int n_seq, long long ctas) {
+  if (n_seq <= 0 || ctas * n_seq > 74) return 0;
+  long long chunk = (tokens * ctas + 3 * 148 - 1) / (3 * 148);
+  chunk = chunk < 256 ? 256 : (chunk + kTT - 1) / kTT * kTT;
+  return tokens / n_seq >= 4 * chunk ? (int)chunk : 0;
+}
+static size_t al256(size_t n) { return (n + 255) / 256 * 256; }
+static size_t ends_bytes(long long slots, int channels, int states) {
+  return al256((size_t)slots * channels * states * 4);
 }
 
 // lane: values of B and C that are read at a time.
@@ -597,7 +712,8 @@ static Args make_args(const cwg_ssm *op, int np, int lane, size_t esz) {
   a.p = *op;
   if (op->tokens <= 1) a.p.ldu = a.p.lddt = a.p.ldz = a.p.ldy = 0, a.p.ldb = a.p.ldc = 0;
   a.per = op->channels / op->groups;
-  a.cblocks = 0;
+  a.cblocks = a.chunk = 0;
+  a.ends = a.sums = nullptr;
   a.vec_state = op->states == np && aligned16(op->state);
   a.vec_a = op->states == np && aligned16(op->A);
   a.vec_bc = op->states == np && ((uintptr_t)op->B % (lane * esz)) == 0 &&
@@ -607,10 +723,17 @@ static Args make_args(const cwg_ssm *op, int np, int lane, size_t esz) {
 }
 
 template <typename T, int L>
-static int prompts(const cwg_ssm *op, cudaStream_t s) {
+static int prompts(const cwg_ssm *op, void *workspace, cudaStream_t s) {
   Args a = make_args(op, kS * L, 4, sizeof(T));
   a.cblocks = (a.per + Prompt<L>::kCH - 1) / Prompt<L>::kCH;
-  const long long blocks = (long long)op->n_seq * a.cblocks * op->groups;
+  const long long ctas = (long long)a.cblocks * op->groups;
+  a.chunk = workspace ? chunk_of(op->tokens, op->n_seq, ctas) : 0;
+  const long long slots = a.chunk ? op->tokens / a.chunk + op->n_seq : op->n_seq;
+  if (a.chunk) {
+    a.ends = static_cast<float *>(workspace);
+    a.sums = a.ends + ends_bytes(slots, op->channels, op->states) / 4;
+  }
+  const long long blocks = slots * ctas;
   if (blocks > 0x7fffffffLL) return -2;
   constexpr int E = 16 / (int)sizeof(T);
   const bool vec = a.per % 8 == 0 && aligned16(op->u) && aligned16(op->dt) && aligned16(op->z) &&
@@ -640,22 +763,27 @@ static int steps(const cwg_ssm *op, cudaStream_t s) {
 }
 
 template <typename T, int L>
-static int launch(const cwg_ssm *op, bool step, cudaStream_t s) {
+static int launch(const cwg_ssm *op, bool step, void *workspace, cudaStream_t s) {
   constexpr int V = L > 1 ? 2 : 1;
-  return step ? steps<T, V, L / V>(op, s) : prompts<T, L>(op, s);
+  return step ? steps<T, V, L / V>(op, s) : prompts<T, L>(op, workspace, s);
 }
 
 template <typename T>
-static int by_states(const cwg_ssm *op, bool step, cudaStream_t s) {
-  if (op->states <= 4) return launch<T, 1>(op, step, s);
-  if (op->states <= 8) return launch<T, 2>(op, step, s);
-  if (op->states <= 16) return launch<T, 4>(op, step, s);
-  if (op->states <= 32) return launch<T, 8>(op, step, s);
-  return launch<T, 16>(op, step, s);
+static int by_states(const cwg_ssm *op, bool step, void *workspace, cudaStream_t s) {
+  if (op->states <= 4) return launch<T, 1>(op, step, workspace, s);
+  if (op->states <= 8) return launch<T, 2>(op, step, workspace, s);
+  if (op->states <= 16) return launch<T, 4>(op, step, workspace, s);
+  if (op->states <= 32) return launch<T, 8>(op, step, workspace, s);
+  return launch<T, 16>(op, step, workspace, s);
 }
 
-static int any(const cwg_ssm *op, bool step, cudaStream_t s) {
-  return op->flags & CWG_BF16 ? by_states<__nv_bfloat16>(op, step, s) : by_states<float>(op, step, s);
+static int any(const cwg_ssm *op, bool step, void *workspace, cudaStream_t s) {
+  return op->flags & CWG_BF16 ? by_states<__nv_bfloat16>(op, step, workspace, s)
+                              : by_states<float>(op, step, workspace, s);
+}
+
+static int channels_per_cta(int states) {
+  return states <= 16 ? 32 : states <= 32 ? Prompt<8>::kCH : Prompt<16>::kCH;
 }
 
 }  // namespace ssm
@@ -663,14 +791,22 @@ static int any(const cwg_ssm *op, bool step, cudaStream_t s) {
 
 extern "C" {
 
-size_t cwgk_ssm_workspace_bytes(int tokens, int n_seq, int channels, int states) { return 256; }
+// Of one group: more groups only make more CTAs and so fewer chunks.
+size_t cwgk_ssm_workspace_bytes(int tokens, int n_seq, int channels, int states) {
+  using namespace cwg::ssm;
+  const int ch = channels_per_cta(states);
+  const int chunk = chunk_of(tokens, n_seq, (channels + ch - 1) / ch);
+  if (!chunk) return 256;
+  const long long slots = tokens / chunk + n_seq;
+  return ends_bytes(slots, channels, states) + al256((size_t)slots * channels * 4);
+}
 
 int cwgk_ssm_scan(const cwg_ssm *op, void *workspace, size_t workspace_bytes, void *stream) {
-  return cwg::ssm::any(op, false, (cudaStream_t)stream);
+  return cwg::ssm::any(op, false, workspace, (cudaStream_t)stream);
 }
 
 int cwgk_ssm_step(const cwg_ssm *op, void *stream) {
-  return cwg::ssm::any(op, true, (cudaStream_t)stream);
+  return cwg::ssm::any(op, true, nullptr, (cudaStream_t)stream);
 }
 
 int cwgk_ssm_read_clear_status(unsigned *status) {

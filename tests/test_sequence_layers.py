@@ -243,6 +243,29 @@ def test_ssm_long_sequence(cuda_dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("lens,ch,groups,n,pad", [
+    ([900, 0, 3500, 1, 800], 40, 1, 16, (0, 0)), ([1024, 1536], 128, 2, 16, (8, 8)),
+    ([2600], 6, 2, 5, (0, 0)), ([1300, 1, 1800], 24, 1, 64, (0, 8)), ([256, 2000], 33, 1, 3, (0, 0)),
+], ids=str)
+def test_ssm_cut_sequences(cuda_dev, dtype, lens, ch, groups, n, pad):
+    """Few channels and long sequences: cut into chunks of time when there is a workspace."""
+    c = ssm_case(dtype, lens, ch, groups, n, 18, pad=pad)
+    assert cwg.ssm_workspace_bytes(len(c["u"]), len(lens), ch, n) > 256
+    check_ssm(c, cuda_dev)
+    check_ssm(c, cuda_dev, workspace=False)
+
+
+def test_ssm_cut_sequences_report_bad_indices(cuda_dev):
+    for starts, slots in (([0, 1500, 1400, 3300], [0, 1, 2]), ([0, 900, 2000, 3300], [1, 1, 7])):
+        c = ssm_case("bf16", [1100, 1100, 1100], 32, 1, 16, 19)
+        c["starts"], c["slots"] = starts, torch.tensor(slots, dtype=torch.int32)
+        with pytest.raises(cwg.CwgError) as e:
+            run_ssm(c, cuda_dev)
+        assert e.value.status == cwg.EINDEX
+        cwg.device_status()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 @pytest.mark.parametrize("rows,ch,groups,n", [(1, 2048, 1, 16), (5, 6, 2, 12), (33, 264, 1, 64),
                                               (70, 128, 4, 4), (3, 70, 1, 23), (9, 64, 1, 8)])
 def test_ssm_step(cuda_dev, dtype, rows, ch, groups, n):
