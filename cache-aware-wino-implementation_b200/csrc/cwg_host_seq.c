@@ -36,6 +36,15 @@ static int overlaps(const void *a, long long lda, long long wa, const void *b, l
   return !(off >= wa * (long long)esz && off + wb * (long long)esz <= step);
 }
 
+/* Whether the byte ranges of two row operands meet. */
+static int ranges_meet(const void *a, long long arow, const void *b, long long brow,
+                       long long arows, long long brows, long long abytes, long long bbytes) {
+  const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;
+  const uintptr_t a1 = a0 + (uintptr_t)((arows > 1 ? (arows - 1) * arow : 0) + abytes);
+  const uintptr_t b1 = b0 + (uintptr_t)((brows > 1 ? (brows - 1) * brow : 0) + bbytes);
+  return a0 < b1 && b0 < a1;
+}
+
 static int act_of(unsigned flags, unsigned allowed) {
   const unsigned act = flags & (CWG_RELU | CWG_SILU);
   if (flags & ~(allowed | CWG_BF16 | CWG_NO_PDL)) return -1;
@@ -159,13 +168,20 @@ int cwg_fp8_quantize(const void *x, long long ldx, void *q, long long ldq, float
                      long long lds, int rows, int cols, int block_rows, unsigned flags,
                      void *stream) {
   if (flags & ~(CWG_BF16 | CWG_NO_PDL)) return CWG_EINVAL;
-  if (rows < 0 || cols <= 0 || (block_rows != 1 && block_rows != 128)) return CWG_EINVAL;
+  if (rows < 0 || rows > kMaxRows || cols <= 0 || cols > kMaxRows ||
+      (block_rows != 1 && block_rows != 128))
+    return CWG_EINVAL;
   if (rows == 0) return CWG_OK;
   const size_t esz = (flags & CWG_BF16) ? 2 : 4;
   const long long kb = ((long long)cols + 127) / 128;
   const long long rb = block_rows == 1 ? rows : ((long long)rows + 127) / 128;
   if (!rows_ok(x, ldx, rows, cols, esz) || !rows_ok(q, ldq, rows, cols, 1) ||
       !rows_ok(scale, lds, rb, kb, 4))
+    return CWG_EINVAL;
+  const long long e = (long long)esz;
+  if (ranges_meet(x, ldx * e, q, ldq, rows, rows, cols * e, cols) ||
+      ranges_meet(x, ldx * e, scale, lds * 4, rows, rb, cols * e, kb * 4) ||
+      ranges_meet(q, ldq, scale, lds * 4, rows, rb, cols, kb * 4))
     return CWG_EINVAL;
   return cwgk_fp8_quantize(x, ldx, q, ldq, scale, lds, rows, cols, block_rows,
                            (flags & CWG_BF16) != 0, !(flags & CWG_NO_PDL), stream);
@@ -176,7 +192,8 @@ int cwg_fp8_matmul(const void *a, long long lda, const float *a_scale, long long
                    const float *bias, void *y, long long ldy, int m, int n, int k,
                    unsigned flags, void *stream) {
   if (flags & ~(CWG_BF16 | CWG_RELU | CWG_NO_PDL)) return CWG_EINVAL;
-  if (m < 0 || n <= 0 || k <= 0) return CWG_EINVAL;
+  if (m < 0 || n <= 0 || k <= 0 || m > kMaxRows || n > kMaxRows || k > kMaxRows)
+    return CWG_EINVAL;
   if (m == 0) return CWG_OK;
   const size_t esz = (flags & CWG_BF16) ? 2 : 4;
   const long long kb = ((long long)k + 127) / 128, nb = ((long long)n + 127) / 128;
@@ -185,6 +202,12 @@ int cwg_fp8_matmul(const void *a, long long lda, const float *a_scale, long long
       !rows_ok(y, ldy, m, n, esz) || ((uintptr_t)bias & 3))
     return CWG_EINVAL;
   if ((m > 1 && (lda & 15)) || (n > 1 && (ldw & 15))) return CWG_EINVAL;
+  const long long e = (long long)esz;
+  if (ranges_meet(a, lda, y, ldy * e, m, m, k, n * e) ||
+      ranges_meet(w, ldw, y, ldy * e, n, m, k, n * e) ||
+      ranges_meet(a_scale, lda_scale * 4, y, ldy * e, m, m, kb * 4, n * e) ||
+      ranges_meet(w_scale, ldw_scale * 4, y, ldy * e, nb, m, kb * 4, n * e))
+    return CWG_EINVAL;
   const cwgk_fp8 op = {a,       w,         lda,       ldw, a_scale, w_scale, bias,
                        lda_scale, ldw_scale, y,         ldy, m,       n,       k,
                        (flags & CWG_RELU) != 0, (flags & CWG_BF16) != 0,

@@ -146,6 +146,9 @@ PyObject *guarded(F &&f) {
   } catch (const std::exception &e) {
     PyErr_SetString(PyExc_ValueError, e.what());
     return nullptr;
+  } catch (...) {
+    PyErr_SetString(PyExc_RuntimeError, "unknown C++ exception");
+    return nullptr;
   }
 }
 

@@ -231,8 +231,9 @@ int cwg_conv3x3_nonfused(const float *x, const float *U, const float *bias, floa
  *
  * y must not overlap the inputs (disjoint columns of one matrix do not overlap):
  * CWG_EINVAL.  All calls are asynchronous on `stream`, allocate nothing and can be
- * captured into a graph; they are programmatic dependent launches (see CWG_NO_PDL, which
- * they take too). */
+ * captured into a graph (make a call of the kind before the first capture: kernels are
+ * loaded and configured at their first launch); they are programmatic dependent launches
+ * (see CWG_NO_PDL, which they take too). */
 
 /* y[t][c] = act(bias[c] + sum_j w[c][j] x[t - width + 1 + j][c]); rows before the
  * sequence come from its line.  w fp32 [channels][width], width 2 .. 4, bias fp32
@@ -282,12 +283,15 @@ int cwg_ssm_step(const cwg_ssm *op, void *stream);
 
 /* ---- 8-bit matrix product with scales per block of 128 (DEVICE pointers) ------- */
 
+/* Streams, graphs and launches as for the sequence layers. */
+
 /* e4m3 values q and fp32 scales of x (fp32, or bf16 with CWG_BF16), [rows][cols]:
  * each group of block_rows rows x 128 columns (cut at the edges) has
  *   scale = max(max |x| / 448, 2^-126),  q = e4m3(x / scale), to nearest even.
  * block_rows 1 (activations) or 128 (weights).  scale [ceil(rows / block_rows)]
  * [ceil(cols / 128)], rows lds apart.  A group that holds an infinity or NaN has an
- * infinite or NaN scale, and its values come back as NaN. */
+ * infinite or NaN scale, and its values come back as NaN.  x, q and scale must not overlap,
+ * from the first row to the last: CWG_EINVAL. */
 int cwg_fp8_quantize(const void *x, long long ldx, void *q, long long ldq, float *scale,
                      long long lds, int rows, int cols, int block_rows, unsigned flags,
                      void *stream);
@@ -297,7 +301,8 @@ int cwg_fp8_quantize(const void *x, long long ldx, void *q, long long ldq, float
  * a e4m3 [m][k], w e4m3 [n][k] (a weight's rows are outputs), as cwg_fp8_quantize
  * writes them with block_rows 1 and 128; a and w 16-byte aligned with lda and ldw
  * multiples of 16 (k itself may be any size >= 1).  y fp32 [m][n], or bf16 with
- * CWG_BF16; bias fp32 [n] or NULL; act: CWG_RELU or none. */
+ * CWG_BF16; bias fp32 [n] or NULL; act: CWG_RELU or none.  y must not overlap the inputs, from
+ * the first row to the last: CWG_EINVAL. */
 int cwg_fp8_matmul(const void *a, long long lda, const float *a_scale, long long lda_scale,
                    const void *w, long long ldw, const float *w_scale, long long ldw_scale,
                    const float *bias, void *y, long long ldy, int m, int n, int k,

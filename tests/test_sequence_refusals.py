@@ -101,6 +101,8 @@ def quantize(**kw):
     (dict(ldx=199), cwg.EINVAL), (dict(ldq=100), cwg.EINVAL), (dict(lds=1), cwg.EINVAL),
     (dict(block_rows=2), cwg.EINVAL), (dict(cols=0), cwg.EINVAL), (dict(rows=-1), cwg.EINVAL),
     (dict(flags=cwg.RELU), cwg.EINVAL), (dict(x=X + 1), cwg.EINVAL), (dict(rows=0), cwg.OK),
+    (dict(q=X), cwg.EINVAL), (dict(scale=X + 64), cwg.EINVAL), (dict(scale=Y + 400), cwg.EINVAL),
+    (dict(cols=(1 << 30) + 1, ldx=1 << 31), cwg.EINVAL),
 ])
 def test_fp8_quantize_refuses(kw, status):
     assert quantize(**kw) == status
@@ -120,7 +122,8 @@ def matmul(**kw):
     (dict(ldw=204), cwg.EINVAL), (dict(lda=192), cwg.EINVAL), (dict(ldy=299), cwg.EINVAL),
     (dict(lda_scale=1), cwg.EINVAL), (dict(ldw_scale=1), cwg.EINVAL), (dict(m=-1), cwg.EINVAL),
     (dict(n=0), cwg.EINVAL), (dict(k=0), cwg.EINVAL), (dict(flags=cwg.SILU), cwg.EINVAL),
-    (dict(bias=S + 2), cwg.EINVAL), (dict(m=0), cwg.OK),
+    (dict(bias=S + 2), cwg.EINVAL), (dict(m=0), cwg.OK), (dict(y=X), cwg.EINVAL),
+    (dict(y=W + 16), cwg.EINVAL), (dict(y=S), cwg.EINVAL), (dict(m=(1 << 30) + 1), cwg.EINVAL),
 ])
 def test_fp8_matmul_refuses(kw, status):
     assert matmul(**kw) == status
