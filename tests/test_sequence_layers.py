@@ -535,3 +535,267 @@ def test_calls_follow_the_current_stream_and_replay(cuda_dev):
     cwg.device_status()
     for a, b, c in zip(want, got, got2):
         assert torch.equal(a, b) and torch.equal(a, c)
+
+
+# ---- the layers of a state space block, one after the other ----------------------------------
+class Block:
+    """Weights of a block and its calls, each checked against its 64-bit reference on the very
+    inputs that it got: quantise, project to x and z, convolve, project to dt, B and C, scan with
+    the gate z, project back."""
+
+    def __init__(self, dev, d_model=136, ch=192, rank=24, n=16, lines=6, seed=31):
+        g = gen(seed)
+        self.dev, self.ch, self.rank, self.n = dev, ch, rank, n
+        self.w = {}
+        for name, out, k in (("in", 2 * ch, d_model), ("x", rank + 2 * n, ch), ("dt", ch, rank),
+                             ("out", d_model, ch)):
+            w = randn(g, out, k, std=k ** -0.5)
+            q = on_dev(torch.zeros(out, k).to(torch.float8_e4m3fn), dev)
+            s = torch.empty(-(-out // 128), -(-k // 128), device=dev)
+            cwg.fp8_quantize(w.to(dev), q, s, 128)
+            self.w[name] = (q, s)
+        self.cw, self.cb = randn(g, ch, 4, std=0.4), randn(g, ch, std=0.1)
+        self.A = -torch.arange(1.0, n + 1).repeat(ch, 1)
+        self.D, self.db = torch.ones(ch), torch.rand(ch, generator=g) * 4 - 5
+        self.conv = torch.zeros(lines, 3, ch, dtype=torch.bfloat16, device=dev)
+        self.h = torch.zeros(lines, ch, n, device=dev)
+
+    def project(self, name, x, bias=None):
+        rows, k = x.shape
+        q = on_dev(torch.zeros(rows, k).to(torch.float8_e4m3fn), self.dev)
+        s = torch.empty(rows, -(-k // 128), device=self.dev)
+        cwg.fp8_quantize(x, q, s, 1, cwg.BF16)
+        want, scale = R.quantize(x.cpu(), 1)
+        assert torch.equal(s.cpu(), scale) and torch.equal(q.float().cpu(), want.float())
+        w, ws = self.w[name]
+        y = torch.empty(rows, w.shape[0], dtype=torch.bfloat16, device=self.dev)
+        cwg.fp8_matmul(q, s, w, ws, bias, y, cwg.BF16)
+        R.close(y, R.matmul(q.cpu(), s.cpu(), w.cpu(), ws.cpu(), None, False, torch.bfloat16), name)
+        return y
+
+    def __call__(self, x, lens, slots, resume, step):
+        dev, ch = self.dev, self.ch
+        slots_d = torch.tensor(slots, dtype=torch.int32, device=dev)
+        starts = offsets(lens)
+        starts_d = torch.tensor(starts, dtype=torch.int32, device=dev)
+        resume_d = torch.tensor(resume, dtype=torch.uint8, device=dev)
+        xz = self.project("in", x)
+        u = torch.empty(len(x), ch, dtype=torch.bfloat16, device=dev)
+        conv, h = self.conv.cpu(), self.h.cpu()
+        cw, cb = self.cw.to(dev), self.cb.to(dev)
+        if step:
+            cwg.conv1d_causal_step(xz[:, :ch], cw, cb, u, self.conv, slots_d, cwg.BF16 | cwg.SILU)
+        else:
+            cwg.conv1d_causal(xz[:, :ch], cw, cb, u, self.conv, starts_d, slots_d, resume_d,
+                              cwg.BF16 | cwg.SILU)
+        proj = self.project("x", u)
+        r, n = self.rank, self.n
+        dt = self.project("dt", proj[:, :r])
+        y = torch.empty_like(u)
+        args = (u, dt, self.A.to(dev), proj[:, r:r + n], proj[:, r + n:], self.D.to(dev),
+                self.db.to(dev), xz[:, ch:], y, self.h)
+        if step:
+            cwg.ssm_step(*args, slots_d, cwg.BF16 | cwg.SOFTPLUS)
+        else:
+            ws = torch.empty(cwg.ssm_workspace_bytes(len(x), len(lens), ch, n),
+                             dtype=torch.uint8, device=dev)
+            cwg.ssm_scan(*args, starts_d, slots_d, resume_d, ws, cwg.BF16 | cwg.SOFTPLUS)
+        cwg.device_status()
+        for b, slot in enumerate(slots):
+            rows = slice(starts[b], starts[b + 1])
+            keep = 1 if resume[b] else 0
+            want, line = R.conv1d(xz[rows, :ch].cpu(), self.cw, self.cb, conv[slot] * keep, "silu")
+            R.close(u[rows], want, f"convolution {b}")
+            assert torch.equal(self.conv[slot].cpu(), line.to(torch.bfloat16))
+            p = proj[rows].cpu()
+            want, state = R.ssm(u[rows].cpu(), dt[rows].cpu(), self.A, p[:, None, r:r + n],
+                                p[:, None, r + n:], self.D, self.db, xz[rows, ch:].cpu(),
+                                h[slot] * keep, True)
+            R.close(y[rows], want, f"scan {b}")
+            R.close(self.h[slot], state, f"state {b}")
+        return self.project("out", y)
+
+
+def test_block_prompts_then_steps(cuda_dev):
+    g = gen(32)
+    block = Block(cuda_dev)
+    x = randn(g, 300, 136, dtype=torch.bfloat16).to(cuda_dev)
+    out = block(x[:200], [70, 1, 129], [4, 0, 2], [0, 0, 0], step=False)
+    assert out.shape == (200, 136) and out.isfinite().all()
+    block(x[200:240], [30, 10], [4, 5], [1, 0], step=False)      # one goes on, one begins
+    for i in range(3):
+        y = block(x[240 + 4 * i:244 + 4 * i], [1] * 4, [2, 4, 5, 0], [1] * 4, step=True)
+        assert y.isfinite().all()
+
+
+def test_prompt_in_pieces_is_the_whole_prompt(cuda_dev):
+    """A prompt cut at any place and resumed, and the same prompt token by token: the
+    convolution gives the same bits, the scan stays within its bound."""
+    c = conv_case("bf16", [90], 72, 4, "silu", 33, tail=0)
+    c["resume"][:] = 1
+    _, whole, line = run_conv(c, cuda_dev)
+    for cuts in ([1], [2, 50], [89], [3, 4, 5, 40]):
+        st, out = c["state"].to(cuda_dev), torch.empty_like(whole)
+        for s, e in zip([0] + cuts, cuts + [90]):
+            cwg.conv1d_causal(c["x"][s:e].to(cuda_dev), c["w"].to(cuda_dev), c["bias"].to(cuda_dev),
+                              out[s:e], st, torch.tensor([0, e - s], dtype=torch.int32,
+                                                         device=cuda_dev),
+                              c["slots"].to(cuda_dev), c["resume"].to(cuda_dev),
+                              cwg.BF16 | cwg.SILU)
+        assert torch.equal(out, whole) and torch.equal(st, line)
+    st, out = c["state"].to(cuda_dev), torch.empty_like(whole)
+    for t in range(90):
+        cwg.conv1d_causal_step(c["x"][t:t + 1].to(cuda_dev), c["w"].to(cuda_dev),
+                               c["bias"].to(cuda_dev), out[t:t + 1], st, c["slots"].to(cuda_dev),
+                               cwg.BF16 | cwg.SILU)
+    assert torch.equal(out, whole) and torch.equal(st, line)
+
+    s = ssm_case("fp32", [90], 40, 1, 16, 34, tail=0)
+    h = s["state"][int(s["slots"][0])]
+    want, end = ssm_want(s, slice(0, 90), h)
+    dev = {k: put(s[k], cuda_dev) for k in ("u", "step", "A", "B", "C", "D", "bias", "z", "slots")}
+    for cuts in ([1], [33, 64], list(range(1, 90))):
+        st, out = s["state"].to(cuda_dev), torch.empty(90, 40, device=cuda_dev)
+        for a, b in zip([0] + cuts, cuts + [90]):
+            rows = [dev[k][a:b] for k in ("u", "step", "B", "C", "z")]
+            call = (rows[0], rows[1], dev["A"], rows[2], rows[3], dev["D"], dev["bias"], rows[4],
+                    out[a:b], st)
+            if b - a == 1:
+                cwg.ssm_step(*call, dev["slots"], cwg.SOFTPLUS)
+            else:
+                cwg.ssm_scan(*call, torch.tensor([0, b - a], dtype=torch.int32, device=cuda_dev),
+                             dev["slots"], torch.ones(1, dtype=torch.uint8, device=cuda_dev), None,
+                             cwg.SOFTPLUS)
+        R.close(out, want, f"cuts {cuts[:3]}")
+        R.close(st[int(s["slots"][0])], end, f"state, cuts {cuts[:3]}")
+
+
+# ---- calls at the edges --------------------------------------------------------------------
+def test_fresh_sequences_do_not_read_their_lines(cuda_dev):
+    c = conv_case("fp32", [3, 1, 0, 40], 32, 4, "silu", 41)
+    s = ssm_case("bf16", [3, 1, 0, 40], 32, 1, 16, 42)
+    for case, check in ((c, check_conv), (s, check_ssm)):
+        fresh = case["slots"][case["resume"] == 0].long()
+        assert len(fresh)
+        case["state"][fresh] = float("nan")
+        case["state"][-1] = torch.where(torch.isnan(case["state"][-1]), 0.0, 1.0)
+        check(case, cuda_dev)
+
+
+def test_no_tokens_still_sets_the_lines(cuda_dev):
+    c = conv_case("bf16", [0, 0], 40, 3, "none", 43, tail=0)
+    c["resume"] = torch.tensor([0, 1], dtype=torch.uint8)
+    check_conv(c, cuda_dev)
+    s = ssm_case("fp32", [0, 0], 40, 1, 16, 44, tail=0)
+    s["resume"] = c["resume"]
+    check_ssm(s, cuda_dev)
+
+
+def test_many_sequences(cuda_dev):
+    """More sequences than the convolution keeps offsets of in shared memory."""
+    lens = [1, 0, 3, 2, 9] * 330
+    check_conv(conv_case("bf16", lens, 8, 4, "silu", 45), cuda_dev)
+    s = ssm_case("fp32", lens[:1200], 8, 1, 4, 46)
+    check_ssm(s, cuda_dev)
+
+
+def test_ordinary_launches_give_the_same_bits(cuda_dev):
+    a, got = decode_calls(cuda_dev)
+    b, want = decode_calls(cuda_dev)
+    orig = cwg.BF16
+    a()
+    try:
+        cwg.BF16 = orig | cwg.NO_PDL
+        b()
+    finally:
+        cwg.BF16 = orig
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_offsets_beyond_32_bits(cuda_dev):
+    """Rows and cache lines more than 2^31 elements (and 2^32 bytes) from the first."""
+    dev = cuda_dev
+    ld, ch, rows = (1 << 28) + 8, 32, 18
+    big = torch.empty(ld * (rows - 1) + 2 * ch, dtype=torch.bfloat16, device=dev)
+    x, y = (big.as_strided((rows, ch), (ld, 1), off) for off in (0, ch))
+    c = conv_case("bf16", [rows], ch, 4, "silu", 47, tail=0)
+    lines = (1 << 31) // (3 * ch) + 3  # 4.3 GB
+    state = torch.empty(lines, 3, ch, dtype=torch.bfloat16, device=dev)
+    slot = torch.tensor([lines - 1], dtype=torch.int32, device=dev)
+    one = torch.ones(1, dtype=torch.uint8, device=dev)
+    starts = torch.tensor([0, rows], dtype=torch.int32, device=dev)
+    x.copy_(c["x"])
+    state[-1] = c["state"][0].to(dev)
+    cwg.conv1d_causal(x, c["w"].to(dev), c["bias"].to(dev), y, state, starts, slot, one,
+                      cwg.BF16 | cwg.SILU)
+    want, line = R.conv1d(c["x"], c["w"], c["bias"], c["state"][0], "silu")
+    R.close(y, want, "rows")
+    assert torch.equal(state[-1].cpu(), line.to(torch.bfloat16))
+    cwg.conv1d_causal_step(x[-1:], c["w"].to(dev), c["bias"].to(dev), y[-1:], state, slot,
+                           cwg.BF16 | cwg.SILU)
+    want, line = R.conv1d(c["x"][-1:], c["w"], c["bias"], line.to(torch.bfloat16), "silu")
+    R.close(y[-1:], want, "step")
+    del state
+
+    s = ssm_case("bf16", [rows], ch, 1, 16, 48, tail=0)
+    u = x
+    u.copy_(s["u"])
+    lines = (1 << 31) // (ch * 16) + 3  # 8.6 GB
+    h = torch.empty(lines, ch, 16, device=dev)
+    h[-1] = s["state"][0].to(dev)
+    dv = {k: put(s[k], dev) for k in ("step", "A", "B", "C", "D", "bias", "z")}
+    cwg.ssm_scan(u, dv["step"], dv["A"], dv["B"], dv["C"], dv["D"], dv["bias"], dv["z"], y, h,
+                 starts, slot * 0 + lines - 1, one, None, cwg.BF16 | cwg.SOFTPLUS)
+    want, end = ssm_want(s, slice(0, rows), s["state"][0])
+    R.close(y, want, "scan")
+    R.close(h[-1], end, "state")
+    before = h[-1].cpu()
+    cwg.ssm_step(u[-1:], dv["step"][-1:], dv["A"], dv["B"][-1:], dv["C"][-1:], dv["D"],
+                 dv["bias"], dv["z"][-1:], y[-1:], h, slot * 0 + lines - 1,
+                 cwg.BF16 | cwg.SOFTPLUS)
+    want, end = ssm_want(s, slice(rows - 1, rows), before)
+    R.close(y[-1:], want, "scan step")
+    R.close(h[-1], end, "state after the step")
+    del h
+
+    q = torch.empty(rows, ch, dtype=torch.float8_e4m3fn, device=dev)
+    sc = torch.empty(rows, 1, device=dev)
+    cwg.fp8_quantize(x, q, sc, 1, cwg.BF16)
+    want, scale = R.quantize(s["u"], 1)
+    assert torch.equal(q.float().cpu(), want.float()) and torch.equal(sc.cpu(), scale)
+    w, w_s = R.quantize(randn(gen(49), ch, ch), 128)
+    cwg.fp8_matmul(q, sc, on_dev(w, dev), w_s.to(dev), None, y, cwg.BF16)
+    R.close(y, R.matmul(want, scale, w, w_s, None, False, torch.bfloat16), "product")
+    cwg.device_status()
+
+
+def test_two_threads_at_once(cuda_dev):
+    """Two host threads, each on a stream of its own, make the same calls as one."""
+    import threading
+
+    plain, want = decode_calls(cuda_dev)
+    for _ in range(20):
+        plain()
+    torch.cuda.synchronize()
+    runs = [decode_calls(cuda_dev) for _ in range(2)]
+    torch.cuda.synchronize()
+    errors = []
+
+    def work(calls):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    calls()
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(c,)) for c, _ in runs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for _, got in runs:
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
