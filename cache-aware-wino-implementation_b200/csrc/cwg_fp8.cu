@@ -278,7 +278,8 @@ static int quantize(QuantArgs a, int block_rows, int pdl, cudaStream_t s) {
   const bool one = a.rows <= 1;
   const bool vec = ((uintptr_t)a.x & 15) == 0 && ((uintptr_t)a.q & 7) == 0 &&
                    a.cols % E == 0 && (one || (a.ldx % E == 0 && a.ldq % 8 == 0));
-  const long long blocks = block_rows != 1 ? a.groups : vec ? (a.groups + 63) / 64 : (a.groups + 7) / 8;
+  const long long blocks =
+      block_rows != 1 ? a.groups : vec ? (a.groups + 63) / 64 : (a.groups + 7) / 8;
   if (a.groups > 0x7fffffffLL - 64) return -2;  // 32-bit group numbers
   const bool one_row = block_rows == 1;
   const auto kernel = one_row ? (vec ? quantize_rows<T, true> : quantize_rows<T, false>)
@@ -308,7 +309,7 @@ constexpr int kGroupK = 8;  // blocks whose scales are staged together
 
 template <int TN>
 struct Cfg {
-  static constexpr int kPromote = TN > 64 ? 8 : 4;       // promoting warps
+  static constexpr int kPromote = TN > 32 ? 8 : 4;       // promoting warps
   static constexpr int kCols = TN * 4 / kPromote;        // columns per promoting thread
   static constexpr int kThreads = (kPromote + 3) * 32;
   static constexpr int kMinBlocks = TN > 64 ? 1 : 2;
@@ -360,8 +361,8 @@ __device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
 __host__ __device__ constexpr uint32_t idesc_fp8(int m, int n) {
   return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float *v) {
-  uint32_t r[16];
+// 16 columns of one lane, and 32; valid after tmem_wait_ld.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t *r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
       "%11, %12, %13, %14, %15}, [%16];"
@@ -370,12 +371,26 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float *v) {
         "=r"(r[14]), "=r"(r[15])
       : "r"(taddr)
       : "memory");
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
+      "%28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
 
@@ -388,6 +403,42 @@ __device__ __forceinline__ void store_out(const MatArgs &a, int row, int col, fl
     static_cast<__nv_bfloat16 *>(a.y)[at] = pack1<__nv_bfloat16>(v);
   else
     static_cast<float *>(a.y)[at] = v;
+}
+// Adds the S ranks' sums of a tile's rows (columns of `part`) rank, rank + S, ... in rank
+// order and stores them: a warp takes a row, a lane four outputs.  All S loads from the
+// other CTAs' shared memory are issued before the first is used.
+template <int S, int TN, int WARPS>
+__device__ __forceinline__ void join_ranks(const MatArgs &p, uint32_t part, int rank, int warp,
+                                           int lane, int m0, int n0, const float (&bias)[4]) {
+  const int col = n0 + lane * 4;
+  uint32_t from[S];
+#pragma unroll
+  for (int r = 0; r < S; ++r) from[r] = mapa_shared(part + lane * 16, (uint32_t)r);
+  for (int j = rank + warp * S; j < TN && m0 + j < p.m; j += WARPS * S) {
+    float4 f[S];
+#pragma unroll
+    for (int r = 0; r < S; ++r) f[r] = ld_cluster4(from[r] + j * 512);
+    float v[4] = {f[0].x, f[0].y, f[0].z, f[0].w};
+#pragma unroll
+    for (int r = 1; r < S; ++r) v[0] += f[r].x, v[1] += f[r].y, v[2] += f[r].z, v[3] += f[r].w;
+    if (p.vec_y && col + 4 <= p.n) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] += bias[e];
+        if (p.relu && v[e] < 0.f) v[e] = 0.f;  // NaN stays
+      }
+      const size_t at = (size_t)(m0 + j) * p.ldy + col;
+      if (p.bf16)
+        seq::store_raw<__nv_bfloat16, 4>(static_cast<__nv_bfloat16 *>(p.y) + at,
+                                         seq::pack<__nv_bfloat16, 4>(v));
+      else
+        seq::store_raw<float, 4>(static_cast<float *>(p.y) + at, seq::pack<float, 4>(v));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (col + e < p.n) store_out(p, m0 + j, col + e, v[e], bias[e]);
+    }
+  }
 }
 
 template <int TN>
@@ -545,25 +596,28 @@ __global__ void __launch_bounds__(Cfg<TN>::kThreads, Cfg<TN>::kMinBlocks)
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
       const float *sc = s_scale + ((g & 1) * kGroupK + k) * TN;
+      uint32_t v[C::kCols];
+      if constexpr (C::kCols == 16) {
+        tmem_ld16(trow + ac * TN, v);
+      } else {
 #pragma unroll
-      for (int j0 = 0; j0 < C::kCols; j0 += 16) {
-        float v[16];
-        tmem_ld16(trow + ac * TN + j0, v);
-        tmem_wait_ld();
-#pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-          const float4 f = *reinterpret_cast<const float4 *>(sc + j0 + j);
-          acc[j0 + j] = fmaf(v[j], f.x, acc[j0 + j]);
-          acc[j0 + j + 1] = fmaf(v[j + 1], f.y, acc[j0 + j + 1]);
-          acc[j0 + j + 2] = fmaf(v[j + 2], f.z, acc[j0 + j + 2]);
-          acc[j0 + j + 3] = fmaf(v[j + 3], f.w, acc[j0 + j + 3]);
-        }
+        for (int j = 0; j < C::kCols; j += 32) tmem_ld32(trow + ac * TN + j, v + j);
       }
-      tc_fence_before();
+      tmem_wait_ld();
+      tc_fence_before();  // all read: the accumulator may be filled again
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(acc_empty + 8 * ac);
-        if (k == kGroupK - 1) mbar_arrive(s_empty + 8 * (g & 1));
+      if (lane == 0) mbar_arrive(acc_empty + 8 * ac);
+#pragma unroll
+      for (int j = 0; j < C::kCols; j += 4) {
+        const float4 f = *reinterpret_cast<const float4 *>(sc + j);
+        acc[j] = fmaf(__uint_as_float(v[j]), f.x, acc[j]);
+        acc[j + 1] = fmaf(__uint_as_float(v[j + 1]), f.y, acc[j + 1]);
+        acc[j + 2] = fmaf(__uint_as_float(v[j + 2]), f.z, acc[j + 2]);
+        acc[j + 3] = fmaf(__uint_as_float(v[j + 3]), f.w, acc[j + 3]);
+      }
+      if (k == kGroupK - 1) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_empty + 8 * (g & 1));
       }
     }
     const int row = quad * 32 + lane, col = n0 + row;
@@ -586,20 +640,20 @@ __global__ void __launch_bounds__(Cfg<TN>::kThreads, Cfg<TN>::kMinBlocks)
 #pragma unroll
       for (int j = 0; j < C::kCols; ++j) part[((warp >> 2) * C::kCols + j) * 128 + row] = acc[j];
     }
-    cluster_sync_all();
-    // rank r finishes the columns r, r + splits, ...
-    const int row = threadIdx.x & 127, lead = (int)(threadIdx.x >> 7);
-    constexpr int kTeams = C::kThreads / 128;
-    const int col = n0 + row;
-    if (lead < kTeams && col < p.n) {
-      const float bias = p.bias ? p.bias[col] : 0.f;
-      for (int j = rank + lead * p.splits; j < TN && m0 + j < p.m; j += kTeams * p.splits) {
-        const uint32_t at = sbase + (uint32_t)(j * 128 + row) * 4;
-        float v = 0.f;
-        for (int r = 0; r < p.splits; ++r) v += ld_cluster(mapa_shared(at, (uint32_t)r));
-        store_out(p, m0 + j, col, v, bias);
-      }
+    float bias[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int col = n0 + lane * 4 + e;
+      bias[e] = p.bias && col < p.n ? p.bias[col] : 0.f;
     }
+    cluster_sync_all();
+    constexpr int kWarps = C::kThreads / 32;
+    if (p.splits == 2)
+      join_ranks<2, TN, kWarps>(p, sbase, rank, warp, lane, m0, n0, bias);
+    else if (p.splits == 4)
+      join_ranks<4, TN, kWarps>(p, sbase, rank, warp, lane, m0, n0, bias);
+    else
+      join_ranks<8, TN, kWarps>(p, sbase, rank, warp, lane, m0, n0, bias);
     __syncwarp();
     cluster_sync_all();  // no CTA leaves while another reads its sums
   }
@@ -663,20 +717,6 @@ __device__ __forceinline__ void mma_fp8_pair(uint32_t d_tmem, uint64_t a_desc, u
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-// 32 columns of one lane; valid after tmem_wait_ld.
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-      "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
-      "%28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
-        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
-        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
       : "memory");
 }
 template <int N>
@@ -844,7 +884,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
           const uint32_t dst = sbase + st * C::kStageBytes;
           mbar_expect_tx(full + 8 * st, C::kStageBytes);
           tma_2d(dst, &map_a, kb * kTileK, m0 + (int)rank * 128, full + 8 * st);
-          tma_2d(dst + 128 * kTileK, &map_w, kb * kTileK, n0 + (int)rank * (C::kN / 2), full + 8 * st);
+          tma_2d(dst + 128 * kTileK, &map_w, kb * kTileK, n0 + (int)rank * (C::kN / 2),
+                 full + 8 * st);
         }
         __syncwarp();
       }

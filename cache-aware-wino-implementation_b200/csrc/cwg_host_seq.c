@@ -45,6 +45,15 @@ static int ranges_meet(const void *a, long long arow, const void *b, long long b
   return a0 < b1 && b0 < a1;
 }
 
+/* Whether `rows` rows of `width` elements share bytes with the cache lines. */
+static int meets_lines(const void *p, long long ld, long long rows, long long width, size_t esz,
+                       const void *state, int n_slots, long long line, size_t line_esz) {
+  if (!p || !state || rows <= 0 || n_slots <= 0) return 0;
+  const __int128 a = (__int128)(uintptr_t)p, s = (__int128)(uintptr_t)state;
+  return a < s + (__int128)n_slots * line * (__int128)line_esz &&
+         s < a + ((__int128)(rows - 1) * ld * (rows > 1) + width) * (__int128)esz;
+}
+
 static int act_of(unsigned flags, unsigned allowed) {
   const unsigned act = flags & (CWG_RELU | CWG_SILU);
   if (flags & ~(allowed | CWG_BF16 | CWG_NO_PDL)) return -1;
@@ -70,7 +79,10 @@ static int conv1d_check(const cwgk_conv1d *p, int rows, unsigned flags) {
     if (!rows_ok(p->x, p->ldx, rows, p->channels, esz) ||
         !rows_ok(p->y, p->ldy, rows, p->channels, esz))
       return CWG_EINVAL;
-    if (overlaps(p->x, p->ldx, p->channels, p->y, p->ldy, p->channels, rows, esz))
+    const long long line = (long long)(p->width - 1) * p->channels;
+    if (overlaps(p->x, p->ldx, p->channels, p->y, p->ldy, p->channels, rows, esz) ||
+        meets_lines(p->x, p->ldx, rows, p->channels, esz, p->state, p->n_slots, line, esz) ||
+        meets_lines(p->y, p->ldy, rows, p->channels, esz, p->state, p->n_slots, line, esz))
       return CWG_EINVAL;
   }
   return CWG_OK;
@@ -112,7 +124,8 @@ static int ssm_check(const cwg_ssm *p, int n_seq) {
   if (!p) return CWG_EINVAL;
   if (p->flags & ~(CWG_BF16 | CWG_SOFTPLUS | CWG_NO_PDL)) return CWG_EINVAL;
   const size_t esz = (p->flags & CWG_BF16) ? 2 : 4;
-  if (p->tokens < 0 || p->tokens > kMaxRows || n_seq < 0 || p->channels <= 0 || p->groups <= 0 || p->states <= 0)
+  if (p->tokens < 0 || p->tokens > kMaxRows || n_seq < 0 || p->channels <= 0 ||
+      p->groups <= 0 || p->states <= 0)
     return CWG_EINVAL;
   if (p->channels % p->groups) return CWG_EINVAL;
   if (p->states > 64) return CWG_EUNSUPPORTED;
@@ -131,6 +144,14 @@ static int ssm_check(const cwg_ssm *p, int n_seq) {
         overlaps(p->z, p->ldz, c, p->y, p->ldy, c, rows, esz) ||
         overlaps(p->B, p->ldb, gn, p->y, p->ldy, c, rows, esz) ||
         overlaps(p->C, p->ldc, gn, p->y, p->ldy, c, rows, esz))
+      return CWG_EINVAL;
+    const long long line = c * p->states;
+    if (meets_lines(p->u, p->ldu, rows, c, esz, p->state, p->n_slots, line, 4) ||
+        meets_lines(p->dt, p->lddt, rows, c, esz, p->state, p->n_slots, line, 4) ||
+        meets_lines(p->z, p->ldz, rows, c, esz, p->state, p->n_slots, line, 4) ||
+        meets_lines(p->B, p->ldb, rows, gn, esz, p->state, p->n_slots, line, 4) ||
+        meets_lines(p->C, p->ldc, rows, gn, esz, p->state, p->n_slots, line, 4) ||
+        meets_lines(p->y, p->ldy, rows, c, esz, p->state, p->n_slots, line, 4))
       return CWG_EINVAL;
   }
   return CWG_OK;

@@ -354,8 +354,9 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads, MODE == kRoomy ? 1 : 0)
             y[t] = s.x + s.y;
           }
         }
-        if constexpr (SUMMARY) {  // the steps pairwise, then with compensation: a sum's rounding enters
-                        // the decay of everything before this chunk
+        // a chunk's steps are added pairwise, then with compensation: their sum's rounding
+        // enters the decay of everything before the chunk
+        if constexpr (SUMMARY) {
 #pragma unroll
           for (int o = 1; o < TG; o *= 2)
 #pragma unroll
@@ -422,8 +423,8 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads, MODE == kRoomy ? 1 : 0)
           [&](int t, int k) { return sh.bc[st][t][k / kS].at(k % kS); });
       if (!SUMMARY)
         copy_rows<T, G::kElem, kS * L, kS, VBC>(
-          e, static_cast<const T *>(p.C) + at * p.ldc + col, (size_t)p.ldc, p.states, rows,
-          [&](int t, int k) { return sh.bc[st][t][k / kS].at(kS + k % kS); });
+            e, static_cast<const T *>(p.C) + at * p.ldc + col, (size_t)p.ldc, p.states, rows,
+            [&](int t, int k) { return sh.bc[st][t][k / kS].at(kS + k % kS); });
       copy_commit();
     };
     // pairs (d, d u); rows past the end have d = 0, which leaves the states as they are

@@ -227,10 +227,11 @@ int cwg_conv3x3_nonfused(const float *x, const float *U, const float *bias, floa
  * operand: a slot >= n_slots, or one that an earlier sequence of the call has
  * too, counts as negative, a sequence whose offsets are not
  * 0 <= starts[b] <= starts[b+1] <= tokens is left out, and
- * cwg_device_status reports CWG_EINDEX.
+ * cwg_device_status reports CWG_EINDEX.  Where offsets descend, what the call leaves in
+ * the rows and lines of its other sequences is unspecified.
  *
- * y must not overlap the inputs (disjoint columns of one matrix do not overlap):
- * CWG_EINVAL.  All calls are asynchronous on `stream`, allocate nothing and can be
+ * y must not overlap the inputs (disjoint columns of one matrix do not overlap), nor
+ * state any of them: CWG_EINVAL.  All calls are asynchronous on `stream`, allocate nothing and can be
  * captured into a graph (make a call of the kind before the first capture: kernels are
  * loaded and configured at their first launch); they are programmatic dependent launches
  * (see CWG_NO_PDL, which they take too). */
@@ -255,7 +256,9 @@ int cwg_conv1d_causal_step(const void *x, long long ldx, const float *w, const f
  *   y[t][c] = (sum_i C[t][g][i] h[c][i] + D[c] u[t][c]) * z[t][c] / (1 + exp(-z[t][c]))
  * A fp32 [channels][states], B and C rows of groups * states columns, D and
  * dt_bias fp32 [channels] or NULL, z or NULL (no gate).  state fp32
- * [n_slots][channels][states].  1 <= states <= 64; groups divides channels. */
+ * [n_slots][channels][states].  1 <= states <= 64; groups divides channels.  Inputs are
+ * meant to be finite: from an infinite step or u on, a channel's y may be NaN where the
+ * formula gives an infinity.  No other channel or sequence is touched by that. */
 typedef struct cwg_ssm {
   const void *u, *dt, *B, *C, *z;
   void *y;

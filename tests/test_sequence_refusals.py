@@ -37,6 +37,8 @@ def conv_step(**kw):
     (dict(ldx=96, ldy=96, y=X + 63 * 4), cwg.EINVAL),   # one shared column
     (dict(slots=None, n_slots=1), cwg.EINVAL),          # line b of too few lines
     (dict(n_slots=-1), cwg.EINVAL), (dict(state=S + 2), cwg.EINVAL),
+    (dict(state=X), cwg.EINVAL), (dict(state=Y + 2556), cwg.EINVAL),  # lines among the rows
+    (dict(state=Y - 4 * 3 * 64 * 4 + 4), cwg.EINVAL), (dict(state=X, n_slots=1 << 30), cwg.EINVAL),
     (dict(n_seq=0), cwg.OK), (dict(tokens=0, state=None), cwg.OK),
 ])
 def test_conv1d_refuses(kw, status):
@@ -71,6 +73,8 @@ def ssm(step=False, workspace=None, size=0, **kw):
     dict(channels=0), dict(groups=0), dict(groups=3), dict(states=0), dict(tokens=-1),
     dict(A=W + 1), dict(D=W + 2), dict(flags=cwg.SILU), dict(flags=cwg.RELU), dict(y=X),
     dict(B=Y, ldb=64), dict(slots=None, n_slots=1), dict(state=S + 1),
+    dict(state=X), dict(state=X + 0x40000), dict(state=X + 0x80000 + 16), dict(state=X + 0xC0000),
+    dict(state=Y + 4), dict(z=S + 16, ldz=64),
 ], ids=str)
 def test_ssm_refuses(step, kw):
     assert ssm(step, **kw) == cwg.EINVAL
