@@ -1152,7 +1152,9 @@ static int resident_pairs() {
   return n;
 }
 
-// The pair kernel where its tiles fill at least half of the pairs.
+// The pair kernel where its tiles fill at least half of the pairs (192 x 11008 x 4096, 43
+// tiles: 24.4 us, 37.9 with tiles of 128 x 128; 512 x 4096 x 4096, 32 tiles: 22.8 and 21.5;
+// 1024 x 2048 x 8192, 32 tiles: 39.2 and 32.8).
 static bool pair_pays(const cwgk_fp8 *op) {
   const long long tiles =
       (long long)((op->m + 255) / 256) * ((op->n + PairCfg::kN - 1) / PairCfg::kN);
@@ -1183,6 +1185,10 @@ static int launch_pair(const cwgk_fp8 *op, cudaStream_t s) {
   return 0;
 }
 
+static long long out_tiles(const cwgk_fp8 *op, int tn) {
+  return (long long)((op->n + 127) / 128) * ((op->m + tn - 1) / tn);
+}
+
 template <int TN>
 static int launch(const cwgk_fp8 *op, cudaStream_t s) {
   using C = Cfg<TN>;
@@ -1191,9 +1197,12 @@ static int launch(const cwgk_fp8 *op, cudaStream_t s) {
   if (!rc) rc = make_map(&map_w, op->w, op->ldw, op->n, op->k, 128);
   if (rc) return rc;
   MatArgs p = make_args(op);
-  const long long tiles = (long long)((op->n + 127) / 128) * ((op->m + TN - 1) / TN);
+  const long long tiles = out_tiles(op, TN);
   int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= 148 * C::kMinBlocks && p.kblocks >= splits * 4)
+  // 16 clusters of 8 do not run at once with one CTA per SM, which they do not fill GPC by
+  // GPC (128 x 2048 x 8192 in 16 of them: 22 us, 14.4 for 32 of four that hold 256 rows)
+  while (splits < 8 && tiles * splits * 2 <= (splits < 4 || TN < 128 ? 148 : 112) * C::kMinBlocks &&
+         p.kblocks >= splits * 4)
     splits *= 2;
   p.splits = splits;
   p.per = (p.kblocks + splits - 1) / splits;
@@ -1237,11 +1246,17 @@ int cwgk_fp8_quantize(const void *x, long long ldx, void *q, long long ldq, floa
 
 int cwgk_fp8_matmul(const cwgk_fp8 *op, void *stream) {
   cudaStream_t s = (cudaStream_t)stream;
-  if (op->m <= 16) return cwg::fp8::launch<16>(op, s);
-  if (op->m <= 32) return cwg::fp8::launch<32>(op, s);
-  if (op->m <= 64) return cwg::fp8::launch<64>(op, s);
-  if (cwg::fp8::pair_pays(op)) return cwg::fp8::launch_pair(op, s);
-  return cwg::fp8::launch<128>(op, s);
+  // Rows per tile.  Small tiles make more CTAs of work that is bound by latencies, as long
+  // as those all run at once, two per SM (72 rows x 2048 x 8192: 10.0 us with tiles of 32
+  // rows, 11.1 with 64, 18.9 with 128; x 11008 x 4096, 258 tiles of 32: 16.1, 21.8, 20.6; 128
+  // rows, 344 tiles: 26.3, 23.8, 22.1).  200 rows x 1024 x 4096, 32 tiles of 64: 8.6 us, 12.8
+  // with 128; x 4096 x 4096, 128 tiles: 14.7 and 14.3.
+  using namespace cwg::fp8;
+  if (op->m <= 16) return launch<16>(op, s);
+  if (op->m <= 32 || (op->m <= 128 && out_tiles(op, 32) <= 2 * 148)) return launch<32>(op, s);
+  if (op->m <= 64 || (op->m <= 256 && out_tiles(op, 64) * 8 <= 2 * 148)) return launch<64>(op, s);
+  if (pair_pays(op)) return launch_pair(op, s);
+  return launch<128>(op, s);
 }
 
 int cwgk_fp8_read_clear_status(unsigned *status) {

@@ -799,3 +799,16 @@ def test_two_threads_at_once(cuda_dev):
     assert not errors
     for _, got in runs:
         assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("pad", [(3, 2), (0, 0)])
+@pytest.mark.parametrize("m,n,k", [
+    (16, 1024, 4096), (9, 2048, 512), (20, 9000, 256),        # tiles of 16 and 32 rows
+    (72, 2048, 2100), (128, 300, 1024), (100, 11008, 140),    # 32 rows, cut 4, 8 and 1 ways
+    (40, 19000, 260), (250, 1000, 700), (130, 260, 3000),     # 64 rows
+    (100, 20000, 130), (384, 1024, 1000), (400, 300, 2000),   # 128 rows, cut 1, 4 and 8 ways
+    (190, 4096, 520),
+])
+def test_fp8_matmul_tiles(cuda_dev, dtype, pad, m, n, k):
+    check_matmul(cuda_dev, m, n, k, dtype, relu=m % 3 == 0, with_bias=n % 3 != 0, pad=pad)
