@@ -146,6 +146,30 @@ __global__ void __launch_bounds__(kConvThreads) conv1d_prompt(const ConvArgs a) 
   Chan<V> w[K], b, h[K - 1];
   load_weights<V, K>(a, c, active, w, b);
 
+  // The run's first rows, and those before it, are on their way while the sequences that begin
+  // in it are looked at.
+  const T *px = x + (size_t)t0 * a.ldx + c;  // of row t
+  T *py = y + (size_t)t0 * a.ldy + c;
+  typename Raw<T, V>::type raw[kAhead], next[kAhead];
+  auto fetch = [&](const T *from, int left) {  // kAhead rows, of which `left` are the run's
+    if (left >= kAhead) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) next[i] = load_raw<T, V>(from + i * a.ldx);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        next[i] = i < left ? load_raw<T, V>(from + i * a.ldx) : zero_raw<T, V>();
+    }
+  };
+  fetch(px, active ? t1 - t0 : 0);
+  typename Raw<T, V>::type before[K - 1];
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j) {
+    const int t = t0 - (K - 1) + j;
+    before[j] = active && t >= 0 && t < a.tokens ? load_raw<T, V>(x + (size_t)t * a.ldx + c)
+                                                 : zero_raw<T, V>();
+  }
+
   // Sequences that begin in this run (the first run also has those that begin
   // before row 0 by a bad offset, the last one those that begin at the end).
   const int first = run == 0 ? 0 : lower_bound(starts, a.n_seq, t0);
@@ -157,6 +181,12 @@ __global__ void __launch_bounds__(kConvThreads) conv1d_prompt(const ConvArgs a) 
       bad = true;
       continue;
     }
+    const int len = end - begin;
+    typename Raw<T, V>::type xs[K - 1];
+#pragma unroll
+    for (int i = 0; i < K - 1; ++i)
+      xs[i] = active && i < len ? load_raw<T, V>(x + (size_t)(begin + i) * a.ldx + c)
+                                : zero_raw<T, V>();
     const int slot = state ? line_of(a.slots, s, a.n_slots, bad) : -1;
     const bool carry = slot >= 0 && a.resume && a.resume[s];
     if (!active) continue;
@@ -164,12 +194,11 @@ __global__ void __launch_bounds__(kConvThreads) conv1d_prompt(const ConvArgs a) 
 #pragma unroll
     for (int j = 0; j < K - 1; ++j)
       h[j].from(carry ? load_raw<T, V>(line + (size_t)j * a.channels) : zero_raw<T, V>());
-    const int len = end - begin;
 #pragma unroll
     for (int i = 0; i < K - 1; ++i) {
       if (i < len) {
         Chan<V> xv;
-        xv.from(load_raw<T, V>(x + (size_t)(begin + i) * a.ldx + c));
+        xv.from(xs[i]);
         store_raw<T, V>(y + (size_t)(begin + i) * a.ldy + c,
                         window_row<T, V, K, ACT>(w, b, h, xv));
         slide<V, K>(h, xv);
@@ -195,25 +224,7 @@ __global__ void __launch_bounds__(kConvThreads) conv1d_prompt(const ConvArgs a) 
   if (s >= 0) begin = starts[s], end = starts[s + 1];
   if (begin < 0 || end > a.tokens) end = begin = 0;
 #pragma unroll
-  for (int j = 0; j < K - 1; ++j) {
-    const int t = t0 - (K - 1) + j;
-    h[j].from(t >= 0 && t < a.tokens ? load_raw<T, V>(x + (size_t)t * a.ldx + c)
-                                     : zero_raw<T, V>());
-  }
-  const T *px = x + (size_t)t0 * a.ldx + c;  // of row t
-  T *py = y + (size_t)t0 * a.ldy + c;
-  typename Raw<T, V>::type raw[kAhead], next[kAhead];
-  auto fetch = [&](const T *from, int left) {  // kAhead rows, of which `left` are the run's
-    if (left >= kAhead) {
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) next[i] = load_raw<T, V>(from + i * a.ldx);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i)
-        next[i] = i < left ? load_raw<T, V>(from + i * a.ldx) : zero_raw<T, V>();
-    }
-  };
-  fetch(px, t1 - t0);
+  for (int j = 0; j < K - 1; ++j) h[j].from(before[j]);
   for (int t = t0; t < t1; t += kAhead) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) raw[i] = next[i];

@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(256) quantize_rows(const QuantArgs a) {
     for (int o = kLanes / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float s = scale_of(m);
     if (ok && lane == 0) a.scale[(size_t)row * a.lds + kb] = s;
-    return s;
+    return m ? s : 1.f;  // zeros, and lanes without a group, need no slow division
   };
   if constexpr (VEC) {
     Eight<T> v[4];
@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(512) quantize_blocks(const QuantArgs a) {
     for (int i = 0; i < 16; ++i) m = max(m, s_max[i]);
     const float s = scale_of(m);
     if (tid == 0) a.scale[(size_t)rb * a.lds + kb] = s;
-    return s;
+    return m ? s : 1.f;  // zeros need no slow division
   };
   if constexpr (VEC) {
     Eight<T> v[4];
@@ -333,6 +333,7 @@ struct MatArgs {
   int m, n, kblocks, per;  // per: k blocks of one cluster rank
   int splits, relu, bf16;
   int vec_y, vec_scale;    // rows of y and of a_scale are 16-byte aligned
+  int pair_y;              // rows of y are 4-byte aligned
 };
 
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, int x, int y,
@@ -737,13 +738,33 @@ __device__ __forceinline__ void pair_tile(const MatArgs &p, int t, int &m0, int 
   n0 = r / rows * PairCfg::kN;
 }
 
+// W bytes, as one access.
+template <int W>
+struct Bytes {
+  typedef uint4 type;
+};
+template <>
+struct Bytes<4> {
+  typedef uint32_t type;
+};
+template <>
+struct Bytes<2> {
+  typedef uint16_t type;
+};
+
 // A warp's 32 rows x COLS columns, 64 bytes of each row at a time through a patch of its
 // own, whose 16-byte pieces are turned by the row so that neither side has bank conflicts:
-// a store instruction then writes 64 bytes of 8 rows instead of 16 bytes of 32.
-template <typename T, int COLS>
+// a store instruction then writes 64 bytes of 8 rows instead of 16 bytes of 32.  W: bytes
+// that y's rows are aligned to; 64 bytes of one or two rows at a time where that is an
+// element (3424 x 844 x 120 bf16: 49 us without the patch, 11).
+template <typename T, int COLS, int W>
 __device__ __forceinline__ void store_rows(uint8_t *patch, const seq::F2 (&acc)[COLS / 2],
                                            const MatArgs &p, int row, int col, int lane) {
   constexpr int E = 16 / (int)sizeof(T), kRound = 4 * E;  // columns per 64 bytes
+  constexpr int kLanes = 64 / W, kRows = 32 / kLanes;     // of one store instruction
+  constexpr int EW = W / (int)sizeof(T);
+  typedef typename Bytes<W>::type Word;
+  row -= lane;
 #pragma unroll
   for (int c0 = 0; c0 < COLS; c0 += kRound) {
 #pragma unroll
@@ -758,13 +779,19 @@ __device__ __forceinline__ void store_rows(uint8_t *patch, const seq::F2 (&acc)[
           seq::pack<T, E>(v);
     }
     __syncwarp();
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int r = g * 8 + lane / 4, c = lane % 4;
-      const uint4 w = *reinterpret_cast<const uint4 *>(patch + r * 64 + ((c ^ (r >> 1)) & 3) * 16);
-      if (row - lane + r < p.m)
-        *reinterpret_cast<uint4 *>(static_cast<T *>(p.y) + (size_t)(row - lane + r) * p.ldy + col +
-                                   c0 + c * E) = w;
+    const int b = lane % kLanes * W, c = col + c0 + b / (int)sizeof(T);
+#pragma unroll(W == 16 ? 4 : 2)
+    for (int g = 0; g < 32 / kRows; ++g) {
+      const int r = g * kRows + lane / kLanes;
+      const uint8_t *from = patch + r * 64 + ((b / 16 ^ (r >> 1)) & 3) * 16 + b % 16;
+      if (row + r >= p.m) continue;
+      T *to = static_cast<T *>(p.y) + (size_t)(row + r) * p.ldy + c;
+      if (c + EW <= p.n) {
+        *reinterpret_cast<Word *>(to) = *reinterpret_cast<const Word *>(from);
+      } else {
+        for (int e = 0; e < EW; ++e)
+          if (c + e < p.n) to[e] = reinterpret_cast<const T *>(from)[e];
+      }
     }
     __syncwarp();
   }
@@ -1023,7 +1050,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
       }
       const int row = m0 + (int)rank * 128 + quad * 32 + lane, col = n0 + half * C::kCols;
       if (!ok || col >= p.n) continue;  // whole warps
-      const int ncol = min(C::kCols, p.n - col);
       if (p.bias) {
         const float *bias = reinterpret_cast<const float *>(smem + C::kBiasOff) +
                             j % 3 * C::kN + half * C::kCols;
@@ -1041,25 +1067,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
           acc[c] = seq::f2(f.x < 0.f ? 0.f : f.x, f.y < 0.f ? 0.f : f.y);  // NaN stays
         }
       }
-      if (ncol == C::kCols && p.vec_y) {
-        if (p.bf16)
-          store_rows<__nv_bfloat16, C::kCols>(patch, acc, p, row, col, lane);
-        else
-          store_rows<float, C::kCols>(patch, acc, p, row, col, lane);
-      } else if (row < p.m) {
-        const size_t at = (size_t)row * p.ldy + col;
-#pragma unroll
-        for (int c = 0; c < C::kCols; ++c) {
-          const float2 f = seq::halves(acc[c / 2]);
-          const float v = c % 2 ? f.y : f.x;
-          if (c < ncol) {
-            if (p.bf16)
-              static_cast<__nv_bfloat16 *>(p.y)[at + c] = pack1<__nv_bfloat16>(v);
-            else
-              static_cast<float *>(p.y)[at + c] = v;
-          }
-        }
-      }
+      if (p.bf16 && p.vec_y)
+        store_rows<__nv_bfloat16, C::kCols, 16>(patch, acc, p, row, col, lane);
+      else if (p.bf16 && p.pair_y)
+        store_rows<__nv_bfloat16, C::kCols, 4>(patch, acc, p, row, col, lane);
+      else if (p.bf16)
+        store_rows<__nv_bfloat16, C::kCols, 2>(patch, acc, p, row, col, lane);
+      else if (p.vec_y)
+        store_rows<float, C::kCols, 16>(patch, acc, p, row, col, lane);
+      else
+        store_rows<float, C::kCols, 4>(patch, acc, p, row, col, lane);
     }
   }
   tc_fence_before();
@@ -1127,6 +1144,7 @@ static MatArgs make_args(const cwgk_fp8 *op) {
   const long long esz = op->bf16 ? 2 : 4;
   p.vec_scale = ((uintptr_t)op->a_scale & 15) == 0 && (op->m <= 1 || op->lda_scale % 4 == 0);
   p.vec_y = ((uintptr_t)op->y & 15) == 0 && (op->m <= 1 || op->ldy * esz % 16 == 0);
+  p.pair_y = ((uintptr_t)op->y & 3) == 0 && (op->m <= 1 || op->ldy * esz % 4 == 0);
   return p;
 }
 

@@ -493,10 +493,15 @@ struct Geo {
   static constexpr int kNP = 4 * V * L;
 };
 
+// How a step's states, A, B and C are read: one at a time; four at a time, where there are
+// whole fours of them; states == 4 V L, in the widest vectors.
+enum { kSingle = 0, kFours = 1, kWhole = 2 };
+
 // One row's B or C of a lane: 4 V values, as they are in memory.
-template <typename T, int V, bool VEC>
+template <typename T, int V, int VEC>
 struct Row4 {
-  static constexpr int E = !VEC ? 1 : V * 4 * (int)sizeof(T) >= 16 ? 16 / (int)sizeof(T) : 4;
+  static constexpr int E =
+      !VEC ? 1 : VEC == kWhole && V * 4 * (int)sizeof(T) >= 16 ? 16 / (int)sizeof(T) : 4;
   typename Raw<T, E>::type raw[4 * V / E];
   __device__ __forceinline__ void load(const T *p, int n) {  // n of them exist
 #pragma unroll
@@ -518,8 +523,7 @@ struct Row4 {
 
 // 4 V states per lane: 8 where there are that many, since what a row costs besides its
 // states (step, shuffles, addresses) is then paid by half as many threads.
-// VEC: states == 4 V L, and state, A, B and C can be read in whole vectors.
-template <typename T, int V, int L, int RR, bool VEC>
+template <typename T, int V, int L, int RR, int VEC>
 __global__ void __launch_bounds__(Geo<V, L>::kThreads) ssm_token(const Args a) {
   griddep_wait();
   griddep_launch_dependents();
@@ -530,6 +534,7 @@ __global__ void __launch_bounds__(Geo<V, L>::kThreads) ssm_token(const Args a) {
   const int ch = tid / L, l = tid % L, i0 = l * 4 * V;
   const int in = cblk * CH + ch, c = group * a.per + in;
   const bool mine = in < a.per;
+  auto exists = [&](int v) { return VEC != kFours || i0 + 4 * v < p.states; };
   const int rows = min(RR, p.tokens - r0);
   const size_t width = (size_t)p.channels * p.states;
   float *state = p.state + (size_t)c * p.states;
@@ -552,7 +557,7 @@ __global__ void __launch_bounds__(Geo<V, L>::kThreads) ssm_token(const Args a) {
     for (int v = 0; v < V; ++v) {
 #pragma unroll
       for (int i = 0; i < kS; ++i) h[k][v][i] = 0.f;
-      if (mine && slot[k] >= 0)
+      if (mine && slot[k] >= 0 && exists(v))
         load_states(state + (size_t)slot[k] * width, i0 + 4 * v, p.states, VEC, h[k][v]);
     }
   }
@@ -580,7 +585,8 @@ __global__ void __launch_bounds__(Geo<V, L>::kThreads) ssm_token(const Args a) {
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     float f[kS] = {0.f, 0.f, 0.f, 0.f};
-    if (mine) load_states(p.A + (size_t)c * p.states, i0 + 4 * v, p.states, VEC, f);
+    if (mine && exists(v))
+      load_states(p.A + (size_t)c * p.states, i0 + 4 * v, p.states, VEC, f);
     a2[2 * v] = f2(f[0] * kLog2e, f[1] * kLog2e);
     a2[2 * v + 1] = f2(f[2] * kLog2e, f[3] * kLog2e);
   }
@@ -642,7 +648,8 @@ __global__ void __launch_bounds__(Geo<V, L>::kThreads) ssm_token(const Args a) {
     if (mine && slot[k] >= 0) {
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        store_states(state + (size_t)slot[k] * width, i0 + 4 * v, p.states, VEC, h[k][v]);
+        if (exists(v))
+          store_states(state + (size_t)slot[k] * width, i0 + 4 * v, p.states, VEC, h[k][v]);
     }
     if (l == from || RR == 1) out[e] = y;
   }
@@ -692,15 +699,18 @@ static int launch_prompt(const Args &a, unsigned blocks, cudaStream_t s) {
 }
 
 // Tokens per chunk when a call's sequences are cut, else 0.  `ctas`: CTAs along the
-// channels.  Cut where at most half of the SMs would have a CTA and sequences are at least
-// four chunks long on average; chunks of 256 tokens or more (8 tiles), as many as make
-// three CTAs per SM (one sequence of 1024 tokens, 1024 channels: 32 us, 41 uncut; of 600: 31
-// and 26; of 8192 tokens and 256, 1024, 2048 channels: 47, 130, 254 us, 300 uncut).
+// channels.  Cut where at most half of the SMs would have a CTA; chunks of 256 tokens or more
+// (8 tiles), as many as make three CTAs per SM.  One sequence is cut from four chunks on (1024
+// tokens, 1024 channels: 32 us, 41 uncut; 600 tokens: 31 and 26; 8192 tokens and 256, 1024,
+// 2048 channels: 47, 130, 254 us, 300 uncut).  Several are cut from two chunks on average,
+// since the longest one's length decides uncut (4096 tokens in two sequences, 1024 channels:
+// 75 us cut; uncut 76 if they are equally long, 100 if one has two thirds; in eight, 256
+// channels: 27 to 30, uncut 22 and 36).
 static int chunk_of(int tokens, int n_seq, long long ctas) {
   if (n_seq <= 0 || ctas * n_seq > 74) return 0;
   long long chunk = (tokens * ctas + 3 * 148 - 1) / (3 * 148);
   chunk = chunk < 256 ? 256 : (chunk + kTT - 1) / kTT * kTT;
-  return tokens / n_seq >= 4 * chunk ? (int)chunk : 0;
+  return tokens / n_seq >= (n_seq > 1 ? 2 : 4) * chunk ? (int)chunk : 0;
 }
 static size_t al256(size_t n) { return (n + 255) / 256 * 256; }
 static size_t ends_bytes(long long slots, int channels, int states) {
@@ -717,7 +727,7 @@ static Args make_args(const cwg_ssm *op, int np, int lane, size_t esz) {
   a.ends = a.sums = nullptr;
   a.vec_state = op->states == np && aligned16(op->state);
   a.vec_a = op->states == np && aligned16(op->A);
-  a.vec_bc = op->states == np && ((uintptr_t)op->B % (lane * esz)) == 0 &&
+  a.vec_bc = op->states % lane == 0 && ((uintptr_t)op->B % (lane * esz)) == 0 &&
              ((uintptr_t)op->C % (lane * esz)) == 0 && a.p.ldb % lane == 0 &&
              a.p.ldc % lane == 0;
   return a;
@@ -755,11 +765,18 @@ static int steps(const cwg_ssm *op, cudaStream_t s) {
   // two rows that share A as soon as every SM has work all the same (256 rows of 4096 x 16:
   // 38.4 us with four)
   const long long blocks = (long long)op->tokens * a.cblocks * op->groups;
-  const bool two = blocks >= 4 * 2 * 148, vec = a.vec_state && a.vec_a && a.vec_bc;
+  const bool two = blocks >= 4 * 2 * 148, whole = a.vec_state && a.vec_a && a.vec_bc;
+  const bool fours = op->states % 4 == 0 && aligned16(op->state) && aligned16(op->A) &&
+                     make_args(op, G::kNP, 4, sizeof(T)).vec_bc;
   const dim3 grid((unsigned)a.cblocks, (unsigned)op->groups,
                   (unsigned)(two ? (op->tokens + 1) / 2 : op->tokens));
-  const auto kernel = two ? (vec ? ssm_token<T, V, L, 2, true> : ssm_token<T, V, L, 2, false>)
-                          : (vec ? ssm_token<T, V, L, 1, true> : ssm_token<T, V, L, 1, false>);
+  // 318 rows of 3456 x 12 bf16: 45 us one at a time, 29 in fours
+  const auto kernel = two     ? (whole   ? ssm_token<T, V, L, 2, kWhole>
+                                 : fours ? ssm_token<T, V, L, 2, kFours>
+                                         : ssm_token<T, V, L, 2, kSingle>)
+                      : whole ? ssm_token<T, V, L, 1, kWhole>
+                      : fours ? ssm_token<T, V, L, 1, kFours>
+                              : ssm_token<T, V, L, 1, kSingle>;
   return start(kernel, grid, G::kThreads, 0, s, a);
 }
 

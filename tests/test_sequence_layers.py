@@ -812,3 +812,47 @@ def test_two_threads_at_once(cuda_dev):
 ])
 def test_fp8_matmul_tiles(cuda_dev, dtype, pad, m, n, k):
     check_matmul(cuda_dev, m, n, k, dtype, relu=m % 3 == 0, with_bias=n % 3 != 0, pad=pad)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("left,right", [(2, 2), (1, 0), (4, 4), (8, 24)])
+def test_fp8_matmul_pairs_row_alignment(cuda_dev, dtype, left, right):
+    """Rows of y that are aligned to 16 bytes, to 4 and to an element."""
+    n = 1690
+    right += -(left + n + right) % (8 if left == 8 else 2)
+    check_matmul(cuda_dev, 1540, n, 260, dtype, relu=left == 2, with_bias=left != 4,
+                 pad=(left, right))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("ch,groups,n", [(520, 1, 12), (514, 2, 20), (516, 2, 4), (330, 1, 23),
+                                         (512, 1, 16), (128, 1, 60)])
+def test_ssm_step_many_rows(cuda_dev, dtype, ch, groups, n):
+    rows = 301
+    c = ssm_case(dtype, [1] * rows, ch, groups, n, 51, tail=0)
+    dev = cuda_dev
+    state = c["state"].to(dev)
+    y = torch.empty_like(c["u"], device=dev)
+    cwg.ssm_step(*(put(c[k], dev) for k in ("u", "step", "A", "B", "C", "D", "bias", "z")), y,
+                 state, put(c["slots"], dev), (cwg.BF16 if dtype == "bf16" else 0) | cwg.SOFTPLUS)
+    cwg.device_status()
+    for i in range(0, rows, 20):
+        slot = int(c["slots"][i])
+        want, new = ssm_want(c, slice(i, i + 1), c["state"][slot])
+        R.close(y[i:i + 1], want, f"row {i}")
+        R.close(state[slot], new, f"state of row {i}")
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("cols", [384, 333])
+def test_fp8_quantize_zeros_and_small_values(cuda_dev, block_rows, cols):
+    x = torch.zeros(260, cols)
+    x[1] = -0.0
+    x[2, ::2] = 3e-39                      # denormal: the scale's lower bound
+    x[3] = torch.linspace(-1e-35, 1e-35, cols)
+    x[200:] = 0.5
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=cuda_dev)
+    want, scale = R.quantize(x, block_rows)
+    s = torch.empty(scale.shape, device=cuda_dev)
+    cwg.fp8_quantize(x.to(cuda_dev), q, s, block_rows)
+    assert torch.equal(s.cpu(), scale) and torch.equal(q.float().cpu(), want.float())
