@@ -1170,13 +1170,8 @@ static int resident_pairs() {
   return n;
 }
 
-// The pair kernel where its tiles fill at least half of the pairs (192 x 11008 x 4096, 43
-// tiles: 24.4 us, 37.9 with tiles of 128 x 128; 512 x 4096 x 4096, 32 tiles: 22.8 and 21.5;
-// 1024 x 2048 x 8192, 32 tiles: 39.2 and 32.8).
-static bool pair_pays(const cwgk_fp8 *op) {
-  const long long tiles =
-      (long long)((op->m + 255) / 256) * ((op->n + PairCfg::kN - 1) / PairCfg::kN);
-  return op->m > 128 && tiles >= 37;
+static long long pair_tiles(const cwgk_fp8 *op) {
+  return (long long)((op->m + 255) / 256) * ((op->n + PairCfg::kN - 1) / PairCfg::kN);
 }
 
 static int launch_pair(const cwgk_fp8 *op, cudaStream_t s) {
@@ -1185,8 +1180,7 @@ static int launch_pair(const cwgk_fp8 *op, cudaStream_t s) {
   if (!rc) rc = make_map(&map_w, op->w, op->ldw, op->n, op->k, PairCfg::kN / 2);
   if (rc) return rc;
   const MatArgs p = make_args(op);
-  const long long tiles =
-      (long long)((op->m + 255) / 256) * ((op->n + PairCfg::kN - 1) / PairCfg::kN);
+  const long long tiles = pair_tiles(op);
   if (tiles * p.kblocks > 0x7fffffffLL) return -2;
   cudaError_t e = smem_attr_once<fp8_matmul_pair>(PairCfg::kSmem);
   if (e == cudaSuccess) {
@@ -1217,9 +1211,7 @@ static int launch(const cwgk_fp8 *op, cudaStream_t s) {
   MatArgs p = make_args(op);
   const long long tiles = out_tiles(op, TN);
   int splits = 1;
-  // 16 clusters of 8 do not run at once with one CTA per SM, which they do not fill GPC by
-  // GPC (128 x 2048 x 8192 in 16 of them: 22 us, 14.4 for 32 of four that hold 256 rows)
-  while (splits < 8 && tiles * splits * 2 <= (splits < 4 || TN < 128 ? 148 : 112) * C::kMinBlocks &&
+  while (splits < 8 && tiles * splits * 2 <= 148 * C::kMinBlocks &&
          p.kblocks >= splits * 4)
     splits *= 2;
   p.splits = splits;
@@ -1265,15 +1257,22 @@ int cwgk_fp8_quantize(const void *x, long long ldx, void *q, long long ldq, floa
 int cwgk_fp8_matmul(const cwgk_fp8 *op, void *stream) {
   cudaStream_t s = (cudaStream_t)stream;
   // Rows per tile.  Small tiles make more CTAs of work that is bound by latencies, as long
-  // as those all run at once, two per SM (72 rows x 2048 x 8192: 10.0 us with tiles of 32
-  // rows, 11.1 with 64, 18.9 with 128; x 11008 x 4096, 258 tiles of 32: 16.1, 21.8, 20.6; 128
-  // rows, 344 tiles: 26.3, 23.8, 22.1).  200 rows x 1024 x 4096, 32 tiles of 64: 8.6 us, 12.8
-  // with 128; x 4096 x 4096, 128 tiles: 14.7 and 14.3.
+  // as those run at once, two per SM (72 rows x 2048 x 8192: 10.0 us with tiles of 32 rows,
+  // 11.1 with 64, 18.9 with 128; x 11008 x 4096, 258 tiles of 32: 16.1, 21.8, 20.6; 128 rows,
+  // 344 tiles: 26.3, 23.8, 22.1).  With more rows the weights, which every tile of rows reads
+  // again, count too: 512 x 1024 x 4096, 128 tiles of 32: 10.1, 10.9, 11.3; 768 rows, 192 tiles:
+  // 15.4, 14.6, 14.1; 1024 x 2048 x 512, 256 tiles of 64: 11.0, 7.6, 9.2; 768 x 4096 x 512, 384
+  // tiles of 64: 16.1, 12.2, 17.7, 8.6 with pairs.  Along a long k the larger tiles win (512 x
+  // 4096 x 4096: 24.0 with 64, 21.5 with 128, 22.8 with pairs; 512 x 2048 x 8192: 24.0, 20.0,
+  // 38.8; 512 x 600 x 3600: 10.8, 11.7, 20.5), and pairs once they fill half of the GPU (192 x
+  // 11008 x 4096, 43 tiles: 37.9 with 128, 24.4).
   using namespace cwg::fp8;
   if (op->m <= 16) return launch<16>(op, s);
-  if (op->m <= 32 || (op->m <= 128 && out_tiles(op, 32) <= 2 * 148)) return launch<32>(op, s);
-  if (op->m <= 64 || (op->m <= 256 && out_tiles(op, 64) * 8 <= 2 * 148)) return launch<64>(op, s);
-  if (pair_pays(op)) return launch_pair(op, s);
+  if (op->m <= 32 || out_tiles(op, 32) <= (op->m <= 128 ? 2 * 148 : 148)) return launch<32>(op, s);
+  const bool long_k = op->k > 31 * kTileK;
+  if (op->m <= 64 || (op->m > 128 && !long_k && out_tiles(op, 64) <= 2 * 148))
+    return launch<64>(op, s);
+  if (op->m > 128 && (!long_k || pair_tiles(op) >= 37)) return launch_pair(op, s);
   return launch<128>(op, s);
 }
 

@@ -805,10 +805,12 @@ def test_two_threads_at_once(cuda_dev):
 @pytest.mark.parametrize("pad", [(3, 2), (0, 0)])
 @pytest.mark.parametrize("m,n,k", [
     (16, 1024, 4096), (9, 2048, 512), (20, 9000, 256),        # tiles of 16 and 32 rows
-    (72, 2048, 2100), (128, 300, 1024), (100, 11008, 140),    # 32 rows, cut 4, 8 and 1 ways
-    (40, 19000, 260), (250, 1000, 700), (130, 260, 3000),     # 64 rows
-    (100, 20000, 130), (384, 1024, 1000), (400, 300, 2000),   # 128 rows, cut 1, 4 and 8 ways
-    (190, 4096, 520),
+    (72, 2048, 2100), (128, 300, 1024), (90, 11008, 140),     # 32 rows, cut 4, 8 and 1 ways
+    (250, 1000, 700), (130, 260, 3000), (1000, 384, 520),
+    (40, 19000, 260), (700, 1000, 1100), (190, 4096, 520),    # 64 rows, cut 1, 2 and 2 ways
+    (1100, 2048, 200), (100, 20000, 130),                     # 64 and 128 rows
+    (400, 1600, 4100), (500, 3000, 4000),                     # 128 rows, cut 2 ways and not
+    (1300, 2048, 260),                                        # pairs
 ])
 def test_fp8_matmul_tiles(cuda_dev, dtype, pad, m, n, k):
     check_matmul(cuda_dev, m, n, k, dtype, relu=m % 3 == 0, with_bias=n % 3 != 0, pad=pad)
