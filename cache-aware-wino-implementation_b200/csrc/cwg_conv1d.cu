@@ -187,8 +187,9 @@ __global__ void __launch_bounds__(kConvThreads) conv1d_prompt(const ConvArgs a) 
     for (int i = 0; i < K - 1; ++i)
       xs[i] = active && i < len ? load_raw<T, V>(x + (size_t)(begin + i) * a.ldx + c)
                                 : zero_raw<T, V>();
+    const unsigned char resume = a.resume ? a.resume[s] : 0;
     const int slot = state ? line_of(a.slots, s, a.n_slots, bad) : -1;
-    const bool carry = slot >= 0 && a.resume && a.resume[s];
+    const bool carry = slot >= 0 && resume;
     if (!active) continue;
     T *line = state + ((size_t)(slot < 0 ? 0 : slot) * (K - 1)) * a.channels + c;
 #pragma unroll

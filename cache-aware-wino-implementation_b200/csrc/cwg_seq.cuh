@@ -216,11 +216,23 @@ __device__ __forceinline__ bool taken_before(const int *slots, int b, int slot) 
 
 // Cache line of sequence b, or -1: no line (a negative slot), or an index that
 // cannot be served (outside the lines, or an earlier sequence's), which `bad`
-// reports.  Called by whole warps with a warp-uniform b.
+// reports.  Called by whole warps with a warp-uniform b.  The first 128 lines of earlier
+// sequences are read along with b's own.
 __device__ __forceinline__ int line_of(const int *slots, int b, int n_slots, bool &bad) {
-  const int slot = slots ? slots[b] : b;
+  if (!slots) {
+    if (b < n_slots) return b;
+    bad = true;
+    return -1;
+  }
+  const int lane = (int)(threadIdx.x & 31);
+  int other[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) other[k] = lane + 32 * k < b ? slots[lane + 32 * k] : -1;
+  const int slot = slots[b];
   if (slot < 0) return -1;
-  if (slot >= n_slots || (slots && taken_before(slots, b, slot))) {
+  const bool hit = other[0] == slot || other[1] == slot || other[2] == slot || other[3] == slot;
+  if (slot >= n_slots || __any_sync(0xffffffffu, hit) ||
+      (b > 128 && taken_before(slots + 128, b - 128, slot))) {
     bad = true;
     return -1;
   }

@@ -267,9 +267,10 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads, MODE == kRoomy ? 1 : 0)
     end = min(end, begin + a.chunk);
   }
   bool bad = false;
+  const unsigned char resume = p.resume ? p.resume[b] : 0;
   const int slot = p.state ? line_of(p.slots, b, p.n_slots, bad) : -1;
   if (bad && report) atomicOr(&g_ssm_status, CWGK_STATUS_INDEX);
-  const bool carry = slot >= 0 && p.resume && p.resume[b];
+  const bool carry = slot >= 0 && resume;
   const int tiles = (end - begin + kTT - 1) / kTT;
 
   if (tid < G::kScan) {
