@@ -700,18 +700,23 @@ static int launch_prompt(const Args &a, unsigned blocks, cudaStream_t s) {
 }
 
 // Tokens per chunk when a call's sequences are cut, else 0.  `ctas`: CTAs along the
-// channels.  Cut where at most half of the SMs would have a CTA; chunks of 256 tokens or more
-// (8 tiles), as many as make three CTAs per SM.  One sequence is cut from four chunks on (1024
-// tokens, 1024 channels: 32 us, 41 uncut; 600 tokens: 31 and 26; 8192 tokens and 256, 1024,
-// 2048 channels: 47, 130, 254 us, 300 uncut).  Several are cut from two chunks on average,
-// since the longest one's length decides uncut (4096 tokens in two sequences, 1024 channels:
-// 75 us cut; uncut 76 if they are equally long, 100 if one has two thirds; in eight, 256
-// channels: 27 to 30, uncut 22 and 36).
+// channels.  Cut where at most half of the SMs would have a CTA.  Chunks of 128 to 256 tokens if
+// all their CTAs then have an SM each (1024 tokens, 256 channels: 16 us, 23 in chunks of 256;
+// 1024 channels: 24 us in four chunks, 29 in eight), else of 256 or more, as many as make three
+// CTAs per SM (8192 tokens and 256, 1024, 2048 channels: 52, 130, 254 us, 300 uncut).  One
+// sequence is cut from three chunks on (512 tokens, 1024 channels: 16 us, 22 uncut), several
+// from two chunks on average, since the longest one's length decides uncut (4096 tokens in two
+// sequences, 1024 channels: 75 us cut; uncut 76 if they are equally long, 100 if one has two
+// thirds; in eight, 256 channels: 27 to 30, uncut 22 and 36).
 static int chunk_of(int tokens, int n_seq, long long ctas) {
   if (n_seq <= 0 || ctas * n_seq > 74) return 0;
-  long long chunk = (tokens * ctas + 3 * 148 - 1) / (3 * 148);
-  chunk = chunk < 256 ? 256 : (chunk + kTT - 1) / kTT * kTT;
-  return tokens / n_seq >= (n_seq > 1 ? 2 : 4) * chunk ? (int)chunk : 0;
+  const long long parts = 148 / ctas - (n_seq - 1);  // each sequence but one: a last, short one
+  auto tiles_of = [](long long n) { return (n + kTT - 1) / kTT * kTT; };
+  long long chunk = tiles_of((tokens + parts - 1) / parts);
+  if (chunk < 128) chunk = 128;
+  if (chunk > 256) chunk = tiles_of((tokens * ctas + 3 * 148 - 1) / (3 * 148));
+  if (chunk < 256 && tokens > parts * chunk) chunk = 256;
+  return tokens / n_seq >= (n_seq > 1 ? 2 : 3) * chunk ? (int)chunk : 0;
 }
 static size_t al256(size_t n) { return (n + 255) / 256 * 256; }
 static size_t ends_bytes(long long slots, int channels, int states) {

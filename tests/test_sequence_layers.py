@@ -858,3 +858,11 @@ def test_fp8_quantize_zeros_and_small_values(cuda_dev, block_rows, cols):
     s = torch.empty(scale.shape, device=cuda_dev)
     cwg.fp8_quantize(x.to(cuda_dev), q, s, block_rows)
     assert torch.equal(s.cpu(), scale) and torch.equal(q.float().cpu(), want.float())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("lens,ch,n", [([384], 32, 16), ([400], 40, 16), ([1025], 7, 12),
+                                       ([600], 1024, 4), ([300, 0, 900], 64, 23),
+                                       ([0, 255, 257, 513], 16, 64)], ids=str)
+def test_ssm_short_chunks(cuda_dev, dtype, lens, ch, n):
+    check_ssm(ssm_case(dtype, lens, ch, 1, n, 53), cuda_dev)
