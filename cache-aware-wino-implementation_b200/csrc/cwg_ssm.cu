@@ -181,11 +181,11 @@ __device__ __forceinline__ int turned(int t, int c8, int j) {
 }
 
 // Shared memory of a CTA: the rows of five tiles (three ahead of the one in work, one
-// behind it), the pairs and sums of two.
-template <typename T, int L>
+// behind it; of three tiles, with one ahead, in kShort), the pairs and sums of two.
+template <typename T, int L, int STAGES>
 struct PromptSmem {
   using G = Prompt<L>;
-  static constexpr int kStages = 5;
+  static constexpr int kStages = STAGES;
   float4 dx[2][kTT][G::kCH / 2];
   float y[2][kTT][G::kPitch];
   LaneBC<T> bc[kStages][kTT][L];
@@ -212,7 +212,14 @@ struct PromptSmem {
 // itself (nine fp32 sequences, 288 CTAs: 30 us, 40 dense; one of 4096 tokens x 2048 channels
 // x 64 states: 233, 324), and costs occupancy when there are many CTAs (eight sequences of
 // 1024 x 4096: 272 us, 232 dense).
-enum { kDense = 0, kRoomy = 1, kSummary = 2 };
+//
+// kShort keeps three tiles instead of five, so that more CTAs fit an SM when there are many
+// sequences of about one tile, whose CTAs last as long as their latencies (18 sequences, 161
+// tokens, 4 groups of 768 channels, 4 states, fp32: 30 us, 34 dense; 19 of 108
+// tokens, 246 channels, 23 states, bf16: 6.4, 8.8).
+enum { kDense = 0, kRoomy = 1, kSummary = 2, kShort = 3 };
+template <int MODE>
+constexpr int kStagesOf = MODE == kShort ? 3 : 5;
 template <typename T, int L, bool VEC, bool VBC, int MODE>
 __global__ void __launch_bounds__(Prompt<L>::kThreads, MODE == kRoomy ? 1 : 0)
     ssm_prompt(const Args a) {
@@ -221,9 +228,10 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads, MODE == kRoomy ? 1 : 0)
   griddep_launch_dependents();
   using G = Prompt<L>;
   constexpr int CH = G::kCH;
-  constexpr int NS = PromptSmem<T, L>::kStages;
+  using Smem = PromptSmem<T, L, kStagesOf<MODE>>;
+  constexpr int NS = Smem::kStages;
   extern __shared__ __align__(16) unsigned char smem[];
-  PromptSmem<T, L> &sh = *reinterpret_cast<PromptSmem<T, L> *>(smem);
+  Smem &sh = *reinterpret_cast<Smem *>(smem);
   const cwg_ssm &p = a.p;
   const int tid = threadIdx.x;
   const int cblk = blockIdx.x % a.cblocks;
@@ -466,9 +474,11 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads, MODE == kRoomy ? 1 : 0)
     // waits is passed; the scan warps need B and C, the element threads each other's rows.
     if (tiles > 0) {
       load(0);
-      load(1);
-      load(2);
-      copy_wait<1>();
+      if constexpr (NS == 5) {
+        load(1);
+        load(2);
+      }
+      copy_wait<NS == 5 ? 1 : 0>();
     }
     named_bar<G::kElem>();
     if (tiles > 0) prepare(0);
@@ -476,9 +486,15 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads, MODE == kRoomy ? 1 : 0)
     for (int i = 0; i < tiles; ++i) {
       if (i > 0 && !SUMMARY) finish(i - 1);
       if (i + 1 < tiles) {
-        load(i + 3);  // where tile i - 2 was
-        prepare(i + 1);
-        copy_wait<1>();  // tile i + 2
+        load(i + NS - 2);  // where tile i - 2 was
+        if constexpr (NS == 5) {
+          prepare(i + 1);
+          copy_wait<1>();  // tile i + 2
+        } else {
+          copy_wait<0>();
+          named_bar<G::kElem>();
+          prepare(i + 1);
+        }
       }
       __syncthreads();
     }
@@ -682,10 +698,12 @@ static int start(K kernel, dim3 grid, unsigned threads, size_t smem, cudaStream_
 
 template <typename T, int L, bool VEC, bool VBC>
 static int launch_prompt(const Args &a, unsigned blocks, cudaStream_t s) {
-  constexpr int bytes = (int)sizeof(PromptSmem<T, L>), threads = Prompt<L>::kThreads;
+  constexpr int bytes = (int)sizeof(PromptSmem<T, L, 5>), threads = Prompt<L>::kThreads;
+  constexpr int short_bytes = (int)sizeof(PromptSmem<T, L, 3>);
   cudaError_t e = smem_attr_once<ssm_prompt<T, L, VEC, VBC, kDense>>(bytes);
   if (e == cudaSuccess) e = smem_attr_once<ssm_prompt<T, L, VEC, VBC, kRoomy>>(bytes);
   if (e == cudaSuccess) e = smem_attr_once<ssm_prompt<T, L, VEC, VBC, kSummary>>(bytes);
+  if (e == cudaSuccess) e = smem_attr_once<ssm_prompt<T, L, VEC, VBC, kShort>>(short_bytes);
   if (e != cudaSuccess) {
     cwgk_set_cuda_error((int)e);
     return -3;
@@ -694,6 +712,8 @@ static int launch_prompt(const Args &a, unsigned blocks, cudaStream_t s) {
     const int rc = start(ssm_prompt<T, L, VEC, VBC, kSummary>, dim3(blocks), threads, bytes, s, a);
     if (rc) return rc;
   }
+  if (blocks > 2 * 148 && a.p.tokens / a.p.n_seq <= kTT)
+    return start(ssm_prompt<T, L, VEC, VBC, kShort>, dim3(blocks), threads, short_bytes, s, a);
   const auto kernel = blocks <= 2 * 148 ? ssm_prompt<T, L, VEC, VBC, kRoomy>
                                         : ssm_prompt<T, L, VEC, VBC, kDense>;
   return start(kernel, dim3(blocks), threads, bytes, s, a);

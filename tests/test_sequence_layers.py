@@ -866,3 +866,12 @@ def test_fp8_quantize_zeros_and_small_values(cuda_dev, block_rows, cols):
                                        ([0, 255, 257, 513], 16, 64)], ids=str)
 def test_ssm_short_chunks(cuda_dev, dtype, lens, ch, n):
     check_ssm(ssm_case(dtype, lens, ch, 1, n, 53), cuda_dev)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("ch,groups,n,pad", [(2100, 1, 4, (0, 0)), (1504, 2, 16, (8, 8)),
+                                             (640, 1, 23, (3, 0)), (512, 4, 64, (0, 0))])
+def test_ssm_many_short_prompts(cuda_dev, dtype, ch, groups, n, pad):
+    """Sequences of a tile on average, one of them of several."""
+    check_ssm(ssm_case(dtype, [9, 0, 1, 150, 31, 33, 2, 64, 5, 7, 3, 4, 8], ch, groups, n, 54,
+                       pad=pad), cuda_dev)
