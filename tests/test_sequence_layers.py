@@ -875,3 +875,28 @@ def test_ssm_many_short_prompts(cuda_dev, dtype, ch, groups, n, pad):
     """Sequences of a tile on average, one of them of several."""
     check_ssm(ssm_case(dtype, [9, 0, 1, 150, 31, 33, 2, 64, 5, 7, 3, 4, 8], ch, groups, n, 54,
                        pad=pad), cuda_dev)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("cols", [384, 333])
+def test_fp8_quantize_bytes(cuda_dev, dtype, block_rows, cols):
+    """The codes themselves: zeros keep their sign, in groups of ordinary, tiny, huge and zero
+    scale, and so do values that round to zero."""
+    g = gen(55)
+    x = torch.randn(260, cols, generator=g)
+    x[:, ::5] = -0.0
+    x[:, 1::5] = 0.0
+    x[:, 2::15] *= 1e-8
+    x[1] *= 1e-30
+    x[2] *= 3e37
+    x[3] = -0.0
+    x[128:256] = -0.0
+    x[130, 7] = 2.0 ** -120
+    x = x.to(DT[dtype])
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=cuda_dev)
+    want, scale = R.quantize(x, block_rows)
+    s = torch.empty(scale.shape, device=cuda_dev)
+    cwg.fp8_quantize(x.to(cuda_dev), q, s, block_rows, cwg.BF16 if dtype == "bf16" else 0)
+    assert torch.equal(s.cpu(), scale)
+    assert torch.equal(q.view(torch.uint8).cpu(), want.contiguous().view(torch.uint8))
