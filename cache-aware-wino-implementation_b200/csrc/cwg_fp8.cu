@@ -1006,7 +1006,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1
       bool begun = false;  // the block's first chunk is on its way already
       for (int kb = 0; kb < p.kblocks; ++kb) {
         const int k = kb % kGroupK;
-        if (k == 0) ok = mbar_wait(s_full + 8 * (g & 1), (g >> 1) & 1, abort);
+        // a wait may have given up for some lanes only, and all have to leave together: where a
+        // chunk is on its way already, at the next block that is waited for, or behind the tile
+        if (k == 0)
+          ok = __all_sync(0xffffffffu,
+                          ok && mbar_wait(s_full + 8 * (g & 1), (g >> 1) & 1, abort));
         const float *sc =
             reinterpret_cast<const float *>(smem + C::kScaleOff + (g & 1) * C::kScaleBytes);
         const float scale =

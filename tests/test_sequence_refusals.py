@@ -155,3 +155,18 @@ def test_python_mirror_names_the_wrong_argument():
 
 def test_strerror_of_bad_index():
     assert "index" in cwg.strerror(cwg.EINDEX)
+
+
+def test_pair_kernel_votes_on_every_wait():
+    """A bounded wait may give up for some lanes of a warp and not for others.  The pair
+    product's warps run tcgen05 instructions and barriers behind their waits, which all lanes
+    have to reach together, so every answer goes through a vote before it is used."""
+    import os
+
+    with open(os.path.join(cwg.HERE, "csrc", "cwg_fp8.cu")) as f:
+        text = f.read()
+    body = text[text.index("fp8_matmul_pair(const"):text.index("static int make_map")]
+    waits = [s for s in body.split(";") if "mbar_wait(" in s]
+    assert len(waits) >= 5
+    for s in waits:
+        assert "__all_sync(" in s, s
