@@ -9,7 +9,8 @@
 #include "../../include/cwg.h"
 #include "cwg_internal.h"
 
-/* Row indices and their tile ends stay inside int. */
+/* Most rows, sequences and channels: indices, their tiles' ends and the middle of two of them
+ * stay inside int. */
 enum { kMaxRows = 1 << 30 };
 
 /* Rows of `width` elements, `ld` apart, aligned to the element. */
@@ -70,7 +71,9 @@ static int lines_ok(const void *state, const int *slots, int n_seq, int n_slots,
 
 static int conv1d_check(const cwgk_conv1d *p, int rows, unsigned flags) {
   const size_t esz = (flags & CWG_BF16) ? 2 : 4;
-  if (rows < 0 || rows > kMaxRows || p->n_seq < 0 || p->channels <= 0) return CWG_EINVAL;
+  if (rows < 0 || rows > kMaxRows || p->n_seq < 0 || p->n_seq > kMaxRows || p->channels <= 0 ||
+      p->channels > kMaxRows)
+    return CWG_EINVAL;
   if (p->width < 2) return CWG_EINVAL;
   if (p->width > 4) return CWG_EUNSUPPORTED;
   if (!p->w || ((uintptr_t)p->w & 3) || ((uintptr_t)p->bias & 3)) return CWG_EINVAL;
@@ -124,8 +127,8 @@ static int ssm_check(const cwg_ssm *p, int n_seq) {
   if (!p) return CWG_EINVAL;
   if (p->flags & ~(CWG_BF16 | CWG_SOFTPLUS | CWG_NO_PDL)) return CWG_EINVAL;
   const size_t esz = (p->flags & CWG_BF16) ? 2 : 4;
-  if (p->tokens < 0 || p->tokens > kMaxRows || n_seq < 0 || p->channels <= 0 ||
-      p->groups <= 0 || p->states <= 0)
+  if (p->tokens < 0 || p->tokens > kMaxRows || n_seq < 0 || n_seq > kMaxRows ||
+      p->channels <= 0 || p->channels > kMaxRows || p->groups <= 0 || p->states <= 0)
     return CWG_EINVAL;
   if (p->channels % p->groups) return CWG_EINVAL;
   if (p->states > 64) return CWG_EUNSUPPORTED;
@@ -158,7 +161,9 @@ static int ssm_check(const cwg_ssm *p, int n_seq) {
 }
 
 size_t cwg_ssm_workspace_bytes(int tokens, int n_seq, int channels, int states) {
-  if (tokens < 0 || n_seq < 0 || channels <= 0 || states <= 0 || states > 64) return 0;
+  if (tokens < 0 || tokens > kMaxRows || n_seq < 0 || n_seq > kMaxRows || channels <= 0 ||
+      channels > kMaxRows || states <= 0 || states > 64)
+    return 0;
   return cwgk_ssm_workspace_bytes(tokens, n_seq, channels, states);
 }
 

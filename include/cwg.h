@@ -213,7 +213,8 @@ int cwg_conv3x3_nonfused(const float *x, const float *U, const float *bias, floa
  *
  * Prompts are packed: sequence b is rows starts[b] .. starts[b+1]-1 (device,
  * int32, n_seq + 1 offsets, ascending, at most `tokens`).  An empty sequence is
- * allowed; rows that belong to no sequence are neither read nor written.
+ * allowed; rows that belong to no sequence are neither read nor written.  At most 2^30 tokens,
+ * sequences and channels.
  *
  * State between calls is kept in cache lines, one per sequence: sequence b uses
  * line slots[b] of `state` (device, int32; NULL: line b).  With resume[b] != 0 a

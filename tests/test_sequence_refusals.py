@@ -170,3 +170,40 @@ def test_pair_kernel_votes_on_every_wait():
     assert len(waits) >= 5
     for s in waits:
         assert "__all_sync(" in s, s
+
+
+BIG = (1 << 30) + 1
+
+
+def test_sizes_beyond_the_row_limit_are_refused():
+    """Channels and sequences are bounded as rows are: index sums stay inside int."""
+    assert conv(channels=BIG, ldx=BIG, ldy=BIG) == cwg.EINVAL
+    assert conv(n_seq=BIG) == cwg.EINVAL
+    assert conv(n_seq=BIG, slots=None, n_slots=BIG) == cwg.EINVAL
+    assert conv_step(channels=(1 << 31) - 1, ldx=1 << 31, ldy=1 << 31) == cwg.EINVAL
+    for step in (False, True):
+        assert ssm(step, channels=BIG, ldu=BIG, lddt=BIG, ldy=BIG) == cwg.EINVAL
+        assert ssm(step, channels=BIG, groups=BIG, states=1, ldu=BIG, lddt=BIG, ldy=BIG, ldb=BIG,
+                   ldc=BIG) == cwg.EINVAL
+    assert ssm(n_seq=BIG) == cwg.EINVAL
+
+
+@pytest.mark.parametrize("size", [
+    (10, 1, (1 << 31) - 1, 16), (10, 1, BIG, 16), (BIG, 1, 64, 16), ((1 << 31) - 1, 1, 64, 16),
+    (10, BIG, 64, 16), (10, (1 << 31) - 1, (1 << 31) - 1, 64),
+])
+def test_workspace_query_beyond_the_limits(size):
+    """In a process of its own: a query must answer 0, whatever it is asked."""
+    import subprocess
+    import sys
+
+    code = f"import sys; sys.path.insert(0, {cwg.HERE!r}); import cwg; " \
+           f"print(cwg.ssm_workspace_bytes{size})"
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stderr
+    assert int(r.stdout) == 0
+
+
+@pytest.mark.parametrize("size", [(1 << 30, 1, 64, 16), (1, 1 << 30, 64, 16), (1 << 30, 1, 1 << 30, 64)])
+def test_workspace_query_at_the_limits(size):
+    assert 0 < cwg.ssm_workspace_bytes(*size) < 1 << 40
