@@ -20,39 +20,62 @@ static int rows_ok(const void *p, long long ld, long long rows, long long width,
   return rows <= 1 ? 1 : ld >= width && ld <= (1LL << 40);
 }
 
+/* Addresses and row distances of checked operands reach 2^72, beyond 64 bits. */
+typedef __int128 wide;
+
 /* Whether two row operands share bytes.  Two column ranges of one matrix have the
  * same row distance and lie apart within it. */
 static int overlaps(const void *a, long long lda, long long wa, const void *b, long long ldb,
                     long long wb, long long rows, size_t esz) {
   if (!a || !b || rows <= 0) return 0;
   if (rows == 1) lda = wa, ldb = wb;
-  const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;
-  const uintptr_t a1 = a0 + (uintptr_t)(((rows - 1) * lda + wa) * (long long)esz);
-  const uintptr_t b1 = b0 + (uintptr_t)(((rows - 1) * ldb + wb) * (long long)esz);
-  if (a1 <= b0 || b1 <= a0) return 0;
+  const wide e = (wide)esz, a0 = (uintptr_t)a, b0 = (uintptr_t)b;
+  if (a0 + ((wide)(rows - 1) * lda + wa) * e <= b0 || b0 + ((wide)(rows - 1) * ldb + wb) * e <= a0)
+    return 0;
   if (lda != ldb || rows == 1) return 1;
-  const long long step = lda * (long long)esz;
-  long long off = (long long)(b0 - a0) % step; /* b's columns behind a's, in one row */
+  const wide step = lda * e;
+  wide off = (b0 - a0) % step; /* b's columns behind a's, in one row */
   if (off < 0) off += step;
-  return !(off >= wa * (long long)esz && off + wb * (long long)esz <= step);
+  return !(off >= wa * e && off + wb * e <= step);
 }
 
 /* Whether the byte ranges of two row operands meet. */
 static int ranges_meet(const void *a, long long arow, const void *b, long long brow,
                        long long arows, long long brows, long long abytes, long long bbytes) {
-  const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;
-  const uintptr_t a1 = a0 + (uintptr_t)((arows > 1 ? (arows - 1) * arow : 0) + abytes);
-  const uintptr_t b1 = b0 + (uintptr_t)((brows > 1 ? (brows - 1) * brow : 0) + bbytes);
-  return a0 < b1 && b0 < a1;
+  const wide a0 = (uintptr_t)a, b0 = (uintptr_t)b;
+  return a0 < b0 + (brows > 1 ? (wide)(brows - 1) * brow : 0) + bbytes &&
+         b0 < a0 + (arows > 1 ? (wide)(arows - 1) * arow : 0) + abytes;
 }
 
-/* Whether `rows` rows of `width` elements share bytes with the cache lines. */
-static int meets_lines(const void *p, long long ld, long long rows, long long width, size_t esz,
-                       const void *state, int n_slots, long long line, size_t line_esz) {
-  if (!p || !state || rows <= 0 || n_slots <= 0) return 0;
-  const __int128 a = (__int128)(uintptr_t)p, s = (__int128)(uintptr_t)state;
-  return a < s + (__int128)n_slots * line * (__int128)line_esz &&
-         s < a + ((__int128)(rows - 1) * ld * (rows > 1) + width) * (__int128)esz;
+/* A dense operand: neighbouring bytes. */
+typedef struct block {
+  const void *p;
+  wide bytes;
+} block;
+
+static int blocks_meet(block a, block b) {
+  const wide a0 = (uintptr_t)a.p, b0 = (uintptr_t)b.p;
+  return a.p && b.p && a.bytes > 0 && b.bytes > 0 && a0 < b0 + b.bytes && b0 < a0 + a.bytes;
+}
+
+/* Whether a dense operand shares bytes with `rows` rows of `width` elements. */
+static int meets_rows(block a, const void *p, long long ld, long long rows, long long width,
+                      size_t esz) {
+  if (!a.p || !p || a.bytes <= 0 || rows <= 0 || width <= 0) return 0;
+  const wide step = (wide)ld * (wide)esz, row = (wide)width * (wide)esz;
+  const wide off = (wide)(uintptr_t)a.p - (wide)(uintptr_t)p; /* of the block's first byte */
+  if (off + a.bytes <= 0 || off >= (rows > 1 ? (rows - 1) * step : 0) + row) return 0;
+  if (off < row) return 1;
+  const wide first = (off - row) / step + 1; /* first row that ends behind the block's start */
+  return first < rows && first * step < off + a.bytes;
+}
+
+/* Whether one of n dense inputs shares bytes with the rows of y or with the cache lines. */
+static int outputs_meet(const block *in, int n, const void *y, long long ldy, long long rows,
+                        long long width, size_t esz, block lines) {
+  for (int i = 0; i < n; ++i)
+    if (meets_rows(in[i], y, ldy, rows, width, esz) || blocks_meet(in[i], lines)) return 1;
+  return 0;
 }
 
 static int act_of(unsigned flags, unsigned allowed) {
@@ -78,16 +101,22 @@ static int conv1d_check(const cwgk_conv1d *p, int rows, unsigned flags) {
   if (p->width > 4) return CWG_EUNSUPPORTED;
   if (!p->w || ((uintptr_t)p->w & 3) || ((uintptr_t)p->bias & 3)) return CWG_EINVAL;
   if (!lines_ok(p->state, p->slots, p->n_seq, p->n_slots, esz)) return CWG_EINVAL;
+  const block lines = {p->state, (wide)p->n_slots * (p->width - 1) * p->channels * (wide)esz};
   if (rows > 0) {
     if (!rows_ok(p->x, p->ldx, rows, p->channels, esz) ||
         !rows_ok(p->y, p->ldy, rows, p->channels, esz))
       return CWG_EINVAL;
-    const long long line = (long long)(p->width - 1) * p->channels;
     if (overlaps(p->x, p->ldx, p->channels, p->y, p->ldy, p->channels, rows, esz) ||
-        meets_lines(p->x, p->ldx, rows, p->channels, esz, p->state, p->n_slots, line, esz) ||
-        meets_lines(p->y, p->ldy, rows, p->channels, esz, p->state, p->n_slots, line, esz))
+        meets_rows(lines, p->x, p->ldx, rows, p->channels, esz) ||
+        meets_rows(lines, p->y, p->ldy, rows, p->channels, esz))
       return CWG_EINVAL;
   }
+  const block in[] = {{p->w, (wide)p->channels * p->width * 4},
+                      {p->bias, (wide)p->channels * 4},
+                      {p->starts, ((wide)p->n_seq + 1) * 4},
+                      {p->slots, (wide)p->n_seq * 4},
+                      {p->resume, p->n_seq}};
+  if (outputs_meet(in, 5, p->y, p->ldy, rows, p->channels, esz, lines)) return CWG_EINVAL;
   return CWG_OK;
 }
 
@@ -123,7 +152,30 @@ int cwg_conv1d_causal_step(const void *x, long long ldx, const float *w, const f
   return cwgk_conv1d_step(&op, stream);
 }
 
-static int ssm_check(const cwg_ssm *p, int n_seq) {
+/* The call's dense inputs; a step looks at neither offsets nor `resume`. */
+enum { kSsmDense = 6 };
+static void ssm_dense(const cwg_ssm *p, int n_seq, int step, block *in) {
+  const wide c = p->channels;
+  in[0] = (block){p->A, c * p->states * 4};
+  in[1] = (block){p->D, c * 4};
+  in[2] = (block){p->dt_bias, c * 4};
+  in[3] = (block){p->slots, (wide)n_seq * 4};
+  in[4] = (block){step ? 0 : p->starts, ((wide)n_seq + 1) * 4};
+  in[5] = (block){step ? 0 : p->resume, n_seq};
+}
+static block ssm_lines(const cwg_ssm *p) {
+  return (block){p->state, (wide)p->n_slots * p->channels * p->states * 4};
+}
+/* Whether a dense operand shares bytes with the call's rows, inputs' or outputs'. */
+static int meets_ssm_rows(block b, const cwg_ssm *p) {
+  const size_t esz = (p->flags & CWG_BF16) ? 2 : 4;
+  const long long rows = p->tokens, c = p->channels, gn = (long long)p->groups * p->states;
+  return meets_rows(b, p->u, p->ldu, rows, c, esz) || meets_rows(b, p->dt, p->lddt, rows, c, esz) ||
+         meets_rows(b, p->z, p->ldz, rows, c, esz) || meets_rows(b, p->B, p->ldb, rows, gn, esz) ||
+         meets_rows(b, p->C, p->ldc, rows, gn, esz) || meets_rows(b, p->y, p->ldy, rows, c, esz);
+}
+
+static int ssm_check(const cwg_ssm *p, int n_seq, int step) {
   if (!p) return CWG_EINVAL;
   if (p->flags & ~(CWG_BF16 | CWG_SOFTPLUS | CWG_NO_PDL)) return CWG_EINVAL;
   const size_t esz = (p->flags & CWG_BF16) ? 2 : 4;
@@ -148,15 +200,12 @@ static int ssm_check(const cwg_ssm *p, int n_seq) {
         overlaps(p->B, p->ldb, gn, p->y, p->ldy, c, rows, esz) ||
         overlaps(p->C, p->ldc, gn, p->y, p->ldy, c, rows, esz))
       return CWG_EINVAL;
-    const long long line = c * p->states;
-    if (meets_lines(p->u, p->ldu, rows, c, esz, p->state, p->n_slots, line, 4) ||
-        meets_lines(p->dt, p->lddt, rows, c, esz, p->state, p->n_slots, line, 4) ||
-        meets_lines(p->z, p->ldz, rows, c, esz, p->state, p->n_slots, line, 4) ||
-        meets_lines(p->B, p->ldb, rows, gn, esz, p->state, p->n_slots, line, 4) ||
-        meets_lines(p->C, p->ldc, rows, gn, esz, p->state, p->n_slots, line, 4) ||
-        meets_lines(p->y, p->ldy, rows, c, esz, p->state, p->n_slots, line, 4))
-      return CWG_EINVAL;
+    if (meets_ssm_rows(ssm_lines(p), p)) return CWG_EINVAL;
   }
+  block in[kSsmDense];
+  ssm_dense(p, n_seq, step, in);
+  if (outputs_meet(in, kSsmDense, p->y, p->ldy, p->tokens, p->channels, esz, ssm_lines(p)))
+    return CWG_EINVAL;
   return CWG_OK;
 }
 
@@ -168,22 +217,28 @@ size_t cwg_ssm_workspace_bytes(int tokens, int n_seq, int channels, int states) 
 }
 
 int cwg_ssm_scan(const cwg_ssm *op, void *workspace, size_t workspace_bytes, void *stream) {
-  const int rc = ssm_check(op, op ? op->n_seq : 0);
+  const int rc = ssm_check(op, op ? op->n_seq : 0, 0);
   if (rc) return rc;
   if (op->n_seq == 0) return CWG_OK;
   if (!op->starts || ((uintptr_t)op->starts & 3)) return CWG_EINVAL;
   if (workspace) {
     if ((uintptr_t)workspace & 255) return CWG_EINVAL;
-    if (workspace_bytes <
-        cwgk_ssm_workspace_bytes(op->tokens, op->n_seq, op->channels, op->states))
-      return CWG_EINVAL;
+    const size_t need =
+        cwgk_ssm_workspace_bytes(op->tokens, op->n_seq, op->channels, op->states);
+    if (workspace_bytes < need) return CWG_EINVAL;
+    const block ws = {workspace, (wide)need};
+    block in[kSsmDense];
+    ssm_dense(op, op->n_seq, 0, in);
+    int meet = meets_ssm_rows(ws, op) || blocks_meet(ws, ssm_lines(op));
+    for (int i = 0; i < kSsmDense; ++i) meet |= blocks_meet(ws, in[i]);
+    if (meet) return CWG_EINVAL;
   }
   if (op->tokens == 0 && !op->state) return CWG_OK;
   return cwgk_ssm_scan(op, workspace, workspace_bytes, stream);
 }
 
 int cwg_ssm_step(const cwg_ssm *op, void *stream) {
-  const int rc = ssm_check(op, op ? op->tokens : 0);
+  const int rc = ssm_check(op, op ? op->tokens : 0, 1);
   if (rc) return rc;
   if (op->tokens == 0) return CWG_OK;
   if (!op->state) return CWG_EINVAL;
@@ -232,7 +287,8 @@ int cwg_fp8_matmul(const void *a, long long lda, const float *a_scale, long long
   if (ranges_meet(a, lda, y, ldy * e, m, m, k, n * e) ||
       ranges_meet(w, ldw, y, ldy * e, n, m, k, n * e) ||
       ranges_meet(a_scale, lda_scale * 4, y, ldy * e, m, m, kb * 4, n * e) ||
-      ranges_meet(w_scale, ldw_scale * 4, y, ldy * e, nb, m, kb * 4, n * e))
+      ranges_meet(w_scale, ldw_scale * 4, y, ldy * e, nb, m, kb * 4, n * e) ||
+      (bias && ranges_meet(bias, 0, y, ldy * e, 1, m, n * 4LL, n * e)))
     return CWG_EINVAL;
   const cwgk_fp8 op = {a,       w,         lda,       ldw, a_scale, w_scale, bias,
                        lda_scale, ldw_scale, y,         ldy, m,       n,       k,

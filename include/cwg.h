@@ -232,7 +232,8 @@ int cwg_conv3x3_nonfused(const float *x, const float *U, const float *bias, floa
  * the rows and lines of its other sequences is unspecified.
  *
  * y must not overlap the inputs (disjoint columns of one matrix do not overlap), nor
- * state any of them: CWG_EINVAL.  All calls are asynchronous on `stream`, allocate nothing and can be
+ * state any of them, weights, biases and index arrays included: CWG_EINVAL.  All calls are
+ * asynchronous on `stream`, allocate nothing and can be
  * captured into a graph (make a call of the kind before the first capture: kernels are
  * loaded and configured at their first launch); they are programmatic dependent launches
  * (see CWG_NO_PDL, which they take too). */
@@ -276,8 +277,8 @@ typedef struct cwg_ssm {
 
 /* Prompts.  Few, long sequences are cut into chunks of time that run side by side,
  * in a caller-owned workspace (256-byte aligned, cwg_ssm_workspace_bytes bytes);
- * workspace NULL: never cut.  Calls whose work overlaps on the GPU need workspaces
- * of their own. */
+ * workspace NULL: never cut.  It must not overlap any operand (CWG_EINVAL).  Calls whose
+ * work overlaps on the GPU need workspaces of their own. */
 size_t cwg_ssm_workspace_bytes(int tokens, int n_seq, int channels, int states);
 int cwg_ssm_scan(const cwg_ssm *op, void *workspace, size_t workspace_bytes, void *stream);
 

@@ -207,3 +207,112 @@ def test_workspace_query_beyond_the_limits(size):
 @pytest.mark.parametrize("size", [(1 << 30, 1, 64, 16), (1, 1 << 30, 64, 16), (1 << 30, 1, 1 << 30, 64)])
 def test_workspace_query_at_the_limits(size):
     assert 0 < cwg.ssm_workspace_bytes(*size) < 1 << 40
+
+
+# ---- operands that share bytes --------------------------------------------------------------
+# conv(): x and y are 10 rows of 256 bytes, w 1024 bytes, state 4 lines of 768, 3 offsets
+Y_END, S_END = Y + 10 * 256, S + 4 * 768
+
+
+@pytest.mark.parametrize("kw", [
+    dict(w=Y), dict(w=Y - 1020), dict(w=Y_END - 4), dict(bias=Y + 256), dict(bias=Y - 252),
+    dict(starts=Y_END - 4), dict(starts=Y - 8), dict(slots=Y - 4), dict(slots=Y + 8),
+    dict(resume=Y - 1), dict(resume=Y_END - 1),
+    dict(w=S), dict(w=S - 1020), dict(bias=S_END - 4), dict(starts=S - 8), dict(slots=S_END - 4),
+    dict(resume=S + 1), dict(resume=S - 1),
+], ids=str)
+def test_conv1d_refuses_outputs_over_dense_operands(kw):
+    assert conv(**kw) == cwg.EINVAL
+
+
+@pytest.mark.parametrize("kw", [dict(w=Y), dict(bias=Y + 4), dict(slots=Y + 3 * 256 - 4),
+                                dict(w=S), dict(bias=S + 4), dict(slots=S_END - 4)], ids=str)
+def test_conv1d_step_refuses_outputs_over_dense_operands(kw):
+    assert conv_step(**kw) == cwg.EINVAL
+
+
+def refused_by_arguments(status):
+    """Whether a call ended in the checks; without a GPU the others end in a CUDA error."""
+    return status in (cwg.EINVAL, cwg.EUNSUPPORTED)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="would read the fake addresses")
+@pytest.mark.parametrize("call", [
+    lambda: conv(), lambda: conv_step(), lambda: ssm(), lambda: ssm(True), lambda: quantize(),
+    lambda: matmul(),
+    # dense operands right before and behind y and the cache lines
+    lambda: conv(w=Y - 1024, bias=Y_END, starts=S - 12, slots=S_END, resume=Y - 1026),
+    # and between the columns that a wider matrix gives to y
+    lambda: conv(ldy=128, bias=Y + 256, slots=Y + 504, starts=Y + 768, resume=Y + 1022),
+    lambda: ssm(ldy=128, D=Y + 256, dt_bias=Y + 9 * 512 + 256, slots=Y + 504),
+    # one row: the distance to the next says nothing
+    lambda: conv(tokens=1, ldy=1 << 40, bias=Y + 256),
+    # disjoint columns of one matrix, far apart rows
+    lambda: conv(ldx=1 << 40, ldy=1 << 40, y=X + 256, state=None),
+])
+def test_operands_that_share_no_byte_pass_the_checks(call):
+    assert not refused_by_arguments(call())
+
+
+A_BYTES, H_END = 64 * 16 * 4, S + 4 * 64 * 16 * 4
+
+
+@pytest.mark.parametrize("step", [False, True])
+@pytest.mark.parametrize("kw", [
+    dict(A=Y), dict(A=Y - A_BYTES + 4), dict(D=Y_END - 4), dict(dt_bias=Y - 252),
+    dict(slots=Y - 4), dict(A=S), dict(A=H_END - 4), dict(D=S - 252), dict(dt_bias=S + 64),
+    dict(slots=H_END - 4),
+], ids=str)
+def test_ssm_refuses_outputs_over_dense_operands(step, kw):
+    assert ssm(step, **kw) == cwg.EINVAL
+
+
+@pytest.mark.parametrize("kw", [dict(starts=Y - 8), dict(starts=Y_END - 4), dict(resume=Y - 1),
+                                dict(starts=H_END - 4), dict(resume=S - 1)], ids=str)
+def test_ssm_scan_refuses_outputs_over_offsets(kw):
+    assert ssm(**kw) == cwg.EINVAL
+
+
+# one sequence that is cut: 4096 rows of 64 channels, 16 states
+LONG = dict(u=X, dt=X + 0x1000000, B=X + 0x2000000, C=X + 0x3000000, y=X + 0x4000000, z=X + 0x5000000,
+            ldz=64, A=X + 0x6000000, D=X + 0x6010000, dt_bias=X + 0x6020000, starts=X + 0x6030000,
+            slots=X + 0x6040000, resume=X + 0x6050000, state=X + 0x7000000, tokens=4096, n_seq=1)
+WS = 0x20000000
+
+
+@pytest.mark.parametrize("name,size", [
+    ("u", 4096 * 256), ("dt", 4096 * 256), ("B", 4096 * 64), ("C", 4096 * 64), ("y", 4096 * 256),
+    ("z", 4096 * 256), ("A", A_BYTES), ("D", 256), ("dt_bias", 256), ("starts", 8), ("slots", 4),
+    ("resume", 1), ("state", 4 * A_BYTES)])
+def test_ssm_refuses_a_workspace_over_an_operand(name, size):
+    need = cwg.ssm_workspace_bytes(4096, 1, 64, 16)
+    assert need > 256
+    at = WS + 0x10000  # the operand begins inside the workspace, and ends inside it
+    assert ssm(workspace=at - need + 256, size=need, **dict(LONG, **{name: at})) == cwg.EINVAL
+    at = WS - size + (1 if name == "resume" else 4)
+    assert ssm(workspace=WS, size=need, **dict(LONG, **{name: at})) == cwg.EINVAL
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="would read the fake addresses")
+def test_ssm_workspace_beside_the_operands_passes_the_checks():
+    need = cwg.ssm_workspace_bytes(4096, 1, 64, 16)
+    assert not refused_by_arguments(ssm(workspace=WS, size=need, **dict(LONG, D=WS - 256)))
+    assert not refused_by_arguments(ssm(workspace=WS, size=need, **dict(LONG, D=WS + need)))
+
+
+@pytest.mark.parametrize("kw", [dict(bias=Y), dict(bias=Y - 1196), dict(bias=Y + 4 * 1200 + 1196),
+                                dict(bias=Y + 1204, ldy=400)], ids=str)
+def test_fp8_matmul_refuses_a_bias_inside_y(kw):
+    assert matmul(**kw) == cwg.EINVAL
+
+
+def test_overlaps_of_far_apart_rows():
+    """Row distances whose products with the rows pass 64 bits: (2^22 + 1) rows of fp32 at 2^40."""
+    far, rows = 1 << 40, (1 << 22) + 1
+    assert conv(tokens=rows, ldx=far, ldy=far, y=X + 4 * far, state=None) == cwg.EINVAL
+    assert conv(tokens=rows, ldx=far, ldy=far, y=X + 4 * far + 252, state=None) == cwg.EINVAL
+    assert conv(tokens=rows, ldx=far, ldy=far, x=X + 4 * far, y=X, state=None) == cwg.EINVAL
+    assert conv(tokens=rows, ldy=far, bias=Y + 4 * far, state=None) == cwg.EINVAL
+    assert quantize(rows=rows, ldx=far, q=X + 8 * far) == cwg.EINVAL
+    assert matmul(m=4 * (rows - 1) + 1, lda=far, y=X + far) == cwg.EINVAL
+    assert matmul(m=rows, ldy=far, bias=Y + (1 << 50)) == cwg.EINVAL
