@@ -223,8 +223,7 @@ int cwg_ssm_scan(const cwg_ssm *op, void *workspace, size_t workspace_bytes, voi
   if (!op->starts || ((uintptr_t)op->starts & 3)) return CWG_EINVAL;
   if (workspace) {
     if ((uintptr_t)workspace & 255) return CWG_EINVAL;
-    const size_t need =
-        cwgk_ssm_workspace_bytes(op->tokens, op->n_seq, op->channels, op->states);
+    const size_t need = cwgk_ssm_call_bytes(op);
     if (workspace_bytes < need) return CWG_EINVAL;
     const block ws = {workspace, (wide)need};
     block in[kSsmDense];
@@ -234,7 +233,7 @@ int cwg_ssm_scan(const cwg_ssm *op, void *workspace, size_t workspace_bytes, voi
     if (meet) return CWG_EINVAL;
   }
   if (op->tokens == 0 && !op->state) return CWG_OK;
-  return cwgk_ssm_scan(op, workspace, workspace_bytes, stream);
+  return cwgk_ssm_scan(op, workspace, stream);
 }
 
 int cwg_ssm_step(const cwg_ssm *op, void *stream) {

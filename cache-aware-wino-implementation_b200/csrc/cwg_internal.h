@@ -156,8 +156,8 @@ int cwgk_conv1d_step(const cwgk_conv1d *op, void *stream); /* n_seq rows */
 /* Selective scan (csrc/cwg_ssm.cu); op as the public call takes it, checked. */
 struct cwg_ssm;
 size_t cwgk_ssm_workspace_bytes(int tokens, int n_seq, int channels, int states);
-int cwgk_ssm_scan(const struct cwg_ssm *op, void *workspace, size_t workspace_bytes,
-                  void *stream);
+size_t cwgk_ssm_call_bytes(const struct cwg_ssm *op); /* what this call uses, 256 if nothing */
+int cwgk_ssm_scan(const struct cwg_ssm *op, void *workspace, void *stream);
 int cwgk_ssm_step(const struct cwg_ssm *op, void *stream);
 
 /* 8-bit product (csrc/cwg_fp8.cu), arguments checked by the host entry. */

@@ -743,6 +743,10 @@ static size_t ends_bytes(long long slots, int channels, int states) {
   return al256((size_t)slots * channels * states * 4);
 }
 
+static size_t workspace_bytes(long long slots, int channels, int states) {
+  return ends_bytes(slots, channels, states) + al256((size_t)slots * channels * 4);
+}
+
 // lane: values of B and C that are read at a time.
 static Args make_args(const cwg_ssm *op, int np, int lane, size_t esz) {
   Args a;
@@ -835,17 +839,27 @@ static int channels_per_cta(int states) {
 
 extern "C" {
 
-// Of one group: more groups only make more CTAs and so fewer chunks.
+// An upper bound over all calls of at most so many tokens and sequences, and any groups.  A
+// cut call has n_seq <= 74 / ctas, chunks of at least 128 tokens, and of at least tokens x ctas /
+// 444 (see chunk_of: else all of its CTAs have an SM, ctas chunks <= 148); more groups make more
+// CTAs along the channels than one.
 size_t cwgk_ssm_workspace_bytes(int tokens, int n_seq, int channels, int states) {
   using namespace cwg::ssm;
   const int ch = channels_per_cta(states);
-  const int chunk = chunk_of(tokens, n_seq, (channels + ch - 1) / ch);
-  if (!chunk) return 256;
-  const long long slots = tokens / chunk + n_seq;
-  return ends_bytes(slots, channels, states) + al256((size_t)slots * channels * 4);
+  const long long ctas = (channels + ch - 1) / ch;
+  if (ctas > 74 || n_seq < 1 || tokens < 3 * 128) return 256;
+  const long long chunks = tokens / 128 < 444 / ctas ? tokens / 128 : 444 / ctas;
+  return workspace_bytes(chunks + (n_seq < 74 / ctas ? n_seq : 74 / ctas), channels, states);
 }
 
-int cwgk_ssm_scan(const cwg_ssm *op, void *workspace, size_t workspace_bytes, void *stream) {
+size_t cwgk_ssm_call_bytes(const cwg_ssm *op) {
+  using namespace cwg::ssm;
+  const int ch = channels_per_cta(op->states), per = op->channels / op->groups;
+  const int chunk = chunk_of(op->tokens, op->n_seq, (long long)((per + ch - 1) / ch) * op->groups);
+  return chunk ? workspace_bytes(op->tokens / chunk + op->n_seq, op->channels, op->states) : 256;
+}
+
+int cwgk_ssm_scan(const cwg_ssm *op, void *workspace, void *stream) {
   return cwg::ssm::any(op, false, workspace, (cudaStream_t)stream);
 }
 

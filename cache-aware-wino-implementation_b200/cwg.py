@@ -328,6 +328,7 @@ def conv1d_causal_step(x, w, bias, y, state, slots=None, flags: int = 0, stream=
 
 
 def ssm_workspace_bytes(tokens: int, n_seq: int, channels: int, states: int) -> int:
+    """Bytes that serve every scan of at most `tokens` tokens in at most `n_seq` sequences."""
     return int(lib().cwg_ssm_workspace_bytes(tokens, n_seq, channels, states))
 
 

@@ -276,9 +276,11 @@ typedef struct cwg_ssm {
 } cwg_ssm;
 
 /* Prompts.  Few, long sequences are cut into chunks of time that run side by side,
- * in a caller-owned workspace (256-byte aligned, cwg_ssm_workspace_bytes bytes);
- * workspace NULL: never cut.  It must not overlap any operand (CWG_EINVAL).  Calls whose
- * work overlaps on the GPU need workspaces of their own. */
+ * in a caller-owned workspace (256-byte aligned).  cwg_ssm_workspace_bytes(tokens, n_seq,
+ * ...) bytes serve every call of at most so many tokens and sequences, of those channels
+ * and states and any groups; a call that is given less than it uses is refused, and so is
+ * one whose workspace overlaps an operand (CWG_EINVAL).  workspace NULL: never cut.  Calls
+ * whose work overlaps on the GPU need workspaces of their own. */
 size_t cwg_ssm_workspace_bytes(int tokens, int n_seq, int channels, int states);
 int cwg_ssm_scan(const cwg_ssm *op, void *workspace, size_t workspace_bytes, void *stream);
 

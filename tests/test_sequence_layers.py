@@ -900,3 +900,27 @@ def test_fp8_quantize_bytes(cuda_dev, dtype, block_rows, cols):
     cwg.fp8_quantize(x.to(cuda_dev), q, s, block_rows, cwg.BF16 if dtype == "bf16" else 0)
     assert torch.equal(s.cpu(), scale)
     assert torch.equal(q.view(torch.uint8).cpu(), want.contiguous().view(torch.uint8))
+
+
+@pytest.mark.parametrize("groups", [1, 4])
+def test_ssm_one_workspace_for_calls_of_many_sizes(cuda_dev, groups):
+    """A workspace for the largest call serves every smaller one, cut or not, and is not left."""
+    ch, n = 256, 16
+    size = cwg.ssm_workspace_bytes(2100, 4, ch, n)
+    whole = torch.full((size + 4096,), 0x5a, dtype=torch.uint8, device=cuda_dev)
+    for lens in ([2100], [1500, 600], [600], [512], [384], [0, 1000, 900, 200], [70, 3]):
+        c = ssm_case("bf16", lens, ch, groups, n, 56, tail=0)
+        y, state = torch.empty_like(c["u"], device=cuda_dev), c["state"].to(cuda_dev)
+        dv = {k: put(c[k], cuda_dev) for k in ("u", "step", "A", "B", "C", "D", "bias", "z")}
+        cwg.ssm_scan(*dv.values(), y, state,
+                     torch.tensor(c["starts"], dtype=torch.int32, device=cuda_dev),
+                     c["slots"].to(cuda_dev), c["resume"].to(cuda_dev), whole[:size],
+                     cwg.BF16 | cwg.SOFTPLUS)
+        cwg.device_status()
+        for b, slot in enumerate(c["slots"].tolist()):
+            rows = slice(c["starts"][b], c["starts"][b + 1])
+            h = c["state"][slot] if c["resume"][b] else torch.zeros_like(c["state"][slot])
+            want, new = ssm_want(c, rows, h)
+            R.close(y[rows], want, f"{lens}: sequence {b}")
+            R.close(state[slot], new, f"{lens}: state of sequence {b}")
+        assert (whole[size:] == 0x5a).all()

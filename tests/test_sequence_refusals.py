@@ -316,3 +316,39 @@ def test_overlaps_of_far_apart_rows():
     assert quantize(rows=rows, ldx=far, q=X + 8 * far) == cwg.EINVAL
     assert matmul(m=4 * (rows - 1) + 1, lda=far, y=X + far) == cwg.EINVAL
     assert matmul(m=rows, ldy=far, bias=Y + (1 << 50)) == cwg.EINVAL
+
+
+# ---- one workspace for calls of many sizes ----------------------------------------------------
+def test_workspace_of_the_largest_call_serves_smaller_ones():
+    """The query never falls where tokens or sequences grow: one workspace serves every call of
+    at most as many."""
+    tokens = (0, 1, 100, 255, 256, 383, 384, 511, 512, 513, 600, 767, 768, 1000, 1024, 1500, 2048,
+              4095, 4096, 6127, 8192, 20000, 1 << 17, 1 << 30)
+    seqs = (0, 1, 2, 3, 4, 7, 8, 16, 37, 74, 75, 1000, 1 << 30)
+    for ch, n in ((1, 1), (64, 16), (219, 4), (1024, 16), (1184, 16), (2048, 64), (2368, 16),
+                  (4096, 16), (40, 33), (600, 64)):
+        size = [[cwg.ssm_workspace_bytes(t, s, ch, n) for s in seqs] for t in tokens]
+        for i in range(len(tokens)):
+            for j in range(len(seqs)):
+                assert size[i][j] >= 256
+                assert i == 0 or size[i][j] >= size[i - 1][j], (tokens[i], seqs[j], ch, n)
+                assert j == 0 or size[i][j] >= size[i][j - 1], (tokens[i], seqs[j], ch, n)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="would read the fake addresses")
+@pytest.mark.parametrize("largest,calls", [
+    ((8192, 16), [(8192, 1), (8192, 2), (4096, 1), (600, 1), (512, 1), (384, 1), (10, 5)]),
+    ((600, 1), [(513, 1), (512, 1), (511, 1), (385, 1), (1, 1)]),
+    ((1024, 3), [(1024, 1), (1024, 2), (768, 2), (512, 2)]),
+])
+def test_calls_accept_the_largest_ones_workspace(largest, calls):
+    size = cwg.ssm_workspace_bytes(*largest, 1024, 16)
+    for tokens, n in calls:
+        for groups in (1, 2, 64):
+            op = dict(LONG, tokens=tokens, n_seq=n, channels=1024, groups=groups, ldu=1024,
+                      lddt=1024, ldz=1024, ldy=1024, ldb=16 * groups, ldc=16 * groups,
+                      **{k: X + (i << 28) for i, k in enumerate(("u", "dt", "B", "C", "y", "z"))},
+                      state=X + (6 << 28), n_slots=16)
+            op.update({k: X + (7 << 28) + (i << 20) for i, k in enumerate(
+                ("A", "D", "dt_bias", "starts", "slots", "resume"))})
+            assert not refused_by_arguments(ssm(workspace=8 << 28, size=size, **op)), (tokens, n)
