@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import sys
 from dataclasses import dataclass
 
 import numpy as np
@@ -254,8 +255,19 @@ def conv3x3_fused_host(x_host: int, U, bias, y_host: int, workspace, workspace_b
 def device_status(stream=None) -> None:
     """Raises CwgError(ETIMEOUT) if a bounded device wait gave up since the last check,
     CwgError(ERANGE) if an fp16 tensor-core operand overflowed, or CwgError(EINDEX) if a
-    sequence layer met a bad offset or cache line."""
-    _check(lib().cwg_device_status(_stream(stream)), "device status")
+    sequence layer met a bad offset or cache line.  Waits for `stream`, whose calls it then
+    reports; without one for both streams that calls without one run on: the default stream and
+    torch's current stream.  Calls on other streams may still be running."""
+    streams = [_stream(stream)]
+    torch = sys.modules.get("torch")
+    if stream is None and torch is not None and torch.cuda.is_initialized():
+        current = torch.cuda.current_stream().cuda_stream
+        if current:
+            streams.append(current)
+    # the codes of failures grow with their weight: ECUDA, ETIMEOUT, ERANGE, EINDEX
+    bad = [st for st in [lib().cwg_device_status(s) for s in streams] if st != OK]
+    if bad:
+        _check(max(bad), "device status")
 
 
 def selftest_wait_timeout(stream=None) -> None:

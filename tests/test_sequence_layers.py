@@ -924,3 +924,28 @@ def test_ssm_one_workspace_for_calls_of_many_sizes(cuda_dev, groups):
             R.close(y[rows], want, f"{lens}: sequence {b}")
             R.close(state[slot], new, f"{lens}: state of sequence {b}")
         assert (whole[size:] == 0x5a).all()
+
+
+# ---- status and codes ----------------------------------------------------------------------
+@pytest.mark.parametrize("default_stream", [False, True])
+def test_device_status_waits_for_the_calls_that_it_reports(cuda_dev, default_stream):
+    """Without a stream the status is that of torch's current stream, where the tensor calls
+    run, and of the default one: a bad line behind other work on either is not missed."""
+    dev = cuda_dev
+    x, y, state = (torch.zeros(*shape, device=dev) for shape in ((2, 64), (2, 64), (2, 3, 64)))
+    w, slots = torch.zeros(64, 4, device=dev), torch.tensor([0, 9], dtype=torch.int32, device=dev)
+    cwg.conv1d_causal_step(x, w, None, y, state)  # a kernel's first launch may wait for the GPU
+    cwg.device_status()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(torch.cuda.default_stream() if default_stream else side):
+        torch.cuda._sleep(200_000_000)  # about 0.1 s
+        cwg.conv1d_causal_step(x, w, None, y, state, slots)
+    try:
+        with torch.cuda.stream(side), pytest.raises(cwg.CwgError) as e:
+            cwg.device_status()
+        assert e.value.status == cwg.EINDEX
+        cwg.device_status()  # cleared
+    finally:
+        torch.cuda.synchronize()
+        cwg.lib().cwg_device_status(None)
