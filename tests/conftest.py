@@ -17,15 +17,22 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (B200, sm_100a)")
 
 
-@pytest.hookimpl(wrapper=True)
-def pytest_runtest_call(item):
-    """A comparison with the reference's own C is skipped where its source tree is missing."""
+# Tests that compare with the reference's own C and cannot tell by themselves that it is missing.
+NEEDS_REFERENCE = {"test_c_driver_output_equals_reference_bitwise"}
+
+
+def pytest_collection_modifyitems(items):
+    """They are skipped where there are no sources to build it from.  Where there are, a library
+    that was not built is a failure, and so it is in every other test."""
     import oracle
 
-    try:
-        return (yield)
-    except oracle.ReferenceNotBuilt as e:
-        pytest.skip(str(e))
+    import __graft_entry__ as entry
+
+    if oracle.ref_available() or entry.reference_source():
+        return
+    for item in items:
+        if getattr(item, "originalname", item.name) in NEEDS_REFERENCE:
+            item.add_marker(pytest.mark.skip(reason="the reference's sources are not here"))
 
 
 def load_golden(name):
