@@ -144,12 +144,12 @@ __device__ __forceinline__ float rcp(float v) {
 }
 constexpr float kLog2e = 1.4426950408889634f;
 
-// v / (1 + exp(-v)).  fp32 results take expf and a rounded division.  For bf16 results,
-// whose half step is 2^-8 of the value, ex2 and a reciprocal (2 ulp each; the exponent's
-// rounding adds |v| 2^-24) stay below 2^-19 for |v| up to 16, where the result or exp(-v)
-// is beyond bf16's reach; 5 instructions instead of about 30.  Results below 1e-36 in
-// magnitude (v under -87) come out as zero.  Both give NaN for
-// v = -infinity, as the formula does.
+// v / (1 + exp(-v)).  fp32 results take expf and a rounded division; below -88.7 expf is
+// infinite and the result zero (3e-37 at most is lost).  For bf16 results, whose half step is
+// 2^-8 of the value, ex2 and a reciprocal (2 ulp each) with the exponent's two roundings, which
+// add 2 |v| u, stay within (8 + 2 |v|) u, u = 2^-24: 2^-16 at v = -87; 5 instructions instead of
+// about 30.  Results below 1.1e-36 in magnitude (v under -87.3) come out as zero.  Both give NaN
+// for v = -infinity, as the formula does.
 template <typename T>
 __device__ __forceinline__ float silu(float v) {
   if constexpr (sizeof(T) == 4)

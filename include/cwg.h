@@ -213,8 +213,8 @@ int cwg_conv3x3_nonfused(const float *x, const float *U, const float *bias, floa
  *
  * Prompts are packed: sequence b is rows starts[b] .. starts[b+1]-1 (device,
  * int32, n_seq + 1 offsets, ascending, at most `tokens`).  An empty sequence is
- * allowed; rows that belong to no sequence are neither read nor written.  At most 2^30 tokens,
- * sequences and channels.
+ * allowed; rows that belong to no sequence are not written, and affect no result.  At most
+ * 2^30 tokens, sequences and channels.
  *
  * State between calls is kept in cache lines, one per sequence: sequence b uses
  * line slots[b] of `state` (device, int32; NULL: line b).  With resume[b] != 0 a
@@ -284,8 +284,8 @@ typedef struct cwg_ssm {
 size_t cwg_ssm_workspace_bytes(int tokens, int n_seq, int channels, int states);
 int cwg_ssm_scan(const cwg_ssm *op, void *workspace, size_t workspace_bytes, void *stream);
 
-/* One token of each of op->tokens sequences (at most 65535): row i, line slots[i], updated
- * in place. */
+/* One token of each of op->tokens sequences (at most 65535, and as many groups): row i, line
+ * slots[i], updated in place. */
 int cwg_ssm_step(const cwg_ssm *op, void *stream);
 
 /* ---- 8-bit matrix product with scales per block of 128 (DEVICE pointers) ------- */
@@ -308,8 +308,10 @@ int cwg_fp8_quantize(const void *x, long long ldx, void *q, long long ldq, float
  * a e4m3 [m][k], w e4m3 [n][k] (a weight's rows are outputs), as cwg_fp8_quantize
  * writes them with block_rows 1 and 128; a and w 16-byte aligned with lda and ldw
  * multiples of 16 (k itself may be any size >= 1).  y fp32 [m][n], or bf16 with
- * CWG_BF16; bias fp32 [n] or NULL; act: CWG_RELU or none.  y must not overlap the inputs, from
- * the first row to the last: CWG_EINVAL. */
+ * CWG_BF16; bias fp32 [n] or NULL; act: CWG_RELU or none.  The two scales of a block are
+ * multiplied first, in fp32: a product beyond its range gives an infinity or NaN, one below
+ * 2^-126 loses precision.  y must not overlap the inputs, from the first row to the last:
+ * CWG_EINVAL. */
 int cwg_fp8_matmul(const void *a, long long lda, const float *a_scale, long long lda_scale,
                    const void *w, long long ldw, const float *w_scale, long long ldw_scale,
                    const float *bias, void *y, long long ldy, int m, int n, int k,

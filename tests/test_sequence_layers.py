@@ -949,3 +949,36 @@ def test_device_status_waits_for_the_calls_that_it_reports(cuda_dev, default_str
     finally:
         torch.cuda.synchronize()
         cwg.lib().cwg_device_status(None)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_silu_of_large_negative_values(cuda_dev, dtype):
+    """The convolution's activation and the scan's gate down to -100: within the stated error as
+    far as results are above 1.1e-36, and next to zero beyond."""
+    v = (-torch.arange(0, 1601) / 16).to(DT[dtype])  # exact in fp32, rounded once in bf16
+    ch = len(v)
+    x = v[None]
+    w = torch.tensor([0.0, 1.0]).repeat(ch, 1)
+    flags = cwg.BF16 if dtype == "bf16" else 0
+    y, state = torch.empty_like(x, device=cuda_dev), torch.zeros(1, 1, ch, dtype=DT[dtype])
+    cwg.conv1d_causal_step(x.to(cuda_dev), w.to(cuda_dev), None, y, state.to(cuda_dev), None,
+                           flags | cwg.SILU)
+    # decay 1, step 1, u B C = 1: the gate's argument is all that counts
+    one, ab = torch.ones(1, ch, dtype=DT[dtype]), torch.ones(1, 1, dtype=DT[dtype])
+    gated = torch.empty_like(y)
+    cwg.ssm_step(one.to(cuda_dev), one.to(cuda_dev), torch.zeros(ch, 1, device=cuda_dev),
+                 ab.to(cuda_dev), ab.to(cuda_dev), None, None, x.to(cuda_dev), gated,
+                 torch.zeros(1, ch, 1, device=cuda_dev), None, flags)
+    gated_prompt = torch.empty_like(y)
+    cwg.ssm_scan(one.to(cuda_dev), one.to(cuda_dev), torch.zeros(ch, 1, device=cuda_dev),
+                 ab.to(cuda_dev), ab.to(cuda_dev), None, None, x.to(cuda_dev), gated_prompt, None,
+                 torch.tensor([0, 1], dtype=torch.int32, device=cuda_dev), flags=flags)
+    z = x.to(torch.float64)
+    want = R.silu(z)
+    normal = z >= -87
+    assert normal.sum() > 1300 and (~normal).sum() > 100
+    bound = (R.silu_error(z, DT[dtype]) + R.U) * want.abs()
+    bound = R.half_step(DT[dtype]) * (want.abs() + bound) + bound
+    for got in (y, gated, gated_prompt):
+        off = (got.cpu().to(torch.float64) - want).abs()
+        assert (off <= torch.where(normal, bound, 1.5e-36)).all()
