@@ -55,6 +55,14 @@ __device__ __forceinline__ void store_states(float *line, int i0, int n, bool ve
   }
 }
 
+// A log2(e), kept finite: rows behind a sequence's last token have a step of zero, which has to
+// leave the states as they are, and zero times an infinity would not.
+__device__ __forceinline__ float decay_rate(float A) {
+  constexpr float kMost = 3.402823466e38f;
+  const float v = A * kLog2e;
+  return fabsf(v) > kMost ? copysignf(kMost, v) : v;  // NaN stays
+}
+
 // ---- prompts --------------------------------------------------------------------
 // One CTA per (sequence, block of kCH channels of one group) walks the sequence in tiles
 // of kTT tokens, its warps in two roles that work on neighbouring tiles at the same time:
@@ -295,6 +303,8 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads, MODE == kRoomy ? 1 : 0)
     float *line = p.state + (size_t)(slot < 0 ? 0 : slot) * width + at;
     if (mine) {
       load_states(p.A + at, i0, p.states, a.vec_a, A2);
+#pragma unroll
+      for (int k = 0; k < kS; ++k) A2[k] = decay_rate(A2[k]);
       float *ends = a.ends + (size_t)head * width + at;  // of the sequence's first chunk
       const bool vec = p.states == kS * L;
       if (part == 0 && (SUMMARY || parts == 1)) {
@@ -310,7 +320,7 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads, MODE == kRoomy ? 1 : 0)
           load_states(ends + (size_t)j * width, i0, p.states, vec, e);
           const float d = a.sums[(size_t)(head + j) * p.channels + c0 + ch];
 #pragma unroll
-          for (int k = 0; k < kS; ++k) h[k] = fmaf(ex2(d * (A2[k] * kLog2e)), h[k], e[k]);
+          for (int k = 0; k < kS; ++k) h[k] = fmaf(ex2(d * A2[k]), h[k], e[k]);
         }
       }
     }
@@ -318,7 +328,7 @@ __global__ void __launch_bounds__(Prompt<L>::kThreads, MODE == kRoomy ? 1 : 0)
     F2 a2[kS / 2], hh[kS / 2];
 #pragma unroll
     for (int k = 0; k < kS / 2; ++k) {
-      a2[k] = f2(A2[2 * k] * kLog2e, A2[2 * k + 1] * kLog2e);
+      a2[k] = f2(A2[2 * k], A2[2 * k + 1]);
       hh[k] = f2(h[2 * k], h[2 * k + 1]);
     }
     const int at0 = turned(0, ch >> 3, (ch & 7) >> 1) * 4 + (ch & 1) * 2;

@@ -982,3 +982,24 @@ def test_silu_of_large_negative_values(cuda_dev, dtype):
     for got in (y, gated, gated_prompt):
         off = (got.cpu().to(torch.float64) - want).abs()
         assert (off <= torch.where(normal, bound, 1.5e-36)).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("lens", [[5, 1], [37], [32, 64], [700]], ids=str)
+def test_ssm_states_that_forget_at_once(cuda_dev, dtype, lens):
+    """A = -infinity, or so large that A log2(e) is beyond fp32: exp(step A) is zero for every
+    step, so a state is its last token's drive, wherever the last tile of 32 tokens ends."""
+    ch, n = 40, 6
+    c = ssm_case(dtype, lens, ch, 1, n, 57, gate=False, extras=False, tail=0)
+    c["step"] = c["step"] + 0.125
+    c["A"][:, 1::3], c["A"][:, 2::3] = -float("inf"), -3e38
+    for workspace in (False, True):
+        _, y, state = run_ssm(c, cuda_dev, workspace)
+        for b, slot in enumerate(c["slots"].tolist()):
+            t = c["starts"][b + 1] - 1
+            drive = (c["step"][t].double() * c["u"][t].double())[:, None] * c["B"][t].double()
+            off = (state[slot].cpu().double() - drive)[:, [1, 2, 4, 5]].abs()
+            # step times u and the product with B round once each
+            assert (off <= (2.1 * R.U * drive.abs() + 1e-37)[:, [1, 2, 4, 5]]).all()
+            assert state[slot].isfinite().all()
+        assert y.isfinite().all()
