@@ -1003,3 +1003,65 @@ def test_ssm_states_that_forget_at_once(cuda_dev, dtype, lens):
             assert (off <= (2.1 * R.U * drive.abs() + 1e-37)[:, [1, 2, 4, 5]]).all()
             assert state[slot].isfinite().all()
         assert y.isfinite().all()
+
+
+@pytest.mark.parametrize("tokens,ch", [(2100, 64), (700, 1100)])  # cut into chunks, and not
+def test_captured_prompts_serve_changing_batches(cuda_dev, tokens, ch):
+    """Prompts' calls captured once and replayed with other offsets, lines and inputs in the same
+    tensors, a padded batch among them, give the bits of the same calls made eagerly."""
+    dev, bf, n, lines = cuda_dev, torch.bfloat16, 6, 8
+    g = gen(58)
+    w, w_s = R.quantize(randn(g, 2 * ch, 136, std=0.1), 128)
+    w, w_s = on_dev(w, dev), w_s.to(dev)
+    cw, cb = randn(g, ch, 4).to(dev), randn(g, ch).to(dev)
+    A, D = -torch.rand(ch, 16, generator=g).to(dev), randn(g, ch).to(dev)
+
+    def buffers():
+        x = torch.zeros(tokens, 136, dtype=bf, device=dev)
+        q = on_dev(torch.zeros(tokens, 136).to(torch.float8_e4m3fn), dev)
+        s = torch.empty(tokens, 2, device=dev)
+        xz = torch.zeros(tokens, 2 * ch, dtype=bf, device=dev)
+        bc = torch.zeros(tokens, 32, dtype=bf, device=dev)
+        u, y = (torch.zeros(tokens, ch, dtype=bf, device=dev) for _ in range(2))
+        conv = torch.zeros(lines, 3, ch, dtype=bf, device=dev)
+        h = torch.zeros(lines, ch, 16, device=dev)
+        starts = torch.zeros(n + 1, dtype=torch.int32, device=dev)
+        slots = torch.full((n,), -1, dtype=torch.int32, device=dev)
+        resume = torch.zeros(n, dtype=torch.uint8, device=dev)
+        ws = torch.empty(cwg.ssm_workspace_bytes(tokens, n, ch, 16), dtype=torch.uint8, device=dev)
+
+        def calls():
+            cwg.fp8_quantize(x, q, s, 1, cwg.BF16)
+            cwg.fp8_matmul(q, s, w, w_s, None, xz, cwg.BF16)
+            cwg.conv1d_causal(xz[:, :ch], cw, cb, u, conv, starts, slots, resume,
+                              cwg.BF16 | cwg.SILU)
+            cwg.ssm_scan(u, xz[:, ch:], A, bc[:, :16], bc[:, 16:], D, None, xz[:, ch:], y, h,
+                         starts, slots, resume, ws, cwg.BF16 | cwg.SOFTPLUS)
+        return calls, (x, bc, starts, slots, resume), (xz, u, y, conv, h)
+
+    eager, ins, want = buffers()
+    captured, ins2, got = buffers()
+    eager()
+    captured()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured()
+    batches = (([tokens], [3], [0]), ([tokens // 2, 1, tokens // 3], [3, 0, 7], [1, 0, 0]),
+               ([], [], []), ([5, 0, 9, 64, 2, 33], [7, 1, 0, 3, 4, 5], [1, 1, 1, 1, 0, 0]))
+    for lens, slot, keep in batches:
+        pad = n - len(lens)
+        data = (randn(g, tokens, 136, dtype=bf), randn(g, tokens, 32, dtype=bf),
+                torch.tensor(offsets(lens) + [sum(lens)] * pad, dtype=torch.int32),
+                torch.tensor(slot + [-1] * pad, dtype=torch.int32),
+                torch.tensor(keep + [0] * pad, dtype=torch.uint8))
+        for to in (ins, ins2):
+            for a, b in zip(to, data):
+                a.copy_(b)
+        eager()
+        graph.replay()
+        torch.cuda.synchronize()
+        cwg.device_status()
+        for a, b in zip(want, got):
+            assert torch.equal(a, b), lens
+        assert want[2].isfinite().all()
